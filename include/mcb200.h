@@ -404,11 +404,121 @@ int mcb_linear(const mcb_linear_args* args, void* stream);
 int mcb_linear_supported(const mcb_linear_args* args);
 
 /* ---------------------------------------------------------------------------------------------
+ * The paged cache: K and V in pages of page_size positions (a power of two, 16 to 1024), layout
+ * (n_pages, Hkv, page_size, D) bf16 -- one head's page is one contiguous block --, each request's
+ * pages named by a row of a block table, the batch's new tokens packed (request r's are
+ * [cu_new[r], cu_new[r + 1])).  D = 64 or 128.  Not in the reference, whose KVCache gives every
+ * row T_max positions (modelcore/cache.py:22-25).
+ *
+ * mcb_page_plan: one step's bookkeeping from the lengths alone.  Request r holds cache_seqlens[r]
+ * positions and takes new_lens[r] new tokens: cu_new, the tokens' positions and slots (page *
+ * page_size + offset), and table entries for the pages the request starts to use, taken in request
+ * order from the free queue: entries [head, tail) of free_pages, counter x at x % n_pages,
+ * free_state = {head, tail}, both only growing.  free_state_out (may be free_state) gets the head
+ * after the taken pages; nothing else is moved (cache_seqlens is the caller's to advance), so the
+ * same inputs plan the same step again.  Tokens from the sum of new_lens up to N are padding:
+ * position and slot -1.  When the queue runs out the missing pages are -1, their tokens' slots -1,
+ * and the device error 5 is set; a request past max_pages sets error 1, more new tokens than N
+ * error 7, a table entry outside the pool error 6.
+ *
+ * mcb_page_release: the pages of the requests with done[r] != 0 go to the queue's tail in request
+ * order; seqlens_out (may be cache_seqlens) gets 0 for them and cache_seqlens for the others.
+ * More pages than the pool has room for (a request released twice) set device error 5.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  const int32_t* cache_seqlens;   /* (R,)                                                       */
+  const int32_t* new_lens;        /* (R,)                                                       */
+  int32_t* block_table;           /* (R, max_pages), rows table_stride apart                    */
+  const int32_t* free_pages;      /* (n_pages,) the queue                                       */
+  const int64_t* free_state;      /* (2,) head, tail                                            */
+  int64_t* free_state_out;        /* (2,)                                                       */
+  int32_t* cu_new;                /* (R + 1,)                                                   */
+  int32_t* positions;             /* (N,)                                                       */
+  int64_t* slot_map;              /* (N,)                                                       */
+  int64_t table_stride;           /* elements                                                   */
+  int32_t R, N, n_pages, max_pages, page_size;
+} mcb_page_plan_args;
+
+int mcb_page_plan(const mcb_page_plan_args* args, void* stream);
+
+typedef struct {
+  const int32_t* done;            /* (R,)                                                       */
+  const int32_t* cache_seqlens;   /* (R,)                                                       */
+  const int32_t* block_table;     /* (R, max_pages)                                             */
+  int32_t* free_pages;            /* (n_pages,)                                                 */
+  const int64_t* free_state;      /* (2,)                                                       */
+  int64_t* free_state_out;        /* (2,)                                                       */
+  int32_t* seqlens_out;           /* (R,)                                                       */
+  int64_t table_stride;
+  int32_t R, n_pages, max_pages, page_size;
+} mcb_page_release_args;
+
+int mcb_page_release(const mcb_page_release_args* args, void* stream);
+
+/* mcb_paged_append_rope: mcb_kv_append_rope for packed tokens and a paged cache: q_out = scale *
+ * rms_norm(rope(q)) at each token's position, k the same (raw with rotate_k = 0) and v written to
+ * the token's slot.  k = v = NULL: only q.  A token of position -1 (padding) gets a zero q_out, one
+ * of slot -1 writes nothing.  round_each = 1 rounds every step to bf16 as mcb_kv_append_rope does
+ * (the same bits), 0 keeps fp32 and rounds once. */
+typedef struct {
+  const void* q;                  /* (N, Hq, D) bf16, element strides q_stride (token, head)    */
+  const void* k;                  /* (N, Hkv, D) bf16 or NULL                                   */
+  const void* v;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  void* q_out;                    /* (N, Hq, D) bf16 contiguous                                 */
+  void* k_pages;                  /* (n_pages, Hkv, page_size, D) bf16                          */
+  void* v_pages;
+  const int32_t* positions;       /* (N,)                                                       */
+  const int64_t* slot_map;        /* (N,)                                                       */
+  const void* cos;                /* (rot_len, D/2) bf16                                        */
+  const void* sin;
+  int32_t N, Hq, Hkv, D, n_pages, page_size, rot_len;
+  float eps, scale;
+  int32_t rotate_k, round_each;
+} mcb_paged_append_args;
+
+int mcb_paged_append_rope(const mcb_paged_append_args* args, void* stream);
+
+/* mcb_paged_attn: out[t, h] = softmax_c(q[t, h] . K[c, h / G] * softmax_scale) . V[c, h / G] for
+ * the packed new tokens t of every request, over the request's keys c at positions c <= pos and
+ * (window < 0 or pos - c <= window), pos = cache_seqlens[r] + t - cu_new[r].  The new tokens' keys
+ * and values are already in the pages.  Tokens past cu_new[R] get zeros; nothing past a request's
+ * last position, or before the first its tokens see, reaches the result, whatever the pages hold
+ * there.  max_new: an upper bound on the requests' new tokens when the caller knows one, 0 when
+ * not: it chooses which kernels are launched, never the result's meaning. */
+typedef struct {
+  const void* q;                  /* (N, Hq, D) bf16, element strides q_stride (token, head)    */
+  int64_t q_stride[2];
+  const void* k_pages;            /* (n_pages, Hkv, page_size, D) bf16                          */
+  const void* v_pages;
+  const int32_t* block_table;     /* (R, max_pages), rows table_stride apart                    */
+  int64_t table_stride;
+  const int32_t* cache_seqlens;   /* (R,) positions before the new tokens                       */
+  const int32_t* cu_new;          /* (R + 1,)                                                   */
+  void* out;                      /* (N, Hq, D) bf16 contiguous                                 */
+  int32_t R, N, Hq, Hkv, D, n_pages, max_pages, page_size;
+  int32_t window;
+  int32_t max_new;
+  float softmax_scale;
+  void* workspace;                /* mcb_paged_attn_workspace_size() bytes, 256-byte aligned    */
+  size_t workspace_bytes;
+  int32_t* counters;              /* mcb_paged_attn_counter_count() int32, zero before the first
+                                     call, left zero by every completed one                     */
+  size_t counter_count;
+} mcb_paged_attn_args;
+
+size_t mcb_paged_attn_workspace_size(const mcb_paged_attn_args* args);
+size_t mcb_paged_attn_counter_count(const mcb_paged_attn_args* args);
+int mcb_paged_attn(const mcb_paged_attn_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Device-side status.  Kernels never trap: an out-of-range position (a cache or rotary table
  * overflow) or a timed-out pipeline wait sets a device error word and skips the access.
  * mcb_device_error synchronises `stream`, returns the word in *code and clears it.
  * Codes: 0 none, 1 position beyond Tmax, 2 position beyond the rotary table, 3 pipeline wait
- * timed out, 4 token id outside the embedding table.
+ * timed out, 4 token id outside the embedding table, 5 the free pages do not match the request
+ * (too few to take, or returned twice), 6 a page or slot outside the pool, 7 more new tokens than
+ * the packed batch holds.
  * ------------------------------------------------------------------------------------------- */
 int mcb_device_error(int32_t* code, void* stream);
 

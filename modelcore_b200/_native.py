@@ -34,6 +34,9 @@ DEVICE_ERRORS = {
     2: "position beyond the rotary table",
     3: "pipeline wait timed out",
     4: "token id outside the embedding table",
+    5: "the free pages do not match the request (too few to take, or returned twice)",
+    6: "a page or slot outside the pool",
+    7: "more new tokens than the packed batch holds",
 }
 
 ABI_VERSION = 9
@@ -61,6 +64,12 @@ EXPORTED_SYMBOLS = (
     "mcb_linear",
     "mcb_linear_supported",
     "mcb_softcap_argmax",
+    "mcb_page_plan",
+    "mcb_page_release",
+    "mcb_paged_append_rope",
+    "mcb_paged_attn_workspace_size",
+    "mcb_paged_attn_counter_count",
+    "mcb_paged_attn",
     "mcb_device_error",
     "mcb_launch_count",
     "mcb_last_attn_kernel",
@@ -187,6 +196,63 @@ class LinearArgs(ctypes.Structure):
     ]
 
 
+_i64x2 = ctypes.c_int64 * 2
+
+
+class PagePlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache_seqlens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("free_state", ctypes.c_void_p), ("free_state_out", ctypes.c_void_p),
+        ("cu_new", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("slot_map", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("R", ctypes.c_int32), ("N", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class PageReleaseArgs(ctypes.Structure):
+    _fields_ = [
+        ("done", ctypes.c_void_p), ("cache_seqlens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("free_state", ctypes.c_void_p), ("free_state_out", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("R", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_stride", _i64x2), ("k_stride", _i64x2), ("v_stride", _i64x2),
+        ("q_out", ctypes.c_void_p), ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("slot_map", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+        ("N", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("rot_len", ctypes.c_int32), ("eps", ctypes.c_float), ("scale", ctypes.c_float),
+        ("rotate_k", ctypes.c_int32), ("round_each", ctypes.c_int32),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_stride", _i64x2),
+        ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("cache_seqlens", ctypes.c_void_p), ("cu_new", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("R", ctypes.c_int32), ("N", ctypes.c_int32), ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("window", ctypes.c_int32), ("max_new", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("counters", ctypes.c_void_p), ("counter_count", ctypes.c_size_t),
+    ]
+
+
 class McbError(RuntimeError):
     """A C-ABI call returned a non-zero mcb_status."""
 
@@ -241,6 +307,13 @@ def _declare(lib):
     lib.mcb_device_error.argtypes = [P(ctypes.c_int32), ctypes.c_void_p]
     lib.mcb_launch_count.restype = ctypes.c_uint64
     lib.mcb_launch_count.argtypes = []
+    for name, cls in (("mcb_page_plan", PagePlanArgs), ("mcb_page_release", PageReleaseArgs),
+                      ("mcb_paged_append_rope", PagedAppendArgs), ("mcb_paged_attn", PagedAttnArgs)):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [P(cls), ctypes.c_void_p]
+    for name in ("mcb_paged_attn_workspace_size", "mcb_paged_attn_counter_count"):
+        getattr(lib, name).restype = ctypes.c_size_t
+        getattr(lib, name).argtypes = [P(PagedAttnArgs)]
     lib.mcb_last_attn_kernel.restype = ctypes.c_int
     lib.mcb_last_attn_kernel.argtypes = [ctypes.c_char_p, ctypes.c_size_t]
 

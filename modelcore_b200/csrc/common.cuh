@@ -18,6 +18,9 @@ enum DeviceError : int {
   kErrPositionBeyondRotary = 2,
   kErrWaitTimeout = 3,
   kErrTokenOutOfRange = 4,
+  kErrPagesExhausted = 5,
+  kErrPageOutOfRange = 6,
+  kErrTooManyTokens = 7,
 };
 // Defined once here: the library is a single translation unit (mcb200.cu).
 __device__ int g_device_error = 0;

@@ -20,6 +20,9 @@
 #include "decode_attn_split.cuh"
 #include "kv_append.cuh"
 #include "kv_copy.cuh"
+#include "paged_append.cuh"
+#include "paged_attn.cuh"
+#include "paged_plan.cuh"
 #include "prefill_attn.cuh"
 #include "decode_proj.cuh"
 #include "sample.cuh"
@@ -1671,3 +1674,5 @@ int mcb_device_error(int32_t* code, void* stream) {
 }
 
 }  // extern "C"
+
+#include "paged_api.cuh"

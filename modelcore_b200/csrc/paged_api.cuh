@@ -1,0 +1,308 @@
+// C-ABI entry points of the paged cache (declared in include/mcb200.h): host-side validation and
+// launches.  Included by mcb200.cu, whose helpers it uses.
+#pragma once
+
+namespace {
+
+// Runs a C entry's body: no C++ exception (a failed host allocation) leaves the library.
+template <typename F>
+int guarded(const char* what, F body) {
+  try {
+    return body();
+  } catch (...) {
+    try {
+      return fail(MCB_ERR_CUDA, "%s: host allocation failed", what);
+    } catch (...) {
+      return MCB_ERR_CUDA;
+    }
+  }
+}
+
+int page_shift_of(int page_size) {
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+int check_page_size(int page_size, const char* who) {
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 1024)", who, page_size);
+  return MCB_OK;
+}
+
+int check_pool(int n_pages, int page_size, int max_pages, const char* who) {
+  if (n_pages <= 0 || max_pages <= 0)
+    return fail(MCB_ERR_INVALID_ARG, "%s: n_pages %d and max_pages %d must be positive", who, n_pages, max_pages);
+  if (static_cast<long long>(max_pages) * page_size > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: max_pages %d * page_size %d positions a request (at most 2^31 - 1)", who,
+                max_pages, page_size);
+  return check_page_size(page_size, who);
+}
+
+// Launches one cluster of `ctas` CTAs (the whole grid) with programmatic stream serialization.
+template <typename P>
+cudaError_t launch_one_cluster(void (*kernel)(P), int ctas, int threads, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+int page_plan(const mcb_page_plan_args* a, void* stream) {
+  const char* who = "mcb_page_plan";
+  if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (a->R < 0 || a->N < 0) return fail(MCB_ERR_INVALID_ARG, "%s: bad sizes R=%d N=%d", who, a->R, a->N);
+  int rc = check_pool(a->n_pages, a->page_size, a->max_pages, who);
+  if (rc != MCB_OK) return rc;
+  if (a->cu_new == nullptr || a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr ||
+      (a->R > 0 && (a->cache_seqlens == nullptr || a->new_lens == nullptr || a->block_table == nullptr)) ||
+      (a->N > 0 && (a->positions == nullptr || a->slot_map == nullptr)))
+    return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
+  if (a->table_stride < a->max_pages)
+    return fail(MCB_ERR_INVALID_ARG, "%s: table_stride %lld below max_pages %d", who,
+                static_cast<long long>(a->table_stride), a->max_pages);
+  mcb::PagePlanParams p = {};
+  p.seqlens = a->cache_seqlens;
+  p.new_lens = a->new_lens;
+  p.block_table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.free_pages = a->free_pages;
+  p.free_state = reinterpret_cast<const long long*>(a->free_state);
+  p.free_state_out = reinterpret_cast<long long*>(a->free_state_out);
+  p.cu_new = a->cu_new;
+  p.positions = a->positions;
+  p.slot_map = reinterpret_cast<long long*>(a->slot_map);
+  p.R = a->R;
+  p.N = a->N;
+  p.n_pages = a->n_pages;
+  p.max_pages = a->max_pages;
+  p.page_shift = page_shift_of(a->page_size);
+  // a thread a row up to 1,024, and about two tokens a thread before another CTA joins
+  const int threads = a->R <= 256 && a->N <= 512 ? 256 : mcb::kPlanMaxThreads;
+  const int ctas = std::clamp((a->N + 2 * threads - 1) / (2 * threads), 1, mcb::kPlanMaxCluster);
+  cudaError_t e = launch_one_cluster(mcb::page_plan_kernel, ctas, threads, static_cast<cudaStream_t>(stream), p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "page_plan launch");
+  return MCB_OK;
+}
+
+int page_release(const mcb_page_release_args* a, void* stream) {
+  const char* who = "mcb_page_release";
+  if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (a->R < 0) return fail(MCB_ERR_INVALID_ARG, "%s: bad size R=%d", who, a->R);
+  int rc = check_pool(a->n_pages, a->page_size, a->max_pages, who);
+  if (rc != MCB_OK) return rc;
+  if (a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr ||
+      (a->R > 0 && (a->done == nullptr || a->cache_seqlens == nullptr || a->block_table == nullptr ||
+                    a->seqlens_out == nullptr)))
+    return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
+  if (a->table_stride < a->max_pages)
+    return fail(MCB_ERR_INVALID_ARG, "%s: table_stride %lld below max_pages %d", who,
+                static_cast<long long>(a->table_stride), a->max_pages);
+  mcb::PageReleaseParams p = {};
+  p.done = a->done;
+  p.seqlens = a->cache_seqlens;
+  p.block_table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.free_pages = a->free_pages;
+  p.free_state = reinterpret_cast<const long long*>(a->free_state);
+  p.free_state_out = reinterpret_cast<long long*>(a->free_state_out);
+  p.seqlens_out = a->seqlens_out;
+  p.R = a->R;
+  p.n_pages = a->n_pages;
+  p.max_pages = a->max_pages;
+  p.page_shift = page_shift_of(a->page_size);
+  const int threads = mcb::kPlanMaxThreads;
+  const long long most = static_cast<long long>(a->R) * a->max_pages;  // pages that can come back
+  const int ctas = static_cast<int>(std::clamp<long long>(most / (4 * threads), 1, mcb::kPlanMaxCluster));
+  cudaError_t e = launch_one_cluster(mcb::page_release_kernel, ctas, threads, static_cast<cudaStream_t>(stream), p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "page_release launch");
+  return MCB_OK;
+}
+
+bool rows16(const void* p, const int64_t* strides) {
+  return aligned(p, 16) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
+}
+
+int check_paged_heads(int D, const char* who) {
+  if (D != 64 && D != 128) return fail(MCB_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", who, D);
+  return MCB_OK;
+}
+
+int paged_append(const mcb_paged_append_args* a, void* stream) {
+  const char* who = "mcb_paged_append_rope";
+  if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (a->N < 0 || a->Hq <= 0 || a->Hkv <= 0)
+    return fail(MCB_ERR_INVALID_ARG, "%s: bad sizes N=%d Hq=%d Hkv=%d", who, a->N, a->Hq, a->Hkv);
+  int rc = check_paged_heads(a->D, who);
+  if (rc != MCB_OK) return rc;
+  const bool kv = a->k != nullptr;
+  if (kv != (a->v != nullptr)) return fail(MCB_ERR_INVALID_ARG, "%s: k and v come together", who);
+  if (a->N == 0) return MCB_OK;
+  if (a->q == nullptr || a->q_out == nullptr || a->positions == nullptr || a->cos == nullptr || a->sin == nullptr ||
+      (kv && (a->k_pages == nullptr || a->v_pages == nullptr || a->slot_map == nullptr)))
+    return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
+  if (a->rot_len <= 0) return fail(MCB_ERR_INVALID_ARG, "%s: rot_len %d", who, a->rot_len);
+  if (kv) {
+    rc = check_page_size(a->page_size, who);
+    if (rc != MCB_OK) return rc;
+    if (a->n_pages <= 0) return fail(MCB_ERR_INVALID_ARG, "%s: n_pages %d", who, a->n_pages);
+  }
+  for (int i = 0; i < 2; ++i)
+    if (a->q_stride[i] < 0 || (kv && (a->k_stride[i] < 0 || a->v_stride[i] < 0)))
+      return fail(MCB_ERR_INVALID_ARG, "%s: negative stride", who);
+  if (!rows16(a->q, a->q_stride) || !aligned(a->q_out, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16) ||
+      (kv && (!rows16(a->k, a->k_stride) || !rows16(a->v, a->v_stride) || !aligned(a->k_pages, 16) ||
+              !aligned(a->v_pages, 16))))
+    return fail(MCB_ERR_ALIGNMENT, "%s: head vectors, tables and pages must start on 16-byte boundaries", who);
+  mcb::PagedAppendParams p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.k = static_cast<const uint16_t*>(a->k);
+  p.v = static_cast<const uint16_t*>(a->v);
+  for (int i = 0; i < 2; ++i) {
+    p.qs[i] = a->q_stride[i];
+    p.ks[i] = a->k_stride[i];
+    p.vs[i] = a->v_stride[i];
+  }
+  p.q_out = static_cast<uint16_t*>(a->q_out);
+  p.k_pages = static_cast<uint16_t*>(a->k_pages);
+  p.v_pages = static_cast<uint16_t*>(a->v_pages);
+  p.positions = a->positions;
+  p.slot_map = reinterpret_cast<const long long*>(a->slot_map);
+  p.cos = static_cast<const uint16_t*>(a->cos);
+  p.sin = static_cast<const uint16_t*>(a->sin);
+  p.N = a->N;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.page_shift = kv ? page_shift_of(a->page_size) : 0;
+  p.n_slots = static_cast<long long>(a->n_pages) * a->page_size;
+  p.rot_len = a->rot_len;
+  p.eps = a->eps;
+  p.scale = a->scale;
+  p.nk = kv ? a->Hkv : 0;
+  p.rotate_k = a->rotate_k != 0;
+  p.total_vectors = static_cast<long long>(a->N) * (p.Hq + 2ll * p.nk);
+  if (p.total_vectors > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: %lld vectors in one call (at most 2^31 - 1)", who, p.total_vectors);
+  const long long vpw = 32 / (a->D / 16), wpb = mcb::kAppendVecThreads / 32;
+  const long long blocks = std::min<long long>((p.total_vectors + vpw * wpb - 1) / (vpw * wpb),
+                                               static_cast<long long>(kAppendVecCtasPerSm) * device_sm_count());
+  const dim3 grid(static_cast<unsigned>(blocks)), block(mcb::kAppendVecThreads);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (a->D == 64)
+    e = a->round_each ? launch_pdl(mcb::paged_append_kernel<64, true>, grid, block, 0, st, p)
+                      : launch_pdl(mcb::paged_append_kernel<64, false>, grid, block, 0, st, p);
+  else
+    e = a->round_each ? launch_pdl(mcb::paged_append_kernel<128, true>, grid, block, 0, st, p)
+                      : launch_pdl(mcb::paged_append_kernel<128, false>, grid, block, 0, st, p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_append launch");
+  return MCB_OK;
+}
+
+// Shape checks of mcb_paged_attn: what its size queries need as well.
+int check_paged_attn(const mcb_paged_attn_args* a, const char* who) {
+  if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (a->R < 0 || a->N < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->max_new < 0)
+    return fail(MCB_ERR_INVALID_ARG, "%s: bad sizes R=%d N=%d Hq=%d Hkv=%d max_new=%d", who, a->R, a->N, a->Hq,
+                a->Hkv, a->max_new);
+  if (a->Hq % a->Hkv != 0)
+    return fail(MCB_ERR_INVALID_ARG, "%s: Hq %d must be divisible by Hkv %d", who, a->Hq, a->Hkv);
+  if (a->Hq / a->Hkv > 128)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: %d query heads a kv head (at most 128)", who, a->Hq / a->Hkv);
+  int rc = check_paged_heads(a->D, who);
+  if (rc != MCB_OK) return rc;
+  rc = check_pool(a->n_pages, a->page_size, a->max_pages, who);
+  if (rc != MCB_OK) return rc;
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3e38f)
+    return fail(MCB_ERR_INVALID_ARG, "%s: softmax_scale %g must be positive and finite", who, a->softmax_scale);
+  if (static_cast<long long>(a->n_pages) * a->Hkv > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: n_pages %d * Hkv %d above 2^31 - 1", who, a->n_pages, a->Hkv);
+  return MCB_OK;
+}
+
+int paged_attn(const mcb_paged_attn_args* a, void* stream) {
+  const char* who = "mcb_paged_attn";
+  int rc = check_paged_attn(a, who);
+  if (rc != MCB_OK) return rc;
+  if (a->N == 0) return MCB_OK;
+  if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr ||
+      a->cu_new == nullptr || (a->R > 0 && (a->block_table == nullptr || a->cache_seqlens == nullptr)))
+    return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
+  if (a->q_stride[0] < 0 || a->q_stride[1] < 0 || a->table_stride < a->max_pages)
+    return fail(MCB_ERR_INVALID_ARG, "%s: negative q stride or table_stride below max_pages", who);
+  if (!rows16(a->q, a->q_stride) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
+    return fail(MCB_ERR_ALIGNMENT, "%s: q rows, out and pages must start on 16-byte boundaries", who);
+  mcb::PagedAttnParams p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.qs[0] = a->q_stride[0];
+  p.qs[1] = a->q_stride[1];
+  p.k_pages = static_cast<const uint16_t*>(a->k_pages);
+  p.v_pages = static_cast<const uint16_t*>(a->v_pages);
+  p.block_table = a->block_table;
+  p.table_stride = a->table_stride;
+  p.seqlens = a->cache_seqlens;
+  p.cu_new = a->cu_new;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.R = a->R;
+  p.N = a->N;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.G = a->Hq / a->Hkv;
+  p.n_pages = a->n_pages;
+  p.max_pages = a->max_pages;
+  p.page_shift = page_shift_of(a->page_size);
+  p.window = a->window;
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  const long long warps = static_cast<long long>(a->N) * a->Hq;
+  const dim3 grid(static_cast<unsigned>((warps + 3) / 4)), block(128);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = a->D == 64 ? launch_pdl(mcb::paged_attn_plain_kernel<64>, grid, block, 0, st, p)
+                             : launch_pdl(mcb::paged_attn_plain_kernel<128>, grid, block, 0, st, p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attn launch");
+  return MCB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mcb_page_plan(const mcb_page_plan_args* a, void* stream) {
+  return guarded("mcb_page_plan", [&] { return page_plan(a, stream); });
+}
+int mcb_page_release(const mcb_page_release_args* a, void* stream) {
+  return guarded("mcb_page_release", [&] { return page_release(a, stream); });
+}
+int mcb_paged_append_rope(const mcb_paged_append_args* a, void* stream) {
+  return guarded("mcb_paged_append_rope", [&] { return paged_append(a, stream); });
+}
+size_t mcb_paged_attn_workspace_size(const mcb_paged_attn_args* a) {
+  (void)a;
+  return 0;
+}
+size_t mcb_paged_attn_counter_count(const mcb_paged_attn_args* a) {
+  (void)a;
+  return 0;
+}
+int mcb_paged_attn(const mcb_paged_attn_args* a, void* stream) {
+  return guarded("mcb_paged_attn", [&] { return paged_attn(a, stream); });
+}
+
+}  // extern "C"

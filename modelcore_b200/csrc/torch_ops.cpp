@@ -15,6 +15,9 @@
 //   linear          mcb_linear's plain, residual, gated and norm-out projections (the decode
 //                   step's, modelcore/components/linear.py:14 with block.py:57-59, mlp.py:89-90)
 //   add_rms_norm    the residual add and the next RMSNorm (block.py:57-59, norm.py:43-44)
+//   page_plan, page_release, paged_append_rope, paged_attn
+//                   the paged cache: one step's block tables and slots, a finished request's
+//                   pages back, the append and the attention over pages (include/mcb200.h)
 //
 // Every op runs on the current CUDA stream of its tensors' device, checks dtypes, devices and
 // dimensions here (TORCH_CHECK: a RuntimeError in Python) and leaves sizes, strides and
@@ -29,7 +32,9 @@
 
 #include <cmath>
 #include <limits>
+#include <map>
 #include <mutex>
+#include <tuple>
 #include <vector>
 
 #include "../../include/mcb200.h"
@@ -385,6 +390,247 @@ void add_rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& delta, c
   check_status(mcb_add_rms_norm(&a, stream_of(x)), "mcb200::add_rms_norm");
 }
 
+// -- the paged cache -------------------------------------------------------------------------
+int32_t to_i32(int64_t v, const char* name) {
+  TORCH_CHECK(v >= std::numeric_limits<int32_t>::min() && v <= std::numeric_limits<int32_t>::max(), name, " is ", v,
+              ", outside 32 bits");
+  return static_cast<int32_t>(v);
+}
+
+void int_vec(const at::Tensor& t, const char* name, int64_t n, const at::Tensor& ref, at::ScalarType dtype) {
+  need(t, name, 1, dtype);
+  same_device(ref, t, name);
+  TORCH_CHECK(t.size(0) == n && t.is_contiguous(), name, " must be a contiguous (", n, ",) ", dtype, " tensor, got ",
+              t.sizes());
+}
+
+// Checks a block table and returns its row stride (one row's is arbitrary in torch).
+int64_t check_block_table(const at::Tensor& t, int64_t rows, const at::Tensor& ref) {
+  need(t, "block_table", 2, at::kInt);
+  same_device(ref, t, "block_table");
+  TORCH_CHECK(t.size(0) == rows && (t.size(1) <= 1 || rows == 0 || t.stride(1) == 1) &&
+                  (rows <= 1 || t.stride(0) >= t.size(1)),
+              "block_table must be (", rows, ", max_pages) with contiguous rows, got ", t.sizes(), " strides ",
+              t.strides());
+  return rows <= 1 ? t.size(1) : t.stride(0);
+}
+
+// (N, H, D) packed head vectors with any token and head strides
+void packed_strides(const at::Tensor& t, const char* name, int64_t (&s)[2]) {
+  TORCH_CHECK(t.stride(2) == 1, name, ": the head dimension must be contiguous");
+  s[0] = t.stride(0);
+  s[1] = t.stride(1);
+}
+
+void check_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
+  need(k, "k_pages", 4, at::kBFloat16);
+  need(v, "v_pages", 4, at::kBFloat16);
+  same_device(q, k, "k_pages");
+  same_device(q, v, "v_pages");
+  TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && k.sizes() == v.sizes() && k.size(3) == q.size(2),
+              "k_pages and v_pages must be contiguous (n_pages, Hkv, page_size, ", q.size(2), "), got ", k.sizes(),
+              " and ", v.sizes());
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache_seqlens, const at::Tensor& new_lens,
+                                                         const at::Tensor& block_table, const at::Tensor& free_pages,
+                                                         const at::Tensor& free_state, const at::Tensor& free_state_out,
+                                                         int64_t page_size, int64_t num_tokens) {
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  c10::cuda::CUDAGuard guard(cache_seqlens.device());
+  const int64_t R = cache_seqlens.size(0);
+  int_vec(cache_seqlens, "cache_seqlens", R, cache_seqlens, at::kInt);
+  int_vec(new_lens, "new_lens", R, cache_seqlens, at::kInt);
+  const int64_t table_stride = check_block_table(block_table, R, cache_seqlens);
+  int_vec(free_pages, "free_pages", free_pages.size(0), cache_seqlens, at::kInt);
+  int_vec(free_state, "free_state", 2, cache_seqlens, at::kLong);
+  int_vec(free_state_out, "free_state_out", 2, cache_seqlens, at::kLong);
+  TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative, got ", num_tokens);
+  at::Tensor cu = at::empty({R + 1}, cache_seqlens.options());
+  at::Tensor pos = at::empty({num_tokens}, cache_seqlens.options());
+  at::Tensor slots = at::empty({num_tokens}, cache_seqlens.options().dtype(at::kLong));
+  mcb_page_plan_args a = {};
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.free_pages = free_pages.data_ptr<int32_t>();
+  a.free_state = free_state.data_ptr<int64_t>();
+  a.free_state_out = free_state_out.data_ptr<int64_t>();
+  a.cu_new = cu.data_ptr<int32_t>();
+  a.positions = pos.data_ptr<int32_t>();
+  a.slot_map = slots.data_ptr<int64_t>();
+  a.table_stride = table_stride;
+  a.R = to_i32(R, "R");
+  a.N = to_i32(num_tokens, "num_tokens");
+  a.n_pages = to_i32(free_pages.size(0), "n_pages");
+  a.max_pages = to_i32(block_table.size(1), "max_pages");
+  a.page_size = to_i32(page_size, "page_size");
+  check_status(mcb_page_plan(&a, stream_of(cache_seqlens)), "mcb200::page_plan");
+  return {cu, pos, slots};
+}
+
+void page_release(const at::Tensor& done, const at::Tensor& cache_seqlens, const at::Tensor& block_table,
+                  const at::Tensor& free_pages, const at::Tensor& free_state, const at::Tensor& free_state_out,
+                  const at::Tensor& seqlens_out, int64_t page_size) {
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  c10::cuda::CUDAGuard guard(cache_seqlens.device());
+  const int64_t R = cache_seqlens.size(0);
+  int_vec(cache_seqlens, "cache_seqlens", R, cache_seqlens, at::kInt);
+  int_vec(done, "done", R, cache_seqlens, at::kInt);
+  int_vec(seqlens_out, "seqlens_out", R, cache_seqlens, at::kInt);
+  const int64_t table_stride = check_block_table(block_table, R, cache_seqlens);
+  int_vec(free_pages, "free_pages", free_pages.size(0), cache_seqlens, at::kInt);
+  int_vec(free_state, "free_state", 2, cache_seqlens, at::kLong);
+  int_vec(free_state_out, "free_state_out", 2, cache_seqlens, at::kLong);
+  mcb_page_release_args a = {};
+  a.done = done.data_ptr<int32_t>();
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.free_pages = free_pages.data_ptr<int32_t>();
+  a.free_state = free_state.data_ptr<int64_t>();
+  a.free_state_out = free_state_out.data_ptr<int64_t>();
+  a.seqlens_out = seqlens_out.data_ptr<int32_t>();
+  a.table_stride = table_stride;
+  a.R = to_i32(R, "R");
+  a.n_pages = to_i32(free_pages.size(0), "n_pages");
+  a.max_pages = to_i32(block_table.size(1), "max_pages");
+  a.page_size = to_i32(page_size, "page_size");
+  check_status(mcb_page_release(&a, stream_of(cache_seqlens)), "mcb200::page_release");
+}
+
+at::Tensor paged_append_rope(const at::Tensor& q, const std::optional<at::Tensor>& k,
+                             const std::optional<at::Tensor>& v, const std::optional<at::Tensor>& k_pages,
+                             const std::optional<at::Tensor>& v_pages, const at::Tensor& positions,
+                             const std::optional<at::Tensor>& slot_map, const at::Tensor& cos, const at::Tensor& sin,
+                             std::optional<double> eps, double scale, bool rotate_k, bool round_each) {
+  need(q, "q", 3, at::kBFloat16);
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t N = q.size(0), D = q.size(2);
+  int_vec(positions, "positions", N, q, at::kInt);
+  for (const at::Tensor* t : {&cos, &sin}) {
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->dim() >= 1 &&
+                    t->size(-1) == D / 2,
+                "the rotary tables must be contiguous bf16 CUDA tensors with D/2 = ", D / 2, " columns");
+    same_device(q, *t, "rotary table");
+  }
+  TORCH_CHECK(cos.numel() == sin.numel(), "the rotary tables differ in length");
+  const bool kv = k.has_value();
+  TORCH_CHECK(kv == v.has_value() && kv == k_pages.has_value() && kv == v_pages.has_value() &&
+                  kv == slot_map.has_value(),
+              "k, v, k_pages, v_pages and slot_map come together (all or none)");
+  at::Tensor q_out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  mcb_paged_append_args a = {};
+  a.q = q.data_ptr();
+  packed_strides(q, "q", a.q_stride);
+  a.q_out = q_out.data_ptr();
+  a.Hkv = 1;
+  if (kv) {
+    need(*k, "k", 3, at::kBFloat16);
+    need(*v, "v", 3, at::kBFloat16);
+    same_device(q, *k, "k");
+    same_device(q, *v, "v");
+    check_pages(*k_pages, *v_pages, q);
+    TORCH_CHECK(k->sizes() == v->sizes() && k->size(0) == N && k->size(1) == k_pages->size(1) && k->size(2) == D,
+                "k and v must be (", N, ", ", k_pages->size(1), ", ", D, "), got ", k->sizes(), " and ", v->sizes());
+    int_vec(*slot_map, "slot_map", N, q, at::kLong);
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    packed_strides(*k, "k", a.k_stride);
+    packed_strides(*v, "v", a.v_stride);
+    a.k_pages = k_pages->data_ptr();
+    a.v_pages = v_pages->data_ptr();
+    a.slot_map = slot_map->data_ptr<int64_t>();
+    a.Hkv = to_i32(k_pages->size(1), "Hkv");
+    a.n_pages = to_i32(k_pages->size(0), "n_pages");
+    a.page_size = to_i32(k_pages->size(2), "page_size");
+  }
+  a.positions = positions.data_ptr<int32_t>();
+  a.cos = cos.data_ptr();
+  a.sin = sin.data_ptr();
+  a.rot_len = to_i32(D >= 2 ? cos.numel() / (D / 2) : 0, "rot_len");
+  a.N = to_i32(N, "N");
+  a.Hq = to_i32(q.size(1), "Hq");
+  a.D = to_i32(D, "D");
+  a.eps = norm_eps(eps);
+  a.scale = static_cast<float>(scale);
+  a.rotate_k = rotate_k ? 1 : 0;
+  a.round_each = round_each ? 1 : 0;
+  // an empty tensor's data pointer is null: nothing to do, but only after the checks above
+  if (N > 0) check_status(mcb_paged_append_rope(&a, stream_of(q)), "mcb200::paged_append_rope");
+  return q_out;
+}
+
+// The arrival counters of paged_attn, zero before their first use and left zero by every call: one
+// array per stream, so calls on two streams never share one; a stream under capture gets its own
+// array per capture (zeroed by a node of that graph), so graphs replayed side by side do not either.
+int32_t* paged_counters(const at::Tensor& q, size_t count) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, void*, unsigned long long>, std::vector<at::Tensor>> arrays;
+  const auto stream = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+  if (status != cudaStreamCaptureStatusActive) id = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  auto& bufs = arrays[{q.device().index(), static_cast<void*>(stream), id}];
+  if (bufs.empty() || static_cast<size_t>(bufs.back().numel()) < count) {
+    const int64_t n = std::max<int64_t>(static_cast<int64_t>(count), 1 << 14);
+    bufs.push_back(at::zeros({n}, q.options().dtype(at::kInt)));
+  }
+  return bufs.back().data_ptr<int32_t>();
+}
+
+at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                      const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
+                      int64_t window, std::optional<double> softmax_scale, int64_t max_new) {
+  need(q, "q", 3, at::kBFloat16);
+  c10::cuda::CUDAGuard guard(q.device());
+  check_pages(k_pages, v_pages, q);
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  const int64_t R = cache_seqlens.size(0);
+  int_vec(cache_seqlens, "cache_seqlens", R, q, at::kInt);
+  int_vec(cu_new, "cu_new", R + 1, q, at::kInt);
+  const int64_t table_stride = check_block_table(block_table, R, q);
+  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  mcb_paged_attn_args a = {};
+  a.q = q.data_ptr();
+  packed_strides(q, "q", a.q_stride);
+  a.k_pages = k_pages.data_ptr();
+  a.v_pages = v_pages.data_ptr();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.table_stride = table_stride;
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.cu_new = cu_new.data_ptr<int32_t>();
+  a.out = out.data_ptr();
+  a.R = to_i32(R, "R");
+  a.N = to_i32(q.size(0), "N");
+  a.Hq = to_i32(q.size(1), "Hq");
+  a.Hkv = to_i32(k_pages.size(1), "Hkv");
+  a.D = to_i32(q.size(2), "D");
+  a.n_pages = to_i32(k_pages.size(0), "n_pages");
+  a.max_pages = to_i32(block_table.size(1), "max_pages");
+  a.page_size = to_i32(k_pages.size(2), "page_size");
+  a.window = window < 0 ? -1 : to_i32(window, "window");
+  a.max_new = to_i32(max_new, "max_new");
+  a.softmax_scale = softmax_scale.has_value() ? static_cast<float>(*softmax_scale)
+                                              : static_cast<float>(1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  if (a.N == 0) return out;
+  at::Tensor ws;
+  const size_t bytes = mcb_paged_attn_workspace_size(&a);
+  if (bytes > 0) {
+    ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  const size_t count = mcb_paged_attn_counter_count(&a);
+  if (count > 0) {
+    a.counters = paged_counters(q, count);
+    a.counter_count = count;
+  }
+  check_status(mcb_paged_attn(&a, stream_of(q)), "mcb200::paged_attn");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mcb200, m) {
@@ -405,6 +651,19 @@ TORCH_LIBRARY(mcb200, m) {
   m.def(
       "linear(Tensor x, Tensor weight, Tensor(a!) out, Tensor? res=None, Tensor(b!)? h_out=None, "
       "float? eps=None, bool gated=False, bool pdl=False) -> ()");
+  m.def(
+      "page_plan(Tensor cache_seqlens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, "
+      "Tensor free_state, Tensor(b!) free_state_out, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "page_release(Tensor done, Tensor cache_seqlens, Tensor block_table, Tensor(a!) free_pages, "
+      "Tensor free_state, Tensor(b!) free_state_out, Tensor(c!) seqlens_out, int page_size) -> ()");
+  m.def(
+      "paged_append_rope(Tensor q, Tensor? k, Tensor? v, Tensor(a!)? k_pages, Tensor(b!)? v_pages, "
+      "Tensor positions, Tensor? slot_map, Tensor cos, Tensor sin, float? eps=None, float scale=1.2, "
+      "bool rotate_k=True, bool round_each=True) -> Tensor");
+  m.def(
+      "paged_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cache_seqlens, "
+      "Tensor cu_new, int window=-1, float? softmax_scale=None, int max_new=0) -> Tensor");
   m.def("add_rms_norm(Tensor x, Tensor? delta, Tensor(a!)? x_out, Tensor(b!) h_out, float? eps=None) -> ()");
 }
 
@@ -416,4 +675,8 @@ TORCH_LIBRARY_IMPL(mcb200, CUDA, m) {
   m.impl("kv_advance", &kv_advance);
   m.impl("linear", &linear);
   m.impl("add_rms_norm", &add_rms_norm);
+  m.impl("page_plan", &page_plan);
+  m.impl("page_release", &page_release);
+  m.impl("paged_append_rope", &paged_append_rope);
+  m.impl("paged_attn", &paged_attn);
 }

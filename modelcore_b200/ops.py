@@ -8,6 +8,7 @@ CPU path: non-CUDA or non-bf16 tensors raise.
 """
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -666,6 +667,83 @@ def gated_silu(gate, up, out=None):
     args.rows, args.H = rows, H
     check(_native.load().mcb_gated_silu(ctypes.byref(args), _stream(gate)))
     return out
+
+
+class PagePlan(NamedTuple):
+    """One step of a packed batch over a paged cache (page_plan)."""
+    cu_new: torch.Tensor      # (R + 1,) int32: request r's new tokens are [cu_new[r], cu_new[r + 1])
+    positions: torch.Tensor   # (num_tokens,) int32, -1 for padding
+    slot_map: torch.Tensor    # (num_tokens,) int64: page * page_size + offset, -1 for none
+    free_state: torch.Tensor  # (2,) int64: the queue's head and tail after the step
+
+
+def _paged():
+    """The paged operators, torch.ops.mcb200 (C++ over the same C ABI: a call costs a third of a
+    ctypes one on the host, which a decode step of small launches feels)."""
+    from . import torch_ops  # noqa: F401  (registers them; raises without the built library)
+    return torch.ops.mcb200
+
+
+def page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state, *, page_size, num_tokens,
+              free_state_out=None):
+    """One step's bookkeeping of a paged cache on the GPU, from the requests' lengths: request r
+    holds cache_seqlens[r] positions and takes new_lens[r] new tokens ((R,) int32, any of them 0).
+
+    Writes into block_table (R, max_pages) int32 the pages each request starts to use, taken in
+    request order from the queue free_pages (n_pages,) int32, whose entries between the counters
+    free_state = (head, tail) int64 are free (counter x at x % n_pages).  Returns a PagePlan; its
+    positions and slot_map have num_tokens entries, those past the sum of new_lens padding (-1).
+    cache_seqlens and free_state are not moved -- free_state_out (a new tensor, or the one given,
+    which may be free_state) holds the counters after the step -- so the same inputs plan the
+    same step.  page_size: a power of two, 16 to 1024.
+
+    Device errors (ops.device_error): 5 when the queue runs out (missing pages and their slots
+    are -1), 1 when a request outgrows its table row, 7 when new_lens exceed num_tokens."""
+    if free_state_out is None:
+        free_state_out = torch.empty_like(free_state)
+    cu, pos, slots = _paged().page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state,
+                                        free_state_out, page_size, num_tokens)
+    return PagePlan(cu, pos, slots, free_state_out)
+
+
+def page_release(done, cache_seqlens, block_table, free_pages, free_state, *, page_size,
+                 free_state_out=None, seqlens_out=None):
+    """Returns the pages of the requests with done[r] != 0 ((R,) int32) to the queue's tail, in
+    request order (free_pages is written in place).  Returns (free_state, seqlens) after it: new
+    tensors, or free_state_out / seqlens_out, which may be the inputs.  The table keeps its stale
+    entries: a length of 0 makes them unreachable."""
+    if free_state_out is None:
+        free_state_out = torch.empty_like(free_state)
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens)
+    _paged().page_release(done, cache_seqlens, block_table, free_pages, free_state, free_state_out,
+                          seqlens_out, page_size)
+    return free_state_out, seqlens_out
+
+
+def paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin, *, eps=None, scale=1.2,
+                      rotate_k=True, round_each=True):
+    """kv_append_rope for packed tokens and a paged cache: rope at positions (N,) int32, rms_norm and
+    scale of q (N, Hq, D) and k (N, Hkv, D), k and v written to slot_map (N,) int64 of k_pages /
+    v_pages (n_pages, Hkv, page_size, D); bf16, D 64 or 128, any token and head strides in multiples
+    of 8 elements.  k = v = k_pages = v_pages = slot_map = None: a layer that reads another layer's
+    pages.  Padding (position -1) gives a zero q, slot -1 writes nothing.  round_each: every step
+    rounded to bf16, the bits of kv_append_rope (a paged cache then holds what KVCache holds);
+    False keeps fp32 and rounds once.  Returns the processed q."""
+    return _paged().paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin, eps, scale,
+                                      rotate_k, round_each)
+
+
+def paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, *, window=-1, softmax_scale=None,
+               max_new=0):
+    """Attention of packed new tokens q (N, Hq, D) over a paged cache whose pages already hold their
+    keys and values: request r's tokens [cu_new[r], cu_new[r + 1]) sit at positions cache_seqlens[r]
+    on and see every earlier position and their own, within `window` back (< 0: all).  Chunks of
+    prompts and single-token steps mix freely.  max_new: the largest number of new tokens of a
+    request when the caller knows it (0: unknown; a decode step with 1 needs one launch less).
+    Returns (N, Hq, D) bf16, zeros past cu_new[R]."""
+    return _paged().paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new,
+                               -1 if window is None else window, softmax_scale, max_new)
 
 
 def device_error(device=None):

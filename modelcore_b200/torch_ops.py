@@ -25,6 +25,15 @@ functions, so that torch.compile can trace through them:
         into out (and h_out)
     torch.ops.mcb200.add_rms_norm(x, delta, x_out, h_out, eps=None)
         the residual add and the next RMSNorm (ops.add_rms_norm), into x_out and h_out
+    torch.ops.mcb200.page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state,
+                               free_state_out, page_size, num_tokens) -> cu_new, positions, slot_map
+    torch.ops.mcb200.page_release(done, cache_seqlens, block_table, free_pages, free_state,
+                                  free_state_out, seqlens_out, page_size)
+    torch.ops.mcb200.paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin,
+                                       eps=None, scale=1.2, rotate_k=True, round_each=True) -> q'
+    torch.ops.mcb200.paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, window=-1,
+                                softmax_scale=None, max_new=0) -> y
+        the paged cache (modelcore_b200.ops documents each)
 
 bf16 slots only (the fp8 cache format is reached through modelcore_b200.ops).  The results are
 those of the ctypes entry points bit for bit: one library does the work.  Without the built
@@ -38,7 +47,7 @@ from . import _native
 from .build import TORCH_OPS_PATH
 
 OPS = ("kv_append_rope", "kv_broadcast", "decode_attn", "append_attn", "kv_advance", "linear",
-       "add_rms_norm")
+       "add_rms_norm", "page_plan", "page_release", "paged_append_rope", "paged_attn")
 
 
 def _register_fakes():
@@ -48,9 +57,15 @@ def _register_fakes():
     def nothing(*args, **kwargs):
         return None
 
+    def plan(cache_seqlens, new_lens, block_table, free_pages, free_state, free_state_out, page_size,
+             num_tokens):
+        ints = [cache_seqlens.new_empty(n) for n in (cache_seqlens.shape[0] + 1, num_tokens)]
+        return (*ints, cache_seqlens.new_empty(num_tokens, dtype=torch.int64))
+
     for name, fn in (("kv_append_rope", like_q), ("decode_attn", like_q), ("append_attn", like_q),
                      ("kv_broadcast", nothing), ("kv_advance", nothing), ("linear", nothing),
-                     ("add_rms_norm", nothing)):
+                     ("add_rms_norm", nothing), ("page_plan", plan), ("page_release", nothing),
+                     ("paged_append_rope", like_q), ("paged_attn", like_q)):
         torch.library.register_fake(f"mcb200::{name}")(fn)
 
 
