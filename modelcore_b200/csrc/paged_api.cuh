@@ -231,9 +231,90 @@ int check_paged_attn(const mcb_paged_attn_args* a, const char* who) {
   if (rc != MCB_OK) return rc;
   if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3e38f)
     return fail(MCB_ERR_INVALID_ARG, "%s: softmax_scale %g must be positive and finite", who, a->softmax_scale);
-  if (static_cast<long long>(a->n_pages) * a->Hkv > INT32_MAX)
+  if ((a->n_pages + 1ll) * a->Hkv > INT32_MAX)
     return fail(MCB_ERR_UNSUPPORTED, "%s: n_pages %d * Hkv %d above 2^31 - 1", who, a->n_pages, a->Hkv);
   return MCB_OK;
+}
+
+// The pages as a 4-D map {64 columns, position, D / 64 panels, page * Hkv + head}: a box of `box`
+// positions of one head's page is one contiguous block, landing as D / 64 swizzled panels.
+int encode_page_map(CUtensorMap* map, const void* base, const mcb_paged_attn_args* a, int box, int panels) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(MCB_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t D = static_cast<cuuint64_t>(a->D), page = static_cast<cuuint64_t>(a->page_size);
+  cuuint64_t dims[4] = {64, page, D / 64, static_cast<cuuint64_t>(a->n_pages) * static_cast<cuuint64_t>(a->Hkv)};
+  cuuint64_t strides[3] = {D * 2, 128, page * D * 2};
+  cuuint32_t boxes[4] = {64u, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(panels), 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MCB_ERR_CUDA, "cuTensorMapEncodeTiled(pages) failed (CUresult %d)", (int)r);
+  return MCB_OK;
+}
+
+template <int D, int NQT>
+struct PagedDecodeVariant {
+  // 128-KB and 48-KB rings: one CTA an SM at head size 128, three (two with 16 query rows) at 64
+  static constexpr int STAGES = D == 64 ? 3 : 4;
+  using Cfg = mcb::PagedDecodeConfig<D, NQT, STAGES>;
+  static constexpr auto kernel = mcb::paged_decode_kernel<D, NQT, STAGES>;
+
+  // CTAs resident on the device (the shared-memory limit raised once); one an SM without a device.
+  static int grid() {
+    static std::atomic<uint64_t> done{0};
+    static std::mutex mu;
+    static int cache[64] = {0};
+    const int per_sm = per_device(cache, mu, [] {
+      int n = 0;
+      if (ensure_smem(kernel, Cfg::SMEM_BYTES, done) != cudaSuccess ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, mcb::kPdThreads, Cfg::SMEM_BYTES) != cudaSuccess)
+        cudaGetLastError();
+      return n;
+    });
+    return device_sm_count() * std::max(per_sm, 1);
+  }
+
+  static int launch(const mcb_paged_attn_args* a, const mcb::PagedAttnParams& p, cudaStream_t st) {
+    CUtensorMap km, vm;
+    const int box = std::min(a->page_size, mcb::kPdTile);
+    int rc = encode_page_map(&km, a->k_pages, a, box, D / 64);
+    if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, D / 64);
+    if (rc != MCB_OK) return rc;
+    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid())), dim3(mcb::kPdThreads),
+                               static_cast<size_t>(Cfg::SMEM_BYTES), st, km, vm, p);
+    g_launches++;
+    note_attn_kernel("paged_decode_kernel", D, NQT, STAGES, false);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "paged_decode launch");
+    return MCB_OK;
+  }
+};
+
+// How a call runs, from its shapes alone.
+struct PagedAttnPlan {
+  int nqt;            // decode kernel: 8 nqt query rows a unit
+  int grid;           // its CTAs
+  size_t part_o, part_lse, ws_bytes, counters;
+};
+
+template <typename F>
+auto with_decode_variant(int D, int nqt, F f) {
+  if (D == 64) return nqt == 1 ? f(PagedDecodeVariant<64, 1>{}) : f(PagedDecodeVariant<64, 2>{});
+  return nqt == 1 ? f(PagedDecodeVariant<128, 1>{}) : f(PagedDecodeVariant<128, 2>{});
+}
+
+PagedAttnPlan plan_paged_attn(const mcb_paged_attn_args* a) {
+  PagedAttnPlan pl = {};
+  const long long G = a->Hq / a->Hkv;
+  pl.nqt = a->max_new > 0 && a->max_new * G <= 8 ? 1 : 2;
+  pl.grid = with_decode_variant(a->D, pl.nqt, [](auto v) { return decltype(v)::grid(); });
+  const size_t rows = static_cast<size_t>(pl.grid) * 2 * 8 * pl.nqt;
+  pl.part_o = round256(rows * a->D * 4);
+  pl.part_lse = round256(rows * 4);
+  pl.ws_bytes = pl.part_o + pl.part_lse;
+  pl.counters = static_cast<size_t>(pl.grid);
+  return pl;
 }
 
 int paged_attn(const mcb_paged_attn_args* a, void* stream) {
@@ -248,17 +329,24 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
     return fail(MCB_ERR_INVALID_ARG, "%s: negative q stride or table_stride below max_pages", who);
   if (!rows16(a->q, a->q_stride) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
     return fail(MCB_ERR_ALIGNMENT, "%s: q rows, out and pages must start on 16-byte boundaries", who);
+  const PagedAttnPlan pl = plan_paged_attn(a);
+  if (a->workspace == nullptr || a->workspace_bytes < pl.ws_bytes || !aligned(a->workspace, 256))
+    return fail(MCB_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, got %zu", who, pl.ws_bytes,
+                a->workspace_bytes);
+  if (a->counters == nullptr || a->counter_count < pl.counters)
+    return fail(MCB_ERR_WORKSPACE, "%s: %zu counters are needed, got %zu", who, pl.counters, a->counter_count);
   mcb::PagedAttnParams p = {};
   p.q = static_cast<const uint16_t*>(a->q);
   p.qs[0] = a->q_stride[0];
   p.qs[1] = a->q_stride[1];
-  p.k_pages = static_cast<const uint16_t*>(a->k_pages);
-  p.v_pages = static_cast<const uint16_t*>(a->v_pages);
   p.block_table = a->block_table;
   p.table_stride = a->table_stride;
   p.seqlens = a->cache_seqlens;
   p.cu_new = a->cu_new;
   p.out = static_cast<uint16_t*>(a->out);
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
+  p.counters = a->counters;
   p.R = a->R;
   p.N = a->N;
   p.Hq = a->Hq;
@@ -269,15 +357,11 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
   p.page_shift = page_shift_of(a->page_size);
   p.window = a->window;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  const long long warps = static_cast<long long>(a->N) * a->Hq;
-  const dim3 grid(static_cast<unsigned>((warps + 3) / 4)), block(128);
+  p.few_rows = 8 * pl.nqt;
+  p.all = 1;
+  p.fill = 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = a->D == 64 ? launch_pdl(mcb::paged_attn_plain_kernel<64>, grid, block, 0, st, p)
-                             : launch_pdl(mcb::paged_attn_plain_kernel<128>, grid, block, 0, st, p);
-  g_launches++;
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "paged_attn launch");
-  return MCB_OK;
+  return with_decode_variant(a->D, pl.nqt, [&](auto v) { return decltype(v)::launch(a, p, st); });
 }
 
 }  // namespace
@@ -294,12 +378,22 @@ int mcb_paged_append_rope(const mcb_paged_append_args* a, void* stream) {
   return guarded("mcb_paged_append_rope", [&] { return paged_append(a, stream); });
 }
 size_t mcb_paged_attn_workspace_size(const mcb_paged_attn_args* a) {
-  (void)a;
-  return 0;
+  size_t n = 0;
+  guarded("mcb_paged_attn_workspace_size", [&] {
+    const int rc = check_paged_attn(a, "mcb_paged_attn_workspace_size");
+    if (rc == MCB_OK) n = plan_paged_attn(a).ws_bytes;
+    return rc;
+  });
+  return n;
 }
 size_t mcb_paged_attn_counter_count(const mcb_paged_attn_args* a) {
-  (void)a;
-  return 0;
+  size_t n = 0;
+  guarded("mcb_paged_attn_counter_count", [&] {
+    const int rc = check_paged_attn(a, "mcb_paged_attn_counter_count");
+    if (rc == MCB_OK) n = plan_paged_attn(a).counters;
+    return rc;
+  });
+  return n;
 }
 int mcb_paged_attn(const mcb_paged_attn_args* a, void* stream) {
   return guarded("mcb_paged_attn", [&] { return paged_attn(a, stream); });

@@ -87,6 +87,11 @@ def test_attention_rejects_bad_arguments():
         (dict(q_stride=(-256, 64)), INVALID, "negative"), (dict(q_stride=(256, 60)), ALIGNMENT, "16-byte"),
         (dict(v_pages=P + 8), ALIGNMENT, "16-byte"), (dict(n_pages=1 << 30, Hkv=4), UNSUPPORTED, "2^31")])
     assert _call("mcb_paged_attn", PagedAttnArgs, good, N=0)[0] == 0
+    WORKSPACE, ws = _native.MCB_ERR_WORKSPACE, dict(workspace=P, workspace_bytes=1 << 30)
+    _rejects("mcb_paged_attn", PagedAttnArgs, good, [
+        ({}, WORKSPACE, "workspace"), (dict(workspace=P, workspace_bytes=16), WORKSPACE, "workspace"),
+        (dict(ws, workspace=P + 16), WORKSPACE, "256-byte"), (dict(ws, counters=None), WORKSPACE, "counters"),
+        (dict(ws, counters=P, counter_count=3), WORKSPACE, "counters")])
 
 
 def test_shape_functions_on_meta_tensors():
