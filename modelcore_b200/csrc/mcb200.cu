@@ -21,7 +21,7 @@
 #include "kv_append.cuh"
 #include "kv_copy.cuh"
 #include "paged_append.cuh"
-#include "paged_decode.cuh"
+#include "paged_chunk.cuh"
 #include "paged_plan.cuh"
 #include "prefill_attn.cuh"
 #include "decode_proj.cuh"

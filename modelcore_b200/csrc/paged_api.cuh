@@ -133,7 +133,7 @@ int page_release(const mcb_page_release_args* a, void* stream) {
   return MCB_OK;
 }
 
-bool rows16(const void* p, const int64_t* strides) {
+bool rows16(const void* p, const int64_t (&strides)[2]) {
   return aligned(p, 16) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
 }
 
@@ -291,11 +291,54 @@ struct PagedDecodeVariant {
   }
 };
 
-// How a call runs, from its shapes alone.
+// Packed queries as a 3-D map {D, Hq, N}; a box is 64 columns x the G heads of a kv head x the tokens
+// of a query tile, rows in (token, head) order.
+int encode_packed_q_map(CUtensorMap* map, const mcb_paged_attn_args* a, const int64_t (&stride)[2], int tpb) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(MCB_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(a->D), static_cast<cuuint64_t>(a->Hq), static_cast<cuuint64_t>(a->N)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2};
+  cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(a->Hq / a->Hkv), static_cast<cuuint32_t>(tpb)};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a->q), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MCB_ERR_CUDA, "cuTensorMapEncodeTiled(packed q) failed (CUresult %d)", (int)r);
+  return MCB_OK;
+}
+
+template <int D>
+int launch_paged_chunk(const mcb_paged_attn_args* a, const mcb::PagedChunkParams& p, const int64_t (&q_stride)[2],
+                       int grid, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int smem = mcb::PagedChunkConfig<D>::kSmem;
+  CUtensorMap qm, km, vm;
+  const int box = std::min(a->page_size, mcb::kPcTile);
+  int rc = encode_packed_q_map(&qm, a, q_stride, p.tpb);
+  if (rc == MCB_OK) rc = encode_page_map(&km, a->k_pages, a, box, 1);
+  if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, 1);
+  if (rc != MCB_OK) return rc;
+  cudaError_t e = ensure_smem(mcb::paged_chunk_kernel<D>, smem, done);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_chunk)");
+  e = launch_pdl(mcb::paged_chunk_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(mcb::kPcThreads),
+                 static_cast<size_t>(smem), st, qm, km, vm, p);
+  g_launches++;
+  note_attn_kernel("paged_chunk_kernel", D, 0, 0, false);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_chunk launch");
+  e = launch_pdl(mcb::paged_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 4), dim3(256), 0, st, p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_combine launch");
+  return MCB_OK;
+}
+
+// How a call runs, from its shapes alone: which kernels, their grids, and the workspace's parts
+// (the decode kernel's partials, then the chunk kernel's partials and its cut units).
 struct PagedAttnPlan {
-  int nqt;            // decode kernel: 8 nqt query rows a unit
-  int grid;           // its CTAs
-  size_t part_o, part_lse, ws_bytes, counters;
+  bool decode, chunk;
+  int nqt, decode_grid, chunk_grid;
+  size_t d_o, d_lse, c_o, c_lse, c_cuts, ws_bytes, counters;
 };
 
 template <typename F>
@@ -307,13 +350,25 @@ auto with_decode_variant(int D, int nqt, F f) {
 PagedAttnPlan plan_paged_attn(const mcb_paged_attn_args* a) {
   PagedAttnPlan pl = {};
   const long long G = a->Hq / a->Hkv;
-  pl.nqt = a->max_new > 0 && a->max_new * G <= 8 ? 1 : 2;
-  pl.grid = with_decode_variant(a->D, pl.nqt, [](auto v) { return decltype(v)::grid(); });
-  const size_t rows = static_cast<size_t>(pl.grid) * 2 * 8 * pl.nqt;
-  pl.part_o = round256(rows * a->D * 4);
-  pl.part_lse = round256(rows * 4);
-  pl.ws_bytes = pl.part_o + pl.part_lse;
-  pl.counters = static_cast<size_t>(pl.grid);
+  const long long most = a->max_new > 0 ? a->max_new * G : 1ll << 40;  // query rows a kv head of a request
+  pl.nqt = most <= 8 ? 1 : 2;
+  pl.decode = G <= 16;
+  pl.chunk = most > 16;  // (always when G > 16)
+  if (pl.decode) {
+    pl.decode_grid = with_decode_variant(a->D, pl.nqt, [](auto v) { return decltype(v)::grid(); });
+    const size_t rows = static_cast<size_t>(pl.decode_grid) * 2 * 8 * pl.nqt;
+    pl.d_o = round256(rows * a->D * 4);
+    pl.d_lse = round256(rows * 4);
+    pl.counters = static_cast<size_t>(pl.decode_grid);
+  }
+  if (pl.chunk) {
+    pl.chunk_grid = device_sm_count();
+    const size_t rows = static_cast<size_t>(pl.chunk_grid) * 2 * 256;
+    pl.c_o = round256(rows * a->D * 4);
+    pl.c_lse = round256(rows * 4);
+    pl.c_cuts = round256(pl.chunk_grid * sizeof(mcb::PagedCut));
+  }
+  pl.ws_bytes = pl.d_o + pl.d_lse + pl.c_o + pl.c_lse + pl.c_cuts;
   return pl;
 }
 
@@ -327,25 +382,26 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
     return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
   if (a->q_stride[0] < 0 || a->q_stride[1] < 0 || a->table_stride < a->max_pages)
     return fail(MCB_ERR_INVALID_ARG, "%s: negative q stride or table_stride below max_pages", who);
-  if (!rows16(a->q, a->q_stride) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
+  // the stride of a dimension of one is arbitrary (and not used)
+  const int64_t q_stride[2] = {a->N > 1 ? a->q_stride[0] : static_cast<int64_t>(a->Hq) * a->D,
+                               a->Hq > 1 ? a->q_stride[1] : a->D};
+  if (!rows16(a->q, q_stride) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
     return fail(MCB_ERR_ALIGNMENT, "%s: q rows, out and pages must start on 16-byte boundaries", who);
   const PagedAttnPlan pl = plan_paged_attn(a);
   if (a->workspace == nullptr || a->workspace_bytes < pl.ws_bytes || !aligned(a->workspace, 256))
     return fail(MCB_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, got %zu", who, pl.ws_bytes,
                 a->workspace_bytes);
-  if (a->counters == nullptr || a->counter_count < pl.counters)
+  if (pl.counters > 0 && (a->counters == nullptr || a->counter_count < pl.counters))
     return fail(MCB_ERR_WORKSPACE, "%s: %zu counters are needed, got %zu", who, pl.counters, a->counter_count);
   mcb::PagedAttnParams p = {};
   p.q = static_cast<const uint16_t*>(a->q);
-  p.qs[0] = a->q_stride[0];
-  p.qs[1] = a->q_stride[1];
+  p.qs[0] = q_stride[0];
+  p.qs[1] = q_stride[1];
   p.block_table = a->block_table;
   p.table_stride = a->table_stride;
   p.seqlens = a->cache_seqlens;
   p.cu_new = a->cu_new;
   p.out = static_cast<uint16_t*>(a->out);
-  p.part_o = static_cast<float*>(a->workspace);
-  p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
   p.counters = a->counters;
   p.R = a->R;
   p.N = a->N;
@@ -357,11 +413,29 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
   p.page_shift = page_shift_of(a->page_size);
   p.window = a->window;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  p.few_rows = 8 * pl.nqt;
-  p.all = 1;
-  p.fill = 1;
+  p.few_rows = pl.decode ? 8 * pl.nqt : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return with_decode_variant(a->D, pl.nqt, [&](auto v) { return decltype(v)::launch(a, p, st); });
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  if (pl.decode) {
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_lse = reinterpret_cast<float*>(ws + pl.d_o);
+    p.all = !pl.chunk;
+    p.fill = !pl.chunk;
+    rc = with_decode_variant(a->D, pl.nqt, [&](auto v) { return decltype(v)::launch(a, p, st); });
+    if (rc != MCB_OK || !pl.chunk) return rc;
+  }
+  ws += pl.d_o + pl.d_lse;
+  mcb::PagedChunkParams c = {};
+  c.a = p;
+  c.a.part_o = reinterpret_cast<float*>(ws);
+  c.a.part_lse = reinterpret_cast<float*>(ws + pl.c_o);
+  c.a.all = 0;
+  c.a.fill = 1;
+  c.cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.c_o + pl.c_lse);
+  c.tpb = mcb::kPcTile / p.G;
+  c.wait_last = pl.decode;
+  return a->D == 64 ? launch_paged_chunk<64>(a, c, q_stride, pl.chunk_grid, st)
+                    : launch_paged_chunk<128>(a, c, q_stride, pl.chunk_grid, st);
 }
 
 }  // namespace

@@ -60,14 +60,16 @@ __device__ __forceinline__ PagedRow paged_row(const PagedAttnParams& p, int r) {
   PagedRow x;
   x.tok0 = min(max(p.cu_new[r], 0), p.N);
   x.T = min(max(p.cu_new[r + 1], x.tok0), p.N) - x.tok0;
-  x.L = max(p.seqlens[r], 0);
+  // a request that does not fit its table (reported by paged_row_fits) stays inside it
+  const long long cap = static_cast<long long>(p.max_pages) << p.page_shift;
+  x.L = static_cast<int>(min(static_cast<long long>(max(p.seqlens[r], 0)), max(cap - x.T, 0ll)));
   return x;
 }
 
 // Whether a request's lengths fit the table (the caller reports once).
 __device__ __forceinline__ bool paged_row_fits(const PagedAttnParams& p, int r, const PagedRow& x) {
   return p.seqlens[r] >= 0 &&
-         static_cast<long long>(x.L) + x.T <= (static_cast<long long>(p.max_pages) << p.page_shift);
+         static_cast<long long>(p.seqlens[r]) + x.T <= (static_cast<long long>(p.max_pages) << p.page_shift);
 }
 
 constexpr int kPdTile = 64;  // keys a tile
@@ -211,7 +213,7 @@ __device__ __forceinline__ void paged_merge(const float* part_o, const float* pa
       }
     }
   }
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   uint16_t* dst = row_out(n) + lane * PER_LANE;
   if constexpr (PER_LANE == 4)
     *reinterpret_cast<uint2*>(dst) =
@@ -545,13 +547,13 @@ __global__ void __launch_bounds__(kPdThreads)
         ltot = fmaf(st_l[ww * ROWS + n], f, ltot);
         o = fmaf(mbuf[(ww * ROWS + n) * C::OPITCH + d], f, o);
       }
-      o = ltot > 0.f ? o / ltot : 0.f;
+      o = ltot == 0.f ? 0.f : o / ltot;  // (a NaN stays one)
       if (complete) {
         row_out(n)[d] = float_to_bf16_bits(o);
       } else {
         const long long prow = (static_cast<long long>(blockIdx.x) * 2 + slot) * ROWS + n;
         p.part_o[prow * D + d] = o;
-        if (d == 0) p.part_lse[prow] = ltot > 0.f ? mmax * p.scale_log2 + __log2f(ltot) : -CUDART_INF_F;
+        if (d == 0) p.part_lse[prow] = ltot == 0.f ? -CUDART_INF_F : mmax * p.scale_log2 + __log2f(ltot);
       }
     }
     if (!complete) {
