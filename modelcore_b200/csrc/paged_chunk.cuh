@@ -12,25 +12,26 @@
 // after, merges them (spread over the GPU: one CTA merging a unit cut eighteen ways would take
 // longer than its share of the products).
 //
-// Roles of a CTA's ten warps:
-//   warp 0      TMA producer: Q0, Q1 per unit; K_j, V_j into a two-stage ring that runs on across
-//               units, one box a (page chunk, 64-column panel); lanes hold the next page numbers
-//   warp 1      allocates TMEM; lane 0 issues the products
+// Roles of a CTA's warps:
+//   warp 0      TMA producer and walker: describes each unit (or the part of one in this CTA's share)
+//               in shared memory for the other roles, loads Q0, Q1, then K_j and V_j into rings of
+//               two that run on across units, one box a (page chunk, 64-column panel)
+//   warp 1      allocates TMEM; one elected lane issues the products
 //                 S_t = Q_t K_j^T   M=128 N=128 K=D  (both operands from shared memory)
 //                 O_t += P_t V_j    M=128 N=D K=128  (P from TMEM)
-//   warps 2-5   softmax of Q0, warps 6-9 of Q1: one thread a query row
+//   warps 4-7   softmax of Q0, warps 8-11 of Q1: one thread a query row
+// Warps 2, 3 only complete a warpgroup: warps 0-3 give registers back (setmaxnreg) and the softmax
+// warps take them, a score row being 128 registers.
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each).  D = 128 fills the 512 columns, so P (bf16)
 // is written over S and the issue order is PV0_j S0_j+1 PV1_j S1_j+1: one tile's products run
 // during the other's softmax.  With D = 64 P has columns of its own, and S_j+1 is computed as soon
 // as S_j has been read.
 //
-// Softmax without a maximum on the critical path: the exponent's reference m is a maximum the row
-// has really had (its first tile's), moved only when it must be.  A tile in which every row has an m
-// and nothing is masked is exponentiated at once; P and l may then exceed 1 -- fp32 and bf16 reach
-// 2^127 -- and only when a row's sum over the tile leaves 2^100 is the tile redone with a new m (S is
-// still in TMEM) and O and l rescaled.  Other tiles (masked edges, a row's first keys) take the
-// maximum first and move m when it grew by 2^8.  Rounding: P to bf16 for the product; l sums the
-// unrounded values.
+// Softmax without a maximum on the critical path: the exponent's reference m is the maximum of the
+// first 64 keys a row saw, and stays.  P and l may then exceed 1 -- fp32 and bf16 reach 2^127 -- and
+// only when a row's sum over 64 keys leaves 2^100 is m moved to their maximum, those 64 redone (S is
+// still in TMEM) and O, l and the tile's other half of P rescaled.  Rounding: P to bf16 for the
+// product; l sums the unrounded values.
 // Some of the exponentials run as a polynomial on the FMA pipe (exp2_poly_pair): the 16 a clock
 // an SM of the special function unit would otherwise take as long as the products.
 //
@@ -47,7 +48,10 @@
 namespace mcb {
 
 constexpr int kPcTile = 128;      // query rows a tile, keys a key tile
-constexpr int kPcThreads = 320;   // producer, issuer, 2 x 4 softmax warps
+constexpr int kPcThreads = 384;   // producer, issuer, two idle, 2 x 4 softmax warps
+constexpr int kPcWarps = kPcThreads / 32;
+// registers a thread after the split: 128 (88 + 2 x 208) of the launch's 384 x 168
+constexpr int kPcFewRegs = 120, kPcManyRegs = 192;
 
 // What paged_combine_kernel needs of the unit that starts in a CTA's share and ends after it.
 struct PagedCut {
@@ -75,7 +79,8 @@ struct PagedChunkConfig {
   static constexpr int kVOff = kKOff + 2 * kTileBytes;
   static constexpr int kBarOff = kVOff + 2 * kTileBytes;
   static constexpr int kScanOff = kBarOff + 256;
-  static constexpr int kBytes = kScanOff + 256 + 1024;
+  static constexpr int kSegOff = kScanOff + 128;
+  static constexpr int kBytes = kSegOff + 4 * 64 + 1024;
   // above half of an SM's shared memory: two CTAs never meet on one SM, whose TMEM each needs whole
   static constexpr int kSmem = kBytes > 118784 ? kBytes : 118784;
 };
@@ -87,6 +92,30 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
       : "memory");
+}
+
+// mbar_wait_or_abort in few instructions: it is inlined at some twenty places of one kernel, whose
+// roles run side by side and share the instruction cache.
+__device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      record_error(kErrWaitTimeout);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -165,6 +194,21 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
   return u;
 }
 
+// The part of a unit in one CTA's share, as the producer describes it to the other roles.
+struct ChunkSeg {
+  int seg;             // key tiles (0: no more parts)
+  int kt0;             // the first one's first key
+  int lo, hi;          // the unit's visible keys
+  int b0, e0, b1, e1;  // the tiles [b, e) of each query tile, counted from the first here
+  int pos0;            // position of the unit's first token
+  int c0, c1;          // tokens in Q0, Q1
+  int tok;             // the unit's first token in the packed batch
+  int h;               // kv head
+  int part;            // -1: the whole unit; else the slot of the partial result
+  int pad[2];
+};
+static_assert(sizeof(ChunkSeg) == 64, "four descriptions of 64 bytes");
+
 struct ChunkWalk {
   ChunkUnit u;
   int h, local;
@@ -220,6 +264,94 @@ __device__ __forceinline__ void chunk_rows(const PagedChunkParams& p, int row_a,
   }
 }
 
+// 64 TMEM columns of this warp's lanes, not waited for; tmem_ld_wait64 orders every use after it.
+__device__ __forceinline__ void tmem_ld64_nowait(uint32_t taddr, uint32_t (&r)[64]) {
+#pragma unroll
+  for (int i = 0; i < 64; i += 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[i + 0]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]),
+          "=r"(r[i + 6]), "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]),
+          "=r"(r[i + 12]), "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15]), "=r"(r[i + 16]), "=r"(r[i + 17]),
+          "=r"(r[i + 18]), "=r"(r[i + 19]), "=r"(r[i + 20]), "=r"(r[i + 21]), "=r"(r[i + 22]), "=r"(r[i + 23]),
+          "=r"(r[i + 24]), "=r"(r[i + 25]), "=r"(r[i + 26]), "=r"(r[i + 27]), "=r"(r[i + 28]), "=r"(r[i + 29]),
+          "=r"(r[i + 30]), "=r"(r[i + 31])
+        : "r"(taddr + i)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait64(uint32_t (&r)[64]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; i += 16)  // (empty: the values are not usable before this point)
+    asm volatile(""
+                 : "+r"(r[i + 0]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                   "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
+                   "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
+}
+
+// Columns of the half row outside [lo, hi) to -inf: one unsigned compare a column.
+__device__ __forceinline__ void mask64(uint32_t (&s)[64], int lo, int hi) {
+  const uint32_t width = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+#pragma unroll
+  for (int c = 0; c < 64; ++c)
+    if (static_cast<uint32_t>(c - lo) >= width) s[c] = __float_as_uint(-INFINITY);
+}
+
+__device__ __forceinline__ float max64(const uint32_t (&s)[64]) {
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      m4[u] = fmax3(m4[u], __uint_as_float(s[8 * c + 2 * u]), __uint_as_float(s[8 * c + 2 * u + 1]));
+  return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+}
+
+// Half a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; three
+// pairs of eight by the polynomial, whose inputs' maximum goes to pmax.  A masked score (-inf) gives
+// 0 or, in the polynomial's columns, 2^-125: nothing beside a row's sum, which is about 1 or more.
+__device__ __forceinline__ void exp64(const uint32_t (&s)[64], uint64_t sc2, uint64_t nm2, uint32_t (&w)[32],
+                                      uint64_t& acc0, uint64_t& acc1, float& pmax) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const uint64_t x = fma2(static_cast<uint64_t>(s[2 * c]) | static_cast<uint64_t>(s[2 * c + 1]) << 32, sc2, nm2);
+    const int u = c & 7;
+    uint64_t e;
+    if (u == 2 || u == 5 || u == 7) {
+      pmax = fmax3(pmax, lo_f(x), hi_f(x));
+      e = exp2_poly_pair(x);
+    } else {
+      e = pair_f32(fast_exp2(lo_f(x)), fast_exp2(hi_f(x)));
+    }
+    if (u & 1) acc1 = add2(acc1, e);
+    else acc0 = add2(acc0, e);
+    w[c] = pack_bf16x2_rn(lo_f(e), hi_f(e));
+  }
+}
+
+// This warp's rows of O (D columns) times alpha; its packed first half of P (32 columns) times alpha.
+template <int D>
+__device__ __noinline__ void tmem_scale(uint32_t addr, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(addr + c * 32, o);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+    tmem_st32(addr + c * 32, o);
+  }
+}
+__device__ __noinline__ void tmem_scale_bf16(uint32_t addr, float alpha) {
+  tmem_st_wait();
+  uint32_t o[32];
+  tmem_ld32(addr, o);
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    o[e] = pack_bf16x2_rn(__uint_as_float(o[e] << 16) * alpha, __uint_as_float(o[e] & 0xffff0000u) * alpha);
+  tmem_st32(addr, o);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -232,25 +364,31 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
   uint64_t* q_full = bars + 0;
   uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;    // [2]
-  uint64_t* v_full = bars + 4;    // [2]
-  uint64_t* kv_empty = bars + 6;  // [2]
-  uint64_t* s_full = bars + 8;    // [2] per query tile
-  uint64_t* p_full = bars + 10;   // [2] 128 arrivals
-  uint64_t* s_free = bars + 12;   // [2] 128 arrivals (SEP): S has been read
-  uint64_t* pv_done = bars + 14;  // [2] (SEP): a P V product has completed
-  uint64_t* o_done = bars + 16;
-  uint64_t* epi_done = bars + 17; // 256 arrivals, once a unit
-  uint64_t* drained = bars + 18;
-  constexpr int kNumBars = 19;
+  uint64_t* k_full = bars + 2;     // [2]
+  uint64_t* v_full = bars + 4;     // [2]
+  uint64_t* k_empty = bars + 6;    // [2]
+  uint64_t* v_empty = bars + 8;    // [2]
+  uint64_t* s_full = bars + 10;    // [2] per query tile
+  uint64_t* p_full = bars + 12;    // [2] 128 arrivals
+  uint64_t* s_free = bars + 14;    // [2] 128 arrivals (SEP): S has been read
+  uint64_t* pv_done = bars + 16;   // [2] (SEP): a P V product has completed
+  uint64_t* o_done = bars + 18;
+  uint64_t* epi_done = bars + 19;  // 256 arrivals, once a unit
+  uint64_t* drained = bars + 20;
+  // [4] a description is there.  The producer writes description x after q_empty(x - 1), so after
+  // epi_done(x - 3): every softmax thread is past x - 3, and the four in the ring are never behind
+  uint64_t* seg_full = bars + 21;
+  constexpr int kNumBars = 25;
+  static_assert((kNumBars + 4) * 8 <= 256, "barriers, TMEM slot, abort flag and start in 256 bytes");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars + 1);
   int* ctl = reinterpret_cast<int*>(bars + kNumBars + 2);  // start: r, qb, h, local
-  long long* warp_tot = reinterpret_cast<long long*>(smem + Cfg::kScanOff);  // [10]
+  long long* warp_tot = reinterpret_cast<long long*>(smem + Cfg::kScanOff);  // [12]
+  ChunkSeg* segs = reinterpret_cast<ChunkSeg*>(smem + Cfg::kSegOff);         // [4]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBars; ++i) mbar_init(bars + i, i >= 10 && i < 14 ? 128 : i == 17 ? 256 : 1);
+    for (int i = 0; i < kNumBars; ++i) mbar_init(bars + i, i >= 12 && i < 16 ? 128 : i == 19 ? 256 : 1);
     *abort_flag = 0;
     fence_mbarrier_init();
     prefetch_tensormap(&qmap);
@@ -267,7 +405,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   }
 
   // ---- the sequence's length and this CTA's first tile ----
-  const int per = (p.a.R + 9) / 10;
+  const int per = (p.a.R + kPcWarps - 1) / kPcWarps;
   const int row_a = min(warp * per, p.a.R), row_b = min(row_a + per, p.a.R);
   long long mine = 0;
   chunk_rows(p, row_a, row_b, [&](int, int, int n) {
@@ -283,7 +421,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   tc_fence_after();
   long long total = 0, before = 0;
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
+  for (int i = 0; i < kPcWarps; ++i) {
     if (i < warp) before += warp_tot[i];
     total += warp_tot[i];
   }
@@ -320,214 +458,263 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const uint32_t base = smem_u32(smem);
-  ChunkWalk w;
-  w.t = t_begin;
-  if (active) {
-    const PagedRow x = paged_row(p.a, ctl[0]);
-    w.u = chunk_unit(p, x, ctl[0], ctl[1], chunk_blocks(p, x));
-    w.h = ctl[2];
-    w.local = ctl[3];
-  }
-
-  if (warp == 0) {
-    // ---------------- producer warp ----------------
-    const uint64_t pol = l2_policy_evict_first();
-    const int box_shift = min(p.a.page_shift, 7);  // positions a box: min(page, 128)
-    const int box = 1 << box_shift, nch = kPcTile >> box_shift;
-    const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
-    const uint32_t q_bytes = static_cast<uint32_t>(p.tpb * p.a.G) * 128u;
-    int g = 0, k = 0;
-    bool ok = true;
-    while (ok && w.t < t_end) {
-      const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
-      if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait_or_abort(q_empty, (k - 1) & 1, abort_flag));
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (w.u.c1 > 0 ? 2 : 1) * Cfg::kPanels * q_bytes);
-        for (int t = 0; t < (w.u.c1 > 0 ? 2 : 1); ++t)
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
+    return __all_sync(0xffffffffu, mbar_wait_small(bar, parity, abort_flag)) != 0;
+  };
+  // the x-th description, once it is there; false on a timeout
+  auto next_seg = [&](int x, ChunkSeg& d) {
+    if (!wait(&seg_full[x & 3], (x >> 2) & 1)) return false;
+    const int4* src = reinterpret_cast<const int4*>(&segs[x & 3]);
+    int4* dst = reinterpret_cast<int4*>(&d);
 #pragma unroll
-          for (int pn = 0; pn < Cfg::kPanels; ++pn)
-            tma_load_3d(smem + t * Cfg::kTileBytes + pn * kPcTile * 128, &qmap, q_full, pn * 64, w.h * p.a.G,
-                        w.u.row.tok0 + (w.u.qb * 2 + t) * p.tpb, pol);
+    for (int i = 0; i < 4; ++i) dst[i] = src[i];
+    return true;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcFewRegs));
+    if (warp == 0) {
+      // ---------------- producer and walker ----------------
+      const uint64_t pol = l2_policy_evict_first();
+      const int box_shift = min(p.a.page_shift, 7);  // positions a box: min(page, 128)
+      const int box = 1 << box_shift, nch = kPcTile >> box_shift;
+      const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+      const uint32_t q_bytes = static_cast<uint32_t>(p.tpb * p.a.G) * 128u;
+      ChunkWalk w;
+      w.t = t_begin;
+      if (active) {
+        const PagedRow x = paged_row(p.a, ctl[0]);
+        w.u = chunk_unit(p, x, ctl[0], ctl[1], chunk_blocks(p, x));
+        w.h = ctl[2];
+        w.local = ctl[3];
       }
-      ++k;
-      const int32_t* table = p.a.block_table + w.u.r * p.a.table_stride;
-      int pbase = -1, pg = 0;  // lane l holds the page of chunk pbase + l
-      for (int i = 0; i < seg; ++i, ++g) {
-        const int st = g & 1;
-        const int c0 = (w.u.kb + (w.local + i) * kPcTile) >> box_shift;
-        if (pbase < 0 || c0 + nch > pbase + 32) {
-          pbase = c0;
-          const long long key = static_cast<long long>(c0 + lane) << box_shift;
-          pg = p.a.n_pages;  // outside the pool: a box there reads zeros
-          if (key <= w.u.hi && key + box > w.u.lo) {
-            pg = table[key >> p.a.page_shift];
-            if (pg < 0 || pg >= p.a.n_pages) {
-              record_error(kErrPageOutOfRange);
-              pg = p.a.n_pages;
+      int g = 0, k = 0;
+      bool ok = true;
+      while (ok && w.t < t_end) {
+        const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
+        if (k > 0 && !(ok = wait(q_empty, (k - 1) & 1))) break;
+        if (lane == 0) {
+          const bool whole = w.local == 0 && seg == w.u.n;
+          ChunkSeg d;
+          d.seg = seg;
+          d.kt0 = w.u.kb + w.local * kPcTile;
+          d.lo = w.u.lo;
+          d.hi = w.u.hi;
+          d.b0 = max(w.u.b0 - w.local, 0);
+          d.e0 = min(w.u.e0 - w.local, seg);
+          d.b1 = max(w.u.b1 - w.local, 0);
+          d.e1 = min(w.u.e1 - w.local, seg);
+          d.pos0 = w.u.row.L + w.u.qb * 2 * p.tpb;
+          d.c0 = w.u.c0;
+          d.c1 = w.u.c1;
+          d.tok = w.u.row.tok0 + w.u.qb * 2 * p.tpb;
+          d.h = w.h;
+          d.part = whole ? -1 : k > 0 ? 1 : 0;
+          d.pad[0] = d.pad[1] = 0;
+          segs[k & 3] = d;
+          mbar_arrive(&seg_full[k & 3]);
+          const long long start = w.t - w.local;
+          if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
+            PagedCut c;
+            c.tok0 = d.tok;
+            c.tok1 = d.tok + d.c0 + d.c1;
+            c.h = w.h;
+            c.g_last = share_owner(start + w.u.n - 1, total, ng);
+            c.slot1 = d.part;
+            c.pad[0] = c.pad[1] = c.pad[2] = 0;
+            p.cuts[blockIdx.x] = c;
+          }
+          mbar_arrive_expect_tx(q_full, (w.u.c1 > 0 ? 2 : 1) * Cfg::kPanels * q_bytes);
+          for (int t = 0; t < (w.u.c1 > 0 ? 2 : 1); ++t)
+#pragma unroll
+            for (int pn = 0; pn < Cfg::kPanels; ++pn)
+              tma_load_3d(smem + t * Cfg::kTileBytes + pn * kPcTile * 128, &qmap, q_full, pn * 64, w.h * p.a.G,
+                          d.tok + t * p.tpb, pol);
+        }
+        __syncwarp();
+        ++k;
+        const int32_t* table = p.a.block_table + w.u.r * p.a.table_stride;
+        int pbase = -1, pg = 0;  // lane l holds the page of chunk pbase + l
+        for (int i = 0; ok && i < seg; ++i, ++g) {
+          const int st = __shfl_sync(0xffffffffu, g & 1, 0);
+          const int c0 = (w.u.kb + (w.local + i) * kPcTile) >> box_shift;
+          if (pbase < 0 || c0 + nch > pbase + 32) {
+            pbase = c0;
+            const long long key = static_cast<long long>(c0 + lane) << box_shift;
+            pg = p.a.n_pages;  // outside the pool: a box there reads zeros
+            if (key <= w.u.hi && key + box > w.u.lo) {
+              pg = table[key >> p.a.page_shift];
+              if (pg < 0 || pg >= p.a.n_pages) {
+                record_error(kErrPageOutOfRange);
+                pg = p.a.n_pages;
+              }
+            }
+          }
+          // the tile's chunks with visible keys: [ch0, ch1)
+          const int ch0 = max((w.u.lo >> box_shift) - c0, 0), ch1 = min((w.u.hi >> box_shift) - c0 + 1, nch);
+          const uint32_t bytes = static_cast<uint32_t>(max(ch1 - ch0, 0)) * Cfg::kPanels * box_bytes;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* full = kv ? &v_full[st] : &k_full[st];
+            if (g >= 2 && !(ok = wait(kv ? &v_empty[st] : &k_empty[st], ((g >> 1) - 1) & 1))) break;
+            if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+            __syncwarp();
+            uint8_t* dst = smem + (kv ? Cfg::kVOff : Cfg::kKOff) + st * Cfg::kTileBytes;
+            for (int ch = ch0; ch < ch1; ++ch) {
+              const int row = __shfl_sync(0xffffffffu, pg, (c0 - pbase + ch) & 31) * p.a.Hkv + w.h;
+              const int pos = ((c0 + ch) << box_shift) & ((1 << p.a.page_shift) - 1);
+              if (elect_one()) {
+#pragma unroll
+                for (int pn = 0; pn < Cfg::kPanels; ++pn)
+                  tma_load_4d(dst + pn * kPcTile * 128 + ch * box_bytes, kv ? &vmap : &kmap, full, 0, pos, pn, row, pol);
+              }
+              __syncwarp();
             }
           }
         }
-        // lane l: chunk l / panels, panel l % panels
-        const int ch = lane / Cfg::kPanels, pn = lane % Cfg::kPanels;
-        const int page = __shfl_sync(0xffffffffu, pg, (c0 - pbase + ch) & 31);
-        const int key0 = (c0 + ch) << box_shift;
-        const bool load = ch < nch && key0 <= w.u.hi && key0 + box > w.u.lo;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box_bytes;
-        if (g >= 2) {
-          ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&kv_empty[st], ((g >> 1) - 1) & 1, abort_flag));
-          if (!ok) break;
+        if (!ok) break;
+        w.t += seg;
+        w.local += seg;
+        if (w.local == w.u.n && w.t < t_end) chunk_next(p, w);
+      }
+      if (ok && lane == 0) {
+        segs[k & 3].seg = 0;
+        mbar_arrive(&seg_full[k & 3]);
+      }
+      if (*abort_flag && lane == 0) {  // the copies in flight land before the CTA can exit
+        for (int f = max(0, g - 2); f <= g; ++f) {
+          if (f < g) mbar_wait(&k_full[f & 1], (f >> 1) & 1);
+          if (f < g) mbar_wait(&v_full[f & 1], (f >> 1) & 1);
         }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&k_full[st], bytes);
-          mbar_arrive_expect_tx(&v_full[st], bytes);
+        if (k > 0) mbar_wait(q_full, (k - 1) & 1);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // ---------------- product issuer ----------------
+      // The whole warp waits, converged, and one elected lane issues: the descriptors are then
+      // warp-uniform (a base and constants) and an MMA costs the warp an instruction or two.  Issued
+      // from a lane-0 branch each took a dozen, and with two busy softmax warps on the same scheduler
+      // the tensor cores starved: 2,400 FLOP a clock an SM against 8,000 in this form (both products
+      // back to back beside fp32 work; 8,192 at most).  Everything else a product needs is waited
+      // for before its P, and a tile's P V and next S go in one block: nothing but the two products
+      // lies between a P and the next S.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPcTile, 0);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = smem_desc_sw128(base, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(base + Cfg::kKOff, 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(base + Cfg::kVOff, kPcTile * 128, 1024);
+      int g = 0;
+      uint32_t pv_par = 0, s_par = 0, s_any = 0;  // bit t: parity of tile t's products so far (and any S)
+      bool ok = true;
+      ChunkSeg d;
+      for (int k = 0; ok; ++k) {
+        if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+        ok = wait(q_full, k & 1);
+        // Step j: for each tile P V of key tile j and S of j + 1 (j = -1: the first S); K is free after
+        // its last S, V after its last P V, Q after the unit's last S
+#pragma unroll 1
+        for (int j = -1; ok && j < d.seg; ++j) {
+          const bool pv1 = j >= d.b1 && j < d.e1, s1 = j + 1 >= d.b1 && j + 1 < d.e1;
+          const bool pv0 = j >= d.b0 && j < d.e0, s0 = j + 1 >= d.b0 && j + 1 < d.e0;
+          const int gj = g + j, st = __shfl_sync(0xffffffffu, gj & 1, 0), st1 = st ^ 1;
+          if (pv0 || pv1) ok = wait(&v_full[st], (gj >> 1) & 1);
+          if (ok && (s0 || s1)) ok = wait(&k_full[st1], ((gj + 1) >> 1) & 1);
+#pragma unroll 1
+          for (int t = 0; ok && t < 2; ++t) {
+            const bool pv = t ? pv1 : pv0, sn = t ? s1 : s0;
+            const uint32_t bit = 1u << t;
+            const int flags = __shfl_sync(0xffffffffu,
+                                          (j > (t ? d.b1 : d.b0) ? 1 : 0) | (t || !pv1 ? 2 : 0) | (t || !s1 ? 4 : 0) |
+                                              ((t || !s1) && j + 1 == d.seg - 1 ? 8 : 0),
+                                          0);
+            if (SEP && sn && (s_any & bit) && !(ok = wait(&s_free[t], ((s_par >> t) & 1) ^ 1))) break;
+            if (!SEP && pv && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (half == (SEP ? 0 : 1)) {
+                if (sn) {
+                  const uint64_t qa = q_desc + t * (Cfg::kTileBytes >> 4), ka = k_desc + st1 * (Cfg::kTileBytes >> 4);
+                  if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                      const int off = (kk >> 2) * ((kPcTile * 128) >> 4) + (kk & 3) * (32 >> 4);
+                      umma_ss(tm + t * kPcTile, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[t]);
+                    if (flags & 4) umma_commit(&k_empty[st1]);
+                    if (flags & 8) umma_commit(q_empty);
+                  }
+                  __syncwarp();
+                  s_par ^= bit;
+                  s_any |= bit;
+                }
+              } else if (pv) {
+                if (SEP && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
+                if (SEP) tc_fence_after();
+                const uint32_t pa = tm + (SEP ? Cfg::kPCol + t * (kPcTile / 2) : t * kPcTile);
+                const uint64_t va = v_desc + st * (Cfg::kTileBytes >> 4);
+                if (elect_one()) {
+#pragma unroll
+                  for (int kk = 0; kk < kPcTile / 16; ++kk)
+                    umma_ts(tm + Cfg::kOCol + t * D, pa + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o,
+                            kk > 0 ? 1u : flags & 1u);
+                  if (SEP) umma_commit(&pv_done[t]);
+                  if (flags & 2) umma_commit(&v_empty[st]);
+                }
+                __syncwarp();
+                pv_par ^= bit;
+              }
+            }
+          }
         }
+        if (ok && k > 0) ok = wait(epi_done, (k - 1) & 1);
+        if (ok && elect_one()) umma_commit(o_done);
         __syncwarp();
-        if (load) {
-          const int pos = key0 & ((1 << p.a.page_shift) - 1);
-          uint8_t* dst = smem + st * Cfg::kTileBytes + pn * kPcTile * 128 + ch * box_bytes;
-          tma_load_4d(dst + Cfg::kKOff, &kmap, &k_full[st], 0, pos, pn, page * p.a.Hkv + w.h, pol);
-          tma_load_4d(dst + Cfg::kVOff, &vmap, &v_full[st], 0, pos, pn, page * p.a.Hkv + w.h, pol);
-        }
+        g += d.seg;
       }
-      if (!ok) break;
-      w.t += seg;
-      w.local += seg;
-      if (w.local == w.u.n && w.t < t_end) chunk_next(p, w);
+      if (elect_one()) umma_commit(drained);  // every product has completed before TMEM is freed
+      __syncwarp();
+      mbar_wait(drained, 0);
+      __syncwarp();
     }
-    if (*abort_flag && lane == 0) {  // the copies in flight land before the CTA can exit
-      for (int f = max(0, g - 2); f < g; ++f) {
-        mbar_wait(&k_full[f & 1], (f >> 1) & 1);
-        mbar_wait(&v_full[f & 1], (f >> 1) & 1);
-      }
-      if (k > 0) mbar_wait(q_full, (k - 1) & 1);
-    }
-    __syncwarp();
-  } else if (warp == 1 && lane == 0) {
-    // ---------------- product issuer ----------------
-    constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPcTile, 0);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
-    int g = 0, k = 0;
-    int pv_total[2] = {0, 0}, s_total[2] = {0, 0};
-    bool ok = true;
-    while (ok && w.t < t_end) {
-      const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
-      // this segment's key tiles [b, e) of each query tile, from w.local
-      const int b0 = max(w.u.b0 - w.local, 0), e0 = min(w.u.e0 - w.local, seg);
-      const int b1 = max(w.u.b1 - w.local, 0), e1 = min(w.u.e1 - w.local, seg);
-      const int s_here = max(e0 - b0, 0) + max(e1 - b1, 0);
-      ok = mbar_wait_or_abort(q_full, k & 1, abort_flag);
-      int k_waited = -1, v_waited = -1, s_issued = 0;
-      int pv_unit[2] = {0, 0};
-      auto on = [&](int t, int j) { return t == 0 ? j >= b0 && j < e0 : j >= b1 && j < e1; };
-      auto issue_s = [&](int t, int j) -> bool {
-        const int gj = g + j;
-        if (SEP && s_total[t] > 0 && !mbar_wait_or_abort(&s_free[t], (s_total[t] - 1) & 1, abort_flag)) return false;
-        ++s_total[t];
-        if (k_waited < j) {
-          if (!mbar_wait_or_abort(&k_full[gj & 1], (gj >> 1) & 1, abort_flag)) return false;
-          k_waited = j;
-        }
-        tc_fence_after();
-        const uint32_t qa = base + t * Cfg::kTileBytes, ka = base + Cfg::kKOff + (gj & 1) * Cfg::kTileBytes;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kPcTile * 128) + (kk & 3) * 32;
-          umma_ss(tmem + t * kPcTile, smem_desc_sw128(qa + off, 16, 1024), smem_desc_sw128(ka + off, 16, 1024),
-                  idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
-        if (++s_issued == s_here) umma_commit(q_empty);
-        return true;
-      };
-      auto issue_pv = [&](int t, int j) -> bool {
-        const int gj = g + j;
-        if (!mbar_wait_or_abort(&p_full[t], pv_total[t] & 1, abort_flag)) return false;
-        if (v_waited < j) {
-          if (!mbar_wait_or_abort(&v_full[gj & 1], (gj >> 1) & 1, abort_flag)) return false;
-          v_waited = j;
-        }
-        tc_fence_after();
-        const uint32_t va = base + Cfg::kVOff + (gj & 1) * Cfg::kTileBytes;
-        const uint32_t pa = tmem + (SEP ? Cfg::kPCol + t * (kPcTile / 2) : t * kPcTile);
-#pragma unroll
-        for (int kk = 0; kk < kPcTile / 16; ++kk)
-          umma_ts(tmem + Cfg::kOCol + t * D, pa + kk * 8, smem_desc_sw128(va + kk * 16 * 128, kPcTile * 128, 1024),
-                  idesc_o, (pv_unit[t] > 0 || kk > 0) ? 1u : 0u);
-        if (SEP) umma_commit(&pv_done[t]);
-        ++pv_unit[t];
-        ++pv_total[t];
-        return true;
-      };
-      if (ok && on(0, 0)) ok = issue_s(0, 0);
-      if (ok && on(1, 0)) ok = issue_s(1, 0);
-      for (int j = 0; ok && j < seg; ++j) {
-        if constexpr (SEP) {
-          if (ok && on(0, j + 1)) ok = issue_s(0, j + 1);
-          if (ok && on(0, j)) ok = issue_pv(0, j);
-          if (ok && on(1, j + 1)) ok = issue_s(1, j + 1);
-          if (ok && on(1, j)) ok = issue_pv(1, j);
-          if (ok) umma_commit(&kv_empty[(g + j) & 1]);
-        } else {
-          if (ok && on(0, j)) ok = issue_pv(0, j);
-          if (ok && on(0, j + 1)) ok = issue_s(0, j + 1);
-          if (ok && on(1, j)) ok = issue_pv(1, j);
-          if (ok) umma_commit(&kv_empty[(g + j) & 1]);
-          if (ok && on(1, j + 1)) ok = issue_s(1, j + 1);
-        }
-      }
-      if (ok && k > 0) ok = mbar_wait_or_abort(epi_done, (k - 1) & 1, abort_flag);
-      if (ok) umma_commit(o_done);
-      g += seg;
-      ++k;
-      w.t += seg;
-      w.local += seg;
-      if (w.local == w.u.n && w.t < t_end) chunk_next(p, w);
-    }
-    umma_commit(drained);  // every product has completed before TMEM is freed
-    mbar_wait(drained, 0);
-  } else if (warp >= 2) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPcManyRegs));
     // ---------------- softmax: four warps a query tile, one thread a row ----------------
-    const int t = (warp - 2) >> 2;
+    const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;         // TMEM lanes 32 * quarter .. +31
     const int row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + t * kPcTile;
     const uint32_t o_addr = tmem + lane_off + Cfg::kOCol + t * D;
     const uint32_t p_addr = SEP ? tmem + lane_off + Cfg::kPCol + t * (kPcTile / 2) : s_addr;
-    const int rt = row / p.a.G, rh = row - rt * p.a.G;  // the row's token in the tile, head in the group
+    const int rt = row / p.a.G;           // the row's token in the tile
     const float sc = p.a.scale_log2;
-    int g = 0, k = 0, s_cnt = 0;
-    int seg_index = 0;
+    const uint64_t sc2 = pair_f32(sc, sc);
+    int g = 0, s_cnt = 0;
     bool ok = true;
-    while (ok && w.t < t_end) {
-      const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
-      const int cnt_tok = t ? w.u.c1 : w.u.c0;
-      const int jb = max((t ? w.u.b1 : w.u.b0) - w.local, 0), je = min((t ? w.u.e1 : w.u.e0) - w.local, seg);
-      const int first = (w.u.qb * 2 + t) * p.tpb;  // the tile's first token of the request
+    for (int k = 0; ok; ++k) {
+      ChunkSeg d;
+      if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+      const int cnt_tok = t ? d.c1 : d.c0;
+      const int jb = t ? d.b1 : d.b0, je = t ? d.e1 : d.e0;
       const bool valid = rt < cnt_tok;             // (rows past tpb * G have rt >= tpb)
-      const int pos = w.u.row.L + first + rt;
-      const int pos0 = w.u.row.L + first, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
-      const int see_hi = min(pos, w.u.hi), see_lo = p.a.window >= 0 ? pos - p.a.window : 0;
+      const int pos0 = d.pos0 + t * p.tpb, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
+      const int see_hi = min(pos0 + rt, d.hi), see_lo = p.a.window >= 0 ? pos0 + rt - p.a.window : 0;
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
       int cnt = 0;
       for (int j = jb; j < je; ++j, ++cnt, ++s_cnt) {
-        if (!__all_sync(0xffffffffu, mbar_wait_or_abort(&s_full[t], s_cnt & 1, abort_flag))) {
-          ok = false;
-          break;
-        }
+        if (!(ok = wait(&s_full[t], s_cnt & 1))) break;
         tc_fence_after();
-        const int kt = w.u.kb + (w.local + j) * kPcTile;  // the tile's first key
-        if (kt < w.u.lo || kt + kPcTile - 1 > w.u.hi) {
+        const int kt = d.kt0 + j * kPcTile;  // the tile's first key
+        if (kt < d.lo || kt + kPcTile - 1 > d.hi) {
           // rows of V outside [lo, hi] to zero, a thread a row
-          const int gj = g + j;
-          if (!__all_sync(0xffffffffu, mbar_wait_or_abort(&v_full[gj & 1], (gj >> 1) & 1, abort_flag))) {
-            ok = false;
-            break;
-          }
-          if (kt + row < w.u.lo || kt + row > w.u.hi) {
-            const uint32_t at = base + Cfg::kVOff + (gj & 1) * Cfg::kTileBytes + row * 128;
+          const int st = (g + j) & 1;
+          if (!(ok = wait(&v_full[st], ((g + j) >> 1) & 1))) break;
+          if (kt + row < d.lo || kt + row > d.hi) {
+            const uint32_t at = base + Cfg::kVOff + st * Cfg::kTileBytes + row * 128;
 #pragma unroll
             for (int c = 0; c < 8 * Cfg::kPanels; ++c)
               sts128(at + (c >> 3) * (kPcTile * 128) + (c & 7) * 16, make_uint4(0, 0, 0, 0));
@@ -535,126 +722,78 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           fence_proxy_async_shared();
         }
         if (!warp_rows) {  // no query row in this warp's quarter: P may be anything
-          if (SEP) mbar_arrive(&s_free[t]);
-          if (SEP && cnt > 0 &&
-              !__all_sync(0xffffffffu, mbar_wait_or_abort(&pv_done[t], (s_cnt - 1) & 1, abort_flag))) {
-            ok = false;
-            break;
+          if (SEP) {
+            mbar_arrive(&s_free[t]);
+            if (cnt > 0 && !(ok = wait(&pv_done[t], (s_cnt - 1) & 1))) break;
           }
           tc_fence_before();
           mbar_arrive(&p_full[t]);
           continue;
         }
-        const bool full = kt + kPcTile - 1 <= min(pos0, w.u.hi) && (p.a.window < 0 || pos1 - kt <= p.a.window);
-        uint32_t sr[128];
-        tmem_ld128(s_addr, sr);
-        float alpha = 1.f, sum;
-        bool redo = !full || __any_sync(0xffffffffu, valid && m_used == -INFINITY);
-        if (!redo) {
-          const uint64_t sc2 = pair_f32(sc, sc), nm2 = pair_f32(-m_used, -m_used);
-          uint64_t acc0 = 0, acc1 = 0;
-          float pmax = -INFINITY;  // of the polynomial's inputs
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {  // 16 keys -> 8 words of P
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              const uint64_t x = fma2(static_cast<uint64_t>(sr[16 * c + 2 * u]) |
-                                          static_cast<uint64_t>(sr[16 * c + 2 * u + 1]) << 32,
-                                      sc2, nm2);
-              uint64_t e;
-              if (u == 2 || u == 5 || u == 7) {  // three pairs of eight
-                pmax = fmax3(pmax, lo_f(x), hi_f(x));
-                e = exp2_poly_pair(x);
-              } else {
-                e = pair_f32(fast_exp2(lo_f(x)), fast_exp2(hi_f(x)));
+        const bool full = kt + kPcTile - 1 <= min(pos0, d.hi) && (p.a.window < 0 || pos1 - kt <= p.a.window);
+        const int c_lo = max(0, see_lo - kt), c_hi = valid ? min(kPcTile, see_hi - kt + 1) : 0;
+        // SEP: P's columns and O are free once the last P V has completed (else S's completion says so)
+        auto pv_settled = [&] {
+          if (!SEP || cnt == 0) return;
+          if (!wait(&pv_done[t], (s_cnt - 1) & 1)) ok = false;
+          tc_fence_after();
+        };
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+          float sum;
+          bool redo = false;
+          while (true) {
+            uint32_t a[64];
+            tmem_ld64_nowait(s_addr + 64 * h, a);
+            tmem_ld_wait64(a);
+            if (!full) mask64(a, c_lo - 64 * h, c_hi - 64 * h);
+            if (redo || __any_sync(0xffffffffu, valid && m_used == -INFINITY)) {
+              const float mx = max64(a) * sc;
+              if (m_used == -INFINITY) {  // the first keys this row sees
+                m_used = mx;
+                l = 0.f;
+              } else if (redo) {
+                const float m_new = redo && valid && mx > m_used + 8.f ? mx : m_used;
+                const float alpha = fast_exp2(m_used - m_new);
+                m_used = m_new;
+                l *= alpha;
+                pv_settled();
+                if (cnt > 0) tmem_scale<D>(o_addr, alpha);
+                if (h) tmem_scale_bf16(p_addr, alpha);
               }
-              if (u & 1) acc1 = add2(acc1, e);
-              else acc0 = add2(acc0, e);
-              sr[8 * c + u] = pack_bf16x2_rn(lo_f(e), hi_f(e));  // registers of scores already consumed
             }
+            const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+            uint64_t acc0 = 0, acc1 = 0;
+            float pmax = -INFINITY;
+            exp64(a, sc2, pair_f32(neg_m, neg_m), w, acc0, acc1, pmax);
+            acc0 = add2(acc0, acc1);
+            sum = lo_f(acc0) + hi_f(acc0);
+            if (redo || !__any_sync(0xffffffffu, valid && !(sum < 1.2676506e30f && pmax < 100.f))) break;  // 2^100
+            redo = true;
           }
-          acc0 = add2(acc0, acc1);
-          sum = lo_f(acc0) + hi_f(acc0);
-          redo = __any_sync(0xffffffffu, valid && !(sum < 1.2676506e30f && pmax < 100.f));  // 2^100
-          if (redo) tmem_ld128(s_addr, sr);
-        }
-        if (redo) {
-          if (!full) {
-            // this row sees the columns [c_lo, c_hi): one unsigned compare a column
-            const int c_hi = valid ? min(kPcTile, see_hi - kt + 1) : 0;
-            const int c_lo = max(0, see_lo - kt);
-            const uint32_t width = c_hi > c_lo ? static_cast<uint32_t>(c_hi - c_lo) : 0u;
-#pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (static_cast<uint32_t>(c - c_lo) >= width) sr[c] = __float_as_uint(-INFINITY);
-          }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 16; ++c)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              m4[u] = fmax3(m4[u], __uint_as_float(sr[8 * c + 2 * u]), __uint_as_float(sr[8 * c + 2 * u + 1]));
-          const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
-          if (mx > m_used + 8.f) {
-            alpha = fast_exp2(m_used - mx);  // 0 when m_used is -inf
-            m_used = mx;
-            l *= alpha;
-          }
-          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-          float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            const float e0 = fast_exp2(fmaf(__uint_as_float(sr[2 * c]), sc, neg_m));
-            const float e1 = fast_exp2(fmaf(__uint_as_float(sr[2 * c + 1]), sc, neg_m));
-            s0 += e0;
-            s1 += e1;
-            sr[c] = pack_bf16x2_rn(e0, e1);
-          }
-          sum = s0 + s1;
-        }
-        if constexpr (SEP) {
-          // S is read; P's columns and O are free once the last product has completed
-          tc_fence_before();
-          mbar_arrive(&s_free[t]);
-          if (cnt > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait_or_abort(&pv_done[t], (s_cnt - 1) & 1, abort_flag))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_st16_nowait(p_addr + 16 * c, *reinterpret_cast<const uint32_t(*)[16]>(&sr[16 * c]));
-        l += sum;
-        if (cnt > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c * 32, o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(o_addr + c * 32, o);
-          }
+          l += sum;
+          if (h == 0) pv_settled();
+          tmem_st16_nowait(p_addr + 32 * h, *reinterpret_cast<const uint32_t(*)[16]>(&w[0]));
+          tmem_st16_nowait(p_addr + 32 * h + 16, *reinterpret_cast<const uint32_t(*)[16]>(&w[16]));
         }
         tmem_st_wait();
+        if (!ok) break;
         tc_fence_before();
+        if (SEP) mbar_arrive(&s_free[t]);
         mbar_arrive(&p_full[t]);
       }
       if constexpr (SEP) {
-        if (ok && cnt > 0 && !__all_sync(0xffffffffu, mbar_wait_or_abort(&pv_done[t], (s_cnt - 1) & 1, abort_flag)))
-          ok = false;
+        if (ok && cnt > 0) ok = wait(&pv_done[t], (s_cnt - 1) & 1);
       }
-      if (ok && !__all_sync(0xffffffffu, mbar_wait_or_abort(o_done, k & 1, abort_flag))) ok = false;
+      if (ok) ok = wait(o_done, k & 1);
       if (ok) {
         tc_fence_after();
-        const bool complete = w.local == 0 && seg == w.u.n;
         const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
-        const int tok = w.u.row.tok0 + first + rt;
-        if (complete) {
+        if (d.part < 0) {
           if (warp_rows) {
-            uint16_t* dst = p.a.out + (static_cast<long long>(tok) * p.a.Hq + w.h * p.a.G + rh) * D;
+            const int tok = d.tok + t * p.tpb + rt;
+            uint16_t* dst = p.a.out + (static_cast<long long>(tok) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G)) * D;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
@@ -672,7 +811,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             }
           }
         } else {
-          const long long prow = (static_cast<long long>(blockIdx.x) * 2 + (seg_index ? 1 : 0)) * 256 + t * 128 + row;
+          const long long prow = (static_cast<long long>(blockIdx.x) * 2 + d.part) * 256 + t * 128 + row;
           if (valid) p.a.part_lse[prow] = l == 0.f ? -INFINITY : m_used + __log2f(l);
           if (warp_rows && cnt > 0) {
             float* dst = p.a.part_o + prow * D;
@@ -688,29 +827,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                                   __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
             }
           }
-          if (threadIdx.x == 64) {
-            const long long start = w.t - w.local;
-            if (share_owner(start, total, ng) == static_cast<int>(blockIdx.x)) {
-              PagedCut c;
-              c.tok0 = w.u.row.tok0 + w.u.qb * 2 * p.tpb;
-              c.tok1 = c.tok0 + w.u.c0 + w.u.c1;
-              c.h = w.h;
-              c.g_last = share_owner(start + w.u.n - 1, total, ng);
-              c.slot1 = seg_index ? 1 : 0;
-              c.pad[0] = c.pad[1] = c.pad[2] = 0;
-              p.cuts[blockIdx.x] = c;
-            }
-          }
         }
       }
       tc_fence_before();
       mbar_arrive(epi_done);  // O is read: the issuer may let the next unit's o_done complete
-      g += seg;
-      ++k;
-      ++seg_index;
-      w.t += seg;
-      w.local += seg;
-      if (w.local == w.u.n && w.t < t_end) chunk_next(p, w);
+      g += d.seg;
     }
   }
   tc_fence_before();
