@@ -19,19 +19,19 @@
 //   warp 1      allocates TMEM; one elected lane issues the products
 //                 S_t = Q_t K_j^T   M=128 N=128 K=D  (both operands from shared memory)
 //                 O_t += P_t V_j    M=128 N=D K=128  (P from TMEM)
-//   warps 4-7   softmax of Q0, warps 8-11 of Q1: one thread a query row
-// Warps 2, 3 only complete a warpgroup: warps 0-3 give registers back (setmaxnreg) and the softmax
-// warps take them, a score row being 128 registers.
+//   warps 4-11  softmax of Q0, warps 12-19 of Q1: two threads a query row, 64 key columns each
+// Two threads a row because a thread's instructions are in order: one warp a scheduler works at
+// two to three cycles an instruction, and a tile's softmax is what the next product waits for.
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each).  D = 128 fills the 512 columns, so P (bf16)
 // is written over S and the issue order is PV0_j S0_j+1 PV1_j S1_j+1: one tile's products run
 // during the other's softmax.  With D = 64 P has columns of its own, and S_j+1 is computed as soon
 // as S_j has been read.
 //
-// Softmax without a maximum on the critical path: the exponent's reference m is the maximum of the
-// first 64 keys a row saw, and stays.  P and l may then exceed 1 -- fp32 and bf16 reach 2^127 -- and
-// only when a row's sum over 64 keys leaves 2^100 is m moved to their maximum, those 64 redone (S is
-// still in TMEM) and O, l and the tile's other half of P rescaled.  Rounding: P to bf16 for the
-// product; l sums the unrounded values.
+// Softmax without a maximum on the critical path: the exponent's reference m is the row's maximum over
+// the first tile in which it sees a key, and stays.  P and l may then exceed 1 -- fp32 and bf16
+// reach 2^127 -- and only when a row's sum over its 64 columns of a tile leaves 2^100 is m moved
+// (see overflow()).  The two threads of a row thus need not meet in a tile.  Rounding: P to bf16 for
+// the product; l sums the unrounded values.
 // Some of the exponentials run as a polynomial on the FMA pipe (exp2_poly_pair): the 16 a clock
 // an SM of the special function unit would otherwise take as long as the products.
 //
@@ -48,10 +48,8 @@
 namespace mcb {
 
 constexpr int kPcTile = 128;      // query rows a tile, keys a key tile
-constexpr int kPcThreads = 384;   // producer, issuer, two idle, 2 x 4 softmax warps
+constexpr int kPcThreads = 640;   // producer, issuer, two idle warps, 2 x 8 softmax warps
 constexpr int kPcWarps = kPcThreads / 32;
-// registers a thread after the split: 128 (88 + 2 x 208) of the launch's 384 x 168
-constexpr int kPcFewRegs = 120, kPcManyRegs = 192;
 
 // What paged_combine_kernel needs of the unit that starts in a CTA's share and ends after it.
 struct PagedCut {
@@ -78,9 +76,11 @@ struct PagedChunkConfig {
   static constexpr int kKOff = 2 * kTileBytes;           // Q0, Q1, then K and V, two stages each
   static constexpr int kVOff = kKOff + 2 * kTileBytes;
   static constexpr int kBarOff = kVOff + 2 * kTileBytes;
-  static constexpr int kScanOff = kBarOff + 256;
-  static constexpr int kSegOff = kScanOff + 128;
-  static constexpr int kBytes = kSegOff + 4 * 64 + 1024;
+  static constexpr int kScanOff = kBarOff + 320;
+  static constexpr int kSegOff = kScanOff + 256;
+  // per query tile and row quarter: what the two warps exchange (PagedPair)
+  static constexpr int kPairOff = kSegOff + 4 * 64;
+  static constexpr int kBytes = kPairOff + 2 * 4 * 1024 + 1024;
   // above half of an SM's shared memory: two CTAs never meet on one SM, whose TMEM each needs whole
   static constexpr int kSmem = kBytes > 118784 ? kBytes : 118784;
 };
@@ -94,14 +94,25 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
-// mbar_wait_or_abort in few instructions: it is inlined at some twenty places of one kernel, whose
-// roles run side by side and share the instruction cache.
+// A bounded wait that polls rarely: try_wait suspends the warp for up to 20 us at a time (a plain one
+// returns after a fraction of that, and the polls of sixteen waiting warps took a third of the
+// schedulers' issue slots from the warps at work).
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_try_wait_long(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
+  while (!mbar_try_wait_long(bar, parity)) {
     if (*abort) return false;
     if (global_timer_ns() - t0 > kWaitLimitNs) {
       record_error(kErrWaitTimeout);
@@ -109,6 +120,7 @@ __device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, 
       return false;
     }
   }
+  return true;
 }
 
 // True in one lane of a converged warp.
@@ -194,6 +206,18 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
   return u;
 }
 
+// What the two warps of a row quarter share: per-row values they exchange (two slots), the rows' m
+// after an overflow and how many there were, and each warp's progress -- 2 n + 1: overflow in its
+// n-th tile, 2 n + 2: its P of the n-th tile is stored.
+struct PagedPair {
+  float xch[2][2][32];
+  float m[32];
+  int events;
+  int progress[2];
+  int pad[93];
+};
+static_assert(sizeof(PagedPair) == 1024, "eight of 1 KB");
+
 // The part of a unit in one CTA's share, as the producer describes it to the other roles.
 struct ChunkSeg {
   int seg;             // key tiles (0: no more parts)
@@ -264,61 +288,38 @@ __device__ __forceinline__ void chunk_rows(const PagedChunkParams& p, int row_a,
   }
 }
 
-// 64 TMEM columns of this warp's lanes, not waited for; tmem_ld_wait64 orders every use after it.
-__device__ __forceinline__ void tmem_ld64_nowait(uint32_t taddr, uint32_t (&r)[64]) {
-#pragma unroll
-  for (int i = 0; i < 64; i += 32)
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[i + 0]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]),
-          "=r"(r[i + 6]), "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]),
-          "=r"(r[i + 12]), "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15]), "=r"(r[i + 16]), "=r"(r[i + 17]),
-          "=r"(r[i + 18]), "=r"(r[i + 19]), "=r"(r[i + 20]), "=r"(r[i + 21]), "=r"(r[i + 22]), "=r"(r[i + 23]),
-          "=r"(r[i + 24]), "=r"(r[i + 25]), "=r"(r[i + 26]), "=r"(r[i + 27]), "=r"(r[i + 28]), "=r"(r[i + 29]),
-          "=r"(r[i + 30]), "=r"(r[i + 31])
-        : "r"(taddr + i)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait64(uint32_t (&r)[64]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 64; i += 16)  // (empty: the values are not usable before this point)
-    asm volatile(""
-                 : "+r"(r[i + 0]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                   "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
-                   "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
-}
-
-// Columns of the half row outside [lo, hi) to -inf: one unsigned compare a column.
-__device__ __forceinline__ void mask64(uint32_t (&s)[64], int lo, int hi) {
+// The maximum of this thread's 64 scores; with mask, columns outside [lo, hi) are first set to -inf in
+// TMEM.  Out of line, as all that a tile in a row's interior does not run: see mbar_wait_small.
+__device__ __noinline__ float tmem_prep(uint32_t addr, bool mask, int lo, int hi) {
   const uint32_t width = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 32) {
+    uint32_t a[32];
+    tmem_ld32(addr + c, a);
+    if (mask) {
 #pragma unroll
-  for (int c = 0; c < 64; ++c)
-    if (static_cast<uint32_t>(c - lo) >= width) s[c] = __float_as_uint(-INFINITY);
+      for (int e = 0; e < 32; ++e)
+        if (static_cast<uint32_t>(c + e - lo) >= width) a[e] = __float_as_uint(-INFINITY);
+      tmem_st32(addr + c, a);
+    }
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) mx = fmax3(mx, __uint_as_float(a[e]), __uint_as_float(a[e + 1]));
+  }
+  return mx;
 }
 
-__device__ __forceinline__ float max64(const uint32_t (&s)[64]) {
-  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      m4[u] = fmax3(m4[u], __uint_as_float(s[8 * c + 2 * u]), __uint_as_float(s[8 * c + 2 * u + 1]));
-  return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-}
-
-// Half a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; three
+// 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; two
 // pairs of eight by the polynomial, whose inputs' maximum goes to pmax.  A masked score (-inf) gives
 // 0 or, in the polynomial's columns, 2^-125: nothing beside a row's sum, which is about 1 or more.
-__device__ __forceinline__ void exp64(const uint32_t (&s)[64], uint64_t sc2, uint64_t nm2, uint32_t (&w)[32],
+__device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uint64_t nm2, uint32_t (&w)[16],
                                       uint64_t& acc0, uint64_t& acc1, float& pmax) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
+  for (int c = 0; c < 16; ++c) {
     const uint64_t x = fma2(static_cast<uint64_t>(s[2 * c]) | static_cast<uint64_t>(s[2 * c + 1]) << 32, sc2, nm2);
     const int u = c & 7;
     uint64_t e;
-    if (u == 2 || u == 5 || u == 7) {
+    if (u == 2 || u == 6) {
       pmax = fmax3(pmax, lo_f(x), hi_f(x));
       e = exp2_poly_pair(x);
     } else {
@@ -330,26 +331,51 @@ __device__ __forceinline__ void exp64(const uint32_t (&s)[64], uint64_t sc2, uin
   }
 }
 
-// This warp's rows of O (D columns) times alpha; its packed first half of P (32 columns) times alpha.
-template <int D>
-__device__ __noinline__ void tmem_scale(uint32_t addr, float alpha) {
+// `cols` accumulator columns of this warp's rows times alpha; 32 packed columns of P times alpha.
+__device__ __noinline__ void tmem_scale(uint32_t addr, int cols, float alpha) {
 #pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < cols; c += 32) {
     uint32_t o[32];
-    tmem_ld32(addr + c * 32, o);
+    tmem_ld32(addr + c, o);
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-    tmem_st32(addr + c * 32, o);
+    tmem_st32(addr + c, o);
   }
 }
 __device__ __noinline__ void tmem_scale_bf16(uint32_t addr, float alpha) {
-  tmem_st_wait();
   uint32_t o[32];
   tmem_ld32(addr, o);
 #pragma unroll
   for (int e = 0; e < 32; ++e)
     o[e] = pack_bf16x2_rn(__uint_as_float(o[e] << 16) * alpha, __uint_as_float(o[e] & 0xffff0000u) * alpha);
   tmem_st32(addr, o);
+}
+
+// Half a row of O times inv, as bf16 to out or as fp32 to part (the other null); valid: this row exists.
+template <int COLS>
+__device__ __noinline__ void chunk_store(uint32_t o_addr, float inv, bool valid, uint16_t* out, float* part) {
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t o[32];
+    tmem_ld32(o_addr + c, o);
+    if (!valid) continue;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+    if (part != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        *reinterpret_cast<uint4*>(part + c + 4 * e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = pack_bf16x2_rn(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
+        *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
 }
 
 template <int D>
@@ -369,27 +395,32 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   uint64_t* k_empty = bars + 6;    // [2]
   uint64_t* v_empty = bars + 8;    // [2]
   uint64_t* s_full = bars + 10;    // [2] per query tile
-  uint64_t* p_full = bars + 12;    // [2] 128 arrivals
-  uint64_t* s_free = bars + 14;    // [2] 128 arrivals (SEP): S has been read
+  uint64_t* p_full = bars + 12;    // [2] 256 arrivals
+  uint64_t* s_free = bars + 14;    // [2] 256 arrivals (SEP): S has been read
   uint64_t* pv_done = bars + 16;   // [2] (SEP): a P V product has completed
   uint64_t* o_done = bars + 18;
-  uint64_t* epi_done = bars + 19;  // 256 arrivals, once a unit
+  uint64_t* epi_done = bars + 19;  // 512 arrivals, once a unit
   uint64_t* drained = bars + 20;
   // [4] a description is there.  The producer writes description x after q_empty(x - 1), so after
   // epi_done(x - 3): every softmax thread is past x - 3, and the four in the ring are never behind
   uint64_t* seg_full = bars + 21;
-  constexpr int kNumBars = 25;
-  static_assert((kNumBars + 4) * 8 <= 256, "barriers, TMEM slot, abort flag and start in 256 bytes");
+  uint64_t* pairs = bars + 25;     // [2][4] 2 arrivals: the two warps of a tile's row quarter
+  constexpr int kNumBars = 33;
+  static_assert((kNumBars + 4) * 8 <= 320, "barriers, TMEM slot, abort flag and start in 320 bytes");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars + 1);
   int* ctl = reinterpret_cast<int*>(bars + kNumBars + 2);  // start: r, qb, h, local
-  long long* warp_tot = reinterpret_cast<long long*>(smem + Cfg::kScanOff);  // [12]
+  long long* warp_tot = reinterpret_cast<long long*>(smem + Cfg::kScanOff);  // [20]
   ChunkSeg* segs = reinterpret_cast<ChunkSeg*>(smem + Cfg::kSegOff);         // [4]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBars; ++i) mbar_init(bars + i, i >= 12 && i < 16 ? 128 : i == 19 ? 256 : 1);
+    for (int i = 0; i < kNumBars; ++i) mbar_init(bars + i, i >= 12 && i < 16 ? 256 : i == 19 ? 512 : i >= 25 ? 2 : 1);
     *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) {
+      PagedPair* pr = reinterpret_cast<PagedPair*>(smem + Cfg::kPairOff) + i;
+      pr->events = pr->progress[0] = pr->progress[1] = 0;
+    }
     fence_mbarrier_init();
     prefetch_tensormap(&qmap);
     prefetch_tensormap(&kmap);
@@ -472,7 +503,6 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcFewRegs));
     if (warp == 0) {
       // ---------------- producer and walker ----------------
       const uint64_t pol = l2_policy_evict_first();
@@ -553,7 +583,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           // the tile's chunks with visible keys: [ch0, ch1)
           const int ch0 = max((w.u.lo >> box_shift) - c0, 0), ch1 = min((w.u.hi >> box_shift) - c0 + 1, nch);
           const uint32_t bytes = static_cast<uint32_t>(max(ch1 - ch0, 0)) * Cfg::kPanels * box_bytes;
-#pragma unroll
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             uint64_t* full = kv ? &v_full[st] : &k_full[st];
             if (g >= 2 && !(ok = wait(kv ? &v_empty[st] : &k_empty[st], ((g >> 1) - 1) & 1))) break;
@@ -615,58 +645,66 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         // its last S, V after its last P V, Q after the unit's last S
 #pragma unroll 1
         for (int j = -1; ok && j < d.seg; ++j) {
-          const bool pv1 = j >= d.b1 && j < d.e1, s1 = j + 1 >= d.b1 && j + 1 < d.e1;
           const bool pv0 = j >= d.b0 && j < d.e0, s0 = j + 1 >= d.b0 && j + 1 < d.e0;
+          const bool pv1 = j >= d.b1 && j < d.e1, s1 = j + 1 >= d.b1 && j + 1 < d.e1;
           const int gj = g + j, st = __shfl_sync(0xffffffffu, gj & 1, 0), st1 = st ^ 1;
           if (pv0 || pv1) ok = wait(&v_full[st], (gj >> 1) & 1);
           if (ok && (s0 || s1)) ok = wait(&k_full[st1], ((gj + 1) >> 1) & 1);
+          const uint64_t ka = k_desc + st1 * (Cfg::kTileBytes >> 4), va = v_desc + st * (Cfg::kTileBytes >> 4);
 #pragma unroll 1
           for (int t = 0; ok && t < 2; ++t) {
             const bool pv = t ? pv1 : pv0, sn = t ? s1 : s0;
+            const bool last_v = t || !pv1, last_k = t || !s1, last_q = last_k && j + 1 == d.seg - 1;
+            const uint32_t more = j > (t ? d.b1 : d.b0) ? 1u : 0u;
+            const uint32_t o_col = tm + Cfg::kOCol + t * D;
+            const uint32_t p_col = tm + (SEP ? Cfg::kPCol + t * (kPcTile / 2) : t * kPcTile);
+            const uint64_t qa = q_desc + t * (Cfg::kTileBytes >> 4);
+            auto do_s = [&] {
+#pragma unroll 1
+              for (int pn = 0; pn < Cfg::kPanels; ++pn)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_ss(tm + t * kPcTile, qa + pn * ((kPcTile * 128) >> 4) + kk * 2, ka + pn * ((kPcTile * 128) >> 4) + kk * 2,
+                          idesc_s, pn + kk > 0 ? 1u : 0u);
+              umma_commit(&s_full[t]);
+              if (last_k) umma_commit(&k_empty[st1]);
+              if (last_q) umma_commit(q_empty);
+            };
+            auto do_pv = [&] {
+#pragma unroll 1
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_ts(o_col, p_col + half * (SEP ? 32 : 64) + kk * 8, va + (half * 4 + kk) * ((16 * 128) >> 4),
+                          idesc_o, half + kk > 0 ? 1u : more);
+              if (SEP) umma_commit(&pv_done[t]);
+              if (last_v) umma_commit(&v_empty[st]);
+            };
             const uint32_t bit = 1u << t;
-            const int flags = __shfl_sync(0xffffffffu,
-                                          (j > (t ? d.b1 : d.b0) ? 1 : 0) | (t || !pv1 ? 2 : 0) | (t || !s1 ? 4 : 0) |
-                                              ((t || !s1) && j + 1 == d.seg - 1 ? 8 : 0),
-                                          0);
-            if (SEP && sn && (s_any & bit) && !(ok = wait(&s_free[t], ((s_par >> t) & 1) ^ 1))) break;
-            if (!SEP && pv && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (half == (SEP ? 0 : 1)) {
-                if (sn) {
-                  const uint64_t qa = q_desc + t * (Cfg::kTileBytes >> 4), ka = k_desc + st1 * (Cfg::kTileBytes >> 4);
-                  if (elect_one()) {
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                      const int off = (kk >> 2) * ((kPcTile * 128) >> 4) + (kk & 3) * (32 >> 4);
-                      umma_ss(tm + t * kPcTile, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&s_full[t]);
-                    if (flags & 4) umma_commit(&k_empty[st1]);
-                    if (flags & 8) umma_commit(q_empty);
-                  }
-                  __syncwarp();
-                  s_par ^= bit;
-                  s_any |= bit;
-                }
-              } else if (pv) {
-                if (SEP && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
-                if (SEP) tc_fence_after();
-                const uint32_t pa = tm + (SEP ? Cfg::kPCol + t * (kPcTile / 2) : t * kPcTile);
-                const uint64_t va = v_desc + st * (Cfg::kTileBytes >> 4);
-                if (elect_one()) {
-#pragma unroll
-                  for (int kk = 0; kk < kPcTile / 16; ++kk)
-                    umma_ts(tm + Cfg::kOCol + t * D, pa + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o,
-                            kk > 0 ? 1u : flags & 1u);
-                  if (SEP) umma_commit(&pv_done[t]);
-                  if (flags & 2) umma_commit(&v_empty[st]);
-                }
+            if constexpr (SEP) {
+              if (sn) {
+                if ((s_any & bit) && !(ok = wait(&s_free[t], ((s_par >> t) & 1) ^ 1))) break;
+                tc_fence_after();
+                if (elect_one()) do_s();
                 __syncwarp();
-                pv_par ^= bit;
               }
+              if (pv) {
+                if (!(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
+                tc_fence_after();
+                if (elect_one()) do_pv();
+                __syncwarp();
+              }
+            } else {
+              if (pv && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
+              tc_fence_after();
+              if (elect_one()) {
+                if (pv) do_pv();
+                if (sn) do_s();
+              }
+              __syncwarp();
             }
+            if (pv) pv_par ^= bit;
+            if (sn) s_par ^= bit, s_any |= bit;
           }
         }
         if (ok && k > 0) ok = wait(epi_done, (k - 1) & 1);
@@ -680,20 +718,33 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPcManyRegs));
-    // ---------------- softmax: four warps a query tile, one thread a row ----------------
-    const int t = (warp - 4) >> 2;
+    // ---------------- softmax: eight warps a query tile, two threads a row ----------------
+    const int t = (warp - 4) >> 3, hh = ((warp - 4) >> 2) & 1;  // query tile; half of the key columns
     const int quarter = warp & 3;         // TMEM lanes 32 * quarter .. +31
     const int row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_off + t * kPcTile;
-    const uint32_t o_addr = tmem + lane_off + Cfg::kOCol + t * D;
-    const uint32_t p_addr = SEP ? tmem + lane_off + Cfg::kPCol + t * (kPcTile / 2) : s_addr;
+    const uint32_t s_addr = tmem + lane_off + t * kPcTile + hh * 64;
+    const uint32_t o_addr = tmem + lane_off + Cfg::kOCol + t * D + hh * (D / 2);
+    // P over this thread's own columns of S, or in its own
+    const uint32_t p_addr = SEP ? tmem + lane_off + Cfg::kPCol + t * (kPcTile / 2) + hh * 32 : s_addr;
     const int rt = row / p.a.G;           // the row's token in the tile
     const float sc = p.a.scale_log2;
     const uint64_t sc2 = pair_f32(sc, sc);
-    int g = 0, s_cnt = 0;
+    uint64_t* pair = pairs + t * 4 + quarter;
+    PagedPair* pr = reinterpret_cast<PagedPair*>(smem + Cfg::kPairOff) + t * 4 + quarter;
+    volatile int* progress = pr->progress;
+    volatile int* events = &pr->events;
+    int g = 0, s_cnt = 0, ex = 0, seen = 0;
     bool ok = true;
+    // The other thread's v (of this row): written to slot ex % 2 and read after both warps have
+    // arrived; a slot is written again two exchanges later, when both have read it.
+    auto exchange = [&](float v) -> float {
+      pr->xch[ex & 1][hh][lane] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      if (!wait(pair, ex & 1)) ok = false;
+      return pr->xch[ex++ & 1][hh ^ 1][lane];
+    };
     for (int k = 0; ok; ++k) {
       ChunkSeg d;
       if (!(ok = next_seg(k, d)) || d.seg == 0) break;
@@ -701,85 +752,145 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const int jb = t ? d.b1 : d.b0, je = t ? d.e1 : d.e0;
       const bool valid = rt < cnt_tok;             // (rows past tpb * G have rt >= tpb)
       const int pos0 = d.pos0 + t * p.tpb, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
-      const int see_hi = min(pos0 + rt, d.hi), see_lo = p.a.window >= 0 ? pos0 + rt - p.a.window : 0;
+      // this thread's columns of the key tile at kt: [see_lo - kt, see_hi - kt]
+      const int see_hi = min(pos0 + rt, d.hi) - 64 * hh;
+      const int see_lo = (p.a.window >= 0 ? pos0 + rt - p.a.window : 0) - 64 * hh;
+      // a key tile starting in [full_lo, full_hi] is seen whole by every row
+      const int full_hi = min(pos0, d.hi) - (kPcTile - 1), full_lo = p.a.window >= 0 ? pos1 - p.a.window : 0;
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
+      bool all_m = false;  // every row here has an m
       int cnt = 0;
       for (int j = jb; j < je; ++j, ++cnt, ++s_cnt) {
+        const int kt = d.kt0 + j * kPcTile;  // the tile's first key
+        const bool full = kt >= full_lo && kt <= full_hi;
         if (!(ok = wait(&s_full[t], s_cnt & 1))) break;
         tc_fence_after();
-        const int kt = d.kt0 + j * kPcTile;  // the tile's first key
-        if (kt < d.lo || kt + kPcTile - 1 > d.hi) {
-          // rows of V outside [lo, hi] to zero, a thread a row
-          const int st = (g + j) & 1;
-          if (!(ok = wait(&v_full[st], ((g + j) >> 1) & 1))) break;
-          if (kt + row < d.lo || kt + row > d.hi) {
-            const uint32_t at = base + Cfg::kVOff + st * Cfg::kTileBytes + row * 128;
-#pragma unroll
-            for (int c = 0; c < 8 * Cfg::kPanels; ++c)
-              sts128(at + (c >> 3) * (kPcTile * 128) + (c & 7) * 16, make_uint4(0, 0, 0, 0));
-          }
-          fence_proxy_async_shared();
-        }
-        if (!warp_rows) {  // no query row in this warp's quarter: P may be anything
-          if (SEP) {
-            mbar_arrive(&s_free[t]);
-            if (cnt > 0 && !(ok = wait(&pv_done[t], (s_cnt - 1) & 1))) break;
-          }
-          tc_fence_before();
-          mbar_arrive(&p_full[t]);
-          continue;
-        }
-        const bool full = kt + kPcTile - 1 <= min(pos0, d.hi) && (p.a.window < 0 || pos1 - kt <= p.a.window);
-        const int c_lo = max(0, see_lo - kt), c_hi = valid ? min(kPcTile, see_hi - kt + 1) : 0;
         // SEP: P's columns and O are free once the last P V has completed (else S's completion says so)
         auto pv_settled = [&] {
           if (!SEP || cnt == 0) return;
           if (!wait(&pv_done[t], (s_cnt - 1) & 1)) ok = false;
           tc_fence_after();
         };
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-          float sum;
-          bool redo = false;
-          while (true) {
-            uint32_t a[64];
-            tmem_ld64_nowait(s_addr + 64 * h, a);
-            tmem_ld_wait64(a);
-            if (!full) mask64(a, c_lo - 64 * h, c_hi - 64 * h);
-            if (redo || __any_sync(0xffffffffu, valid && m_used == -INFINITY)) {
-              const float mx = max64(a) * sc;
-              if (m_used == -INFINITY) {  // the first keys this row sees
-                m_used = mx;
-                l = 0.f;
-              } else if (redo) {
-                const float m_new = redo && valid && mx > m_used + 8.f ? mx : m_used;
-                const float alpha = fast_exp2(m_used - m_new);
-                m_used = m_new;
-                l *= alpha;
-                pv_settled();
-                if (cnt > 0) tmem_scale<D>(o_addr, alpha);
-                if (h) tmem_scale_bf16(p_addr, alpha);
-              }
+        if (__builtin_expect(!full || cnt == 0 || !warp_rows, 0)) {
+          if (kt < d.lo || kt + kPcTile - 1 > d.hi) {
+            // rows of V outside [lo, hi] to zero, a thread a row and half of its bytes
+            const int st = (g + j) & 1;
+            if (!(ok = wait(&v_full[st], ((g + j) >> 1) & 1))) break;
+            if (kt + row < d.lo || kt + row > d.hi) {
+              const uint32_t at = base + Cfg::kVOff + st * Cfg::kTileBytes + row * 128;
+#pragma unroll
+              for (int c = 0; c < 4 * Cfg::kPanels; ++c)
+                sts128(at + (Cfg::kPanels == 2 ? hh * (kPcTile * 128) + c * 16 : (hh * 4 + c) * 16),
+                       make_uint4(0, 0, 0, 0));
             }
-            const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-            uint64_t acc0 = 0, acc1 = 0;
-            float pmax = -INFINITY;
-            exp64(a, sc2, pair_f32(neg_m, neg_m), w, acc0, acc1, pmax);
-            acc0 = add2(acc0, acc1);
-            sum = lo_f(acc0) + hi_f(acc0);
-            if (redo || !__any_sync(0xffffffffu, valid && !(sum < 1.2676506e30f && pmax < 100.f))) break;  // 2^100
-            redo = true;
+            fence_proxy_async_shared();
           }
-          l += sum;
-          if (h == 0) pv_settled();
-          tmem_st16_nowait(p_addr + 32 * h, *reinterpret_cast<const uint32_t(*)[16]>(&w[0]));
-          tmem_st16_nowait(p_addr + 32 * h + 16, *reinterpret_cast<const uint32_t(*)[16]>(&w[16]));
+          if (!warp_rows) {  // no query row in this quarter: P may be anything
+            pv_settled();
+            if (!ok) break;
+            tc_fence_before();
+            if (SEP) mbar_arrive(&s_free[t]);
+            mbar_arrive(&p_full[t]);
+            continue;
+          }
         }
+        if (__builtin_expect(*events != seen, 0)) {  // the other warp moved m (in an earlier tile: see overflow below)
+          seen = *events;
+          const float m_new = pr->m[lane];
+          if (m_new != m_used) l *= fast_exp2(m_used - m_new);
+          m_used = m_new;
+        }
+        if (__builtin_expect(!full || !all_m, 0)) {
+          float mx = tmem_prep(s_addr, !full, max(0, see_lo - kt), valid ? min(64, see_hi - kt + 1) : 0) * sc;
+          if (!all_m) {  // (the same in both warps)
+            mx = fmaxf(mx, exchange(mx));
+            if (m_used == -INFINITY) {  // the first keys this row sees
+              m_used = mx;
+              l = 0.f;
+            }
+            all_m = !__any_sync(0xffffffffu, valid && m_used == -INFINITY);
+          }
+        }
+        uint32_t w0[16], w1[16];  // P of the first and the second 32 columns
+        float sum;
+        bool redone = false;
+        while (true) {
+          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+          const uint64_t nm2 = pair_f32(neg_m, neg_m);
+          uint64_t acc0 = 0, acc1 = 0;
+          float pmax = -INFINITY;
+          {
+            uint32_t a[32];
+            tmem_ld32(s_addr, a);
+            exp32(a, sc2, nm2, w0, acc0, acc1, pmax);
+            tmem_ld32(s_addr + 32, a);
+            exp32(a, sc2, nm2, w1, acc0, acc1, pmax);
+          }
+          acc0 = add2(acc0, acc1);
+          sum = lo_f(acc0) + hi_f(acc0);
+          const bool over = valid && !(sum < 1.2676506e30f && pmax < 100.f);  // 2^100
+          if (__builtin_expect(redone || !__any_sync(0xffffffffu, over), 1)) break;
+          // Overflow: m moves to the maximum of the rows that need it, and what was computed with the
+          // old one is rescaled.  The other warp of the pair either has overflowed too -- both then
+          // take the rows' common maximum and redo their columns -- or has stored its P of this tile
+          // and waits for the next S, which this warp holds up: this warp rescales that P and O, and
+          // the other one finds the new m (events) before its next tile.
+          redone = true;
+          if (lane == 0) progress[hh] = 2 * s_cnt + 1;
+          int other = 0;
+#pragma unroll 1
+          for (int n = 1 << 24; n > 0; --n) {
+            other = progress[hh ^ 1];
+            if (other > 2 * s_cnt || *abort_flag) break;
+          }
+          if (__any_sync(0xffffffffu, other <= 2 * s_cnt)) {
+            if (lane == 0) {
+              record_error(kErrWaitTimeout);
+              *abort_flag = 1;
+            }
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const bool both = __any_sync(0xffffffffu, other == 2 * s_cnt + 1);
+          float mx = tmem_prep(s_addr, false, 0, 0) * sc;
+          bool move = over;
+          if (both) {
+            mx = fmaxf(mx, exchange(mx));
+            move = exchange(move ? 1.f : 0.f) != 0.f || move;
+            if (!ok) break;
+          }
+          float alpha = 1.f;
+          if (move && mx > m_used) {
+            alpha = fast_exp2(m_used - mx);
+            m_used = mx;
+            l *= alpha;
+          }
+          pv_settled();
+          if (both) {
+            if (cnt > 0) tmem_scale(o_addr, D / 2, alpha);
+          } else {
+            if (cnt > 0) tmem_scale(o_addr - hh * (D / 2), D, alpha);
+            tmem_scale_bf16(SEP ? p_addr + (hh ? -32 : 32) : p_addr + (hh ? -64 : 64), alpha);
+            pr->m[lane] = m_used;
+            __syncwarp();
+            seen = *events + 1;
+            __syncwarp();
+            if (lane == 0) *events = seen;
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
+        l += sum;
+        pv_settled();
+        tmem_st16_nowait(p_addr, w0);
+        tmem_st16_nowait(p_addr + 16, w1);
         tmem_st_wait();
         if (!ok) break;
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) progress[hh] = 2 * s_cnt + 2;
         if (SEP) mbar_arrive(&s_free[t]);
         mbar_arrive(&p_full[t]);
       }
@@ -787,47 +898,24 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (ok && cnt > 0) ok = wait(&pv_done[t], (s_cnt - 1) & 1);
       }
       if (ok) ok = wait(o_done, k & 1);
-      if (ok) {
+      if (ok && warp_rows) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
-        if (d.part < 0) {
-          if (warp_rows) {
-            const int tok = d.tok + t * p.tpb + rt;
-            uint16_t* dst = p.a.out + (static_cast<long long>(tok) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G)) * D;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + c * 32, o);
-              if (valid)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  uint4 v;
-                  v.x = pack_bf16x2(__uint_as_float(o[8 * e + 0]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-                  v.y = pack_bf16x2(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-                  v.z = pack_bf16x2(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-                  v.w = pack_bf16x2(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
-                  *reinterpret_cast<uint4*>(dst + c * 32 + 8 * e) = v;
-                }
-            }
-          }
-        } else {
-          const long long prow = (static_cast<long long>(blockIdx.x) * 2 + d.part) * 256 + t * 128 + row;
-          if (valid) p.a.part_lse[prow] = l == 0.f ? -INFINITY : m_used + __log2f(l);
-          if (warp_rows && cnt > 0) {
-            float* dst = p.a.part_o + prow * D;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + c * 32, o);
-              if (valid)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  *reinterpret_cast<float4*>(dst + c * 32 + 4 * e) =
-                      make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                  __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
-            }
-          }
+        if (*events != seen) {
+          seen = *events;
+          const float m_new = pr->m[lane];
+          if (m_new != m_used) l *= fast_exp2(m_used - m_new);
+          m_used = m_new;
         }
+        const float other = exchange(l);
+        l = hh ? other + l : l + other;              // one order for both
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
+        const long long prow = (static_cast<long long>(blockIdx.x) * 2 + d.part) * 256 + t * 128 + row;
+        if (d.part >= 0 && valid && hh == 0) p.a.part_lse[prow] = l == 0.f ? -INFINITY : m_used + __log2f(l);
+        const int tok = d.tok + t * p.tpb + rt;
+        uint16_t* out =
+            p.a.out + (static_cast<long long>(tok) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G)) * D + hh * (D / 2);
+        if (cnt > 0)
+          chunk_store<D / 2>(o_addr, inv, valid, out, d.part >= 0 ? p.a.part_o + prow * D + hh * (D / 2) : nullptr);
       }
       tc_fence_before();
       mbar_arrive(epi_done);  // O is read: the issuer may let the next unit's o_done complete
