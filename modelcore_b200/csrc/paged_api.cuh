@@ -231,6 +231,8 @@ int check_paged_attn(const mcb_paged_attn_args* a, const char* who) {
   if (rc != MCB_OK) return rc;
   if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3e38f)
     return fail(MCB_ERR_INVALID_ARG, "%s: softmax_scale %g must be positive and finite", who, a->softmax_scale);
+  if (static_cast<long long>(a->N) * a->Hq > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: N %d * Hq %d above 2^31 - 1", who, a->N, a->Hq);
   if ((a->n_pages + 1ll) * a->Hkv > INT32_MAX)
     return fail(MCB_ERR_UNSUPPORTED, "%s: n_pages %d * Hkv %d above 2^31 - 1", who, a->n_pages, a->Hkv);
   return MCB_OK;
@@ -326,7 +328,7 @@ int launch_paged_chunk(const mcb_paged_attn_args* a, const mcb::PagedChunkParams
   note_attn_kernel("paged_chunk_kernel", D, 0, 0, false);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_chunk launch");
-  e = launch_pdl(mcb::paged_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 4), dim3(256), 0, st, p);
+  e = launch_pdl(mcb::paged_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 8), dim3(256), 0, st, p);
   g_launches++;
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_combine launch");

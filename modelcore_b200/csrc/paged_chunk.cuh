@@ -16,22 +16,23 @@
 //   warp 0      TMA producer and walker: describes each unit (or the part of one in this CTA's share)
 //               in shared memory for the other roles, loads Q0, Q1, then K_j and V_j into rings of
 //               two that run on across units, one box a (page chunk, 64-column panel)
-//   warp 1      allocates TMEM; one elected lane issues the products
-//                 S_t = Q_t K_j^T   M=128 N=128 K=D  (both operands from shared memory)
-//                 O_t += P_t V_j    M=128 N=D K=128  (P from TMEM)
-//   warps 4-11  softmax of Q0, warps 12-19 of Q1: two threads a query row, 64 key columns each
-// Two threads a row because a thread's instructions are in order: one warp a scheduler works at
-// two to three cycles an instruction, and a tile's softmax is what the next product waits for.
-// TMEM: S0, S1 (128 columns each), O0, O1 (D each).  D = 128 fills the 512 columns, so P (bf16)
-// is written over S and the issue order is PV0_j S0_j+1 PV1_j S1_j+1: one tile's products run
-// during the other's softmax.  With D = 64 P has columns of its own, and S_j+1 is computed as soon
-// as S_j has been read.
+//   warps 1, 2  (warp 1 allocates TMEM) products of Q0, of Q1, by halves h of a key tile
+//                 S_th = Q_t K_jh^T     M=128 N=64 K=D   (both operands from shared memory)
+//                 O_t += P_th V_jh      M=128 N=D K=64   (P from TMEM)
+//   warps 4-11  softmax of Q0, warps 12-19 of Q1: two threads a query row, one a half of the keys
+// TMEM: four S_th of 64 columns (the bf16 P_th is written over its S_th), O0, O1 (D columns each): all
+// 512 columns at D = 128.  A half is a chain of its own, S -> softmax -> P V -> next S, and the four
+// chains take turns on the tensor cores, so the softmax of three runs while a fourth's products do.
+// With whole tiles (N = 128, two chains) a chain's softmax had to fit beside one other chain's
+// products, which it does not (1,600 cycles against 1,024), and both then waited: 3,700 cycles a key
+// tile where the products take 2,048.  N = 64 costs the tensor cores a quarter more (S reads Q from
+// shared memory once for 64 keys: 384 cycles for 256 worth) and the rest overlaps.
 //
 // Softmax without a maximum on the critical path: the exponent's reference m is the row's maximum over
 // the first tile in which it sees a key, and stays.  P and l may then exceed 1 -- fp32 and bf16
-// reach 2^127 -- and only when a row's sum over its 64 columns of a tile leaves 2^100 is m moved
-// (see overflow()).  The two threads of a row thus need not meet in a tile.  Rounding: P to bf16 for
-// the product; l sums the unrounded values.
+// reach 2^127 -- and only when a row's sum over 64 keys leaves 2^100 is m moved (see `over` below).
+// The two threads of a row thus need not meet in a tile.  Rounding: P to bf16 for the product; l sums
+// the unrounded values.
 // Some of the exponentials run as a polynomial on the FMA pipe (exp2_poly_pair): the 16 a clock
 // an SM of the special function unit would otherwise take as long as the products.
 //
@@ -70,9 +71,7 @@ template <int D>
 struct PagedChunkConfig {
   static constexpr int kPanels = D / 64;
   static constexpr int kTileBytes = kPanels * kPcTile * 128;
-  static constexpr bool kSepP = D == 64;                 // P in columns of its own
-  static constexpr uint32_t kPCol = 2 * kPcTile;         // (kSepP) P0, P1: 64 columns each
-  static constexpr uint32_t kOCol = kSepP ? 3 * kPcTile : 2 * kPcTile;
+  static constexpr uint32_t kOCol = 2 * kPcTile;         // TMEM: S (and P) below, O0, O1 above
   static constexpr int kKOff = 2 * kTileBytes;           // Q0, Q1, then K and V, two stages each
   static constexpr int kVOff = kKOff + 2 * kTileBytes;
   static constexpr int kBarOff = kVOff + 2 * kTileBytes;
@@ -108,8 +107,19 @@ __device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parit
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait_long(bar, parity)) return true;
+  if (mbar_test_wait(bar, parity) || mbar_try_wait_long(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
   while (!mbar_try_wait_long(bar, parity)) {
@@ -152,10 +162,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // (2^a, 2^b) of a pair, each clamped below at 2^-125, as exp2_poly3: x = n + f, n = round(x) by the
 // 1.5 * 2^23 constant, a cubic for 2^f, and n added to the exponent (the constant's own bits leave
 // the word when shifted by 23).  Packed except the clamp and the exponent.  Above 2^127 the result
-// is meaningless: the caller watches the inputs' maximum.  A NaN comes out as 3.4e38, which the
-// caller's bound on the sum catches.
-__device__ __forceinline__ uint64_t exp2_poly_pair(uint64_t x) {
+// is meaningless: the caller watches the inputs' maximum.  A NaN in x leaves one in acc.
+__device__ __forceinline__ uint64_t exp2_poly_pair(uint64_t x, uint64_t& acc) {
   const uint64_t xc = pair_f32(max_nan(lo_f(x), -125.f), max_nan(hi_f(x), -125.f));
+  acc = fma2(xc, 0ull, acc);
   const uint64_t magic = pair_f32(12582912.f, 12582912.f), unmagic = pair_f32(-12582912.f, -12582912.f);
   const uint64_t t = add2(xc, magic);
   const uint64_t f = fma2(add2(t, unmagic), pair_f32(-1.f, -1.f), xc);
@@ -208,7 +218,8 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
 
 // What the two warps of a row quarter share: per-row values they exchange (two slots), the rows' m
 // after an overflow and how many there were, and each warp's progress -- 2 n + 1: overflow in its
-// n-th tile, 2 n + 2: its P of the n-th tile is stored.
+// n-th tile, 2 n + 2: its P of the n-th tile is stored (or, the first half's warp, a part of a unit
+// ended before its n-th tile and the products of all its P are complete).
 struct PagedPair {
   float xch[2][2][32];
   float m[32];
@@ -321,7 +332,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uin
     uint64_t e;
     if (u == 2 || u == 6) {
       pmax = fmax3(pmax, lo_f(x), hi_f(x));
-      e = exp2_poly_pair(x);
+      e = exp2_poly_pair(x, acc1);
     } else {
       e = pair_f32(fast_exp2(lo_f(x)), fast_exp2(hi_f(x)));
     }
@@ -351,29 +362,49 @@ __device__ __noinline__ void tmem_scale_bf16(uint32_t addr, float alpha) {
   tmem_st32(addr, o);
 }
 
-// Half a row of O times inv, as bf16 to out or as fp32 to part (the other null); valid: this row exists.
+// COLS columns of this warp's rows of O times inv: as bf16 to out at row `orow` (-1: no such row), or as
+// fp32 to part, whose layout is [4 columns][row] so that the lanes' stores join.  For out four lanes
+// transpose 4 x 16 bytes by shuffles and write 64 contiguous bytes of a row together (a store of 32
+// rows' separate 16 bytes takes the LSU 32 cycles, these 8).
 template <int COLS>
-__device__ __noinline__ void chunk_store(uint32_t o_addr, float inv, bool valid, uint16_t* out, float* part) {
+__device__ __noinline__ void chunk_store(uint32_t o_addr, float inv, int orow, uint16_t* out, long long pitch,
+                                         float* part) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = 0; c < COLS; c += 32) {
     uint32_t o[32];
     tmem_ld32(o_addr + c, o);
-    if (!valid) continue;
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
     if (part != nullptr) {
+      if (orow >= 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        *reinterpret_cast<uint4*>(part + c + 4 * e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-    } else {
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(part + (c / 4 + e) * (256 * 4)) =
+              make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      continue;
+    }
+    uint32_t v[4][4];  // four 16-byte chunks of this lane's row
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t v[4];
+    for (int e = 0; e < 16; ++e)
+      v[e >> 2][e & 3] = pack_bf16x2_rn(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[i] = pack_bf16x2_rn(__uint_as_float(o[8 * e + 2 * i]), __uint_as_float(o[8 * e + 2 * i + 1]));
-        *reinterpret_cast<uint4*>(out + c + 8 * e) = make_uint4(v[0], v[1], v[2], v[3]);
+    for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i & b) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & b) ? v[i][e] : v[i | b][e], b);
+          if (lane & b) v[i][e] = got;
+          else v[i | b][e] = got;
+        }
       }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // now v[i]: this lane's chunk of the group's i-th row
+      const int ri = __shfl_sync(0xffffffffu, orow, (lane & ~3) + i);
+      if (ri >= 0)
+        *reinterpret_cast<uint4*>(out + ri * pitch + c + (lane & 3) * 8) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
     }
   }
 }
@@ -383,7 +414,6 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const PagedChunkParams p) {
   using Cfg = PagedChunkConfig<D>;
-  constexpr bool SEP = Cfg::kSepP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -394,18 +424,17 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   uint64_t* v_full = bars + 4;     // [2]
   uint64_t* k_empty = bars + 6;    // [2]
   uint64_t* v_empty = bars + 8;    // [2]
-  uint64_t* s_full = bars + 10;    // [2] per query tile
-  uint64_t* p_full = bars + 12;    // [2] 256 arrivals
-  uint64_t* s_free = bars + 14;    // [2] 256 arrivals (SEP): S has been read
-  uint64_t* pv_done = bars + 16;   // [2] (SEP): a P V product has completed
+  uint64_t* s_full = bars + 10;    // [4] chain (query tile) * 2 + half
+  uint64_t* p_full = bars + 14;    // [4] 128 arrivals
   uint64_t* o_done = bars + 18;
   uint64_t* epi_done = bars + 19;  // 512 arrivals, once a unit
   uint64_t* drained = bars + 20;
+  uint64_t* pv_end = bars + 33;    // [2] per query tile: a part's last product of the first half is complete
   // [4] a description is there.  The producer writes description x after q_empty(x - 1), so after
   // epi_done(x - 3): every softmax thread is past x - 3, and the four in the ring are never behind
   uint64_t* seg_full = bars + 21;
   uint64_t* pairs = bars + 25;     // [2][4] 2 arrivals: the two warps of a tile's row quarter
-  constexpr int kNumBars = 33;
+  constexpr int kNumBars = 35;
   static_assert((kNumBars + 4) * 8 <= 320, "barriers, TMEM slot, abort flag and start in 320 bytes");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars + 1);
@@ -415,7 +444,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kNumBars; ++i) mbar_init(bars + i, i >= 12 && i < 16 ? 256 : i == 19 ? 512 : i >= 25 ? 2 : 1);
+    for (int i = 0; i < kNumBars; ++i) {
+      // two arrivals: what both issuers hand back or end with, and the pairs
+      const bool two = i == 1 || (i >= 6 && i < 10) || i == 18 || i == 20 || (i >= 25 && i < 33);
+      mbar_init(bars + i, i >= 14 && i < 18 ? 128 : i == 19 ? 512 : two ? 2 : 1);
+    }
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) {
       PagedPair* pr = reinterpret_cast<PagedPair*>(smem + Cfg::kPairOff) + i;
@@ -619,93 +652,73 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (k > 0) mbar_wait(q_full, (k - 1) & 1);
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ---------------- product issuer ----------------
+    } else if (warp < 3) {
+      // ---------------- product issuers, one a query tile ----------------
       // The whole warp waits, converged, and one elected lane issues: the descriptors are then
       // warp-uniform (a base and constants) and an MMA costs the warp an instruction or two.  Issued
       // from a lane-0 branch each took a dozen, and with two busy softmax warps on the same scheduler
       // the tensor cores starved: 2,400 FLOP a clock an SM against 8,000 in this form (both products
-      // back to back beside fp32 work; 8,192 at most).  Everything else a product needs is waited
-      // for before its P, and a tile's P V and next S go in one block: nothing but the two products
-      // lies between a P and the next S.
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPcTile, 0);
+      // back to back beside fp32 work; 8,192 at most).  A warp a tile, because issuing blocks until
+      // the tensor cores are nearly done: with one warp they idled while it went through its waits.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
+      const int t = __shfl_sync(0xffffffffu, warp - 1, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint64_t q_desc = smem_desc_sw128(base, 16, 1024);
+      const uint64_t q_desc = smem_desc_sw128(base + t * Cfg::kTileBytes, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(base + Cfg::kKOff, 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(base + Cfg::kVOff, kPcTile * 128, 1024);
       int g = 0;
-      uint32_t pv_par = 0, s_par = 0, s_any = 0;  // bit t: parity of tile t's products so far (and any S)
+      uint32_t parity = 0;  // of this tile's P so far
       bool ok = true;
       ChunkSeg d;
       for (int k = 0; ok; ++k) {
         if (!(ok = next_seg(k, d)) || d.seg == 0) break;
         ok = wait(q_full, k & 1);
-        // Step j: for each tile P V of key tile j and S of j + 1 (j = -1: the first S); K is free after
-        // its last S, V after its last P V, Q after the unit's last S
+        const int b = t ? d.b1 : d.b0, e = t ? d.e1 : d.e0;  // this tile's key tiles
+        if (b >= e && lane == 0) mbar_arrive(q_empty);
+        // Step j, half by half: P V of key tile j and S of j + 1 (j = -1: the first S).  Every key tile
+        // is waited for and handed back by both issuers, used or not: each stage's phases stay in step.
 #pragma unroll 1
         for (int j = -1; ok && j < d.seg; ++j) {
-          const bool pv0 = j >= d.b0 && j < d.e0, s0 = j + 1 >= d.b0 && j + 1 < d.e0;
-          const bool pv1 = j >= d.b1 && j < d.e1, s1 = j + 1 >= d.b1 && j + 1 < d.e1;
+          const bool pv = j >= b && j < e, sn = j + 1 >= b && j + 1 < e, next = j + 1 < d.seg;
           const int gj = g + j, st = __shfl_sync(0xffffffffu, gj & 1, 0), st1 = st ^ 1;
-          if (pv0 || pv1) ok = wait(&v_full[st], (gj >> 1) & 1);
-          if (ok && (s0 || s1)) ok = wait(&k_full[st1], ((gj + 1) >> 1) & 1);
-          const uint64_t ka = k_desc + st1 * (Cfg::kTileBytes >> 4), va = v_desc + st * (Cfg::kTileBytes >> 4);
+          if (j >= 0) ok = wait(&v_full[st], (gj >> 1) & 1);
+          if (ok && next) ok = wait(&k_full[st1], ((gj + 1) >> 1) & 1);
 #pragma unroll 1
-          for (int t = 0; ok && t < 2; ++t) {
-            const bool pv = t ? pv1 : pv0, sn = t ? s1 : s0;
-            const bool last_v = t || !pv1, last_k = t || !s1, last_q = last_k && j + 1 == d.seg - 1;
-            const uint32_t more = j > (t ? d.b1 : d.b0) ? 1u : 0u;
-            const uint32_t o_col = tm + Cfg::kOCol + t * D;
-            const uint32_t p_col = tm + (SEP ? Cfg::kPCol + t * (kPcTile / 2) : t * kPcTile);
-            const uint64_t qa = q_desc + t * (Cfg::kTileBytes >> 4);
-            auto do_s = [&] {
-#pragma unroll 1
-              for (int pn = 0; pn < Cfg::kPanels; ++pn)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                  umma_ss(tm + t * kPcTile, qa + pn * ((kPcTile * 128) >> 4) + kk * 2, ka + pn * ((kPcTile * 128) >> 4) + kk * 2,
-                          idesc_s, pn + kk > 0 ? 1u : 0u);
-              umma_commit(&s_full[t]);
-              if (last_k) umma_commit(&k_empty[st1]);
-              if (last_q) umma_commit(q_empty);
-            };
-            auto do_pv = [&] {
-#pragma unroll 1
-              for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                  umma_ts(o_col, p_col + half * (SEP ? 32 : 64) + kk * 8, va + (half * 4 + kk) * ((16 * 128) >> 4),
-                          idesc_o, half + kk > 0 ? 1u : more);
-              if (SEP) umma_commit(&pv_done[t]);
-              if (last_v) umma_commit(&v_empty[st]);
-            };
-            const uint32_t bit = 1u << t;
-            if constexpr (SEP) {
-              if (sn) {
-                if ((s_any & bit) && !(ok = wait(&s_free[t], ((s_par >> t) & 1) ^ 1))) break;
-                tc_fence_after();
-                if (elect_one()) do_s();
-                __syncwarp();
-              }
+          for (int h = 0; ok && h < 2; ++h) {
+            if (pv && !(ok = wait(&p_full[t * 2 + h], parity))) break;
+            tc_fence_after();
+            const uint32_t s_col = tm + t * kPcTile + h * 64;
+            if (elect_one()) {
               if (pv) {
-                if (!(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
-                tc_fence_after();
-                if (elect_one()) do_pv();
-                __syncwarp();
+                const uint64_t va = v_desc + st * (Cfg::kTileBytes >> 4) + h * ((64 * 128) >> 4);
+                const uint32_t more = j > b || h ? 1u : 0u;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_ts(tm + Cfg::kOCol + t * D, s_col + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o,
+                          kk > 0 ? 1u : more);
+                if (!h && j == e - 1) umma_commit(&pv_end[t]);
+                if (h) umma_commit(&v_empty[st]);
               }
-            } else {
-              if (pv && !(ok = wait(&p_full[t], (pv_par >> t) & 1))) break;
-              tc_fence_after();
-              if (elect_one()) {
-                if (pv) do_pv();
-                if (sn) do_s();
+              if (sn) {
+                const uint64_t ka = k_desc + st1 * (Cfg::kTileBytes >> 4) + h * ((64 * 128) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const int off = (kk >> 2) * ((kPcTile * 128) >> 4) + (kk & 3) * (32 >> 4);
+                  umma_ss(s_col, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[t * 2 + h]);
+                if (h) umma_commit(&k_empty[st1]);
+                if (h && j + 1 == e - 1) umma_commit(q_empty);
               }
-              __syncwarp();
             }
-            if (pv) pv_par ^= bit;
-            if (sn) s_par ^= bit, s_any |= bit;
+            __syncwarp();
           }
+          if (lane == 0) {
+            if (!pv && j >= 0) mbar_arrive(&v_empty[st]);
+            if (!sn && next) mbar_arrive(&k_empty[st1]);
+          }
+          parity ^= pv ? 1u : 0u;
         }
         if (ok && k > 0) ok = wait(epi_done, (k - 1) & 1);
         if (ok && elect_one()) umma_commit(o_done);
@@ -719,30 +732,32 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     }
   } else {
     // ---------------- softmax: eight warps a query tile, two threads a row ----------------
-    const int t = (warp - 4) >> 3, hh = ((warp - 4) >> 2) & 1;  // query tile; half of the key columns
+    const int t = (warp - 4) >> 3, hh = ((warp - 4) >> 2) & 1;  // query tile; half of the keys
     const int quarter = warp & 3;         // TMEM lanes 32 * quarter .. +31
     const int row = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_off + t * kPcTile + hh * 64;
-    const uint32_t o_addr = tmem + lane_off + Cfg::kOCol + t * D + hh * (D / 2);
-    // P over this thread's own columns of S, or in its own
-    const uint32_t p_addr = SEP ? tmem + lane_off + Cfg::kPCol + t * (kPcTile / 2) + hh * 32 : s_addr;
+    const uint32_t s_addr = tmem + lane_off + t * kPcTile + hh * 64;  // S, and P over it
+    const uint32_t o_addr = tmem + lane_off + Cfg::kOCol + t * D;
     const int rt = row / p.a.G;           // the row's token in the tile
     const float sc = p.a.scale_log2;
     const uint64_t sc2 = pair_f32(sc, sc);
     uint64_t* pair = pairs + t * 4 + quarter;
+    uint64_t* my_s = &s_full[t * 2 + hh];
+    uint64_t* my_p = &p_full[t * 2 + hh];
     PagedPair* pr = reinterpret_cast<PagedPair*>(smem + Cfg::kPairOff) + t * 4 + quarter;
     volatile int* progress = pr->progress;
     volatile int* events = &pr->events;
-    int g = 0, s_cnt = 0, ex = 0, seen = 0;
+    int g = 0, s_cnt = 0, ex = 0, seen = 0, ends = 0;
     bool ok = true;
     // The other thread's v (of this row): written to slot ex % 2 and read after both warps have
     // arrived; a slot is written again two exchanges later, when both have read it.
     auto exchange = [&](float v) -> float {
       pr->xch[ex & 1][hh][lane] = v;
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pair);
       if (!wait(pair, ex & 1)) ok = false;
+      tc_fence_after();
       return pr->xch[ex++ & 1][hh ^ 1][lane];
     };
     for (int k = 0; ok; ++k) {
@@ -752,64 +767,62 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const int jb = t ? d.b1 : d.b0, je = t ? d.e1 : d.e0;
       const bool valid = rt < cnt_tok;             // (rows past tpb * G have rt >= tpb)
       const int pos0 = d.pos0 + t * p.tpb, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
-      // this thread's columns of the key tile at kt: [see_lo - kt, see_hi - kt]
-      const int see_hi = min(pos0 + rt, d.hi) - 64 * hh;
-      const int see_lo = (p.a.window >= 0 ? pos0 + rt - p.a.window : 0) - 64 * hh;
-      // a key tile starting in [full_lo, full_hi] is seen whole by every row
-      const int full_hi = min(pos0, d.hi) - (kPcTile - 1), full_lo = p.a.window >= 0 ? pos1 - p.a.window : 0;
+      const int see_hi = min(pos0 + rt, d.hi), see_lo = p.a.window >= 0 ? pos0 + rt - p.a.window : 0;
+      // 64 keys starting in [full_lo, full_hi] are seen whole by every row
+      const int full_hi = min(pos0, d.hi) - 63, full_lo = p.a.window >= 0 ? pos1 - p.a.window : 0;
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
-      bool all_m = false;  // every row here has an m
+      bool all_m = !warp_rows;  // every row here has an m
+      int kt = d.kt0 + jb * kPcTile + hh * 64;  // the first of this half's keys
+      auto new_m = [&] {  // the other warp moved m after an overflow
+        seen = *events;
+        const float m = pr->m[lane];
+        if (m != m_used) l *= fast_exp2(m_used - m);
+        m_used = m;
+      };
       int cnt = 0;
-      for (int j = jb; j < je; ++j, ++cnt, ++s_cnt) {
-        const int kt = d.kt0 + j * kPcTile;  // the tile's first key
-        const bool full = kt >= full_lo && kt <= full_hi;
-        if (!(ok = wait(&s_full[t], s_cnt & 1))) break;
+      for (int j = jb; j < je; ++j, ++cnt, ++s_cnt, kt += kPcTile) {
+        const bool plain = kt >= full_lo && kt <= full_hi && all_m && warp_rows;
+        if (!(ok = wait(my_s, s_cnt & 1))) break;
         tc_fence_after();
-        // SEP: P's columns and O are free once the last P V has completed (else S's completion says so)
-        auto pv_settled = [&] {
-          if (!SEP || cnt == 0) return;
-          if (!wait(&pv_done[t], (s_cnt - 1) & 1)) ok = false;
-          tc_fence_after();
-        };
-        if (__builtin_expect(!full || cnt == 0 || !warp_rows, 0)) {
-          if (kt < d.lo || kt + kPcTile - 1 > d.hi) {
-            // rows of V outside [lo, hi] to zero, a thread a row and half of its bytes
+        if (__builtin_expect(*events != seen, 0)) new_m();
+        if (__builtin_expect(!plain, 0)) {
+          if (kt < d.lo || kt + 63 > d.hi) {
+            // rows of V outside [lo, hi] to zero: 64 rows, two threads a row
             const int st = (g + j) & 1;
             if (!(ok = wait(&v_full[st], ((g + j) >> 1) & 1))) break;
-            if (kt + row < d.lo || kt + row > d.hi) {
-              const uint32_t at = base + Cfg::kVOff + st * Cfg::kTileBytes + row * 128;
+            const int vr = row >> 1;
+            if (kt + vr < d.lo || kt + vr > d.hi) {
+              const uint32_t at = base + Cfg::kVOff + st * Cfg::kTileBytes + (hh * 64 + vr) * 128;
 #pragma unroll
               for (int c = 0; c < 4 * Cfg::kPanels; ++c)
-                sts128(at + (Cfg::kPanels == 2 ? hh * (kPcTile * 128) + c * 16 : (hh * 4 + c) * 16),
+                sts128(at + (Cfg::kPanels == 2 ? (row & 1) * (kPcTile * 128) + c * 16 : ((row & 1) * 4 + c) * 16),
                        make_uint4(0, 0, 0, 0));
             }
             fence_proxy_async_shared();
           }
           if (!warp_rows) {  // no query row in this quarter: P may be anything
-            pv_settled();
-            if (!ok) break;
             tc_fence_before();
-            if (SEP) mbar_arrive(&s_free[t]);
-            mbar_arrive(&p_full[t]);
+            mbar_arrive(my_p);
             continue;
           }
-        }
-        if (__builtin_expect(*events != seen, 0)) {  // the other warp moved m (in an earlier tile: see overflow below)
-          seen = *events;
-          const float m_new = pr->m[lane];
-          if (m_new != m_used) l *= fast_exp2(m_used - m_new);
-          m_used = m_new;
-        }
-        if (__builtin_expect(!full || !all_m, 0)) {
+          const bool full = kt >= full_lo && kt <= full_hi;
           float mx = tmem_prep(s_addr, !full, max(0, see_lo - kt), valid ? min(64, see_hi - kt + 1) : 0) * sc;
-          if (!all_m) {  // (the same in both warps)
+          if (!all_m) {
+            // (the same in both warps, which are both at their tile j: no product of O is in flight)
             mx = fmaxf(mx, exchange(mx));
-            if (m_used == -INFINITY) {  // the first keys this row sees
+            float alpha = 1.f;
+            if (mx > m_used + 64.f) {  // a row's first keys, or far above its m
+              alpha = fast_exp2(m_used - mx);  // 0 when m was -inf
               m_used = mx;
-              l = 0.f;
+              l *= alpha;
             }
             all_m = !__any_sync(0xffffffffu, valid && m_used == -INFINITY);
+            if (cnt > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+              tmem_scale(o_addr + hh * (D / 2), D / 2, alpha);
+              exchange(0.f);  // both halves of O are scaled before either P can be used
+            }
+            if (!ok) break;
           }
         }
         uint32_t w0[16], w1[16];  // P of the first and the second 32 columns
@@ -829,37 +842,44 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           acc0 = add2(acc0, acc1);
           sum = lo_f(acc0) + hi_f(acc0);
-          const bool over = valid && !(sum < 1.2676506e30f && pmax < 100.f);  // 2^100
+          const bool over = valid && (sum >= 1.2676506e30f || pmax >= 100.f);  // 2^100 (not a NaN)
           if (__builtin_expect(redone || !__any_sync(0xffffffffu, over), 1)) break;
-          // Overflow: m moves to the maximum of the rows that need it, and what was computed with the
-          // old one is rescaled.  The other warp of the pair either has overflowed too -- both then
-          // take the rows' common maximum and redo their columns -- or has stored its P of this tile
-          // and waits for the next S, which this warp holds up: this warp rescales that P and O, and
-          // the other one finds the new m (events) before its next tile.
+          // Overflow (never where the maximum has just been exchanged, so all_m holds for both warps
+          // from here on and they meet only below).  m moves to the maximum of the rows that need it, and
+          // what was computed with the old one is rescaled.  The products of a query tile are issued
+          // first half, second half, first half, ..., and this warp holds up its own: the other warp
+          //   - has overflowed too (odd progress): both take the rows' common maximum and redo theirs; or
+          //   - has stored the P whose product comes after this one's -- the first half's warp (hh = 0)
+          //     in tile n waits for the second's tile n, the second's for the first's tile n + 1 -- so
+          //     every product of O before is complete (its S was), and it waits for a next S that
+          //     cannot come: this warp rescales that P and O, and the other finds the new m (events)
+          //     before its next tile.
           redone = true;
+          __syncwarp();
           if (lane == 0) progress[hh] = 2 * s_cnt + 1;
+          const int need = 2 * (s_cnt + hh) + 1, low = 2 * (s_cnt - 1 + hh) + 1;
           int other = 0;
+          bool there = false;
+          const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
-          for (int n = 1 << 24; n > 0; --n) {
-            other = progress[hh ^ 1];
-            if (other > 2 * s_cnt || *abort_flag) break;
+          while (!there && !*abort_flag && global_timer_ns() - t0 < kWaitLimitNs) {
+            other = __shfl_sync(0xffffffffu, progress[hh ^ 1], 0);
+            there = other >= need || other == low;
+            __syncwarp();
           }
-          if (__any_sync(0xffffffffu, other <= 2 * s_cnt)) {
-            if (lane == 0) {
-              record_error(kErrWaitTimeout);
-              *abort_flag = 1;
-            }
+          if (__any_sync(0xffffffffu, !there)) {
+            if (lane == 0 && !*abort_flag) record_error(kErrWaitTimeout);
+            *abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const bool both = __any_sync(0xffffffffu, other == 2 * s_cnt + 1);
+          const bool both = other & 1;
           float mx = tmem_prep(s_addr, false, 0, 0) * sc;
           bool move = over;
           if (both) {
             mx = fmaxf(mx, exchange(mx));
             move = exchange(move ? 1.f : 0.f) != 0.f || move;
-            if (!ok) break;
           }
           float alpha = 1.f;
           if (move && mx > m_used) {
@@ -867,55 +887,51 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             m_used = mx;
             l *= alpha;
           }
-          pv_settled();
           if (both) {
-            if (cnt > 0) tmem_scale(o_addr, D / 2, alpha);
+            tmem_scale(o_addr + hh * (D / 2), D / 2, alpha);
+            exchange(0.f);  // both halves of O are scaled before either P can be used
+            if (!ok) break;
           } else {
-            if (cnt > 0) tmem_scale(o_addr - hh * (D / 2), D, alpha);
-            tmem_scale_bf16(SEP ? p_addr + (hh ? -32 : 32) : p_addr + (hh ? -64 : 64), alpha);
+            tmem_scale(o_addr, D, alpha);
+            tmem_scale_bf16(s_addr + (hh ? -64 : 64), alpha);
             pr->m[lane] = m_used;
             __syncwarp();
-            seen = *events + 1;
+            seen = __shfl_sync(0xffffffffu, *events, 0) + 1;
             __syncwarp();
             if (lane == 0) *events = seen;
-            __syncwarp();
           }
         }
         if (!ok) break;
         l += sum;
-        pv_settled();
-        tmem_st16_nowait(p_addr, w0);
-        tmem_st16_nowait(p_addr + 16, w1);
+        tmem_st16_nowait(s_addr, w0);
+        tmem_st16_nowait(s_addr + 16, w1);
         tmem_st_wait();
-        if (!ok) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) progress[hh] = 2 * s_cnt + 2;
-        if (SEP) mbar_arrive(&s_free[t]);
-        mbar_arrive(&p_full[t]);
+        mbar_arrive(my_p);
       }
-      if constexpr (SEP) {
-        if (ok && cnt > 0) ok = wait(&pv_done[t], (s_cnt - 1) & 1);
+      if (ok && cnt > 0) {
+        ok = wait(&pv_end[t], ends & 1);
+        ++ends;
+        if (hh == 0 && lane == 0) progress[0] = 2 * s_cnt + 2;
       }
       if (ok) ok = wait(o_done, k & 1);
       if (ok && warp_rows) {
         tc_fence_after();
-        if (*events != seen) {
-          seen = *events;
-          const float m_new = pr->m[lane];
-          if (m_new != m_used) l *= fast_exp2(m_used - m_new);
-          m_used = m_new;
-        }
+        if (*events != seen) new_m();
         const float other = exchange(l);
         l = hh ? other + l : l + other;              // one order for both
         const float inv = l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
-        const long long prow = (static_cast<long long>(blockIdx.x) * 2 + d.part) * 256 + t * 128 + row;
-        if (d.part >= 0 && valid && hh == 0) p.a.part_lse[prow] = l == 0.f ? -INFINITY : m_used + __log2f(l);
-        const int tok = d.tok + t * p.tpb + rt;
-        uint16_t* out =
-            p.a.out + (static_cast<long long>(tok) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G)) * D + hh * (D / 2);
-        if (cnt > 0)
-          chunk_store<D / 2>(o_addr, inv, valid, out, d.part >= 0 ? p.a.part_o + prow * D + hh * (D / 2) : nullptr);
+        const long long slot = static_cast<long long>(blockIdx.x) * 2 + d.part;
+        if (d.part >= 0 && valid && hh == 0)
+          p.a.part_lse[slot * 256 + t * 128 + row] = l == 0.f ? -INFINITY : m_used + __log2f(l);
+        if (cnt > 0) {
+          const int orow = valid ? (d.tok + t * p.tpb + rt) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G) : -1;
+          float* part = d.part < 0 ? nullptr
+                                   : p.a.part_o + ((slot * (D / 4) + hh * (D / 8)) * 256 + t * 128 + row) * 4;
+          chunk_store<D / 2>(o_addr + hh * (D / 2), inv, orow, p.a.out + hh * (D / 2), D, part);
+        }
       }
       tc_fence_before();
       mbar_arrive(epi_done);  // O is read: the issuer may let the next unit's o_done complete
@@ -935,23 +951,58 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   }
 }
 
-// Merges the units cut between CTAs: blockIdx.x is the CTA whose share the unit starts in,
-// blockIdx.y and the warps divide its 256 rows.
+// Merges the units cut between CTAs: blockIdx.x is the CTA whose share the unit starts in, blockIdx.y
+// 32 of its rows.  A lane is a row, a warp takes every eighth group of four columns (the partials'
+// layout: a load is 512 contiguous bytes); the rows leave through shared memory, whole.
 template <int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedChunkParams p) {
+  __shared__ uint2 rows[32][D / 4 + 1];
+  __shared__ int out_row[32];
   pdl_wait();
   pdl_launch_dependents();
   const PagedCut c = p.cuts[blockIdx.x];
   if (c.h < 0) return;
-  const int rows = p.tpb * p.a.G;
-  auto row_out = [&](int n) {
-    const int rr = n & 127, tok = c.tok0 + (n >> 7) * p.tpb + rr / p.a.G;
-    return p.a.out + (static_cast<long long>(tok) * p.a.Hq + c.h * p.a.G + rr % p.a.G) * D;
-  };
-  for (int n = blockIdx.y * 8 + (threadIdx.x >> 5); n < 256; n += gridDim.y * 8) {
-    const int rr = n & 127;
-    if (rr >= rows || c.tok0 + (n >> 7) * p.tpb + rr / p.a.G >= c.tok1) continue;
-    paged_merge<D, 256>(p.a.part_o, p.a.part_lse, blockIdx.x, c.g_last, c.slot1 != 0, n, row_out);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = blockIdx.y * 32 + lane, rr = n & 127;
+  const int rt = rr / p.a.G, tok = c.tok0 + (n >> 7) * p.tpb + rt;
+  const bool valid = rt < p.tpb && tok < c.tok1;
+  if (!__syncthreads_or(valid)) return;
+  const int cnt = c.g_last - static_cast<int>(blockIdx.x) + 1;
+  auto slot = [&](int k) { return (static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 && c.slot1 ? 1 : 0); };
+  float mx = -CUDART_INF_F, wsum = 0.f;
+  if (valid) {
+    for (int k = 0; k < cnt; ++k) mx = fmaxf(mx, __ldcg(p.a.part_lse + slot(k) * 256 + n));
+    for (int k = 0; k < cnt; ++k) {
+      const float ls = __ldcg(p.a.part_lse + slot(k) * 256 + n);
+      wsum += ls == -CUDART_INF_F ? 0.f : fast_exp2(ls - mx);
+    }
+  }
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
+  if (warp == 0) out_row[lane] = valid ? tok * p.a.Hq + c.h * p.a.G + (rr - rt * p.a.G) : -1;
+#pragma unroll 1
+  for (int q = warp; q < D / 4; q += 8) {
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    if (valid) {
+#pragma unroll 4
+      for (int k = 0; k < cnt; ++k) {
+        const float ls = __ldcg(p.a.part_lse + slot(k) * 256 + n);
+        if (ls == -CUDART_INF_F) continue;  // (its partial was not written)
+        const float w = fast_exp2(ls - mx);
+        const float4 v =
+            __ldcg(reinterpret_cast<const float4*>(p.a.part_o) + (slot(k) * (D / 4) + q) * 256 + n);
+        a[0] = fmaf(w, v.x, a[0]);
+        a[1] = fmaf(w, v.y, a[1]);
+        a[2] = fmaf(w, v.z, a[2]);
+        a[3] = fmaf(w, v.w, a[3]);
+      }
+    }
+    rows[lane][q] = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+    const int r = i / (D / 4), q = i % (D / 4);
+    if (out_row[r] >= 0)
+      *reinterpret_cast<uint2*>(p.a.out + static_cast<long long>(out_row[r]) * D + 4 * q) = rows[r][q];
   }
 }
 
