@@ -435,6 +435,7 @@ typedef struct {
   int32_t* cu_new;                /* (R + 1,)                                                   */
   int32_t* positions;             /* (N,)                                                       */
   int64_t* slot_map;              /* (N,)                                                       */
+  int32_t* counter;               /* one int32, zero before the call and after it               */
   int64_t table_stride;           /* elements                                                   */
   int32_t R, N, n_pages, max_pages, page_size;
 } mcb_page_plan_args;
@@ -449,6 +450,7 @@ typedef struct {
   const int64_t* free_state;      /* (2,)                                                       */
   int64_t* free_state_out;        /* (2,)                                                       */
   int32_t* seqlens_out;           /* (R,)                                                       */
+  int32_t* counter;               /* one int32, zero before the call and after it               */
   int64_t table_stride;
   int32_t R, n_pages, max_pages, page_size;
 } mcb_page_release_args;

@@ -205,7 +205,7 @@ class PagePlanArgs(ctypes.Structure):
         ("block_table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
         ("free_state", ctypes.c_void_p), ("free_state_out", ctypes.c_void_p),
         ("cu_new", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("slot_map", ctypes.c_void_p),
-        ("table_stride", ctypes.c_int64),
+        ("counter", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
         ("R", ctypes.c_int32), ("N", ctypes.c_int32), ("n_pages", ctypes.c_int32),
         ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
     ]
@@ -216,7 +216,7 @@ class PageReleaseArgs(ctypes.Structure):
         ("done", ctypes.c_void_p), ("cache_seqlens", ctypes.c_void_p),
         ("block_table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
         ("free_state", ctypes.c_void_p), ("free_state_out", ctypes.c_void_p),
-        ("seqlens_out", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p), ("counter", ctypes.c_void_p),
         ("table_stride", ctypes.c_int64),
         ("R", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32),
         ("page_size", ctypes.c_int32),

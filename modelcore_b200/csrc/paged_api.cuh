@@ -39,25 +39,6 @@ int check_pool(int n_pages, int page_size, int max_pages, const char* who) {
   return check_page_size(page_size, who);
 }
 
-// Launches one cluster of `ctas` CTAs (the whole grid) with programmatic stream serialization.
-template <typename P>
-cudaError_t launch_one_cluster(void (*kernel)(P), int ctas, int threads, cudaStream_t st, const P& p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 int page_plan(const mcb_page_plan_args* a, void* stream) {
   const char* who = "mcb_page_plan";
   if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
@@ -66,7 +47,7 @@ int page_plan(const mcb_page_plan_args* a, void* stream) {
   if (rc != MCB_OK) return rc;
   if (a->cu_new == nullptr || a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr ||
       (a->R > 0 && (a->cache_seqlens == nullptr || a->new_lens == nullptr || a->block_table == nullptr)) ||
-      (a->N > 0 && (a->positions == nullptr || a->slot_map == nullptr)))
+      a->counter == nullptr || (a->N > 0 && (a->positions == nullptr || a->slot_map == nullptr)))
     return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
   if (a->table_stride < a->max_pages)
     return fail(MCB_ERR_INVALID_ARG, "%s: table_stride %lld below max_pages %d", who,
@@ -87,10 +68,13 @@ int page_plan(const mcb_page_plan_args* a, void* stream) {
   p.n_pages = a->n_pages;
   p.max_pages = a->max_pages;
   p.page_shift = page_shift_of(a->page_size);
+  p.counter = a->counter;
   // a thread a row up to 1,024, and about two tokens a thread before another CTA joins
   const int threads = a->R <= 256 && a->N <= 512 ? 256 : mcb::kPlanMaxThreads;
-  const int ctas = std::clamp((a->N + 2 * threads - 1) / (2 * threads), 1, mcb::kPlanMaxCluster);
-  cudaError_t e = launch_one_cluster(mcb::page_plan_kernel, ctas, threads, static_cast<cudaStream_t>(stream), p);
+  const int ctas = static_cast<int>(std::clamp<long long>((a->N + 2ll * threads - 1) / (2 * threads), 1,
+                                                          device_sm_count()));
+  cudaError_t e = launch_pdl(mcb::page_plan_kernel, dim3(static_cast<unsigned>(ctas)),
+                             dim3(static_cast<unsigned>(threads)), 0, static_cast<cudaStream_t>(stream), p);
   g_launches++;
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "page_plan launch");
@@ -103,7 +87,7 @@ int page_release(const mcb_page_release_args* a, void* stream) {
   if (a->R < 0) return fail(MCB_ERR_INVALID_ARG, "%s: bad size R=%d", who, a->R);
   int rc = check_pool(a->n_pages, a->page_size, a->max_pages, who);
   if (rc != MCB_OK) return rc;
-  if (a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr ||
+  if (a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr || a->counter == nullptr ||
       (a->R > 0 && (a->done == nullptr || a->cache_seqlens == nullptr || a->block_table == nullptr ||
                     a->seqlens_out == nullptr)))
     return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
@@ -123,10 +107,13 @@ int page_release(const mcb_page_release_args* a, void* stream) {
   p.n_pages = a->n_pages;
   p.max_pages = a->max_pages;
   p.page_shift = page_shift_of(a->page_size);
-  const int threads = mcb::kPlanMaxThreads;
-  const long long most = static_cast<long long>(a->R) * a->max_pages;  // pages that can come back
-  const int ctas = static_cast<int>(std::clamp<long long>(most / (4 * threads), 1, mcb::kPlanMaxCluster));
-  cudaError_t e = launch_one_cluster(mcb::page_release_kernel, ctas, threads, static_cast<cudaStream_t>(stream), p);
+  p.counter = a->counter;
+  // at most a table's worth of pages comes back, eight a thread
+  const int threads = a->R <= 256 ? 256 : mcb::kPlanMaxThreads;
+  const long long most = static_cast<long long>(a->R) * a->max_pages;
+  const int ctas = static_cast<int>(std::clamp<long long>(most / (8 * threads), 1, device_sm_count()));
+  cudaError_t e = launch_pdl(mcb::page_release_kernel, dim3(static_cast<unsigned>(ctas)),
+                             dim3(static_cast<unsigned>(threads)), 0, static_cast<cudaStream_t>(stream), p);
   g_launches++;
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "page_release launch");

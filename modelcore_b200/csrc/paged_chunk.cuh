@@ -299,6 +299,29 @@ __device__ __forceinline__ void chunk_rows(const PagedChunkParams& p, int row_a,
   }
 }
 
+// 32 TMEM columns of this warp's lanes, not waited for; tmem_ld_wait32 orders every use after it.
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
 // The maximum of this thread's 64 scores; with mask, columns outside [lo, hi) are first set to -inf in
 // TMEM.  Out of line, as all that a tile in a row's interior does not run: see mbar_wait_small.
 __device__ __noinline__ float tmem_prep(uint32_t addr, bool mask, int lo, int hi) {
@@ -320,8 +343,8 @@ __device__ __noinline__ float tmem_prep(uint32_t addr, bool mask, int lo, int hi
   return mx;
 }
 
-// 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; two
-// pairs of eight by the polynomial, whose inputs' maximum goes to pmax.  A masked score (-inf) gives
+// 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; one
+// pair of eight by the polynomial, whose inputs' maximum goes to pmax.  A masked score (-inf) gives
 // 0 or, in the polynomial's columns, 2^-125: nothing beside a row's sum, which is about 1 or more.
 __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uint64_t nm2, uint32_t (&w)[16],
                                       uint64_t& acc0, uint64_t& acc1, float& pmax) {
@@ -330,7 +353,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uin
     const uint64_t x = fma2(static_cast<uint64_t>(s[2 * c]) | static_cast<uint64_t>(s[2 * c + 1]) << 32, sc2, nm2);
     const int u = c & 7;
     uint64_t e;
-    if (u == 2 || u == 6) {
+    if (u == 4) {
       pmax = fmax3(pmax, lo_f(x), hi_f(x));
       e = exp2_poly_pair(x, acc1);
     } else {
@@ -785,8 +808,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         const bool plain = kt >= full_lo && kt <= full_hi && all_m && warp_rows;
         if (!(ok = wait(my_s, s_cnt & 1))) break;
         tc_fence_after();
+        uint32_t a[32];
+        tmem_ld32_nowait(s_addr, a);  // on its way during the checks
         if (__builtin_expect(*events != seen, 0)) new_m();
         if (__builtin_expect(!plain, 0)) {
+          tmem_ld_wait32(a);
           if (kt < d.lo || kt + 63 > d.hi) {
             // rows of V outside [lo, hi] to zero: 64 rows, two threads a row
             const int st = (g + j) & 1;
@@ -824,6 +850,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             }
             if (!ok) break;
           }
+          tmem_ld32_nowait(s_addr, a);  // (masked)
         }
         uint32_t w0[16], w1[16];  // P of the first and the second 32 columns
         float sum;
@@ -833,13 +860,10 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           const uint64_t nm2 = pair_f32(neg_m, neg_m);
           uint64_t acc0 = 0, acc1 = 0;
           float pmax = -INFINITY;
-          {
-            uint32_t a[32];
-            tmem_ld32(s_addr, a);
-            exp32(a, sc2, nm2, w0, acc0, acc1, pmax);
-            tmem_ld32(s_addr + 32, a);
-            exp32(a, sc2, nm2, w1, acc0, acc1, pmax);
-          }
+          tmem_ld_wait32(a);
+          exp32(a, sc2, nm2, w0, acc0, acc1, pmax);
+          tmem_ld32(s_addr + 32, a);
+          exp32(a, sc2, nm2, w1, acc0, acc1, pmax);
           acc0 = add2(acc0, acc1);
           sum = lo_f(acc0) + hi_f(acc0);
           const bool over = valid && (sum >= 1.2676506e30f || pmax >= 100.f);  // 2^100 (not a NaN)
@@ -900,6 +924,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             __syncwarp();
             if (lane == 0) *events = seen;
           }
+          tmem_ld32_nowait(s_addr, a);
         }
         if (!ok) break;
         l += sum;
@@ -907,9 +932,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         tmem_st16_nowait(s_addr + 16, w1);
         tmem_st_wait();
         tc_fence_before();
+        mbar_arrive(my_p);
         __syncwarp();
         if (lane == 0) progress[hh] = 2 * s_cnt + 2;
-        mbar_arrive(my_p);
       }
       if (ok && cnt > 0) {
         ok = wait(&pv_end[t], ends & 1);

@@ -11,11 +11,11 @@
 // tail (entry x at x mod n_pages).  A plan neither moves the lengths nor overwrites a table entry
 // below first_r, so planning again from the same lengths and counters gives the same answer.
 //
-// One thread-block cluster does a whole call: every CTA scans the lengths itself (1,024 rows at a
-// time, two sums in one 64-bit scan) and expands its share of the tokens and pages.  Integers
-// only, a few KB to a few MB: launch and dependent-load latency bound it, not bytes.  A cluster,
-// not a grid, because free_state_out (and seqlens_out) may be the inputs: every CTA has read them
-// before the cluster barrier, and only then are they written.
+// Every CTA scans the lengths itself (1,024 rows at a time, two sums in one 64-bit scan) and expands
+// its share of the tokens and pages, a thread four (plan) or eight (release) of them with their
+// searches and loads side by side: integers only, a few KB to a few MB, so launch and dependent
+// latencies bound it, not bytes.  free_state_out (and seqlens_out) may be the inputs: the CTA that
+// arrives last, all having read them, writes them.
 #pragma once
 
 #include "common.cuh"
@@ -23,7 +23,6 @@
 namespace mcb {
 
 constexpr int kPlanMaxThreads = 1024;
-constexpr int kPlanMaxCluster = 8;
 
 struct PagePlanParams {
   const int32_t* seqlens;
@@ -36,6 +35,7 @@ struct PagePlanParams {
   int32_t* cu_new;      // (R + 1,)
   int32_t* positions;   // (N,)
   long long* slot_map;  // (N,)
+  int* counter;         // arrivals, zero on entry and left zero
   int R, N, n_pages, max_pages, page_shift;
 };
 
@@ -48,8 +48,22 @@ struct PageReleaseParams {
   const long long* free_state;
   long long* free_state_out;
   int32_t* seqlens_out;
+  int* counter;
   int R, n_pages, max_pages, page_shift;
 };
+
+// Whether this CTA is the last of the grid to arrive; all threads' reads before are then done in every
+// CTA.  `counter` is zero again after the last.
+__device__ __forceinline__ bool last_cta(int* counter) {
+  __shared__ int s_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_last = atom_add_acq_rel_gpu(counter, 1) == static_cast<int>(gridDim.x) - 1;
+    if (s_last) *counter = 0;
+  }
+  __syncthreads();
+  return s_last != 0;
+}
 
 // Inclusive scan of one 64-bit value a thread over the block; `warp_sums` is 33 shared words, the
 // last of them the block's total.
@@ -88,6 +102,21 @@ __device__ __forceinline__ int row_of(const uint32_t* start, int n, uint32_t x) 
   return lo;
 }
 
+// The same for U values at once, in step.
+template <int U>
+__device__ __forceinline__ void rows_of(const uint32_t* start, int n, const uint32_t (&x)[U], int (&row)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) row[u] = 0;
+  int step = 1;
+  while (step < n) step <<= 1;
+  for (step >>= 1; step > 0; step >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = row[u] + step;
+      if (r < n && start[r] <= x[u]) row[u] = r;
+    }
+}
+
 // x mod n for 0 <= x < 2 n.
 __device__ __forceinline__ int wrap(long long x, int n) { return static_cast<int>(x >= n ? x - n : x); }
 
@@ -103,10 +132,11 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, nthr = blockDim.x;
-  const int rank = blockIdx.x, nc = gridDim.x;  // the grid is one cluster
+  const int rank = blockIdx.x, nc = gridDim.x;
   const long long head = p.free_state[0], tail = p.free_state[1];
   const long long avail = min(max(tail - head, 0ll), static_cast<long long>(p.n_pages));
-  const int head0 = static_cast<int>(((head % p.n_pages) + p.n_pages) % p.n_pages);
+  __shared__ int s_head;  // (one thread's division: the first scan's barriers publish it)
+  if (tid == 0) s_head = static_cast<int>(((head % p.n_pages) + p.n_pages) % p.n_pages);
   uint32_t tok0 = 0, page0 = 0;  // sums over the rows of earlier chunks
   if (rank == 0 && tid == 0) p.cu_new[0] = 0;
   for (int base = 0; base < p.R; base += nthr) {
@@ -136,33 +166,46 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
       const int i = row_of(s_page, rows, k);
       const int j = pages_of(s_len[i], p.page_shift, p.max_pages) + static_cast<int>(k - s_page[i]);
       int page = -1;
-      if (k < avail) page = p.free_pages[wrap(static_cast<long long>(head0) + k, p.n_pages)];
+      if (k < avail) page = p.free_pages[wrap(static_cast<long long>(s_head) + k, p.n_pages)];
       else record_error(kErrPagesExhausted);
       p.block_table[(base + i) * p.table_stride + j] = page;
     }
     // positions and slots
-    for (uint32_t t = tok0 + rank * nthr + tid; t < min(tok1, static_cast<uint32_t>(p.N)); t += nc * nthr) {
-      const int i = row_of(s_tok, rows, t);
-      const int row_len = s_len[i];
-      const long long pos = static_cast<long long>(row_len) + (t - s_tok[i]);
-      const long long j = pos >> p.page_shift;
-      int page = -1;
-      if (j < p.max_pages) {
-        const int first = pages_of(row_len, p.page_shift, p.max_pages);
-        if (j < first) {
-          page = p.block_table[(base + i) * p.table_stride + j];
-        } else {
-          const uint32_t k = s_page[i] + static_cast<uint32_t>(j - first);
-          if (k < avail) page = p.free_pages[wrap(static_cast<long long>(head0) + k, p.n_pages)];
-        }
-        if (page < 0 || page >= p.n_pages) {
-          record_error(kErrPageOutOfRange);  // (a page the queue lacked: error 5 came first)
-          page = -1;
+    constexpr int U = 4;
+    const uint32_t tok_end = min(tok1, static_cast<uint32_t>(p.N)), hop = nc * nthr;
+    for (uint32_t t0 = tok0 + rank * nthr + tid; t0 < tok_end; t0 += U * hop) {
+      uint32_t t[U];
+      int i[U], page[U];
+      long long pos[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) t[u] = min(t0 + u * hop, tok_end - 1);
+      rows_of<U>(s_tok, rows, t, i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row_len = s_len[i[u]];
+        pos[u] = static_cast<long long>(row_len) + (t[u] - s_tok[i[u]]);
+        const long long j = pos[u] >> p.page_shift;
+        page[u] = -1;
+        if (j < p.max_pages) {
+          const int first = pages_of(row_len, p.page_shift, p.max_pages);
+          const uint32_t k = s_page[i[u]] + static_cast<uint32_t>(j - first);
+          if (j < first)
+            page[u] = p.block_table[(base + i[u]) * p.table_stride + j];
+          else if (k < avail)
+            page[u] = p.free_pages[wrap(static_cast<long long>(s_head) + k, p.n_pages)];
+          if (page[u] < 0) page[u] = -2;
         }
       }
-      p.positions[t] = static_cast<int>(pos);
-      p.slot_map[t] = page < 0 ? -1 : (static_cast<long long>(page) << p.page_shift) +
-                                          (pos & ((1ll << p.page_shift) - 1));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (t0 + u * hop >= tok_end) break;
+        const bool in = page[u] >= 0 && page[u] < p.n_pages;
+        if (!in && page[u] != -1) record_error(kErrPageOutOfRange);  // (a page the queue lacked: error 5 came first)
+        p.positions[t[u]] = static_cast<int>(pos[u]);
+        p.slot_map[t[u]] = in ? (static_cast<long long>(page[u]) << p.page_shift) +
+                                    (pos[u] & ((1ll << p.page_shift) - 1))
+                              : -1;
+      }
     }
     tok0 = tok1;
     page0 = page1;
@@ -173,8 +216,7 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
     p.positions[t] = -1;
     p.slot_map[t] = -1;
   }
-  cluster_sync();  // every CTA has read the counters
-  if (rank == 0 && tid == 0) {
+  if (last_cta(p.counter) && tid == 0) {
     p.free_state_out[0] = head + min(static_cast<long long>(page0), avail);
     p.free_state_out[1] = tail;
   }
@@ -187,40 +229,66 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
   const int tid = threadIdx.x, nthr = blockDim.x;
   const int rank = blockIdx.x, nc = gridDim.x;
   const long long head = p.free_state[0], tail = p.free_state[1];
-  const long long room = min(max(p.n_pages - (tail - head), 0ll), static_cast<long long>(p.n_pages));
-  const int tail0 = static_cast<int>(((tail % p.n_pages) + p.n_pages) % p.n_pages);
+  const uint32_t room =
+      static_cast<uint32_t>(min(max(p.n_pages - (tail - head), 0ll), static_cast<long long>(p.n_pages)));
+  __shared__ int s_tail;  // (one thread's division: the first scan's barriers publish it)
+  if (tid == 0) s_tail = static_cast<int>(((tail % p.n_pages) + p.n_pages) % p.n_pages);
   uint32_t page0 = 0;
   for (int base = 0; base < p.R; base += nthr) {
     const int r = base + tid, rows = min(nthr, p.R - base);
-    int len = 0, held = 0;
-    bool gone = false;
+    int held = 0;
     if (r < p.R) {
-      len = p.seqlens[r];
-      gone = p.done[r] != 0;
-      if (gone) held = pages_of(max(len, 0), p.page_shift, p.max_pages);
+      const int len = p.seqlens[r];
+      if (p.done[r] != 0) held = pages_of(max(len, 0), p.page_shift, p.max_pages);
     }
     const unsigned long long incl = block_scan(static_cast<unsigned long long>(held), warp_sums);
     const uint32_t page1 = page0 + static_cast<uint32_t>(warp_sums[32]);
     s_page[tid] = page0 + static_cast<uint32_t>(incl) - held;
     __syncthreads();
-    for (uint32_t k = page0 + rank * nthr + tid; k < page1; k += nc * nthr) {
-      const int i = row_of(s_page, rows, k);
-      const int page = p.block_table[(base + i) * p.table_stride + (k - s_page[i])];
-      if (page < 0 || page >= p.n_pages) record_error(kErrPageOutOfRange);
-      if (k >= room) {
-        record_error(kErrPagesExhausted);  // more pages than the pool has: a row released twice
-        continue;
+    // A warp takes 256 consecutive pages at a time.  Where they are one request's -- long requests --
+    // one search finds it, and the entries are a copy; else every lane searches for its own.
+    constexpr int U = 8;
+    const int lane = tid & 31;
+    const uint32_t hop = nc * (nthr >> 5) * 32 * U;
+    for (uint32_t w0 = page0 + (rank * (nthr >> 5) + (tid >> 5)) * 32 * U; w0 < page1; w0 += hop) {
+      const uint32_t k0 = w0 + lane;
+      int page[U];
+      const int row = row_of(s_page, rows, w0);
+      const uint32_t row_end = row + 1 < rows ? s_page[row + 1] : page1;
+      if (row_end - w0 >= 32 * U) {
+        const int32_t* src = p.block_table + (base + row) * p.table_stride + (k0 - s_page[row]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) page[u] = src[32 * u];
+      } else {
+        uint32_t k[U];
+        int i[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = min(k0 + 32 * u, page1 - 1);
+        rows_of<U>(s_page, rows, k, i);
+#pragma unroll
+        for (int u = 0; u < U; ++u) page[u] = p.block_table[(base + i[u]) * p.table_stride + (k[u] - s_page[i[u]])];
       }
-      p.free_pages[wrap(static_cast<long long>(tail0) + k, p.n_pages)] = page;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t k = k0 + 32 * u;
+        if (k >= page1) break;
+        if (static_cast<uint32_t>(page[u]) >= static_cast<uint32_t>(p.n_pages)) record_error(kErrPageOutOfRange);
+        if (k >= room) {
+          record_error(kErrPagesExhausted);  // more pages than the pool has: a row released twice
+        } else {
+          const uint32_t at = s_tail + k;  // below 2 n_pages
+          p.free_pages[at >= static_cast<uint32_t>(p.n_pages) ? at - p.n_pages : at] = page[u];
+        }
+      }
     }
     page0 = page1;
-    cluster_sync();  // every CTA has read this chunk's lengths (and s_page is free again)
-    if (rank == 0 && r < p.R) p.seqlens_out[r] = gone ? 0 : len;
+    __syncthreads();  // s_page is free again
   }
-  cluster_sync();
-  if (rank == 0 && tid == 0) {
+  if (!last_cta(p.counter)) return;
+  for (int r = tid; r < p.R; r += nthr) p.seqlens_out[r] = p.done[r] != 0 ? 0 : p.seqlens[r];
+  if (tid == 0) {
     p.free_state_out[0] = head;
-    p.free_state_out[1] = tail + min(static_cast<long long>(page0), room);
+    p.free_state_out[1] = tail + min(page0, room);
   }
 }
 

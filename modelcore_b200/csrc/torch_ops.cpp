@@ -27,6 +27,7 @@
 // (earlier arrays stay alive: a captured CUDA graph may hold them).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -404,6 +405,12 @@ void int_vec(const at::Tensor& t, const char* name, int64_t n, const at::Tensor&
               t.sizes());
 }
 
+// A new contiguous tensor beside `like`, straight from the caching allocator (at::empty's way through the
+// dispatcher costs a microsecond of host time a tensor, as much as a decode step's small kernels take).
+at::Tensor new_tensor(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType dtype) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
+}
+
 // Checks a block table and returns its row stride (one row's is arbitrary in torch).
 int64_t check_block_table(const at::Tensor& t, int64_t rows, const at::Tensor& ref) {
   need(t, "block_table", 2, at::kInt);
@@ -432,6 +439,26 @@ void check_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) 
               " and ", v.sizes());
 }
 
+// The arrival counters of the paged operators, zero before their first use and left zero by every call: one
+// array per stream, so calls on two streams never share one; a stream under capture gets its own
+// array per capture (zeroed by a node of that graph), so graphs replayed side by side do not either.
+int32_t* paged_counters(const at::Tensor& q, size_t count) {
+  static std::mutex mu;
+  static std::map<std::tuple<int, void*, unsigned long long>, std::vector<at::Tensor>> arrays;
+  const auto stream = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+  if (status != cudaStreamCaptureStatusActive) id = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  auto& bufs = arrays[{q.device().index(), static_cast<void*>(stream), id}];
+  if (bufs.empty() || static_cast<size_t>(bufs.back().numel()) < count) {
+    const int64_t n = std::max<int64_t>(static_cast<int64_t>(count), 1 << 14);
+    bufs.push_back(at::zeros({n}, q.options().dtype(at::kInt)));
+  }
+  return bufs.back().data_ptr<int32_t>();
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache_seqlens, const at::Tensor& new_lens,
                                                          const at::Tensor& block_table, const at::Tensor& free_pages,
                                                          const at::Tensor& free_state, const at::Tensor& free_state_out,
@@ -446,9 +473,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache
   int_vec(free_state, "free_state", 2, cache_seqlens, at::kLong);
   int_vec(free_state_out, "free_state_out", 2, cache_seqlens, at::kLong);
   TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative, got ", num_tokens);
-  at::Tensor cu = at::empty({R + 1}, cache_seqlens.options());
-  at::Tensor pos = at::empty({num_tokens}, cache_seqlens.options());
-  at::Tensor slots = at::empty({num_tokens}, cache_seqlens.options().dtype(at::kLong));
+  at::Tensor cu = new_tensor({R + 1}, cache_seqlens, at::kInt);
+  at::Tensor pos = new_tensor({num_tokens}, cache_seqlens, at::kInt);
+  at::Tensor slots = new_tensor({num_tokens}, cache_seqlens, at::kLong);
   mcb_page_plan_args a = {};
   a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
   a.new_lens = new_lens.data_ptr<int32_t>();
@@ -465,6 +492,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache
   a.n_pages = to_i32(free_pages.size(0), "n_pages");
   a.max_pages = to_i32(block_table.size(1), "max_pages");
   a.page_size = to_i32(page_size, "page_size");
+  a.counter = paged_counters(cache_seqlens, 1);
   check_status(mcb_page_plan(&a, stream_of(cache_seqlens)), "mcb200::page_plan");
   return {cu, pos, slots};
 }
@@ -495,6 +523,7 @@ void page_release(const at::Tensor& done, const at::Tensor& cache_seqlens, const
   a.n_pages = to_i32(free_pages.size(0), "n_pages");
   a.max_pages = to_i32(block_table.size(1), "max_pages");
   a.page_size = to_i32(page_size, "page_size");
+  a.counter = paged_counters(cache_seqlens, 1);
   check_status(mcb_page_release(&a, stream_of(cache_seqlens)), "mcb200::page_release");
 }
 
@@ -518,7 +547,7 @@ at::Tensor paged_append_rope(const at::Tensor& q, const std::optional<at::Tensor
   TORCH_CHECK(kv == v.has_value() && kv == k_pages.has_value() && kv == v_pages.has_value() &&
                   kv == slot_map.has_value(),
               "k, v, k_pages, v_pages and slot_map come together (all or none)");
-  at::Tensor q_out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor q_out = new_tensor(q.sizes(), q, at::kBFloat16);
   mcb_paged_append_args a = {};
   a.q = q.data_ptr();
   packed_strides(q, "q", a.q_stride);
@@ -560,26 +589,6 @@ at::Tensor paged_append_rope(const at::Tensor& q, const std::optional<at::Tensor
   return q_out;
 }
 
-// The arrival counters of paged_attn, zero before their first use and left zero by every call: one
-// array per stream, so calls on two streams never share one; a stream under capture gets its own
-// array per capture (zeroed by a node of that graph), so graphs replayed side by side do not either.
-int32_t* paged_counters(const at::Tensor& q, size_t count) {
-  static std::mutex mu;
-  static std::map<std::tuple<int, void*, unsigned long long>, std::vector<at::Tensor>> arrays;
-  const auto stream = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
-  if (status != cudaStreamCaptureStatusActive) id = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  auto& bufs = arrays[{q.device().index(), static_cast<void*>(stream), id}];
-  if (bufs.empty() || static_cast<size_t>(bufs.back().numel()) < count) {
-    const int64_t n = std::max<int64_t>(static_cast<int64_t>(count), 1 << 14);
-    bufs.push_back(at::zeros({n}, q.options().dtype(at::kInt)));
-  }
-  return bufs.back().data_ptr<int32_t>();
-}
-
 at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
                       const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
                       int64_t window, std::optional<double> softmax_scale, int64_t max_new) {
@@ -591,7 +600,7 @@ at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::
   int_vec(cache_seqlens, "cache_seqlens", R, q, at::kInt);
   int_vec(cu_new, "cu_new", R + 1, q, at::kInt);
   const int64_t table_stride = check_block_table(block_table, R, q);
-  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor out = new_tensor(q.sizes(), q, at::kBFloat16);
   mcb_paged_attn_args a = {};
   a.q = q.data_ptr();
   packed_strides(q, "q", a.q_stride);
@@ -618,7 +627,7 @@ at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::
   at::Tensor ws;
   const size_t bytes = mcb_paged_attn_workspace_size(&a);
   if (bytes > 0) {
-    ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    ws = new_tensor({static_cast<int64_t>(bytes)}, q, at::kByte);
     a.workspace = ws.data_ptr();
     a.workspace_bytes = bytes;
   }

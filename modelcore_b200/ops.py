@@ -677,11 +677,18 @@ class PagePlan(NamedTuple):
     free_state: torch.Tensor  # (2,) int64: the queue's head and tail after the step
 
 
-def _paged():
+class _Paged:
     """The paged operators, torch.ops.mcb200 (C++ over the same C ABI: a call costs a third of a
-    ctypes one on the host, which a decode step of small launches feels)."""
-    from . import torch_ops  # noqa: F401  (registers them; raises without the built library)
-    return torch.ops.mcb200
+    ctypes one on the host, which a decode step of small launches feels), resolved on first use."""
+
+    def __getattr__(self, name):
+        from . import torch_ops  # noqa: F401  (registers them; raises without the built library)
+        op = getattr(torch.ops.mcb200, name).default
+        setattr(self, name, op)
+        return op
+
+
+_PAGED = _Paged()
 
 
 def page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state, *, page_size, num_tokens,
@@ -701,7 +708,7 @@ def page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state, *, p
     are -1), 1 when a request outgrows its table row, 7 when new_lens exceed num_tokens."""
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)
-    cu, pos, slots = _paged().page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state,
+    cu, pos, slots = _PAGED.page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state,
                                         free_state_out, page_size, num_tokens)
     return PagePlan(cu, pos, slots, free_state_out)
 
@@ -716,7 +723,7 @@ def page_release(done, cache_seqlens, block_table, free_pages, free_state, *, pa
         free_state_out = torch.empty_like(free_state)
     if seqlens_out is None:
         seqlens_out = torch.empty_like(cache_seqlens)
-    _paged().page_release(done, cache_seqlens, block_table, free_pages, free_state, free_state_out,
+    _PAGED.page_release(done, cache_seqlens, block_table, free_pages, free_state, free_state_out,
                           seqlens_out, page_size)
     return free_state_out, seqlens_out
 
@@ -730,7 +737,7 @@ def paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin, 
     pages.  Padding (position -1) gives a zero q, slot -1 writes nothing.  round_each: every step
     rounded to bf16, the bits of kv_append_rope (a paged cache then holds what KVCache holds);
     False keeps fp32 and rounds once.  Returns the processed q."""
-    return _paged().paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin, eps, scale,
+    return _PAGED.paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin, eps, scale,
                                       rotate_k, round_each)
 
 
@@ -742,7 +749,7 @@ def paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, *, windo
     prompts and single-token steps mix freely.  max_new: the largest number of new tokens of a
     request when the caller knows it (0: unknown; a decode step with 1 needs one launch less).
     Returns (N, Hq, D) bf16, zeros past cu_new[R]."""
-    return _paged().paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new,
+    return _PAGED.paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new,
                                -1 if window is None else window, softmax_scale, max_new)
 
 

@@ -41,7 +41,7 @@ def _rejects(entry, cls, good, cases):
 
 P = 1 << 20
 PLAN = dict(cache_seqlens=P, new_lens=P, block_table=P, free_pages=P, free_state=P, free_state_out=P, cu_new=P,
-            positions=P, slot_map=P, table_stride=8, R=2, N=4, n_pages=9, max_pages=8, page_size=16)
+            positions=P, slot_map=P, counter=P, table_stride=8, R=2, N=4, n_pages=9, max_pages=8, page_size=16)
 
 
 def test_plan_and_release_reject_bad_arguments():
@@ -50,11 +50,11 @@ def test_plan_and_release_reject_bad_arguments():
               (dict(page_size=24), UNSUPPORTED, "power of two"), (dict(page_size=2048), UNSUPPORTED, "power of two"),
               (dict(max_pages=1 << 28, table_stride=1 << 28), UNSUPPORTED, "positions a request"),
               (dict(table_stride=7), INVALID, "table_stride"), (dict(block_table=None), INVALID, "NULL"),
-              (dict(free_state_out=None), INVALID, "NULL")]
+              (dict(free_state_out=None), INVALID, "NULL"), (dict(counter=None), INVALID, "NULL")]
     _rejects("mcb_page_plan", PagePlanArgs, PLAN,
              common + [(dict(N=-1), INVALID, "N=-1"), (dict(slot_map=None), INVALID, "NULL")])
     release = dict(done=P, cache_seqlens=P, block_table=P, free_pages=P, free_state=P, free_state_out=P,
-                   seqlens_out=P, table_stride=8, R=2, n_pages=9, max_pages=8, page_size=16)
+                   seqlens_out=P, counter=P, table_stride=8, R=2, n_pages=9, max_pages=8, page_size=16)
     _rejects("mcb_page_release", PageReleaseArgs, release, common + [(dict(done=None), INVALID, "NULL")])
 
 
