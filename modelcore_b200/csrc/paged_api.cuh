@@ -244,10 +244,12 @@ int encode_page_map(CUtensorMap* map, const void* base, const mcb_paged_attn_arg
 
 template <int D, int NQT>
 struct PagedDecodeVariant {
-  // 128-KB and 48-KB rings: one CTA an SM at head size 128, three (two with 16 query rows) at 64
+  // 128-KB and 48-KB rings: one CTA an SM at head size 128, three (two with 16 query rows) at 64.  Two
+  // groups of consumer warps where they fit: batch 128 of 16/4 heads of 128, 198 -> 191 us.
   static constexpr int STAGES = D == 64 ? 3 : 4;
-  using Cfg = mcb::PagedDecodeConfig<D, NQT, STAGES>;
-  static constexpr auto kernel = mcb::paged_decode_kernel<D, NQT, STAGES>;
+  static constexpr int GROUPS = D == 128 && NQT == 1 ? 2 : 1;
+  using Cfg = mcb::PagedDecodeConfig<D, NQT, STAGES, GROUPS>;
+  static constexpr auto kernel = mcb::paged_decode_kernel<D, NQT, STAGES, GROUPS>;
 
   // CTAs resident on the device (the shared-memory limit raised once); one an SM without a device.
   static int grid() {
@@ -257,11 +259,11 @@ struct PagedDecodeVariant {
     const int per_sm = per_device(cache, mu, [] {
       int n = 0;
       if (ensure_smem(kernel, Cfg::SMEM_BYTES, done) != cudaSuccess ||
-          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, mcb::kPdThreads, Cfg::SMEM_BYTES) != cudaSuccess)
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, Cfg::THREADS, Cfg::SMEM_BYTES) != cudaSuccess)
         cudaGetLastError();
       return n;
     });
-    return device_sm_count() * std::max(per_sm, 1);
+    return std::min(device_sm_count() * std::max(per_sm, 1), 1024);  // (share_begin's bound)
   }
 
   static int launch(const mcb_paged_attn_args* a, const mcb::PagedAttnParams& p, cudaStream_t st) {
@@ -270,7 +272,7 @@ struct PagedDecodeVariant {
     int rc = encode_page_map(&km, a->k_pages, a, box, D / 64);
     if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, D / 64);
     if (rc != MCB_OK) return rc;
-    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid())), dim3(mcb::kPdThreads),
+    cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(grid())), dim3(Cfg::THREADS),
                                static_cast<size_t>(Cfg::SMEM_BYTES), st, km, vm, p);
     g_launches++;
     note_attn_kernel("paged_decode_kernel", D, NQT, STAGES, false);
@@ -303,7 +305,7 @@ int launch_paged_chunk(const mcb_paged_attn_args* a, const mcb::PagedChunkParams
   constexpr int smem = mcb::PagedChunkConfig<D>::kSmem;
   CUtensorMap qm, km, vm;
   const int box = std::min(a->page_size, mcb::kPcTile);
-  int rc = encode_packed_q_map(&qm, a, q_stride, p.tpb);
+  int rc = encode_packed_q_map(&qm, a, q_stride, p.a.tpb);
   if (rc == MCB_OK) rc = encode_page_map(&km, a->k_pages, a, box, 1);
   if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, 1);
   if (rc != MCB_OK) return rc;
@@ -340,9 +342,11 @@ PagedAttnPlan plan_paged_attn(const mcb_paged_attn_args* a) {
   PagedAttnPlan pl = {};
   const long long G = a->Hq / a->Hkv;
   const long long most = a->max_new > 0 ? a->max_new * G : 1ll << 40;  // query rows a kv head of a request
-  pl.nqt = most <= 8 ? 1 : 2;
   pl.decode = G <= 16;
   pl.chunk = most > 16;  // (always when G > 16)
+  // 8 query rows a unit where every request has no more, and beside the chunk kernel (whose share is
+  // then the requests of 9 to 16 rows too): the variant of 8 reads half as fast again an SM
+  pl.nqt = most <= 8 || (pl.chunk && G <= 8) ? 1 : 2;
   if (pl.decode) {
     pl.decode_grid = with_decode_variant(a->D, pl.nqt, [](auto v) { return decltype(v)::grid(); });
     const size_t rows = static_cast<size_t>(pl.decode_grid) * 2 * 8 * pl.nqt;
@@ -403,6 +407,7 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
   p.window = a->window;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.few_rows = pl.decode ? 8 * pl.nqt : 0;
+  p.tpb = mcb::kPcTile / p.G;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   if (pl.decode) {
@@ -421,7 +426,6 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
   c.a.all = 0;
   c.a.fill = 1;
   c.cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.c_o + pl.c_lse);
-  c.tpb = mcb::kPcTile / p.G;
   c.wait_last = pl.decode;
   return a->D == 64 ? launch_paged_chunk<64>(a, c, q_stride, pl.chunk_grid, st)
                     : launch_paged_chunk<128>(a, c, q_stride, pl.chunk_grid, st);

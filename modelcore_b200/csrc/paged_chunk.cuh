@@ -62,7 +62,6 @@ struct PagedCut {
 struct PagedChunkParams {
   PagedAttnParams a;
   PagedCut* cuts;      // [grid]
-  int tpb;             // tokens a tile
   int wait_last;       // the kernel ahead is this call's decode kernel, whose output this one does
                        // not read: wait for it only before the end
 };
@@ -187,7 +186,7 @@ struct ChunkUnit {
 };
 
 __device__ __forceinline__ int chunk_blocks(const PagedChunkParams& p, const PagedRow& x) {
-  return static_cast<long long>(x.T) * p.a.G > p.a.few_rows ? (x.T + 2 * p.tpb - 1) / (2 * p.tpb) : 0;
+  return static_cast<long long>(x.T) * p.a.G > p.a.few_rows ? (x.T + 2 * p.a.tpb - 1) / (2 * p.a.tpb) : 0;
 }
 
 __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const PagedRow& x, int r, int qb, int nqb) {
@@ -196,9 +195,9 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
   u.r = r;
   u.qb = qb;
   u.nqb = nqb;
-  const int first = qb * 2 * p.tpb, left = x.T - first;
-  u.c0 = min(left, p.tpb);
-  u.c1 = min(max(left - p.tpb, 0), p.tpb);
+  const int first = qb * 2 * p.a.tpb, left = x.T - first;
+  u.c0 = min(left, p.a.tpb);
+  u.c1 = min(max(left - p.a.tpb, 0), p.a.tpb);
   const int cap = static_cast<int>((static_cast<long long>(p.a.max_pages) << p.a.page_shift) - 1);
   auto last_key = [&](int tok) { return static_cast<int>(min(static_cast<long long>(x.L) + tok, static_cast<long long>(cap))); };
   auto first_key = [&](int tok) { return p.a.window >= 0 ? max(0, x.L + tok - p.a.window) : 0; };
@@ -210,7 +209,7 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
   u.e0 = (last_key(first + u.c0 - 1) - u.kb) / kPcTile + 1;
   u.b1 = u.e1 = 0;
   if (u.c1 > 0) {
-    u.b1 = min((min(first_key(first + p.tpb), u.hi) - u.kb) / kPcTile, u.n - 1);
+    u.b1 = min((min(first_key(first + p.a.tpb), u.hi) - u.kb) / kPcTile, u.n - 1);
     u.e1 = u.n;
   }
   return u;
@@ -320,6 +319,12 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])
                :
                : "memory");
+}
+
+// 32 TMEM columns of this warp's lanes to zero.
+__device__ __noinline__ void tmem_zero32(uint32_t taddr) {
+  const uint32_t z[32] = {};
+  tmem_st32(taddr, z);
 }
 
 // The maximum of this thread's 64 scores; with mask, columns outside [lo, hi) are first set to -inf in
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const int box_shift = min(p.a.page_shift, 7);  // positions a box: min(page, 128)
       const int box = 1 << box_shift, nch = kPcTile >> box_shift;
       const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
-      const uint32_t q_bytes = static_cast<uint32_t>(p.tpb * p.a.G) * 128u;
+      const uint32_t q_bytes = static_cast<uint32_t>(p.a.tpb * p.a.G) * 128u;
       ChunkWalk w;
       w.t = t_begin;
       if (active) {
@@ -590,10 +595,10 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           d.e0 = min(w.u.e0 - w.local, seg);
           d.b1 = max(w.u.b1 - w.local, 0);
           d.e1 = min(w.u.e1 - w.local, seg);
-          d.pos0 = w.u.row.L + w.u.qb * 2 * p.tpb;
+          d.pos0 = w.u.row.L + w.u.qb * 2 * p.a.tpb;
           d.c0 = w.u.c0;
           d.c1 = w.u.c1;
-          d.tok = w.u.row.tok0 + w.u.qb * 2 * p.tpb;
+          d.tok = w.u.row.tok0 + w.u.qb * 2 * p.a.tpb;
           d.h = w.h;
           d.part = whole ? -1 : k > 0 ? 1 : 0;
           d.pad[0] = d.pad[1] = 0;
@@ -615,7 +620,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
 #pragma unroll
             for (int pn = 0; pn < Cfg::kPanels; ++pn)
               tma_load_3d(smem + t * Cfg::kTileBytes + pn * kPcTile * 128, &qmap, q_full, pn * 64, w.h * p.a.G,
-                          d.tok + t * p.tpb, pol);
+                          d.tok + t * p.a.tpb, pol);
         }
         __syncwarp();
         ++k;
@@ -789,10 +794,12 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const int cnt_tok = t ? d.c1 : d.c0;
       const int jb = t ? d.b1 : d.b0, je = t ? d.e1 : d.e0;
       const bool valid = rt < cnt_tok;             // (rows past tpb * G have rt >= tpb)
-      const int pos0 = d.pos0 + t * p.tpb, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
+      const int pos0 = d.pos0 + t * p.a.tpb, pos1 = pos0 + cnt_tok - 1;  // the tile's positions
       const int see_hi = min(pos0 + rt, d.hi), see_lo = p.a.window >= 0 ? pos0 + rt - p.a.window : 0;
       // 64 keys starting in [full_lo, full_hi] are seen whole by every row
       const int full_hi = min(pos0, d.hi) - 63, full_lo = p.a.window >= 0 ? pos1 - p.a.window : 0;
+      // ... and 64 keys starting outside [some_lo, some_hi] by none
+      const int some_hi = min(pos1, d.hi), some_lo = p.a.window >= 0 ? pos0 - p.a.window - 63 : 0;
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
       bool all_m = !warp_rows;  // every row here has an m
@@ -832,8 +839,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             mbar_arrive(my_p);
             continue;
           }
-          const bool full = kt >= full_lo && kt <= full_hi;
-          float mx = tmem_prep(s_addr, !full, max(0, see_lo - kt), valid ? min(64, see_hi - kt + 1) : 0) * sc;
+          const bool full = kt >= full_lo && kt <= full_hi, none = kt < some_lo || kt > some_hi;
+          float mx = -INFINITY;
+          if (!none) mx = tmem_prep(s_addr, !full, max(0, see_lo - kt), valid ? min(64, see_hi - kt + 1) : 0) * sc;
           if (!all_m) {
             // (the same in both warps, which are both at their tile j: no product of O is in flight)
             mx = fmaxf(mx, exchange(mx));
@@ -849,6 +857,14 @@ __global__ void __launch_bounds__(kPcThreads, 1)
               exchange(0.f);  // both halves of O are scaled before either P can be used
             }
             if (!ok) break;
+          }
+          if (none) {
+            tmem_zero32(s_addr);
+            tc_fence_before();
+            mbar_arrive(my_p);
+            __syncwarp();
+            if (lane == 0) progress[hh] = 2 * s_cnt + 2;
+            continue;
           }
           tmem_ld32_nowait(s_addr, a);  // (masked)
         }
@@ -952,7 +968,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (d.part >= 0 && valid && hh == 0)
           p.a.part_lse[slot * 256 + t * 128 + row] = l == 0.f ? -INFINITY : m_used + __log2f(l);
         if (cnt > 0) {
-          const int orow = valid ? (d.tok + t * p.tpb + rt) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G) : -1;
+          const int orow = valid ? (d.tok + t * p.a.tpb + rt) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G) : -1;
           float* part = d.part < 0 ? nullptr
                                    : p.a.part_o + ((slot * (D / 4) + hh * (D / 8)) * 256 + t * 128 + row) * 4;
           chunk_store<D / 2>(o_addr + hh * (D / 2), inv, orow, p.a.out + hh * (D / 2), D, part);
@@ -989,8 +1005,8 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedChunkPara
   if (c.h < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = blockIdx.y * 32 + lane, rr = n & 127;
-  const int rt = rr / p.a.G, tok = c.tok0 + (n >> 7) * p.tpb + rt;
-  const bool valid = rt < p.tpb && tok < c.tok1;
+  const int rt = rr / p.a.G, tok = c.tok0 + (n >> 7) * p.a.tpb + rt;
+  const bool valid = rt < p.a.tpb && tok < c.tok1;
   if (!__syncthreads_or(valid)) return;
   const int cnt = c.g_last - static_cast<int>(blockIdx.x) + 1;
   auto slot = [&](int k) { return (static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 && c.slot1 ? 1 : 0); };

@@ -16,11 +16,13 @@
 // Per CTA a producer warp streams K and V tiles by TMA into a ring that is never drained between
 // units: one 4-D box {64 columns, box positions, D / 64 panels, 1} a page chunk, box = min(page, 64),
 // from the maps {64, page, D / 64, n_pages Hkv} over the pool -- a contiguous block, since a head's
-// page is one.  The warp's lanes hold the next 32 chunks' page numbers.  Four consumer warps take
-// 16 keys of every tile each, on the tensor cores with keys on the M side (mma.sync m16n8k16):
+// page is one.  The warp's lanes hold the next 32 chunks' page numbers.  Two groups of four consumer
+// warps take turns at the tiles (a tile is a chain of dependent steps: 16 SMs reach 56 GB/s each
+// with one group, 76 with two; one where registers would spill, 16 rows of 128, and at 64, where
+// three CTAs share an SM), 16 keys a warp, on the tensor cores with keys on the M side (mma.sync m16n8k16):
 //   S^T(16 keys x 8 rows) = K(16 x D) Q^T,  O^T(D x 8 rows) += V^T(D x 16 keys) P^T
 // with an online softmax in fp32 a warp, P rounded to bf16 for the product (its sum l is of the
-// unrounded values), and a merge of the four through shared memory after each unit.
+// unrounded values), and a merge of the eight through shared memory after each unit.
 //
 // Positions of a tile outside [lo, hi] may hold anything (another request's old values, NaN): their
 // scores are replaced by -inf and their value rows are zeroed in shared memory, since 0 * NaN is NaN.
@@ -48,6 +50,7 @@ struct PagedAttnParams {
   int few_rows;                // requests of at most this many query rows a kv head go to the decode kernel
   int all;                     // decode kernel: take every request (the chunk kernel is not launched)
   int fill;                    // this launch zeroes the padding tokens' output
+  int tpb;                     // chunk kernel: tokens a query tile
   float scale_log2;            // softmax_scale * log2(e)
 };
 
@@ -73,11 +76,10 @@ __device__ __forceinline__ bool paged_row_fits(const PagedAttnParams& p, int r, 
 }
 
 constexpr int kPdTile = 64;  // keys a tile
-constexpr int kPdWarps = 4;  // consumer warps, 16 keys of a tile each
-constexpr int kPdThreads = (kPdWarps + 1) * 32;
-
-template <int D, int NQT, int STAGES>
+template <int D, int NQT, int STAGES, int GROUPS>
 struct PagedDecodeConfig {
+  static constexpr int WARPS = 4 * GROUPS;           // consumer warps
+  static constexpr int THREADS = (WARPS + 1) * 32;   // and the producer's
   static constexpr int kRows = 8 * NQT;
   static constexpr int NPANEL = D / 64;
   static constexpr int TILE_BYTES = kPdTile * D * 2;
@@ -85,13 +87,15 @@ struct PagedDecodeConfig {
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int OPITCH = D + 4;
   static constexpr int MERGE_OFFSET = RING_BYTES;
-  static constexpr int MERGE_BYTES = 2 * kPdWarps * kRows * OPITCH * 4;  // two copies, by unit parity
+  static constexpr int MERGE_BYTES = WARPS * kRows * OPITCH * 4;
   static constexpr int STAT_OFFSET = MERGE_OFFSET + MERGE_BYTES;
-  static constexpr int STAT_BYTES = 2 * 2 * kPdWarps * kRows * 4;
+  static constexpr int STAT_BYTES = 2 * WARPS * kRows * 4;
   static constexpr int BAR_OFFSET = STAT_OFFSET + STAT_BYTES;
   static constexpr int SCAN_OFFSET = BAR_OFFSET + 2 * STAGES * 8;
   static constexpr int CTL_OFFSET = SCAN_OFFSET + 33 * 8;
   static constexpr int SMEM_BYTES = CTL_OFFSET + 64 + 1024;
+  // a stage always holds the same group's tiles: its phases are then all waited for by that group
+  static_assert(STAGES % GROUPS == 0, "whole turns");
   static_assert(BAR_OFFSET % 8 == 0 && SCAN_OFFSET % 8 == 0, "alignment");
 };
 
@@ -124,8 +128,15 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedAttnParams& p, const 
   return u;
 }
 
-__device__ __forceinline__ long long share_begin(int c, long long total, int ng) { return c * total / ng; }
+// CTA c's share of `total` tiles among ng <= 1,024 CTAs begins at c total / ng; the CTA whose share
+// holds tile t.  (In 32 bits where they do: a 64-bit division is a hundred dependent instructions.)
+__device__ __forceinline__ long long share_begin(int c, long long total, int ng) {
+  if (total < (1 << 21)) return static_cast<uint32_t>(c) * static_cast<uint32_t>(total) / static_cast<uint32_t>(ng);
+  return c * total / ng;
+}
 __device__ __forceinline__ int share_owner(long long t, long long total, int ng) {
+  if (total < (1 << 21))
+    return static_cast<int>((static_cast<uint32_t>(t + 1) * static_cast<uint32_t>(ng) - 1) / static_cast<uint32_t>(total));
   return static_cast<int>(((t + 1) * ng - 1) / total);
 }
 
@@ -222,11 +233,12 @@ __device__ __forceinline__ void paged_merge(const float* part_o, const float* pa
     *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
 }
 
-template <int D, int NQT, int STAGES>
-__global__ void __launch_bounds__(kPdThreads)
+template <int D, int NQT, int STAGES, int GROUPS>
+__global__ void __launch_bounds__(PagedDecodeConfig<D, NQT, STAGES, GROUPS>::THREADS)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const PagedAttnParams p) {
-  using C = PagedDecodeConfig<D, NQT, STAGES>;
+  using C = PagedDecodeConfig<D, NQT, STAGES, GROUPS>;
+  constexpr int WARPS = C::WARPS;
   constexpr int ROWS = C::kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -236,14 +248,14 @@ __global__ void __launch_bounds__(kPdThreads)
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::BAR_OFFSET);
   uint64_t* empty_bar = full_bar + STAGES;
   unsigned long long* scan = reinterpret_cast<unsigned long long*>(smem + C::SCAN_OFFSET);
-  int* ctl = reinterpret_cast<int*>(smem + C::CTL_OFFSET);  // abort, start r, qb, h, local, last x 2
+  int* ctl = reinterpret_cast<int*>(smem + C::CTL_OFFSET);  // abort; start r, qb, h, local, tok0, T, L; last
   volatile int* abort_flag = ctl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], kPdWarps);
+      mbar_init(&empty_bar[s], 4);
     }
     ctl[0] = 0;
     fence_mbarrier_init();
@@ -254,7 +266,7 @@ __global__ void __launch_bounds__(kPdThreads)
   pdl_launch_dependents();
 
   // ---- the sequence's length, and the unit holding this CTA's first tile ----
-  const int per = (p.R + kPdThreads - 1) / kPdThreads;
+  const int per = (p.R + C::THREADS - 1) / C::THREADS;
   const int row_a = min(static_cast<int>(threadIdx.x) * per, p.R), row_b = min(row_a + per, p.R);
   long long mine = 0;
   for (int r = row_a; r < row_b; ++r) {
@@ -279,10 +291,14 @@ __global__ void __launch_bounds__(kPdThreads)
       for (int qb = 0; qb < nqb; ++qb) {
         const int n = paged_unit<ROWS>(p, x, r, qb, nqb).n;
         if (left < static_cast<long long>(n) * p.Hkv) {
+          const int at = static_cast<int>(left);  // < n * Hkv
           ctl[1] = r;
           ctl[2] = qb;
-          ctl[3] = static_cast<int>(left / n);
-          ctl[4] = static_cast<int>(left % n);
+          ctl[3] = at / n;
+          ctl[4] = at % n;
+          ctl[5] = x.tok0;
+          ctl[6] = x.T;
+          ctl[7] = x.L;
           found = true;
           break;
         }
@@ -293,7 +309,7 @@ __global__ void __launch_bounds__(kPdThreads)
   __syncthreads();
   PagedWalk w;
   {
-    const PagedRow x = paged_row(p, ctl[1]);
+    const PagedRow x = {ctl[5], ctl[6], ctl[7]};
     w.u = paged_unit<ROWS>(p, x, ctl[1], ctl[2], paged_blocks<ROWS>(p, x));
     w.h = ctl[3];
     w.local = ctl[4];
@@ -303,7 +319,7 @@ __global__ void __launch_bounds__(kPdThreads)
   const int box = 1 << box_shift;
   const uint32_t panel_bytes = static_cast<uint32_t>(box) * 128u;
 
-  if (warp == kPdWarps) {
+  if (warp == WARPS) {
     // ---------------- producer warp ----------------
     const uint64_t policy = l2_policy_evict_first();
     const int nch = kPdTile >> box_shift;  // chunks a tile
@@ -361,8 +377,9 @@ __global__ void __launch_bounds__(kPdThreads)
     return static_cast<uint32_t>(row >> box_shift) * panel_bytes * C::NPANEL +
            static_cast<uint32_t>(row & (box - 1)) * 128u;
   };
-  const int krow = warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-  const int vrow = warp * 16 + (lane & 7) + (lane >> 4) * 8;
+  const int part = warp & 3;  // of the tile: keys part * 16 .. +15
+  const int krow = part * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+  const int vrow = part * 16 + (lane & 7) + (lane >> 4) * 8;
   const uint32_t koff = row_offset(krow), voff = row_offset(vrow);
   const uint32_t swz = static_cast<uint32_t>(lane & 7) << 4;
   uint32_t g = 0;
@@ -391,7 +408,6 @@ __global__ void __launch_bounds__(kPdThreads)
     const bool complete = w.local == 0 && seg == u.n;
     const int slot = seg_index == 0 ? 0 : 1;
     const int nvalid = u.r1 - u.r0;
-    const int par = seg_index & 1;
 
     float m_run[NQT][2], l_run[NQT][2], o_acc[NQT][D / 16][4];
     int row_hi[NQT][2], row_lo[NQT][2];
@@ -413,6 +429,7 @@ __global__ void __launch_bounds__(kPdThreads)
     }
 
     for (int i = 0; i < seg; ++i, ++g) {
+      if ((g & (GROUPS - 1)) != static_cast<uint32_t>(warp >> 2)) continue;  // the other group's tile
       const int s = g % STAGES;
       if (mbar_wait_or_abort(&full_bar[s], (g / STAGES) & 1, abort_flag)) {
         const uint32_t kbase = smem_u32(smem + s * C::STAGE_BYTES);
@@ -421,7 +438,7 @@ __global__ void __launch_bounds__(kPdThreads)
         const bool edge = tile0 < u.lo || tile0 + kPdTile - 1 > u.hi;
         if (edge) {
           // value rows outside [lo, hi] to zero (this warp's 16 rows; two lanes a row)
-          const int row = warp * 16 + (lane >> 1);
+          const int row = part * 16 + (lane >> 1);
           if (tile0 + row < u.lo || tile0 + row > u.hi) {
             const uint32_t at = vbase + row_offset(row);
 #pragma unroll
@@ -431,20 +448,24 @@ __global__ void __launch_bounds__(kPdThreads)
           fence_proxy_async_shared();  // TMA refills this stage later
           __syncwarp();
         }
-        float sc[NQT][4];
+        float sc[NQT][4], sd[NQT][4];  // even and odd steps: two dependent chains instead of one
 #pragma unroll
         for (int j = 0; j < NQT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sc[j][c] = 0.f;
+          for (int c = 0; c < 4; ++c) sc[j][c] = sd[j][c] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t chunk = ((kk & 3) * 2 + (lane >> 4)) << 4;
           uint32_t a0, a1, a2, a3;
           ldsm_x4(kbase + koff + (kk >> 2) * panel_bytes + (chunk ^ swz), a0, a1, a2, a3);
 #pragma unroll
-          for (int j = 0; j < NQT; ++j) mma_16816(sc[j], a0, a1, a2, a3, qf[j][kk][0], qf[j][kk][1]);
+          for (int j = 0; j < NQT; ++j) mma_16816(kk & 1 ? sd[j] : sc[j], a0, a1, a2, a3, qf[j][kk][0], qf[j][kk][1]);
         }
-        const int key = tile0 + warp * 16 + (lane >> 2);
+#pragma unroll
+        for (int j = 0; j < NQT; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[j][c] += sd[j][c];
+        const int key = tile0 + part * 16 + (lane >> 2);
 #pragma unroll
         for (int j = 0; j < NQT; ++j) {
 #pragma unroll
@@ -502,11 +523,11 @@ __global__ void __launch_bounds__(kPdThreads)
       load_q(wn, qf);
     }
 
-    // ---- merge the four warps' states; the buffers alternate by unit parity, so one barrier a
-    // unit suffices (a warp writes a copy again only after the next unit's barrier) ----
-    float* mbuf = merge + par * (kPdWarps * ROWS * C::OPITCH);
-    float* st_m = stat + par * (2 * kPdWarps * ROWS);
-    float* st_l = st_m + kPdWarps * ROWS;
+    // ---- merge the warps' states ----
+    float* mbuf = merge;
+    float* st_m = stat;
+    float* st_l = st_m + WARPS * ROWS;
+    if (seg_index > 0) named_barrier(1, WARPS * 32);  // the last unit's have been read
 #pragma unroll
     for (int j = 0; j < NQT; ++j)
 #pragma unroll
@@ -529,19 +550,19 @@ __global__ void __launch_bounds__(kPdThreads)
           dst[d + 8] = o_acc[j][db][e + 2];
         }
       }
-    named_barrier(1, kPdWarps * 32);
+    named_barrier(1, WARPS * 32);
     auto row_out = [&](int n) {
       const int r = u.r0 + n;
       return p.out + (static_cast<long long>(u.row.tok0 + r / p.G) * p.Hq + w.h * p.G + r % p.G) * D;
     };
-    for (int idx = threadIdx.x; idx < nvalid * D; idx += kPdWarps * 32) {
+    for (int idx = threadIdx.x; idx < nvalid * D; idx += WARPS * 32) {
       const int n = idx / D, d = idx - n * D;
       float mmax = -CUDART_INF_F;
 #pragma unroll
-      for (int ww = 0; ww < kPdWarps; ++ww) mmax = fmaxf(mmax, st_m[ww * ROWS + n]);
+      for (int ww = 0; ww < WARPS; ++ww) mmax = fmaxf(mmax, st_m[ww * ROWS + n]);
       float ltot = 0.f, o = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < kPdWarps; ++ww) {
+      for (int ww = 0; ww < WARPS; ++ww) {
         const float mw = st_m[ww * ROWS + n];
         const float f = mw == -CUDART_INF_F ? 0.f : fast_exp2((mw - mmax) * p.scale_log2);
         ltot = fmaf(st_l[ww * ROWS + n], f, ltot);
@@ -558,18 +579,18 @@ __global__ void __launch_bounds__(kPdThreads)
     }
     if (!complete) {
       // the barrier orders every thread's stores before thread 0's release of the counter
-      named_barrier(1, kPdWarps * 32);
+      named_barrier(1, WARPS * 32);
       const long long start = w.t - w.local;  // the unit's first tile
       const int g_first = share_owner(start, total, ng), g_last = share_owner(start + u.n - 1, total, ng);
       if (threadIdx.x == 0) {
         int* counter = p.counters + g_first;
         const bool last = atom_add_acq_rel_gpu(counter, 1) == g_last - g_first;
         if (last) *counter = 0;  // every contributor has arrived: ready for the next call
-        ctl[5 + par] = last;
+        ctl[8] = last;
       }
-      named_barrier(1, kPdWarps * 32);
-      if (ctl[5 + par])
-        for (int n = warp; n < nvalid; n += kPdWarps)
+      named_barrier(1, WARPS * 32);
+      if (ctl[8])
+        for (int n = warp; n < nvalid; n += WARPS)
           paged_merge<D, ROWS>(p.part_o, p.part_lse, g_first, g_last, start != share_begin(g_first, total, ng), n,
                                row_out);
     }
