@@ -398,6 +398,63 @@ def test_large_scores_and_a_given_scale(ops):
     check_attn(ops, [130, 700], [1, 90], 8, 2, 64, 32, -1, scale=1e-4)
 
 
+SPIKES = {
+    # score of key c when q's first element is +1 (integers exact in bf16, times the scale)
+    "one key of a first half": lambda c: 60.0 * (c == 390),
+    "one key of a second half": lambda c: 60.0 * (c == 450),
+    "a jump inside a first half": lambda c: 60.0 * (c >= 400),
+    "a jump inside a second half": lambda c: 60.0 * (c >= 500),
+    "a step every 64 keys": lambda c: 40.0 * (c // 64),
+    "a step every 128 keys": lambda c: 40.0 * (c // 128),
+    "up and down": lambda c: 50.0 * ((c // 64) % 3),
+    "the last keys of the cache": lambda c: 60.0 * (c >= 636),
+}
+
+
+@pytest.mark.parametrize("pattern", SPIKES)
+@pytest.mark.parametrize("D,G,fresh", [(128, 4, 100), (64, 1, 300), (128, 8, 1), (64, 4, 5)])
+def test_scores_that_leap_by_hundreds(ops, pattern, D, G, fresh):
+    """Far more than an exponential's range between one block of keys and the next: every running
+    reference has to move, for some rows and not for others (q's first element is +1, 0 or -1)."""
+    cached = 640
+    c, ks, vs = attn_case([cached], [fresh], 2 * G, 2, D, 64, seed=3)
+    key = torch.arange(cached + fresh, device="cuda")
+    ks[0][..., 0] = SPIKES[pattern](key).to(torch.bfloat16)[:, None]
+    sign = (torch.arange(fresh, device="cuda") % 3 - 1).to(torch.bfloat16)[:, None]
+    q = c["q"].contiguous().mul(0.25)
+    q[..., 0] = sign
+    page = c["table"][0].long()
+    c["kp"][page[key // 64], :, key % 64] = ks[0]
+    scale = 8.0
+    want, bound = attn_ref(q, ks, vs, [cached], [fresh], -1, scale)
+    got = ops.paged_attn(q, c["kp"], c["vp"], c["table"], c["cached"], c["cu"], softmax_scale=scale)
+    err = np.abs(got.double().cpu().numpy() - want)
+    # a score of s = 480 is a sum of fp32 products: off by up to s 2^-20, its weight by that relatively
+    slack = (2.25 * U + 8.0 * 480 * 2.0 ** -20) * bound
+    assert np.isfinite(err).all() and (err <= slack).all(), (err - slack).max()
+
+
+@pytest.mark.parametrize("D,G,fresh", [(128, 4, 200), (64, 1, 300), (128, 4, 1), (64, 12, 1)])
+def test_what_a_row_sees_reaches_it(ops, D, G, fresh):
+    """A NaN key makes the rows that see it NaN and no others; an infinite value is infinite there."""
+    cached = 300
+    for at, what in ((100, "k"), (310, "k"), (20, "v"), (299, "v")):
+        if at >= cached + fresh:
+            continue
+        c, ks, vs = attn_case([cached, 50], [fresh, 3], 2 * G, 2, D, 32, seed=at)
+        page = c["table"][0].long()
+        pool = c["kp"] if what == "k" else c["vp"]
+        pool[page[at // 32], :, at % 32] = float("nan") if what == "k" else float("inf")
+        got = ops.paged_attn(c["q"], c["kp"], c["vp"], c["table"], c["cached"], c["cu"]).float()
+        sees = torch.arange(cached, cached + fresh, device="cuda") >= at
+        assert got[fresh:].isfinite().all()
+        if what == "k":
+            assert torch.equal(got[:fresh].isnan().all(-1).all(-1), sees)
+            assert got[:fresh][~sees].isfinite().all()
+        else:
+            assert (got[:fresh][sees] == float("inf")).all()
+
+
 def test_pages_beyond_32_bit_offsets(ops):
     """A pool of more than 2^31 elements, the requests' pages at its end."""
     pages = (1 << 31) // (2 * 64 * 128) + 200
