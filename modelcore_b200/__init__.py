@@ -2,6 +2,7 @@
 
 Public surface (mirrors modelcore's names for this path):
   KVCache                   modelcore.cache.KVCache on the B200 layout and kernels
+  PagedKVCache              a cache in pages for requests of any length (continuous batching)
   flash_attn                namespace with flash_attn_with_kvcache (modelcore.kernels.flash_attn's)
   flash_attn_with_kvcache   insert + split-K decode attention
   ModelManager              modelcore.ModelManager with the decode path installed (needs modelcore)
@@ -17,9 +18,10 @@ here has a CPU or pure-Python fallback.
 from . import _native, ops
 from .cache import KVCache
 from .flash_attn import flash_attn, flash_attn_with_kvcache
+from .paged import PagedKVCache
 from .sampling import sample_next_token
 
-__all__ = ["KVCache", "flash_attn", "flash_attn_with_kvcache", "ModelManager", "install",
+__all__ = ["KVCache", "PagedKVCache", "flash_attn", "flash_attn_with_kvcache", "ModelManager", "install",
            "uninstall", "GraphDecoder", "sample_next_token", "ops"]
 
 

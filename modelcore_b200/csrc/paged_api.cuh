@@ -181,12 +181,15 @@ int paged_append(const mcb_paged_append_args* a, void* stream) {
   p.scale = a->scale;
   p.nk = kv ? a->Hkv : 0;
   p.rotate_k = a->rotate_k != 0;
-  p.total_vectors = static_cast<long long>(a->N) * (p.Hq + 2ll * p.nk);
-  if (p.total_vectors > INT32_MAX)
-    return fail(MCB_ERR_UNSUPPORTED, "%s: %lld vectors in one call (at most 2^31 - 1)", who, p.total_vectors);
-  const long long vpw = 32 / (a->D / 16), wpb = mcb::kAppendVecThreads / 32;
-  const long long blocks = std::min<long long>((p.total_vectors + vpw * wpb - 1) / (vpw * wpb),
-                                               static_cast<long long>(kAppendVecCtasPerSm) * device_sm_count());
+  const long long heads = p.Hq + 2ll * p.nk, vpw = 32 / (a->D / 16), steps = (heads + vpw - 1) / vpw;
+  if (static_cast<long long>(a->N) * heads > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: %lld vectors in one call (at most 2^31 - 1)", who,
+                static_cast<long long>(a->N) * heads);
+  // a warp a token once tokens fill the resident warps; before that its heads over several
+  const long long wpb = mcb::kAppendVecThreads / 32;
+  const long long resident = static_cast<long long>(kAppendVecCtasPerSm) * device_sm_count();
+  p.parts = static_cast<int>(std::clamp<long long>(resident * wpb / a->N, 1, steps));
+  const long long blocks = std::min<long long>((static_cast<long long>(a->N) * p.parts + wpb - 1) / wpb, resident);
   const dim3 grid(static_cast<unsigned>(blocks)), block(mcb::kAppendVecThreads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;

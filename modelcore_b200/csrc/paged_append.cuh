@@ -8,10 +8,13 @@
 // and one rounding at the end.
 // K page layout (n_pages, Hkv, page, D): slot s is position s % page of page s / page.
 //
-// D/16 lanes a vector, 16-byte loads and stores, grid-stride over groups of vectors, two groups'
-// loads in flight before either's arithmetic: kv_append_rope_vec_kernel's shape.  Bound by HBM
-// (each byte read and written once) for long batches, by launch and dependent-load latency for
-// a decode step.
+// A warp takes a token (or, for few tokens, one of `parts` shares of its heads): the position, the
+// slot and the rotary row are read once for all its heads -- a lane keeps the same 16 table values --
+// and the heads go by in steps of 32 / (D/16) vectors, D/16 lanes each, the next step's loads in flight.
+// With a vector's position and table row read per vector the two dependent loads ahead of every
+// vector bounded it.  16,381 tokens of 16/4 heads of 128 (206 MB): 43 us so, 40 us now, 5.2 TB/s; two
+// or more steps in flight cost registers and with them warps (44 to 65 us).  Bound by HBM (each
+// byte read and written once) for long batches, by launch and dependent-load latency for a decode step.
 #pragma once
 
 #include "common.cuh"
@@ -36,7 +39,7 @@ struct PagedAppendParams {
   float eps, scale;
   int nk;                         // key (and value) vectors a token: Hkv, or 0 without k and v
   int rotate_k;
-  long long total_vectors;
+  int parts;                      // warps a token
 };
 
 // rope_norm_vec_tab with every step in fp32 and one rounding: products and sums fused.
@@ -77,95 +80,67 @@ __device__ __forceinline__ void rope_norm_vec_once(const uint4& x1v, const uint4
   }
 }
 
-struct PagedVec {
-  int j, pos;
-  long long slot;
-  int t;
-  bool active;
-  uint4 x1v, x2v, cv, sv;
-};
-
-template <int D>
-__device__ __forceinline__ void paged_vec_load(const PagedAppendParams& p, long long w, int sub, PagedVec& r) {
-  constexpr int HALF = D / 2;
-  r.active = w < p.total_vectors;
-  const unsigned wv = r.active ? static_cast<unsigned>(w) : 0u;  // total_vectors < 2^31 (host)
-  const unsigned per = static_cast<unsigned>(p.Hq + 2 * p.nk);
-  r.t = static_cast<int>(wv / per);
-  r.j = static_cast<int>(wv - static_cast<unsigned>(r.t) * per);
-  const bool is_q = r.j < p.Hq, is_k = !is_q && r.j < p.Hq + p.nk;
-  const uint16_t* src = is_q ? p.q + r.t * p.qs[0] + r.j * p.qs[1]
-                       : is_k ? p.k + r.t * p.ks[0] + (r.j - p.Hq) * p.ks[1]
-                              : p.v + r.t * p.vs[0] + (r.j - p.Hq - p.nk) * p.vs[1];
-  r.pos = p.positions[r.t];
-  r.slot = is_q ? 0 : p.slot_map[r.t];
-  r.x1v = *reinterpret_cast<const uint4*>(src + 8 * sub);
-  r.x2v = *reinterpret_cast<const uint4*>(src + HALF + 8 * sub);
-}
-
-template <int D>
-__device__ __forceinline__ void paged_vec_tables(const PagedAppendParams& p, int sub, PagedVec& r) {
-  r.cv = r.sv = make_uint4(0, 0, 0, 0);
-  const bool is_v = r.j >= p.Hq + p.nk;
-  if (r.active && !is_v && r.pos >= 0 && r.pos < p.rot_len) {
-    const long long row = static_cast<long long>(r.pos) * (D / 2) + 8 * sub;
-    r.cv = *reinterpret_cast<const uint4*>(p.cos + row);
-    r.sv = *reinterpret_cast<const uint4*>(p.sin + row);
-  }
-}
-
-template <int D, bool EACH>
-__device__ __forceinline__ void paged_vec_store(const PagedAppendParams& p, const PagedVec& r, int sub) {
-  constexpr int HALF = D / 2;
-  const bool is_q = r.j < p.Hq, is_k = !is_q && r.j < p.Hq + p.nk;
-  const bool turn = is_q || (is_k && p.rotate_k);
-  bool rot_ok = r.pos >= 0;
-  if (r.active && turn && r.pos >= p.rot_len) {
-    if (sub == 0) record_error(kErrPositionBeyondRotary);
-    rot_ok = false;
-  }
-  const bool rotate = r.active && turn && rot_ok;
-  uint4 w1, w2;  // every lane takes part in the butterfly
-  if constexpr (EACH) rope_norm_vec_tab<D>(r.x1v, r.x2v, r.cv, r.sv, rotate, p.eps, p.scale, w1, w2);
-  else rope_norm_vec_once<D>(r.x1v, r.x2v, r.cv, r.sv, rotate, p.eps, p.scale, w1, w2);
-  if (!r.active) return;
-  uint16_t* dst;
-  if (is_q) {
-    if (!rotate) w1 = w2 = make_uint4(0, 0, 0, 0);  // a padding token
-    dst = p.q_out + (static_cast<long long>(r.t) * p.Hq + r.j) * D;
-  } else {
-    if (r.slot < 0 || (turn && !rot_ok)) return;
-    if (r.slot >= p.n_slots) {
-      if (sub == 0) record_error(kErrPageOutOfRange);
-      return;
-    }
-    const int h = is_k ? r.j - p.Hq : r.j - p.Hq - p.nk;
-    const long long page = r.slot >> p.page_shift;
-    const long long row = ((page * p.Hkv + h) << p.page_shift) + (r.slot & ((1ll << p.page_shift) - 1));
-    dst = (is_k ? p.k_pages : p.v_pages) + row * D;
-  }
-  *reinterpret_cast<uint4*>(dst + 8 * sub) = w1;
-  *reinterpret_cast<uint4*>(dst + HALF + 8 * sub) = w2;
-}
-
 template <int D, bool EACH>
 __global__ void __launch_bounds__(kAppendVecThreads, 4) paged_append_kernel(const PagedAppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int L = D / 16, VPW = 32 / L;
+  constexpr int L = D / 16, VPW = 32 / L, HALF = D / 2;
   const int lane = threadIdx.x & 31, sub = lane % L;
-  const long long stride = static_cast<long long>(gridDim.x) * (kAppendVecThreads / 32) * VPW;
-  const long long first =
-      (static_cast<long long>(blockIdx.x) * (kAppendVecThreads / 32) + (threadIdx.x >> 5)) * VPW;
-  constexpr int U = 2;
-  for (long long base = first; base < p.total_vectors; base += U * stride) {  // warp-uniform
-    PagedVec v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) paged_vec_load<D>(p, base + u * stride + lane / L, sub, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) paged_vec_tables<D>(p, sub, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) paged_vec_store<D, EACH>(p, v[u], sub);
+  const int heads = p.Hq + 2 * p.nk;
+  const long long items = static_cast<long long>(p.N) * p.parts;
+  const long long warps = static_cast<long long>(gridDim.x) * (kAppendVecThreads / 32);
+  for (long long item = static_cast<long long>(blockIdx.x) * (kAppendVecThreads / 32) + (threadIdx.x >> 5);
+       item < items; item += warps) {
+    const int t = static_cast<int>(item / p.parts), part = static_cast<int>(item - static_cast<long long>(t) * p.parts);
+    const int pos = p.positions[t];
+    const long long slot = p.nk > 0 ? p.slot_map[t] : -1;
+    auto load = [&](int j, uint4& x1, uint4& x2) {
+      x1 = x2 = make_uint4(0, 0, 0, 0);
+      if (j >= heads) return;
+      const uint16_t* src = j < p.Hq          ? p.q + t * p.qs[0] + j * p.qs[1]
+                            : j < p.Hq + p.nk ? p.k + t * p.ks[0] + (j - p.Hq) * p.ks[1]
+                                              : p.v + t * p.vs[0] + (j - p.Hq - p.nk) * p.vs[1];
+      x1 = *reinterpret_cast<const uint4*>(src + 8 * sub);
+      x2 = *reinterpret_cast<const uint4*>(src + HALF + 8 * sub);
+    };
+    const int step = p.parts * VPW;
+    int j = part * VPW + lane / L;
+    uint4 x1, x2;
+    load(j, x1, x2);
+    const bool rot_ok = pos >= 0 && pos < p.rot_len;
+    if (pos >= p.rot_len && part == 0 && lane == 0) record_error(kErrPositionBeyondRotary);
+    const bool slot_ok = slot >= 0 && slot < p.n_slots;
+    if (slot >= p.n_slots && part == 0 && lane == 0) record_error(kErrPageOutOfRange);
+    uint4 cv = make_uint4(0, 0, 0, 0), sv = cv;
+    if (rot_ok) {
+      const long long row = static_cast<long long>(pos) * HALF + 8 * sub;
+      cv = *reinterpret_cast<const uint4*>(p.cos + row);
+      sv = *reinterpret_cast<const uint4*>(p.sin + row);
+    }
+    // the slot's row for head 0; a head further is one page of one head further
+    const long long slot_row = ((slot >> p.page_shift) * p.Hkv << p.page_shift) + (slot & ((1ll << p.page_shift) - 1));
+#pragma unroll 1
+    for (int j0 = part * VPW; j0 < heads; j0 += step, j += step) {  // warp-uniform
+      const uint4 a = x1, b = x2;
+      if (j0 + step < heads) load(j + step, x1, x2);
+      const bool is_q = j < p.Hq, is_k = !is_q && j < p.Hq + p.nk;
+      const bool turn = is_q || (is_k && p.rotate_k);
+      uint4 w1, w2;  // every lane takes part in the butterfly
+      if constexpr (EACH) rope_norm_vec_tab<D>(a, b, cv, sv, turn && rot_ok, p.eps, p.scale, w1, w2);
+      else rope_norm_vec_once<D>(a, b, cv, sv, turn && rot_ok, p.eps, p.scale, w1, w2);
+      if (j >= heads) continue;
+      uint16_t* dst;
+      if (is_q) {
+        if (!rot_ok) w1 = w2 = make_uint4(0, 0, 0, 0);  // a padding token
+        dst = p.q_out + (static_cast<long long>(t) * p.Hq + j) * D;
+      } else {
+        if (!slot_ok || (turn && !rot_ok)) continue;
+        const int h = is_k ? j - p.Hq : j - p.Hq - p.nk;
+        dst = (is_k ? p.k_pages : p.v_pages) + (slot_row + (static_cast<long long>(h) << p.page_shift)) * D;
+      }
+      *reinterpret_cast<uint4*>(dst + 8 * sub) = w1;
+      *reinterpret_cast<uint4*>(dst + HALF + 8 * sub) = w2;
+    }
   }
 }
 
