@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     if (i < warp) before += warp_tot[i];
     total += warp_tot[i];
   }
-  if (p.a.fill) paged_fill(p.a, D);
+  if (p.a.fill) paged_fill(p.a, D, blockDim.x);
   const int ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   const bool active = static_cast<int>(blockIdx.x) < ng;
   const long long t_begin = active ? share_begin(blockIdx.x, total, ng) : 0;

@@ -167,61 +167,64 @@ __device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedWalk& 
   }
 }
 
-// Zeroes the output of the padding tokens, [cu_new[R], N).
-__device__ __forceinline__ void paged_fill(const PagedAttnParams& p, int D) {
+// Zeroes the output of the padding tokens, [cu_new[R], N): threads 0 .. threads - 1 of every CTA.
+__device__ __forceinline__ void paged_fill(const PagedAttnParams& p, int D, int threads) {
   const long long per = static_cast<long long>(p.Hq) * D / 8;  // 16-byte words a token
   const long long from = static_cast<long long>(min(max(p.cu_new[p.R], 0), p.N)) * per;
   uint4* out = reinterpret_cast<uint4*>(p.out);
-  for (long long i = from + static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-       i < static_cast<long long>(p.N) * per; i += static_cast<long long>(gridDim.x) * blockDim.x)
+  for (long long i = from + static_cast<long long>(blockIdx.x) * threads + threadIdx.x;
+       i < static_cast<long long>(p.N) * per; i += static_cast<long long>(gridDim.x) * threads)
     out[i] = make_uint4(0, 0, 0, 0);
 }
 
 // Merges the partials of a cut unit into its output rows, one warp a row: contributors g_first ..
-// g_last (the first one's partial is its last unit's, slot 1 unless the unit began its share).
+// g_last (the first one's partial is its last unit's, slot 1 unless the unit began its share).  Online
+// over 16 contributors at a time, their sums and values all loaded before the first is used: one trip
+// to L2 where a pass for the maximum and four values in flight made five of it (7,000 -> 1,900 cycles; the
+// 3 requests below 9.7 -> 7.2 us).
 template <int D, int ROWS, typename RowOut>
 __device__ __forceinline__ void paged_merge(const float* part_o, const float* part_lse, int g_first, int g_last,
                                             bool first_in_slot1, int n, RowOut row_out) {
   constexpr int PER_LANE = D / 32;
+  constexpr int AHEAD = 16;
   const int lane = threadIdx.x & 31;
   const int cnt = g_last - g_first + 1;
   auto at = [&](int k) {
     return (static_cast<long long>(g_first + k) * 2 + (k == 0 && first_in_slot1 ? 1 : 0)) * ROWS + n;
   };
-  float mx = -CUDART_INF_F;
-  for (int k = lane; k < cnt; k += 32) mx = fmaxf(mx, __ldcg(part_lse + at(k)));
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
-  float acc[PER_LANE], wsum = 0.f;
+  float acc[PER_LANE], wsum = 0.f, mx = -CUDART_INF_F;
 #pragma unroll
   for (int e = 0; e < PER_LANE; ++e) acc[e] = 0.f;
-  for (int k0 = 0; k0 < cnt; k0 += 32) {
-    float wk = 0.f;
-    if (k0 + lane < cnt) {
-      const float ls = __ldcg(part_lse + at(k0 + lane));
-      wk = ls == -CUDART_INF_F ? 0.f : fast_exp2(ls - mx);
+  for (int k0 = 0; k0 < cnt; k0 += AHEAD) {
+    const float ls = lane < AHEAD && k0 + lane < cnt ? __ldcg(part_lse + at(k0 + lane)) : -CUDART_INF_F;
+    float v[AHEAD][PER_LANE];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float* src = part_o + at(min(k0 + j, cnt - 1)) * D + lane * PER_LANE;  // (a weight of 0 beyond cnt)
+      if constexpr (PER_LANE == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+        v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+        v[j][0] = x.x, v[j][1] = x.y;
+      }
     }
-    const int here = min(32, cnt - k0);
-#pragma unroll 4
-    for (int j = 0; j < here; ++j) {
+    float m_new = fmaxf(mx, ls);
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, m));
+    const float alpha = mx == -CUDART_INF_F ? 1.f : fast_exp2(mx - m_new);  // (nothing summed yet)
+    const float wk = ls == -CUDART_INF_F ? 0.f : fast_exp2(ls - m_new);
+    mx = m_new;
+    wsum *= alpha;
+#pragma unroll
+    for (int e = 0; e < PER_LANE; ++e) acc[e] *= alpha;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
       const float w = __shfl_sync(0xffffffffu, wk, j);
       wsum += w;
-      const float* src = part_o + at(k0 + j) * D + lane * PER_LANE;
-      if constexpr (PER_LANE == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-        if (w != 0.f) {
-          acc[0] = fmaf(w, v.x, acc[0]);
-          acc[1] = fmaf(w, v.y, acc[1]);
-          acc[2] = fmaf(w, v.z, acc[2]);
-          acc[3] = fmaf(w, v.w, acc[3]);
-        }
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-        if (w != 0.f) {
-          acc[0] = fmaf(w, v.x, acc[0]);
-          acc[1] = fmaf(w, v.y, acc[1]);
-        }
-      }
+      if (w != 0.f)
+#pragma unroll
+        for (int e = 0; e < PER_LANE; ++e) acc[e] = fmaf(w, v[j][e], acc[e]);
     }
   }
   const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
@@ -262,59 +265,103 @@ __global__ void __launch_bounds__(PagedDecodeConfig<D, NQT, STAGES, GROUPS>::THR
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
   // ---- the sequence's length, and the unit holding this CTA's first tile ----
-  const int per = (p.R + C::THREADS - 1) / C::THREADS;
-  const int row_a = min(static_cast<int>(threadIdx.x) * per, p.R), row_b = min(row_a + per, p.R);
-  long long mine = 0;
-  for (int r = row_a; r < row_b; ++r) {
-    const PagedRow x = paged_row(p, r);
-    if (blockIdx.x == 0 && !paged_row_fits(p, r, x)) record_error(kErrPositionBeyondCache);
-    const int nqb = paged_blocks<ROWS>(p, x);
-    for (int qb = 0; qb < nqb; ++qb) mine += paged_unit<ROWS>(p, x, r, qb, nqb).n;
-  }
-  mine *= p.Hkv;
-  const long long incl = static_cast<long long>(block_scan(static_cast<unsigned long long>(mine), scan));
-  const long long total = static_cast<long long>(scan[32]);
-  if (p.fill) paged_fill(p, D);
-  const int ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  if (static_cast<int>(blockIdx.x) >= ng) return;
-  const long long t_begin = share_begin(blockIdx.x, total, ng), t_end = share_begin(blockIdx.x + 1, total, ng);
-  if (incl - mine <= t_begin && t_begin < incl) {
-    long long left = t_begin - (incl - mine);
-    bool found = false;
-    for (int r = row_a; r < row_b && !found; ++r) {
-      const PagedRow x = paged_row(p, r);
+  // Up to 32 requests every warp does it alone, a request a lane: no barrier, nothing through shared
+  // memory (3 requests of 12 heads of 64 at 500 to 1,023: 7.2 -> 6.6 us; 24 of 32/8 heads of 128: 33.0 -> 32.2); more, the CTA together.
+  PagedWalk w;
+  long long t_end;
+  int ng;
+  long long total;
+  if (p.R <= 32) {
+    PagedRow x = {0, 0, 0};
+    long long mine = 0;
+    if (lane < p.R) {
+      x = paged_row(p, lane);
+      if (blockIdx.x == 0 && warp == 0 && !paged_row_fits(p, lane, x)) record_error(kErrPositionBeyondCache);
       const int nqb = paged_blocks<ROWS>(p, x);
-      for (int qb = 0; qb < nqb; ++qb) {
-        const int n = paged_unit<ROWS>(p, x, r, qb, nqb).n;
-        if (left < static_cast<long long>(n) * p.Hkv) {
-          const int at = static_cast<int>(left);  // < n * Hkv
-          ctl[1] = r;
-          ctl[2] = qb;
-          ctl[3] = at / n;
-          ctl[4] = at % n;
-          ctl[5] = x.tok0;
-          ctl[6] = x.T;
-          ctl[7] = x.L;
-          found = true;
-          break;
-        }
-        left -= static_cast<long long>(n) * p.Hkv;
+      for (int qb = 0; qb < nqb; ++qb) mine += paged_unit<ROWS>(p, x, lane, qb, nqb).n;
+      mine *= p.Hkv;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, m);
+      if (lane >= m) incl += o;
+    }
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    if (static_cast<int>(blockIdx.x) < ng) {
+      w.t = share_begin(blockIdx.x, total, ng);
+      t_end = share_begin(blockIdx.x + 1, total, ng);
+      const int r = __ffs(__ballot_sync(0xffffffffu, w.t < incl)) - 1;  // (w.t < total: some lane's)
+      long long left = w.t - __shfl_sync(0xffffffffu, incl - mine, r);
+      x.tok0 = __shfl_sync(0xffffffffu, x.tok0, r);
+      x.T = __shfl_sync(0xffffffffu, x.T, r);
+      x.L = __shfl_sync(0xffffffffu, x.L, r);
+      const int nqb = paged_blocks<ROWS>(p, x);
+      w.u = paged_unit<ROWS>(p, x, r, 0, nqb);
+      while (left >= static_cast<long long>(w.u.n) * p.Hkv) {
+        left -= static_cast<long long>(w.u.n) * p.Hkv;
+        w.u = paged_unit<ROWS>(p, x, r, w.u.qb + 1, nqb);
       }
+      const uint32_t at = static_cast<uint32_t>(left);  // < n Hkv
+      w.h = static_cast<int>(at / static_cast<uint32_t>(w.u.n));
+      w.local = static_cast<int>(at % static_cast<uint32_t>(w.u.n));
+    }
+  } else {
+    const int per = (p.R + C::THREADS - 1) / C::THREADS;
+    const int row_a = min(static_cast<int>(threadIdx.x) * per, p.R), row_b = min(row_a + per, p.R);
+    long long mine = 0;
+    for (int r = row_a; r < row_b; ++r) {
+      const PagedRow x = paged_row(p, r);
+      if (blockIdx.x == 0 && !paged_row_fits(p, r, x)) record_error(kErrPositionBeyondCache);
+      const int nqb = paged_blocks<ROWS>(p, x);
+      for (int qb = 0; qb < nqb; ++qb) mine += paged_unit<ROWS>(p, x, r, qb, nqb).n;
+    }
+    mine *= p.Hkv;
+    const long long incl = static_cast<long long>(block_scan(static_cast<unsigned long long>(mine), scan));
+    total = static_cast<long long>(scan[32]);
+    ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    if (static_cast<int>(blockIdx.x) < ng) {
+      w.t = share_begin(blockIdx.x, total, ng);
+      t_end = share_begin(blockIdx.x + 1, total, ng);
+      if (incl - mine <= w.t && w.t < incl) {
+        long long left = w.t - (incl - mine);
+        bool found = false;
+        for (int r = row_a; r < row_b && !found; ++r) {
+          const PagedRow x = paged_row(p, r);
+          const int nqb = paged_blocks<ROWS>(p, x);
+          for (int qb = 0; qb < nqb; ++qb) {
+            const int n = paged_unit<ROWS>(p, x, r, qb, nqb).n;
+            if (left < static_cast<long long>(n) * p.Hkv) {
+              const int at = static_cast<int>(left);  // < n * Hkv
+              ctl[1] = r;
+              ctl[2] = qb;
+              ctl[3] = at / n;
+              ctl[4] = at % n;
+              ctl[5] = x.tok0;
+              ctl[6] = x.T;
+              ctl[7] = x.L;
+              found = true;
+              break;
+            }
+            left -= static_cast<long long>(n) * p.Hkv;
+          }
+        }
+      }
+      __syncthreads();
+      const PagedRow x = {ctl[5], ctl[6], ctl[7]};
+      w.u = paged_unit<ROWS>(p, x, ctl[1], ctl[2], paged_blocks<ROWS>(p, x));
+      w.h = ctl[3];
+      w.local = ctl[4];
     }
   }
-  __syncthreads();
-  PagedWalk w;
-  {
-    const PagedRow x = {ctl[5], ctl[6], ctl[7]};
-    w.u = paged_unit<ROWS>(p, x, ctl[1], ctl[2], paged_blocks<ROWS>(p, x));
-    w.h = ctl[3];
-    w.local = ctl[4];
-    w.t = t_begin;
-  }
+  if (p.fill && warp < WARPS) paged_fill(p, D, WARPS * 32);
+  if (static_cast<int>(blockIdx.x) >= ng) return;
   const int box_shift = min(p.page_shift, 6);  // positions a TMA box: min(page, 64)
   const int box = 1 << box_shift;
   const uint32_t panel_bytes = static_cast<uint32_t>(box) * 128u;
@@ -408,6 +455,12 @@ __global__ void __launch_bounds__(PagedDecodeConfig<D, NQT, STAGES, GROUPS>::THR
     const bool complete = w.local == 0 && seg == u.n;
     const int slot = seg_index == 0 ? 0 : 1;
     const int nvalid = u.r1 - u.r0;
+    const long long start = w.t - w.local;  // the unit's first tile, and who has its tiles
+    int g_first = 0, g_last = 0;
+    if (!complete) {
+      g_first = share_owner(start, total, ng);
+      g_last = share_owner(start + u.n - 1, total, ng);
+    }
 
     float m_run[NQT][2], l_run[NQT][2], o_acc[NQT][D / 16][4];
     int row_hi[NQT][2], row_lo[NQT][2];
@@ -580,8 +633,6 @@ __global__ void __launch_bounds__(PagedDecodeConfig<D, NQT, STAGES, GROUPS>::THR
     if (!complete) {
       // the barrier orders every thread's stores before thread 0's release of the counter
       named_barrier(1, WARPS * 32);
-      const long long start = w.t - w.local;  // the unit's first tile
-      const int g_first = share_owner(start, total, ng), g_last = share_owner(start + u.n - 1, total, ng);
       if (threadIdx.x == 0) {
         int* counter = p.counters + g_first;
         const bool last = atom_add_acq_rel_gpu(counter, 1) == g_last - g_first;
