@@ -185,22 +185,22 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
         const int row_len = s_len[i[u]];
         pos[u] = static_cast<long long>(row_len) + (t[u] - s_tok[i[u]]);
         const long long j = pos[u] >> p.page_shift;
-        page[u] = -1;
+        page[u] = -1;  // none: past the table or the queue, which the rows and the table entries report
         if (j < p.max_pages) {
           const int first = pages_of(row_len, p.page_shift, p.max_pages);
           const uint32_t k = s_page[i[u]] + static_cast<uint32_t>(j - first);
-          if (j < first)
-            page[u] = p.block_table[(base + i[u]) * p.table_stride + j];
-          else if (k < avail)
-            page[u] = p.free_pages[wrap(static_cast<long long>(s_head) + k, p.n_pages)];
-          if (page[u] < 0) page[u] = -2;
+          if (j < first || k < avail) {
+            page[u] = j < first ? p.block_table[(base + i[u]) * p.table_stride + j]
+                                : p.free_pages[wrap(static_cast<long long>(s_head) + k, p.n_pages)];
+            if (page[u] < 0) page[u] = p.n_pages;  // no page number: reported below
+          }
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (t0 + u * hop >= tok_end) break;
         const bool in = page[u] >= 0 && page[u] < p.n_pages;
-        if (!in && page[u] != -1) record_error(kErrPageOutOfRange);  // (a page the queue lacked: error 5 came first)
+        if (page[u] >= p.n_pages) record_error(kErrPageOutOfRange);
         p.positions[t[u]] = static_cast<int>(pos[u]);
         p.slot_map[t[u]] = in ? (static_cast<long long>(page[u]) << p.page_shift) +
                                     (pos[u] & ((1ll << p.page_shift) - 1))

@@ -173,6 +173,22 @@ def test_plan_reports_what_does_not_fit(ops, expects_device_error):
     assert ops.device_error()[0] == 7 and p.slot_map.tolist() == [0, 1, 2] and p.cu_new.tolist() == [0, 5]
     run_plan(ops, [5], [1], np.full((1, 4), -1), np.arange(20), [0, 20], 16, 1)
     assert ops.device_error()[0] == 6                                           # a held page the table lacks
+
+
+def test_plan_out_of_pages_over_many_ctas(ops, expects_device_error):
+    """The CTAs that write slots and those that write table entries meet the queue's end in any order:
+    what is reported is the queue's end, and the pages go to the first requests."""
+    R, page, have = 900, 16, 1000
+    fresh = [40] * R  # three pages each
+    for _ in range(20):
+        p, bt, _ = run_plan(ops, [0] * R, fresh, np.full((R, 4), -1), np.arange(have), [0, have], page, 40 * R)
+        assert ops.device_error()[0] == 5
+        assert p.free_state.tolist() == [have, have]
+        k = np.arange(3 * R).reshape(R, 3)
+        assert np.array_equal(bt.cpu().numpy()[:, :3], np.where(k < have, k, -1))
+        t = np.arange(40 * R)
+        k = t // 40 * 3 + t % 40 // page
+        assert np.array_equal(p.slot_map.cpu().numpy(), np.where(k < have, k * page + t % 40 % page, -1))
     ops.page_release(i32([1]), i32([40]), i32([[1, 2, 3]]), i32(np.arange(4)),
                      torch.tensor([0, 3], device="cuda"), page_size=16)
     assert ops.device_error()[0] == 5                                           # three pages into room for one
