@@ -74,7 +74,7 @@ struct PagedChunkConfig {
   static constexpr int kKOff = 2 * kTileBytes;           // Q0, Q1, then K and V, two stages each
   static constexpr int kVOff = kKOff + 2 * kTileBytes;
   static constexpr int kBarOff = kVOff + 2 * kTileBytes;
-  static constexpr int kScanOff = kBarOff + 320;
+  static constexpr int kScanOff = kBarOff + 336;
   static constexpr int kSegOff = kScanOff + 256;
   // per query tile and row quarter: what the two warps exchange (PagedPair)
   static constexpr int kPairOff = kSegOff + 4 * 64;
@@ -454,16 +454,16 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   uint64_t* v_empty = bars + 8;    // [2]
   uint64_t* s_full = bars + 10;    // [4] chain (query tile) * 2 + half
   uint64_t* p_full = bars + 14;    // [4] 128 arrivals
-  uint64_t* o_done = bars + 18;
-  uint64_t* epi_done = bars + 19;  // 512 arrivals, once a unit
+  uint64_t* o_done = bars + 18;    // [2] per query tile: a part's products are complete
+  uint64_t* epi_done = bars + 35;  // [2] 256 arrivals: ... and its O has been read
   uint64_t* drained = bars + 20;
   uint64_t* pv_end = bars + 33;    // [2] per query tile: a part's last product of the first half is complete
   // [4] a description is there.  The producer writes description x after q_empty(x - 1), so after
   // epi_done(x - 3): every softmax thread is past x - 3, and the four in the ring are never behind
   uint64_t* seg_full = bars + 21;
   uint64_t* pairs = bars + 25;     // [2][4] 2 arrivals: the two warps of a tile's row quarter
-  constexpr int kNumBars = 35;
-  static_assert((kNumBars + 4) * 8 <= 320, "barriers, TMEM slot, abort flag and start in 320 bytes");
+  constexpr int kNumBars = 37;
+  static_assert((kNumBars + 4) * 8 <= 336, "barriers, TMEM slot, abort flag and start in 336 bytes");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kNumBars + 1);
   int* ctl = reinterpret_cast<int*>(bars + kNumBars + 2);  // start: r, qb, h, local
@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
       // two arrivals: what both issuers hand back or end with, and the pairs
-      const bool two = i == 1 || (i >= 6 && i < 10) || i == 18 || i == 20 || (i >= 25 && i < 33);
-      mbar_init(bars + i, i >= 14 && i < 18 ? 128 : i == 19 ? 512 : two ? 2 : 1);
+      const bool two = i == 1 || (i >= 6 && i < 10) || i == 20 || (i >= 25 && i < 33);
+      mbar_init(bars + i, i >= 14 && i < 18 ? 128 : i >= 35 ? 256 : two ? 2 : 1);
     }
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) {
@@ -748,8 +748,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           parity ^= pv ? 1u : 0u;
         }
-        if (ok && k > 0) ok = wait(epi_done, (k - 1) & 1);
-        if (ok && elect_one()) umma_commit(o_done);
+        if (ok && k > 0) ok = wait(&epi_done[t], (k - 1) & 1);
+        if (ok && elect_one()) umma_commit(&o_done[t]);
         __syncwarp();
         g += d.seg;
       }
@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         ++ends;
         if (hh == 0 && lane == 0) progress[0] = 2 * s_cnt + 2;
       }
-      if (ok) ok = wait(o_done, k & 1);
+      if (ok) ok = wait(&o_done[t], k & 1);
       if (ok && warp_rows) {
         tc_fence_after();
         if (*events != seen) new_m();
@@ -975,7 +975,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         }
       }
       tc_fence_before();
-      mbar_arrive(epi_done);  // O is read: the issuer may let the next unit's o_done complete
+      mbar_arrive(&epi_done[t]);  // O is read: the issuer may let the next unit's o_done complete
       g += d.seg;
     }
   }
