@@ -33,8 +33,6 @@
 // reach 2^127 -- and only when a row's sum over 64 keys leaves 2^100 is m moved (see `over` below).
 // The two threads of a row thus need not meet in a tile.  Rounding: P to bf16 for the product; l sums
 // the unrounded values.
-// Some of the exponentials run as a polynomial on the FMA pipe (exp2_poly_pair): the 16 a clock
-// an SM of the special function unit would otherwise take as long as the products.
 //
 // A key tile's positions outside the unit's [lo, hi] may hold anything: scores there are replaced
 // by -inf (never computed with), and their rows of V are zeroed in shared memory by the softmax
@@ -160,30 +158,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
 __device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
-// (2^a, 2^b) of a pair, each clamped below at 2^-125, as exp2_poly3: x = n + f, n = round(x) by the
-// 1.5 * 2^23 constant, a cubic for 2^f, and n added to the exponent (the constant's own bits leave
-// the word when shifted by 23).  Packed except the clamp and the exponent.  Above 2^127 the result
-// is meaningless: the caller watches the inputs' maximum.  A NaN in x leaves one in acc.
-__device__ __forceinline__ uint64_t exp2_poly_pair(uint64_t x, uint64_t& acc) {
-  const uint64_t xc = pair_f32(max_nan(lo_f(x), -125.f), max_nan(hi_f(x), -125.f));
-  acc = fma2(xc, 0ull, acc);
-  const uint64_t magic = pair_f32(12582912.f, 12582912.f), unmagic = pair_f32(-12582912.f, -12582912.f);
-  const uint64_t t = add2(xc, magic);
-  const uint64_t f = fma2(add2(t, unmagic), pair_f32(-1.f, -1.f), xc);
-  uint64_t q = fma2(pair_f32(0.0551716648f, 0.0551716648f), f, pair_f32(0.242611125f, 0.242611125f));
-  q = fma2(q, f, pair_f32(0.693260968f, 0.693260968f));
-  q = fma2(q, f, pair_f32(0.999928057f, 0.999928057f));
-  const uint32_t r0 = static_cast<uint32_t>(q) + (static_cast<uint32_t>(t) << 23);
-  const uint32_t r1 = static_cast<uint32_t>(q >> 32) + (static_cast<uint32_t>(t >> 32) << 23);
-  return static_cast<uint64_t>(r0) | static_cast<uint64_t>(r1) << 32;
-}
 
 // A unit (kv head aside): tiles' first tokens and counts, their key-tile ranges from kb.
 struct ChunkUnit {
@@ -357,25 +331,19 @@ __device__ __noinline__ float tmem_prep(uint32_t addr, bool mask, int lo, int hi
   return mx;
 }
 
-// 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc; one
-// pair of eight by the polynomial, whose inputs' maximum goes to pmax.  A masked score (-inf) gives
-// 0 or, in the polynomial's columns, 2^-125: nothing beside a row's sum, which is about 1 or more.
+// 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc.  (A
+// polynomial on the FMA pipe for some of them, to spare the special function unit's 16 a clock, lost: it
+// costs the issue slots that the four chains' warps share.  8,192 after 8,192: 748 us without, 750, 760,
+// 789 and 818 with one pair of sixteen, one, two and three of eight.)
 __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uint64_t nm2, uint32_t (&w)[16],
-                                      uint64_t& acc0, uint64_t& acc1, float& pmax) {
+                                      uint64_t& acc0, uint64_t& acc1) {
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
     const uint64_t x = fma2(static_cast<uint64_t>(s[2 * c]) | static_cast<uint64_t>(s[2 * c + 1]) << 32, sc2, nm2);
-    const int u = c & 7;
-    uint64_t e;
-    if (u == 4) {
-      pmax = fmax3(pmax, lo_f(x), hi_f(x));
-      e = exp2_poly_pair(x, acc1);
-    } else {
-      e = pair_f32(fast_exp2(lo_f(x)), fast_exp2(hi_f(x)));
-    }
-    if (u & 1) acc1 = add2(acc1, e);
-    else acc0 = add2(acc0, e);
-    w[c] = pack_bf16x2_rn(lo_f(e), hi_f(e));
+    const float e0 = fast_exp2(lo_f(x)), e1 = fast_exp2(hi_f(x));
+    if (c & 1) acc1 = add2(acc1, pair_f32(e0, e1));
+    else acc0 = add2(acc0, pair_f32(e0, e1));
+    w[c] = pack_bf16x2_rn(e0, e1);
   }
 }
 
@@ -884,14 +852,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
           const uint64_t nm2 = pair_f32(neg_m, neg_m);
           uint64_t acc0 = 0, acc1 = 0;
-          float pmax = -INFINITY;
           tmem_ld_wait32(a);
-          exp32(a, sc2, nm2, w0, acc0, acc1, pmax);
+          exp32(a, sc2, nm2, w0, acc0, acc1);
           tmem_ld32(s_addr + 32, a);
-          exp32(a, sc2, nm2, w1, acc0, acc1, pmax);
+          exp32(a, sc2, nm2, w1, acc0, acc1);
           acc0 = add2(acc0, acc1);
           sum = lo_f(acc0) + hi_f(acc0);
-          const bool over = valid && (sum >= 1.2676506e30f || pmax >= 100.f);  // 2^100 (not a NaN)
+          const bool over = valid && sum >= 1.2676506e30f;  // 2^100 (not a NaN)
           if (__builtin_expect(redone || !__any_sync(0xffffffffu, over), 1)) break;
           // Overflow (never where the maximum has just been exchanged, so all_m holds for both warps
           // from here on and they meet only below).  m moves to the maximum of the rows that need it, and
