@@ -26,7 +26,11 @@
 // With whole tiles (N = 128, two chains) a chain's softmax had to fit beside one other chain's
 // products, which it does not (1,600 cycles against 1,024), and both then waited: 3,700 cycles a key
 // tile where the products take 2,048.  N = 64 costs the tensor cores a quarter more (S reads Q from
-// shared memory once for 64 keys: 384 cycles for 256 worth) and the rest overlaps.
+// shared memory once for 64 keys: 384 cycles for 256 worth) and the rest overlaps: 2,560 of some 3,300.
+// Measured, 16/4 heads of 128: 8,192 tokens after 8,192 767 us, 1,075 TFLOP/s at the 1.45 GHz that the
+// power limit leaves; five chunks of 2,041 under a window of 1,024 119 us, 600 TFLOP/s -- nine key tiles
+// a unit there, and a unit costs some 12,000 cycles beside its tiles: the first tile's maximum and the
+// masks at both ends (5,500), the last product and O's way out (6,000).
 //
 // Softmax without a maximum on the critical path: the exponent's reference m is the row's maximum over
 // the first tile in which it sees a key, and stays.  P and l may then exceed 1 -- fp32 and bf16
@@ -47,7 +51,7 @@
 namespace mcb {
 
 constexpr int kPcTile = 128;      // query rows a tile, keys a key tile
-constexpr int kPcThreads = 640;   // producer, issuer, two idle warps, 2 x 8 softmax warps
+constexpr int kPcThreads = 640;   // producer, two issuers, an idle warp, 2 x 8 softmax warps
 constexpr int kPcWarps = kPcThreads / 32;
 
 // What paged_combine_kernel needs of the unit that starts in a CTA's share and ends after it.
