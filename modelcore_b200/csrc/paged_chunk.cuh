@@ -685,6 +685,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         ok = wait(q_full, k & 1);
         const int b = t ? d.b1 : d.b0, e = t ? d.e1 : d.e0;  // this tile's key tiles
         if (b >= e && lane == 0) mbar_arrive(q_empty);
+        bool o_read = k == 0;  // the part before has been read out of O_t
         // Step j, half by half: P V of key tile j and S of j + 1 (j = -1: the first S).  Every key tile
         // is waited for and handed back by both issuers, used or not: each stage's phases stay in step.
 #pragma unroll 1
@@ -696,6 +697,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
 #pragma unroll 1
           for (int h = 0; ok && h < 2; ++h) {
             if (pv && !(ok = wait(&p_full[t * 2 + h], parity))) break;
+            // A part's first product overwrites O_t.  Its P says that the warps with rows are past the last
+            // part's end (they meet in the first tile), but a quarter without rows here hands its P over at
+            // once, one of its warps possibly still at the last part's columns.
+            if (pv && !o_read) {
+              if (!(ok = wait(&epi_done[t], (k - 1) & 1))) break;
+              o_read = true;
+            }
             tc_fence_after();
             const uint32_t s_col = tm + t * kPcTile + h * 64;
             if (elect_one()) {
@@ -729,7 +737,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           parity ^= pv ? 1u : 0u;
         }
-        if (ok && k > 0) ok = wait(&epi_done[t], (k - 1) & 1);
+        if (ok && !o_read) ok = wait(&epi_done[t], (k - 1) & 1);
         if (ok && elect_one()) umma_commit(&o_done[t]);
         __syncwarp();
         g += d.seg;
