@@ -203,9 +203,10 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const PagedChunkParams& p, const
 }
 
 // What the two warps of a row quarter share: per-row values they exchange (two slots), the rows' m
-// after an overflow and how many there were, and each warp's progress -- 2 n + 1: overflow in its
-// n-th tile, 2 n + 2: its P of the n-th tile is stored (or, the first half's warp, a part of a unit
-// ended before its n-th tile and the products of all its P are complete).
+// after an overflow and how many there were, and each warp's progress -- 2 n + 1: it waits in the
+// handshake over an overflow in its n-th tile, 2 n: that handshake is over and its P not yet stored, 2 n +
+// 2: its P of the n-th tile is stored (or, the first half's warp, a part of a unit ended before its n-th
+// tile and the products of all its P are complete).
 struct PagedPair {
   float xch[2][2][32];
   float m[32];
@@ -917,6 +918,12 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           if (both) {
             tmem_scale(o_addr + hh * (D / 2), D / 2, alpha);
+            // No longer waiting, and the other is to know before it can look again: it may reach its next
+            // tile and overflow there before this one's P is stored, would take an odd progress left
+            // standing for this warp at the handshake, and wait for it in an exchange that it has left.
+            // (The exchange publishes it.  A warp that goes on alone, below, may leave its odd progress:
+            // that is below the other's `low` from the other's next tile on.)
+            if (lane == 0) progress[hh] = 2 * s_cnt;
             exchange(0.f);  // both halves of O are scaled before either P can be used
             if (!ok) break;
           } else {
