@@ -11,7 +11,7 @@
 // tail (entry x at x mod n_pages).  A plan neither moves the lengths nor overwrites a table entry
 // below first_r, so planning again from the same lengths and counters gives the same answer.
 //
-// Every CTA scans the lengths itself (1,024 rows at a time, two sums in one 64-bit scan) and expands
+// Every CTA scans the lengths itself (1,024 rows at a time, two saturating sums in one scan) and expands
 // its share of the tokens and pages, a thread four (plan) or eight (release) of them with their
 // searches and loads side by side: integers only, a few KB to a few MB, so launch and dependent
 // latencies bound it, not bytes.  free_state_out (and seqlens_out) may be the inputs: the CTA that
@@ -65,14 +65,40 @@ __device__ __forceinline__ bool last_cta(int* counter) {
   return s_last != 0;
 }
 
+// Counts of tokens and pages stop at 2^31, above every N and n_pages: lengths may be anything, and the
+// sum of a few is past 32 bits.  (The saturating sum is associative, so it can be scanned.)
+constexpr uint32_t kCountEnd = 1u << 31;
+__device__ __forceinline__ uint32_t count_add(uint32_t a, uint32_t b) {  // both at most kCountEnd
+  const uint32_t s = a + b;
+  return s < a || s > kCountEnd ? kCountEnd : s;
+}
+__device__ __forceinline__ uint32_t count_of(unsigned long long n) {
+  return static_cast<uint32_t>(n < kCountEnd ? n : kCountEnd);
+}
+
+struct SumAdd {
+  __device__ __forceinline__ unsigned long long operator()(unsigned long long a, unsigned long long b) const {
+    return a + b;
+  }
+};
+struct CountPairAdd {  // two counts in one word
+  __device__ __forceinline__ unsigned long long operator()(unsigned long long a, unsigned long long b) const {
+    const uint32_t lo = count_add(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+    const uint32_t hi = count_add(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32));
+    return static_cast<unsigned long long>(hi) << 32 | lo;
+  }
+};
+
 // Inclusive scan of one 64-bit value a thread over the block; `warp_sums` is 33 shared words, the
 // last of them the block's total.
+template <typename Add = SumAdd>
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warp_sums) {
+  const Add add;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     const unsigned long long o = __shfl_up_sync(0xffffffffu, v, m);
-    if (lane >= m) v += o;
+    if (lane >= m) v = add(o, v);
   }
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
@@ -81,13 +107,13 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
       const unsigned long long o = __shfl_up_sync(0xffffffffu, w, m);
-      if (lane >= m) w += o;
+      if (lane >= m) w = add(o, w);
     }
     warp_sums[lane] = w;
     if (lane == 31) warp_sums[32] = w;
   }
   __syncthreads();
-  return warp > 0 ? v + warp_sums[warp - 1] : v;
+  return warp > 0 ? add(warp_sums[warp - 1], v) : v;
 }
 
 // The last i in [0, n) with start[i] <= x (start[0] <= x): of rows with equal starts, the one that
@@ -127,7 +153,7 @@ __device__ __forceinline__ int pages_of(long long len, int shift, int max_pages)
 
 __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePlanParams p) {
   __shared__ unsigned long long warp_sums[33];
-  __shared__ uint32_t s_tok[kPlanMaxThreads], s_page[kPlanMaxThreads];
+  __shared__ uint32_t s_tok[kPlanMaxThreads + 1], s_page[kPlanMaxThreads + 1];  // (row + 1: its end)
   __shared__ int s_len[kPlanMaxThreads];
   pdl_wait();
   pdl_launch_dependents();
@@ -153,14 +179,20 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
              pages_of(len, p.page_shift, p.max_pages);
     }
     const unsigned long long mine = static_cast<unsigned long long>(need) << 32 | static_cast<uint32_t>(fresh);
-    const unsigned long long incl = block_scan(mine, warp_sums);
+    const unsigned long long incl = block_scan<CountPairAdd>(mine, warp_sums);
     const unsigned long long total = warp_sums[32];
-    s_tok[tid] = tok0 + static_cast<uint32_t>(incl - mine);
-    s_page[tid] = page0 + static_cast<uint32_t>((incl - mine) >> 32);
+    const uint32_t row_tok1 = count_add(tok0, static_cast<uint32_t>(incl));
+    if (tid == 0) {
+      s_tok[0] = tok0;
+      s_page[0] = page0;
+    }
+    s_tok[tid + 1] = row_tok1;
+    s_page[tid + 1] = count_add(page0, static_cast<uint32_t>(incl >> 32));
     s_len[tid] = len;
-    if (rank == 0 && r < p.R) p.cu_new[r + 1] = static_cast<int>(tok0 + static_cast<uint32_t>(incl));
+    if (rank == 0 && r < p.R) p.cu_new[r + 1] = static_cast<int>(min(row_tok1, kCountEnd - 1));
     __syncthreads();
-    const uint32_t tok1 = tok0 + static_cast<uint32_t>(total), page1 = page0 + static_cast<uint32_t>(total >> 32);
+    const uint32_t tok1 = count_add(tok0, static_cast<uint32_t>(total));
+    const uint32_t page1 = count_add(page0, static_cast<uint32_t>(total >> 32));
     // new table entries
     for (uint32_t k = page0 + rank * nthr + tid; k < page1; k += nc * nthr) {
       const int i = row_of(s_page, rows, k);
@@ -242,8 +274,8 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
       if (p.done[r] != 0) held = pages_of(max(len, 0), p.page_shift, p.max_pages);
     }
     const unsigned long long incl = block_scan(static_cast<unsigned long long>(held), warp_sums);
-    const uint32_t page1 = page0 + static_cast<uint32_t>(warp_sums[32]);
-    s_page[tid] = page0 + static_cast<uint32_t>(incl) - held;
+    const uint32_t page1 = count_of(page0 + warp_sums[32]);
+    s_page[tid] = count_of(page0 + incl - held);
     __syncthreads();
     // A warp takes 256 consecutive pages at a time.  Where they are one request's -- long requests --
     // one search finds it, and the entries are a copy; else every lane searches for its own.

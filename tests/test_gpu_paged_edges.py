@@ -49,3 +49,33 @@ def test_references_that_move_again_and_again(ops, pattern, D, G, fresh):
     # a score of up to 1600 x 8 is a sum of fp32 products: off by up to 2^-20 of it
     slack = (2.25 * U + 8.0 * 1600 * 2.0 ** -20) * bound
     assert np.isfinite(err).all() and (err <= slack).all(), (err - slack).max()
+
+
+HUGE = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("new", [[HUGE] * 3, [HUGE] * 5, [20] + [HUGE] * 4 + [20], [HUGE] * 1000, [16] * 1023 + [HUGE] * 3,
+                                 [40] * 1024 + [HUGE] * 1025])
+def test_new_tokens_past_32_bits_stay_in_the_table(ops, expects_device_error, new):
+    """Lengths that sum to 2^32 and more (a tensor never written, say): the errors are set, each row takes the
+    pages of its own table row and no more, what fits the batch is planned, nothing else is written."""
+    R, width, page, N = len(new), 4, 16, 300
+    need = [min(-(-n // page), width) for n in new]
+    have = sum(need) + 10
+    whole = torch.full((R + 4, width), -77, dtype=torch.int32, device="cuda")
+    outs = ops.page_plan(i32([0] * R), i32(new), whole[:R], i32(range(have)), torch.tensor([0, have], device="cuda"),
+                         page_size=page, num_tokens=N)
+    assert ops.device_error()[0] in (1, 7)
+    start = np.concatenate([[0], np.cumsum(need)])
+    want = np.where(np.arange(width)[None] < np.array(need)[:, None], start[:-1, None] + np.arange(width)[None], -77)
+    assert np.array_equal(whole.cpu().numpy(), np.concatenate([want, np.full((4, width), -77)]))
+    assert outs.free_state.tolist() == [sum(need), have]
+    cu = np.minimum(np.concatenate([[0], np.cumsum(np.array(new, dtype=np.int64))]), HUGE)
+    assert outs.cu_new.tolist() == cu.tolist()
+    pos, slots = np.zeros(N, np.int64), np.full(N, -1)
+    for t in range(N):
+        r = int(np.searchsorted(cu, t, side="right")) - 1
+        pos[t] = t - cu[r]
+        if pos[t] < width * page:
+            slots[t] = want[r, pos[t] // page] * page + pos[t] % page
+    assert outs.positions.tolist() == pos.tolist() and outs.slot_map.tolist() == slots.tolist()
