@@ -28,22 +28,23 @@ def test_a_full_block_and_then_a_ragged_one(ops, Hq, Hkv, D, block):
 def test_references_that_move_again_and_again(ops, pattern, D, G, fresh):
     """Scores that leave the exponent's range tile after tile for thousands of keys: the two warps of a row
     quarter move its reference together, or one of them does, in every order, and none waits for one
-    that has gone on (the wait's limit would set a device error)."""
-    cached, scale = 6000, 8.0
-    c, ks, vs = attn_case([cached] * 3, [fresh] * 3, 2 * G, 2, D, 64, seed=7)
+    that has gone on (the wait's limit would set a device error).  Enough requests that an SM has runs of
+    a dozen tiles and more."""
+    cached, scale, R = 6000, 8.0, 24
+    c, ks, vs = attn_case([cached] * R, [fresh] * R, 2 * G, 2, D, 64, seed=7)
     key = torch.arange(cached + fresh, device="cuda")
     n, half = key // 128, key // 64 % 2
     level = {"both halves, every tile": 2 * n + half, "both, then one": 2 * n - n % 2 * half * 3,
              "halves in turn": n + (n + half) % 2 * 2}[pattern]
     rise = (4.0 * level).to(torch.bfloat16)  # (integers up to 400, a multiple of 4: exact)
-    sign = (torch.arange(3 * fresh, device="cuda") % 3 - 1).to(torch.bfloat16)[:, None]
+    sign = (torch.arange(R * fresh, device="cuda") % 3 - 1).to(torch.bfloat16)[:, None]
     q = c["q"].contiguous().mul(0.25)
     q[..., 0] = sign * 4
-    for r in range(3):
+    for r in range(R):
         ks[r][..., 0] = rise[:, None]
         page = c["table"][r].long()
         c["kp"][page[key // 64], :, key % 64] = ks[r]
-    want, bound = attn_ref(q, ks, vs, [cached] * 3, [fresh] * 3, -1, scale)
+    want, bound = attn_ref(q, ks, vs, [cached] * R, [fresh] * R, -1, scale)
     got = ops.paged_attn(q, c["kp"], c["vp"], c["table"], c["cached"], c["cu"], softmax_scale=scale)
     err = np.abs(got.double().cpu().numpy() - want)
     # a score of up to 1600 x 8 is a sum of fp32 products: off by up to 2^-20 of it
