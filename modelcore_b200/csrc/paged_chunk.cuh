@@ -788,8 +788,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const int see_hi = min(pos0 + rt, d.hi), see_lo = p.a.window >= 0 ? pos0 + rt - p.a.window : 0;
       // 64 keys starting in [full_lo, full_hi] are seen whole by every row
       const int full_hi = min(pos0, d.hi) - 63, full_lo = p.a.window >= 0 ? pos1 - p.a.window : 0;
-      // ... and 64 keys starting outside [some_lo, some_hi] by none
-      const int some_hi = min(pos1, d.hi), some_lo = p.a.window >= 0 ? pos0 - p.a.window - 63 : 0;
+      // ... and 64 keys starting outside [some_lo, some_hi] by none (no window takes that below 32 bits)
+      const int some_hi = min(pos1, d.hi), some_lo = p.a.window >= 0 ? max(pos0 - p.a.window, 0) - 63 : 0;
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
       bool all_m = !warp_rows;  // every row here has an m

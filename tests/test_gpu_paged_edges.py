@@ -80,3 +80,11 @@ def test_new_tokens_past_32_bits_stay_in_the_table(ops, expects_device_error, ne
         if pos[t] < width * page:
             slots[t] = want[r, pos[t] // page] * page + pos[t] % page
     assert outs.positions.tolist() == pos.tolist() and outs.slot_map.tolist() == slots.tolist()
+
+
+@pytest.mark.parametrize("window", [HUGE, HUGE - 1, HUGE - 62, HUGE - 200, 2 ** 30, 1000])
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 4, 128), (6, 6, 64)])
+def test_a_window_wider_than_the_positions(ops, window, Hq, Hkv, D):
+    """The widest windows are no windows, for the first tokens of a prompt too."""
+    check_attn(ops, [0, 0, 70, 5], [300, 1, 200, 3], Hq, Hkv, D, 64, window, hints=(0, 300))
+    check_attn(ops, [0, 3, 70, 500], [1, 1, 1, 1], Hq, Hkv, D, 64, window, hints=(0, 1))
