@@ -423,7 +423,9 @@ int mcb_linear_supported(const mcb_linear_args* args);
  *
  * mcb_page_release: the pages of the requests with done[r] != 0 go to the queue's tail in request
  * order; seqlens_out (may be cache_seqlens) gets 0 for them and cache_seqlens for the others.
- * More pages than the pool has room for (a request released twice) set device error 5.
+ * Table entries outside the pool, as the -1 that a plan leaves when the queue runs out, are left
+ * out and set device error 6; more pages than the pool has room for (a request released twice)
+ * set error 5.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
   const int32_t* cache_seqlens;   /* (R,)                                                       */

@@ -52,16 +52,20 @@ struct PageReleaseParams {
   int R, n_pages, max_pages, page_shift;
 };
 
-// Whether this CTA is the last of the grid to arrive; all threads' reads before are then done in every
-// CTA.  `counter` is zero again after the last.
-__device__ __forceinline__ bool last_cta(int* counter) {
-  __shared__ int s_last;
-  __syncthreads();
+// Whether this CTA is the last of the grid to arrive; all threads' reads and writes before are then done
+// in every CTA, and `flag` becomes whether any thread of the grid came with it set.  `counter` is zero
+// again after the last.
+__device__ __forceinline__ bool last_cta(int* counter, bool& flag) {
+  __shared__ int s_last;  // 0: not the last, 1: the last, 3: the last and a flag
+  constexpr int kFlag = 1 << 16;  // (a grid has fewer CTAs)
+  const int mine = __syncthreads_or(flag) ? kFlag + 1 : 1;
   if (threadIdx.x == 0) {
-    s_last = atom_add_acq_rel_gpu(counter, 1) == static_cast<int>(gridDim.x) - 1;
+    const int all = atom_add_acq_rel_gpu(counter, mine) + mine;
+    s_last = (all & (kFlag - 1)) == static_cast<int>(gridDim.x) ? (all >= kFlag ? 3 : 1) : 0;
     if (s_last) *counter = 0;
   }
   __syncthreads();
+  flag = (s_last & 2) != 0;
   return s_last != 0;
 }
 
@@ -248,7 +252,8 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
     p.positions[t] = -1;
     p.slot_map[t] = -1;
   }
-  if (last_cta(p.counter) && tid == 0) {
+  bool unused = false;
+  if (last_cta(p.counter, unused) && tid == 0) {
     p.free_state_out[0] = head + min(static_cast<long long>(page0), avail);
     p.free_state_out[1] = tail;
   }
@@ -265,18 +270,31 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
       static_cast<uint32_t>(min(max(p.n_pages - (tail - head), 0ll), static_cast<long long>(p.n_pages)));
   __shared__ int s_tail;  // (one thread's division: the first scan's barriers publish it)
   if (tid == 0) s_tail = static_cast<int>(((tail % p.n_pages) + p.n_pages) % p.n_pages);
-  uint32_t page0 = 0;
-  for (int base = 0; base < p.R; base += nthr) {
-    const int r = base + tid, rows = min(nthr, p.R - base);
+  // The rows from `base` on: s_page, where each one's pages start in the sequence of all returned ones;
+  // returns where the block's end.
+  auto rows_pages = [&](int base, uint32_t page0) -> uint32_t {
+    const int r = base + tid;
     int held = 0;
     if (r < p.R) {
       const int len = p.seqlens[r];
       if (p.done[r] != 0) held = pages_of(max(len, 0), p.page_shift, p.max_pages);
     }
     const unsigned long long incl = block_scan(static_cast<unsigned long long>(held), warp_sums);
-    const uint32_t page1 = count_of(page0 + warp_sums[32]);
     s_page[tid] = count_of(page0 + incl - held);
+    const uint32_t page1 = count_of(page0 + warp_sums[32]);
     __syncthreads();
+    return page1;
+  };
+  auto no_page = [&](int page) { return static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.n_pages); };
+  auto store = [&](uint32_t k, int page) {  // the k-th returned page, k < room
+    const uint32_t at = s_tail + k;         // below 2 n_pages
+    p.free_pages[at >= static_cast<uint32_t>(p.n_pages) ? at - p.n_pages : at] = page;
+  };
+  uint32_t page0 = 0;
+  bool holes = false;  // entries that name no page
+  for (int base = 0; base < p.R; base += nthr) {
+    const int rows = min(nthr, p.R - base);
+    const uint32_t page1 = rows_pages(base, page0);
     // A warp takes 256 consecutive pages at a time.  Where they are one request's -- long requests --
     // one search finds it, and the entries are a copy; else every lane searches for its own.
     constexpr int U = 8;
@@ -304,21 +322,44 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
       for (int u = 0; u < U; ++u) {
         const uint32_t k = k0 + 32 * u;
         if (k >= page1) break;
-        if (static_cast<uint32_t>(page[u]) >= static_cast<uint32_t>(p.n_pages)) record_error(kErrPageOutOfRange);
-        if (k >= room) {
-          record_error(kErrPagesExhausted);  // more pages than the pool has: a row released twice
-        } else {
-          const uint32_t at = s_tail + k;  // below 2 n_pages
-          p.free_pages[at >= static_cast<uint32_t>(p.n_pages) ? at - p.n_pages : at] = page[u];
-        }
+        holes |= no_page(page[u]);
+        if (k < room) store(k, page[u]);
       }
     }
     page0 = page1;
     __syncthreads();  // s_page is free again
   }
-  if (!last_cta(p.counter)) return;
+  if (!last_cta(p.counter, holes)) return;
+  if (holes) {
+    // Entries that plan left at -1 when the queue ran out, or worse: they are no pages to hand on.  Rare,
+    // so this CTA writes the whole sequence again without them, over what all have written.
+    if (tid == 0) record_error(kErrPageOutOfRange);
+    uint32_t kept = 0;
+    page0 = 0;
+    for (int base = 0; base < p.R; base += nthr) {
+      const int rows = min(nthr, p.R - base);
+      const uint32_t page1 = rows_pages(base, page0);
+      for (uint32_t k0 = page0; k0 < page1; k0 += nthr) {
+        const uint32_t k = k0 + tid;
+        int page = -1;
+        if (k < page1) {
+          const int i = row_of(s_page, rows, k);
+          page = p.block_table[(base + i) * p.table_stride + (k - s_page[i])];
+        }
+        const bool is_page = !no_page(page);
+        const unsigned long long incl = block_scan(is_page ? 1ull : 0ull, warp_sums);
+        if (is_page && kept + incl <= room) store(kept + static_cast<uint32_t>(incl) - 1, page);
+        kept += static_cast<uint32_t>(warp_sums[32]);
+        __syncthreads();  // warp_sums is free again
+      }
+      page0 = page1;
+      __syncthreads();  // s_page is free again
+    }
+    page0 = kept;
+  }
   for (int r = tid; r < p.R; r += nthr) p.seqlens_out[r] = p.done[r] != 0 ? 0 : p.seqlens[r];
   if (tid == 0) {
+    if (page0 > room) record_error(kErrPagesExhausted);  // more pages than the pool has: a row released twice
     p.free_state_out[0] = head;
     p.free_state_out[1] = tail + min(page0, room);
   }

@@ -718,7 +718,8 @@ def page_release(done, cache_seqlens, block_table, free_pages, free_state, *, pa
     """Returns the pages of the requests with done[r] != 0 ((R,) int32) to the queue's tail, in
     request order (free_pages is written in place).  Returns (free_state, seqlens) after it: new
     tensors, or free_state_out / seqlens_out, which may be the inputs.  The table keeps its stale
-    entries: a length of 0 makes them unreachable."""
+    entries: a length of 0 makes them unreachable.  Entries that name no page (the -1 of a plan that
+    ran out) are left out, with device error 6."""
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)
     if seqlens_out is None:

@@ -88,3 +88,50 @@ def test_a_window_wider_than_the_positions(ops, window, Hq, Hkv, D):
     """The widest windows are no windows, for the first tokens of a prompt too."""
     check_attn(ops, [0, 0, 70, 5], [300, 1, 200, 3], Hq, Hkv, D, 64, window, hints=(0, 300))
     check_attn(ops, [0, 3, 70, 500], [1, 1, 1, 1], Hq, Hkv, D, 64, window, hints=(0, 1))
+
+
+def test_release_after_the_queue_ran_out(ops, expects_device_error):
+    """Entries that plan left at -1 for want of pages (or that name no page) do not go into the queue: it holds
+    every real page once again, and later plans take them."""
+    page, n_pages = 16, 10
+    table = torch.full((2, 8), -1, dtype=torch.int32, device="cuda")
+    queue, state = i32(range(n_pages)), torch.tensor([0, n_pages], device="cuda")
+    lens = i32([0, 0])
+    ops.page_plan(lens, i32([96, 96]), table, queue, state, page_size=page, num_tokens=192, free_state_out=state)
+    assert ops.device_error()[0] == 5 and table.tolist() == [[0, 1, 2, 3, 4, 5, -1, -1], [6, 7, 8, 9, -1, -1, -1, -1]]
+    lens.copy_(i32([96, 96]))
+    for done in ([0, 1], [1, 0]):
+        ops.page_release(i32(done), lens, table, queue, state, page_size=page, free_state_out=state, seqlens_out=lens)
+    assert ops.device_error()[0] == 6 and lens.tolist() == [0, 0] and state.tolist() == [10, 20]
+    assert queue.tolist() == [6, 7, 8, 9, 0, 1, 2, 3, 4, 5]
+    plan = ops.page_plan(lens, i32([80, 80]), table, queue, state, page_size=page, num_tokens=160, free_state_out=state)
+    assert ops.device_error()[0] == 0 and sorted(table[:, :5].flatten().tolist()) == list(range(10))
+    assert state.tolist() == [20, 20] and (plan.slot_map >= 0).all()
+
+
+@pytest.mark.parametrize("R,hi,holes", [(3, 100, 0.5), (40, 2000, 0.1), (40, 2000, 0.001), (1500, 3000, 0.02), (700, 60, 1.0)])
+def test_release_of_tables_with_holes(ops, expects_device_error, R, hi, holes):
+    """Holes anywhere, over one CTA and many: the pages go back in order without them."""
+    rng = np.random.default_rng(R)
+    page, cached = 16, rng.integers(0, hi, R)
+    held = -(-cached // page)
+    total = int(held.sum()) + 5
+    table = np.full((R, int(held.max()) + 2), 12345678, np.int64)
+    order, at, want = rng.permutation(total), 0, []
+    done = (rng.random(R) < 0.8).astype(int)
+    for r in range(R):
+        table[r, :held[r]] = order[at:at + held[r]]
+        at += held[r]
+        bad = rng.random(held[r]) < holes
+        table[r, :held[r]][bad] = rng.choice([-1, total, 2 ** 31 - 1, -2 ** 31], bad.sum())
+        want += table[r, :held[r]][~bad].tolist() if done[r] else []
+    queue = np.arange(total) + 1000
+    head, tail = 7 * total + total - 3, 7 * total + total  # three free ones, the queue going round at once
+    got = i32(queue)
+    st, lens = ops.page_release(i32(done), i32(cached), i32(table), got, torch.tensor([head, tail], device="cuda"),
+                                page_size=page)
+    ops.device_error()
+    assert st.tolist() == [head, tail + len(want)] and lens.tolist() == np.where(done, 0, cached).tolist()
+    got = got.cpu().numpy()
+    assert got[(tail + np.arange(len(want))) % total].tolist() == want
+    assert got[(head + np.arange(3)) % total].tolist() == queue[(head + np.arange(3)) % total].tolist()
