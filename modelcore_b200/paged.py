@@ -15,6 +15,9 @@ finished request's pages serve the next:
     cache.advance(step)
     cache.release([2])                                # row 2 is done: its pages are free
 
+A plan takes its pages only when the step is advanced: until then it can be dropped (planned again, or
+never followed), and the cache is what it was.
+
 Everything that depends on the lengths happens on the GPU (ops.page_plan and the kernels that read its
 tables); the class keeps a host mirror of the lengths only to refuse a step that does not fit
 before anything is launched, as KVCache does.
@@ -29,7 +32,7 @@ from .cache import _aligned_zeros
 
 
 class PagedStep(NamedTuple):
-    """One planned step (PagedKVCache.plan)."""
+    """One planned step (PagedKVCache.plan): the cache's current one until it is advanced or dropped."""
     plan: ops.PagePlan
     new_lens: torch.Tensor     # (max_rows,) int32
     host_lens: np.ndarray      # the same, on the host
@@ -73,6 +76,7 @@ class PagedKVCache:
         self.free_pages = torch.arange(n_pages, **ints)
         self.free_state = torch.tensor([0, n_pages], dtype=torch.int64, device=device)
         self._host_lens = np.zeros(max_rows, dtype=np.int64)
+        self._step = None  # the planned step that advance has not followed yet
 
     def _held(self, lens):
         return -(-lens // self.page_size)
@@ -103,9 +107,10 @@ class PagedKVCache:
         return new
 
     def plan(self, new_lens, num_tokens: Optional[int] = None):
-        """Plans a step of new_lens[r] new tokens for each row (missing rows: 0): pages are taken for
+        """Plans a step of new_lens[r] new tokens for each row (missing rows: 0): pages are chosen for
         them and the packed batch's offsets, positions and slots computed, on the GPU.  num_tokens pads
-        the batch (for a fixed shape).  The rows' lengths stay until advance(step)."""
+        the batch (for a fixed shape).  The rows' lengths and the free pages stay until advance(step);
+        planning again drops a step that has not been advanced."""
         new = self._rows(new_lens)
         total = int(new.sum())
         num_tokens = total if num_tokens is None else int(num_tokens)
@@ -119,32 +124,49 @@ class PagedKVCache:
             raise RuntimeError(f"the step needs {self.pages_needed(new)} pages and {self.free_page_count()} are free")
         lens = self._to_device(new)
         p = ops.page_plan(self.cache_seqlens, lens, self.block_table, self.free_pages, self.free_state,
-                          page_size=self.page_size, num_tokens=num_tokens, free_state_out=self.free_state)
-        return PagedStep(p, lens, new, num_tokens, int(new.max(initial=0)))
+                          page_size=self.page_size, num_tokens=num_tokens)
+        self._step = PagedStep(p, lens, new, num_tokens, int(new.max(initial=0)))
+        return self._step
+
+    def _current(self, step):
+        # another plan may have given this one's pages to other rows, and its positions are behind once advanced
+        if step is not self._step:
+            raise RuntimeError("the step is not the planned one: it has been advanced, or dropped by a later plan or "
+                               "by the release of one of its rows")
 
     def append(self, slot, q, k, v, step, cos, sin, *, eps=None, scale=1.2, rotate_k=True, round_each=True):
         """Rope, norm and scale of the packed q (N, Hq, D) and k (N, Hkv, D), k and v into the step's
         slots; k = v = None for a layer that reads slot's pages but adds nothing (modelcore's
         produces_kv=False).  Returns the processed q."""
+        self._current(step)
         pages = (self.k_pages[slot], self.v_pages[slot], step.plan.slot_map) if k is not None else (None,) * 3
         return ops.paged_append_rope(q, k, v, pages[0], pages[1], step.plan.positions, pages[2], cos, sin, eps=eps,
                                      scale=scale, rotate_k=rotate_k, round_each=round_each)
 
     def attend(self, slot, q, step, *, window=-1, softmax_scale=None):
         """Attention of the step's packed queries over their rows' pages of one slot."""
+        self._current(step)
         return ops.paged_attn(q, self.k_pages[slot], self.v_pages[slot], self.block_table, self.cache_seqlens,
                               step.plan.cu_new, window=window, softmax_scale=softmax_scale, max_new=step.max_new)
 
     def advance(self, step):
-        """The step's new tokens become part of their rows."""
+        """The step's new tokens become part of their rows, and its pages theirs."""
+        self._current(step)
+        self._step = None
         self.cache_seqlens.add_(step.new_lens)
+        self.free_state = step.plan.free_state
         self._host_lens += step.host_lens
 
     def release(self, rows):
-        """Frees the pages of the given rows and sets their lengths to 0."""
+        """Frees the pages of the given rows and sets their lengths to 0.  A planned step that has new tokens
+        of one of them is dropped; any other stays the current one."""
         done = np.zeros(self.max_rows, dtype=np.int64)
         done[np.asarray(rows, dtype=np.int64)] = 1
+        if self._step is not None and self._step.host_lens[done != 0].any():
+            self._step = None
         ops.page_release(self._to_device(done), self.cache_seqlens, self.block_table, self.free_pages,
                          self.free_state, page_size=self.page_size, free_state_out=self.free_state,
                          seqlens_out=self.cache_seqlens)
+        if self._step is not None:
+            self._step.plan.free_state[1:].copy_(self.free_state[1:])  # its tail: the pages that have come back
         self._host_lens[done != 0] = 0
