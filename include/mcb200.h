@@ -459,6 +459,14 @@ typedef struct {
 
 int mcb_page_release(const mcb_page_release_args* args, void* stream);
 
+/* mcb_page_release_to: the same, but a request with done[r] != 0 keeps its first keep_lens[r]
+ * positions (clamped to its length; (R,) int32, NULL: none): the pages above them go back and
+ * seqlens_out gets keep_lens.  For a step of which only a part is kept, as drafted tokens that
+ * verification rejects: advance cache_seqlens by the whole step, then release to the kept lengths;
+ * without it the pages that the plan took for the rejected tokens are lost to the queue.
+ * keep_lens must not be seqlens_out. */
+int mcb_page_release_to(const mcb_page_release_args* args, const int32_t* keep_lens, void* stream);
+
 /* mcb_paged_append_rope: mcb_kv_append_rope for packed tokens and a paged cache: q_out = scale *
  * rms_norm(rope(q)) at each token's position, k the same (raw with rotate_k = 0) and v written to
  * the token's slot.  k = v = NULL: only q.  A token of position -1 (padding) gets a zero q_out, one

@@ -66,6 +66,7 @@ EXPORTED_SYMBOLS = (
     "mcb_softcap_argmax",
     "mcb_page_plan",
     "mcb_page_release",
+    "mcb_page_release_to",
     "mcb_paged_append_rope",
     "mcb_paged_attn_workspace_size",
     "mcb_paged_attn_counter_count",
@@ -311,6 +312,8 @@ def _declare(lib):
                       ("mcb_paged_append_rope", PagedAppendArgs), ("mcb_paged_attn", PagedAttnArgs)):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [P(cls), ctypes.c_void_p]
+    lib.mcb_page_release_to.restype = ctypes.c_int
+    lib.mcb_page_release_to.argtypes = [P(PageReleaseArgs), ctypes.c_void_p, ctypes.c_void_p]
     for name in ("mcb_paged_attn_workspace_size", "mcb_paged_attn_counter_count"):
         getattr(lib, name).restype = ctypes.c_size_t
         getattr(lib, name).argtypes = [P(PagedAttnArgs)]

@@ -81,8 +81,7 @@ int page_plan(const mcb_page_plan_args* a, void* stream) {
   return MCB_OK;
 }
 
-int page_release(const mcb_page_release_args* a, void* stream) {
-  const char* who = "mcb_page_release";
+int page_release(const mcb_page_release_args* a, const int32_t* keep_lens, const char* who, void* stream) {
   if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
   if (a->R < 0) return fail(MCB_ERR_INVALID_ARG, "%s: bad size R=%d", who, a->R);
   int rc = check_pool(a->n_pages, a->page_size, a->max_pages, who);
@@ -103,6 +102,7 @@ int page_release(const mcb_page_release_args* a, void* stream) {
   p.free_state = reinterpret_cast<const long long*>(a->free_state);
   p.free_state_out = reinterpret_cast<long long*>(a->free_state_out);
   p.seqlens_out = a->seqlens_out;
+  p.keep_lens = keep_lens;
   p.R = a->R;
   p.n_pages = a->n_pages;
   p.max_pages = a->max_pages;
@@ -442,7 +442,10 @@ int mcb_page_plan(const mcb_page_plan_args* a, void* stream) {
   return guarded("mcb_page_plan", [&] { return page_plan(a, stream); });
 }
 int mcb_page_release(const mcb_page_release_args* a, void* stream) {
-  return guarded("mcb_page_release", [&] { return page_release(a, stream); });
+  return guarded("mcb_page_release", [&] { return page_release(a, nullptr, "mcb_page_release", stream); });
+}
+int mcb_page_release_to(const mcb_page_release_args* a, const int32_t* keep_lens, void* stream) {
+  return guarded("mcb_page_release_to", [&] { return page_release(a, keep_lens, "mcb_page_release_to", stream); });
 }
 int mcb_paged_append_rope(const mcb_paged_append_args* a, void* stream) {
   return guarded("mcb_paged_append_rope", [&] { return paged_append(a, stream); });

@@ -48,6 +48,7 @@ struct PageReleaseParams {
   const long long* free_state;
   long long* free_state_out;
   int32_t* seqlens_out;
+  const int32_t* keep_lens;  // positions that a done request keeps, or null: none
   int* counter;
   int R, n_pages, max_pages, page_shift;
 };
@@ -262,6 +263,7 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_plan_kernel(const PagePl
 __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const PageReleaseParams p) {
   __shared__ unsigned long long warp_sums[33];
   __shared__ uint32_t s_page[kPlanMaxThreads];
+  __shared__ int s_first[kPlanMaxThreads];  // the row's first returned table entry
   pdl_wait();  // no early trigger: like kv_advance, this kernel may write cache_seqlens
   const int tid = threadIdx.x, nthr = blockDim.x;
   const int rank = blockIdx.x, nc = gridDim.x;
@@ -270,17 +272,24 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
       static_cast<uint32_t>(min(max(p.n_pages - (tail - head), 0ll), static_cast<long long>(p.n_pages)));
   __shared__ int s_tail;  // (one thread's division: the first scan's barriers publish it)
   if (tid == 0) s_tail = static_cast<int>(((tail % p.n_pages) + p.n_pages) % p.n_pages);
+  auto kept_len = [&](int r, int len) {  // of a done request
+    return p.keep_lens == nullptr ? 0 : min(max(p.keep_lens[r], 0), max(len, 0));
+  };
   // The rows from `base` on: s_page, where each one's pages start in the sequence of all returned ones;
   // returns where the block's end.
   auto rows_pages = [&](int base, uint32_t page0) -> uint32_t {
     const int r = base + tid;
-    int held = 0;
+    int held = 0, first = 0;
     if (r < p.R) {
       const int len = p.seqlens[r];
-      if (p.done[r] != 0) held = pages_of(max(len, 0), p.page_shift, p.max_pages);
+      if (p.done[r] != 0) {
+        first = pages_of(kept_len(r, len), p.page_shift, p.max_pages);
+        held = pages_of(max(len, 0), p.page_shift, p.max_pages) - first;
+      }
     }
     const unsigned long long incl = block_scan(static_cast<unsigned long long>(held), warp_sums);
     s_page[tid] = count_of(page0 + incl - held);
+    s_first[tid] = first;
     const uint32_t page1 = count_of(page0 + warp_sums[32]);
     __syncthreads();
     return page1;
@@ -306,7 +315,7 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
       const int row = row_of(s_page, rows, w0);
       const uint32_t row_end = row + 1 < rows ? s_page[row + 1] : page1;
       if (row_end - w0 >= 32 * U) {
-        const int32_t* src = p.block_table + (base + row) * p.table_stride + (k0 - s_page[row]);
+        const int32_t* src = p.block_table + (base + row) * p.table_stride + s_first[row] + (k0 - s_page[row]);
 #pragma unroll
         for (int u = 0; u < U; ++u) page[u] = src[32 * u];
       } else {
@@ -316,7 +325,8 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
         for (int u = 0; u < U; ++u) k[u] = min(k0 + 32 * u, page1 - 1);
         rows_of<U>(s_page, rows, k, i);
 #pragma unroll
-        for (int u = 0; u < U; ++u) page[u] = p.block_table[(base + i[u]) * p.table_stride + (k[u] - s_page[i[u]])];
+        for (int u = 0; u < U; ++u)
+          page[u] = p.block_table[(base + i[u]) * p.table_stride + s_first[i[u]] + (k[u] - s_page[i[u]])];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -344,7 +354,7 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
         int page = -1;
         if (k < page1) {
           const int i = row_of(s_page, rows, k);
-          page = p.block_table[(base + i) * p.table_stride + (k - s_page[i])];
+          page = p.block_table[(base + i) * p.table_stride + s_first[i] + (k - s_page[i])];
         }
         const bool is_page = !no_page(page);
         const unsigned long long incl = block_scan(is_page ? 1ull : 0ull, warp_sums);
@@ -357,7 +367,10 @@ __global__ void __launch_bounds__(kPlanMaxThreads) page_release_kernel(const Pag
     }
     page0 = kept;
   }
-  for (int r = tid; r < p.R; r += nthr) p.seqlens_out[r] = p.done[r] != 0 ? 0 : p.seqlens[r];
+  for (int r = tid; r < p.R; r += nthr) {
+    const int len = p.seqlens[r];
+    p.seqlens_out[r] = p.done[r] != 0 ? kept_len(r, len) : len;
+  }
   if (tid == 0) {
     if (page0 > room) record_error(kErrPagesExhausted);  // more pages than the pool has: a row released twice
     p.free_state_out[0] = head;

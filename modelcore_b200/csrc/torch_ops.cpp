@@ -499,7 +499,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache
 
 void page_release(const at::Tensor& done, const at::Tensor& cache_seqlens, const at::Tensor& block_table,
                   const at::Tensor& free_pages, const at::Tensor& free_state, const at::Tensor& free_state_out,
-                  const at::Tensor& seqlens_out, int64_t page_size) {
+                  const at::Tensor& seqlens_out, int64_t page_size, const std::optional<at::Tensor>& keep_lens) {
   need(cache_seqlens, "cache_seqlens", 1, at::kInt);
   c10::cuda::CUDAGuard guard(cache_seqlens.device());
   const int64_t R = cache_seqlens.size(0);
@@ -524,7 +524,13 @@ void page_release(const at::Tensor& done, const at::Tensor& cache_seqlens, const
   a.max_pages = to_i32(block_table.size(1), "max_pages");
   a.page_size = to_i32(page_size, "page_size");
   a.counter = paged_counters(cache_seqlens, 1);
-  check_status(mcb_page_release(&a, stream_of(cache_seqlens)), "mcb200::page_release");
+  const int32_t* keep = nullptr;
+  if (keep_lens.has_value()) {
+    int_vec(*keep_lens, "keep_lens", R, cache_seqlens, at::kInt);
+    keep = keep_lens->data_ptr<int32_t>();
+    TORCH_CHECK(R == 0 || keep != a.seqlens_out, "keep_lens must not be seqlens_out");
+  }
+  check_status(mcb_page_release_to(&a, keep, stream_of(cache_seqlens)), "mcb200::page_release");
 }
 
 at::Tensor paged_append_rope(const at::Tensor& q, const std::optional<at::Tensor>& k,
@@ -665,7 +671,8 @@ TORCH_LIBRARY(mcb200, m) {
       "Tensor free_state, Tensor(b!) free_state_out, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor)");
   m.def(
       "page_release(Tensor done, Tensor cache_seqlens, Tensor block_table, Tensor(a!) free_pages, "
-      "Tensor free_state, Tensor(b!) free_state_out, Tensor(c!) seqlens_out, int page_size) -> ()");
+      "Tensor free_state, Tensor(b!) free_state_out, Tensor(c!) seqlens_out, int page_size, "
+      "Tensor? keep_lens=None) -> ()");
   m.def(
       "paged_append_rope(Tensor q, Tensor? k, Tensor? v, Tensor(a!)? k_pages, Tensor(b!)? v_pages, "
       "Tensor positions, Tensor? slot_map, Tensor cos, Tensor sin, float? eps=None, float scale=1.2, "

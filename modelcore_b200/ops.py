@@ -714,18 +714,23 @@ def page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state, *, p
 
 
 def page_release(done, cache_seqlens, block_table, free_pages, free_state, *, page_size,
-                 free_state_out=None, seqlens_out=None):
+                 free_state_out=None, seqlens_out=None, keep_lens=None):
     """Returns the pages of the requests with done[r] != 0 ((R,) int32) to the queue's tail, in
     request order (free_pages is written in place).  Returns (free_state, seqlens) after it: new
     tensors, or free_state_out / seqlens_out, which may be the inputs.  The table keeps its stale
     entries: a length of 0 makes them unreachable.  Entries that name no page (the -1 of a plan that
-    ran out) are left out, with device error 6."""
+    ran out) are left out, with device error 6.
+
+    keep_lens (R,) int32: a done request keeps that many of its positions (at most all), and the pages
+    above them go back.  So a step is kept in part (drafted tokens, some rejected): advance
+    cache_seqlens by the whole step, then release to the kept lengths -- with done all ones nothing
+    needs to be known on the host.  The pages that the plan took for the rest are otherwise lost."""
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)
     if seqlens_out is None:
         seqlens_out = torch.empty_like(cache_seqlens)
     _PAGED.page_release(done, cache_seqlens, block_table, free_pages, free_state, free_state_out,
-                          seqlens_out, page_size)
+                          seqlens_out, page_size, keep_lens)
     return free_state_out, seqlens_out
 
 

@@ -15,6 +15,8 @@ finished request's pages serve the next:
     cache.advance(step)
     cache.release([2])                                # row 2 is done: its pages are free
 
+Of drafted tokens that were verified in one step, advance(step, kept=[2, 0, 1, 4]) keeps the accepted ones.
+
 A plan takes its pages only when the step is advanced: until then it can be dropped (planned again, or
 never followed), and the cache is what it was.
 
@@ -149,24 +151,40 @@ class PagedKVCache:
         return ops.paged_attn(q, self.k_pages[slot], self.v_pages[slot], self.block_table, self.cache_seqlens,
                               step.plan.cu_new, window=window, softmax_scale=softmax_scale, max_new=step.max_new)
 
-    def advance(self, step):
-        """The step's new tokens become part of their rows, and its pages theirs."""
+    def advance(self, step, kept=None):
+        """The step's new tokens become part of their rows, and its pages theirs.  kept: how many of its new
+        tokens each row keeps, the first ones (a list as plan's; drafted tokens that verification
+        rejects are not kept); the pages that only the others needed are free again."""
         self._current(step)
+        if kept is not None:
+            kept = self._rows(kept)
+            if (kept > step.host_lens).any():
+                row = int((kept - step.host_lens).argmax())
+                raise RuntimeError(f"row {row} has {step.host_lens[row]} new tokens in the step, not {kept[row]} to keep")
         self._step = None
         self.cache_seqlens.add_(step.new_lens)
         self.free_state = step.plan.free_state
-        self._host_lens += step.host_lens
+        if kept is None:
+            self._host_lens += step.host_lens
+            return
+        self._host_lens += kept
+        fewer = kept < step.host_lens
+        if fewer.any():
+            self._release(fewer, self._to_device(self._host_lens))
 
     def release(self, rows):
         """Frees the pages of the given rows and sets their lengths to 0.  A planned step that has new tokens
         of one of them is dropped; any other stays the current one."""
-        done = np.zeros(self.max_rows, dtype=np.int64)
-        done[np.asarray(rows, dtype=np.int64)] = 1
-        if self._step is not None and self._step.host_lens[done != 0].any():
+        done = np.zeros(self.max_rows, dtype=bool)
+        done[np.asarray(rows, dtype=np.int64)] = True
+        if self._step is not None and self._step.host_lens[done].any():
             self._step = None
-        ops.page_release(self._to_device(done), self.cache_seqlens, self.block_table, self.free_pages,
-                         self.free_state, page_size=self.page_size, free_state_out=self.free_state,
-                         seqlens_out=self.cache_seqlens)
+        self._release(done)
         if self._step is not None:
             self._step.plan.free_state[1:].copy_(self.free_state[1:])  # its tail: the pages that have come back
-        self._host_lens[done != 0] = 0
+        self._host_lens[done] = 0
+
+    def _release(self, done, keep_lens=None):
+        ops.page_release(self._to_device(done), self.cache_seqlens, self.block_table, self.free_pages,
+                         self.free_state, page_size=self.page_size, free_state_out=self.free_state,
+                         seqlens_out=self.cache_seqlens, keep_lens=keep_lens)

@@ -28,7 +28,7 @@ functions, so that torch.compile can trace through them:
     torch.ops.mcb200.page_plan(cache_seqlens, new_lens, block_table, free_pages, free_state,
                                free_state_out, page_size, num_tokens) -> cu_new, positions, slot_map
     torch.ops.mcb200.page_release(done, cache_seqlens, block_table, free_pages, free_state,
-                                  free_state_out, seqlens_out, page_size)
+                                  free_state_out, seqlens_out, page_size, keep_lens=None)
     torch.ops.mcb200.paged_append_rope(q, k, v, k_pages, v_pages, positions, slot_map, cos, sin,
                                        eps=None, scale=1.2, rotate_k=True, round_each=True) -> q'
     torch.ops.mcb200.paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, window=-1,

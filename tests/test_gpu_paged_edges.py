@@ -135,3 +135,31 @@ def test_release_of_tables_with_holes(ops, expects_device_error, R, hi, holes):
     got = got.cpu().numpy()
     assert got[(tail + np.arange(len(want))) % total].tolist() == want
     assert got[(head + np.arange(3)) % total].tolist() == queue[(head + np.arange(3)) % total].tolist()
+
+
+@pytest.mark.parametrize("R,hi,page,in_place", [(1, 50, 16, True), (40, 3000, 16, False), (1500, 700, 32, True),
+                                                (64, 30000, 64, False)])
+def test_release_down_to_a_length(ops, R, hi, page, in_place):
+    """keep_lens: below, at and above the length, negative; only of the requests that are done."""
+    rng = np.random.default_rng(R)
+    cached, done = rng.integers(0, hi, R), (rng.random(R) < 0.7).astype(int)
+    keep = np.where(rng.random(R) < 0.2, rng.choice([-3, hi + 5, 0], R), (cached * rng.random(R)).astype(int))
+    held = -(-cached // page)
+    total, width = int(held.sum()) + 4, int(held.max()) + 2
+    table, order, at = np.full((R, width), -1, np.int64), rng.permutation(total), 0
+    left = np.where(done, np.clip(keep, 0, cached), cached)
+    want = []
+    for r in range(R):
+        table[r, :held[r]] = order[at:at + held[r]]
+        at += held[r]
+        want += table[r, -(-left[r] // page):held[r]].tolist()
+    head, tail = 5 * total + 2, 5 * total + 6
+    queue, lens, st = i32(np.arange(total)), i32(cached), torch.tensor([head, tail], device="cuda")
+    out = dict(free_state_out=st, seqlens_out=lens) if in_place else {}
+    st, new = ops.page_release(i32(done), lens, i32(table), queue, st, page_size=page, keep_lens=i32(keep), **out)
+    assert new.tolist() == left.tolist() and st.tolist() == [head, tail + len(want)]
+    assert queue.cpu().numpy()[(tail + np.arange(len(want))) % total].tolist() == want
+    for bad in (i32(keep[:-1]), i32(keep).long(), i32(keep).cpu(), new):
+        with pytest.raises(RuntimeError):
+            ops.page_release(i32(done), i32(cached), i32(table), queue, st, page_size=page, seqlens_out=new,
+                             keep_lens=bad)

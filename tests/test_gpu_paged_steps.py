@@ -104,3 +104,58 @@ def test_a_long_life_with_dropped_plans():
         if rng.random() < 0.9:
             cache.advance(step)
         check(cache)
+
+
+def test_a_step_kept_in_part_gives_the_other_pages_back():
+    cache = make()
+    cache.advance(cache.plan([14, 16, 15]))
+    step = cache.plan([4, 4, 4])
+    with pytest.raises(RuntimeError, match="not 5 to keep"):
+        cache.advance(step, kept=[1, 5, 0])
+    cache.advance(step, kept=[1, 4, 0])  # rows 0 and 2 do not need their second page after all
+    check(cache)
+    assert cache.host_lens().tolist() == [15, 20, 15] and cache.free_page_count() == 6
+    rng = np.random.default_rng(4)
+    cache = make(60, 7, 300)
+    for _ in range(150):
+        lens = cache.host_lens()
+        cache.release(np.nonzero((rng.random(7) < 0.05) | (lens > 240))[0])
+        new = rng.integers(0, 40, 7)
+        while cache.pages_needed(new) > cache.free_page_count():
+            new[rng.integers(0, 7)] = 0
+        step = cache.plan(new)
+        cache.advance(step, kept=rng.integers(0, new + 1))
+        check(cache)
+
+
+def test_what_is_kept_is_what_was_written():
+    """Attention after partial steps against the same tokens written whole: the kept ones are in the rows'
+    pages, the rejected ones in nobody's."""
+    from modelcore_b200 import ops
+    g = torch.Generator("cuda").manual_seed(2)
+    cos, sin = (torch.randn(160, 32, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    new = lambda n: torch.randn(n, 6, 64, device="cuda", generator=g).to(torch.bfloat16).split([2, 2, 2], 1)
+    a, b = make(30), make(30)
+    ks, vs = [[], [], []], [[], [], []]
+    for i in range(20):
+        kept = [(i + r) % 5 for r in range(3)]
+        step = a.plan([4, 4, 4])
+        q, k, v = new(12)
+        a.append(0, q, k, v, step, cos, sin)
+        a.advance(step, kept=kept)
+        for r in range(3):
+            ks[r].append(k[4 * r:4 * r + kept[r]])
+            vs[r].append(v[4 * r:4 * r + kept[r]])
+    check(a)
+    lens = [sum(map(len, x)) for x in ks]
+    step = b.plan(lens)
+    k, v = (torch.cat([torch.cat(x) for x in y]) for y in (ks, vs))
+    b.append(0, k, k, v, step, cos, sin)
+    b.advance(step)
+    assert a.host_lens().tolist() == b.host_lens().tolist() == lens
+    q, k, v = new(6)
+    outs = []
+    for cache in (a, b):
+        step = cache.plan([1, 2, 3])
+        outs.append(cache.attend(0, cache.append(0, q, k, v, step, cos, sin), step))
+    assert torch.equal(*outs) and ops.device_error()[0] == 0
