@@ -36,6 +36,7 @@
 #include <map>
 #include <mutex>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/mcb200.h"
@@ -442,16 +443,29 @@ void check_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) 
 // The arrival counters of the paged operators, zero before their first use and left zero by every call: one
 // array per stream, so calls on two streams never share one; a stream under capture gets its own
 // array per capture (zeroed by a node of that graph), so graphs replayed side by side do not either.
+// A capture's array comes from its graph's memory pool and is let go once the stream is seen outside
+// that capture: the pool then goes with its graph, and a graph that lives on still owns the memory and
+// zeroes it in every replay.
 int32_t* paged_counters(const at::Tensor& q, size_t count) {
+  struct Arrays {
+    std::vector<at::Tensor> eager;
+    unsigned long long capture_id = 0;
+    std::vector<at::Tensor> captured;
+  };
   static std::mutex mu;
-  static std::map<std::tuple<int, void*, unsigned long long>, std::vector<at::Tensor>> arrays;
+  static std::map<std::pair<int, void*>, Arrays> per_stream;
   const auto stream = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
   C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
   if (status != cudaStreamCaptureStatusActive) id = 0;
   std::lock_guard<std::mutex> lock(mu);
-  auto& bufs = arrays[{q.device().index(), static_cast<void*>(stream), id}];
+  Arrays& a = per_stream[{q.device().index(), static_cast<void*>(stream)}];
+  if (a.capture_id != id) {
+    a.captured.clear();
+    a.capture_id = id;
+  }
+  auto& bufs = id != 0 ? a.captured : a.eager;
   if (bufs.empty() || static_cast<size_t>(bufs.back().numel()) < count) {
     const int64_t n = std::max<int64_t>(static_cast<int64_t>(count), 1 << 14);
     bufs.push_back(at::zeros({n}, q.options().dtype(at::kInt)));

@@ -163,3 +163,36 @@ def test_release_down_to_a_length(ops, R, hi, page, in_place):
         with pytest.raises(RuntimeError):
             ops.page_release(i32(done), i32(cached), i32(table), queue, st, page_size=page, seqlens_out=new,
                              keep_lens=bad)
+
+
+def test_captures_leave_no_memory_behind(ops):
+    """Steps captured again and again (a server that meets new shapes) and dropped: what the captures took is
+    given back, and the graphs that live on count arrivals of their own."""
+    c, _, _ = attn_case([3000] * 4, [1] * 4, 16, 4, 128, 16, seed=1)
+    call = lambda: ops.paged_attn(c["q"], c["kp"], c["vp"], c["table"], c["cached"], c["cu"], max_new=1)
+    want = call()
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        return graph, out
+
+    def reserved():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.memory_reserved()
+
+    keep, out = capture()
+    capture()
+    before = reserved()
+    for _ in range(12):
+        graph, got = capture()
+        graph.replay()
+        assert torch.equal(got, want)
+        del graph, got
+    assert reserved() <= before
+    for _ in range(3):
+        out.zero_()
+        keep.replay()
+        assert torch.equal(out, want)
