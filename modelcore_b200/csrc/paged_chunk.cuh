@@ -34,7 +34,10 @@
 //
 // Softmax without a maximum on the critical path: the exponent's reference m is the row's maximum over
 // the first tile in which it sees a key, and stays.  P and l may then exceed 1 -- fp32 and bf16
-// reach 2^127 -- and only when a row's sum over 64 keys leaves 2^100 is m moved (see `over` below).
+// reach 2^127 -- and only when a row's sum over 64 keys leaves 2^32 is m moved (see `over` below).
+// O stays below 2^32 (keys / 64) max|V|: values up to 2^78 for 2^20 keys and more, where a running maximum
+// would carry 2^107.  (At 2^100 it overflowed for values of 2^27.  2^32 is 22 units of score above the first
+// tile's maximum; normed queries and keys of rms 1.2 and head size 128 score within +-16.3.)
 // The two threads of a row thus need not meet in a tile.  Rounding: P to bf16 for the product; l sums
 // the unrounded values.
 //
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             // (the same in both warps, which are both at their tile j: no product of O is in flight)
             mx = fmaxf(mx, exchange(mx));
             float alpha = 1.f;
-            if (mx > m_used + 64.f) {  // a row's first keys, or far above its m
+            if (mx > m_used + 24.f) {  // a row's first keys, or far above its m (64 of 2^24 stay below `over`)
               alpha = fast_exp2(m_used - mx);  // 0 when m was -inf
               m_used = mx;
               l *= alpha;
@@ -871,7 +874,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           exp32(a, sc2, nm2, w1, acc0, acc1);
           acc0 = add2(acc0, acc1);
           sum = lo_f(acc0) + hi_f(acc0);
-          const bool over = valid && sum >= 1.2676506e30f;  // 2^100 (not a NaN)
+          const bool over = valid && sum >= 4294967296.f;  // 2^32 (not a NaN)
           if (__builtin_expect(redone || !__any_sync(0xffffffffu, over), 1)) break;
           // Overflow (never where the maximum has just been exchanged, so all_m holds for both warps
           // from here on and they meet only below).  m moves to the maximum of the rows that need it, and

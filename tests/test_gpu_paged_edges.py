@@ -196,3 +196,27 @@ def test_captures_leave_no_memory_behind(ops):
         out.zero_()
         keep.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("D,G,fresh", [(128, 4, 100), (64, 1, 300), (128, 8, 1), (64, 4, 5)])
+@pytest.mark.parametrize("rise", [7, 14, 30, 60])
+def test_large_values_behind_scores_that_rise(ops, D, G, fresh, rise):
+    """Values of 2^60 (and enough requests that an SM has runs of tiles): weights relative to a reference that
+    lies far behind would carry the sums past fp32's range, the result is finite."""
+    cached, scale, R = 1400, 1.0, 60
+    c, ks, vs = attn_case([cached] * R, [fresh] * R, 2 * G, 2, D, 64, seed=11)
+    key = torch.arange(cached + fresh, device="cuda")
+    up = torch.where(key % 512 >= 128, float(rise), 0.0).to(torch.bfloat16)[:, None]
+    q = c["q"].contiguous().mul(0.25)
+    q[..., 0] = 1
+    for r in range(R):
+        ks[r][..., 0] = up
+        vs[r].mul_(2.0 ** 60)
+        page = c["table"][r].long()
+        for pool, x in ((c["kp"], ks[r]), (c["vp"], vs[r])):
+            pool[page[key // 64], :, key % 64] = x
+    want, bound = attn_ref(q, ks, vs, [cached] * R, [fresh] * R, -1, scale)
+    got = ops.paged_attn(q, c["kp"], c["vp"], c["table"], c["cached"], c["cu"], softmax_scale=scale)
+    err = np.abs(got.double().cpu().numpy() - want)
+    # (a score below 2^7 is a sum of fp32 products: off by 2^-13 at most, its weight by that relatively)
+    assert np.isfinite(err).all() and (err <= (2.25 * U + 8.0 * 2.0 ** -13) * bound).all(), (err / bound).max()
