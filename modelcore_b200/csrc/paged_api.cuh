@@ -120,6 +120,13 @@ int page_release(const mcb_page_release_args* a, const int32_t* keep_lens, const
   return MCB_OK;
 }
 
+// (token, head) strides of packed head vectors; the stride of a dimension of one is arbitrary and not used.
+struct PackedStrides {
+  int64_t s[2];
+  PackedStrides(const int64_t (&given)[2], int tokens, int heads, int D)
+      : s{tokens > 1 ? given[0] : static_cast<int64_t>(heads) * D, heads > 1 ? given[1] : D} {}
+};
+
 bool rows16(const void* p, const int64_t (&strides)[2]) {
   return aligned(p, 16) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
 }
@@ -148,11 +155,13 @@ int paged_append(const mcb_paged_append_args* a, void* stream) {
     if (rc != MCB_OK) return rc;
     if (a->n_pages <= 0) return fail(MCB_ERR_INVALID_ARG, "%s: n_pages %d", who, a->n_pages);
   }
+  const PackedStrides qs(a->q_stride, a->N, a->Hq, a->D), ks(a->k_stride, a->N, a->Hkv, a->D),
+      vs(a->v_stride, a->N, a->Hkv, a->D);
   for (int i = 0; i < 2; ++i)
-    if (a->q_stride[i] < 0 || (kv && (a->k_stride[i] < 0 || a->v_stride[i] < 0)))
+    if (qs.s[i] < 0 || (kv && (ks.s[i] < 0 || vs.s[i] < 0)))
       return fail(MCB_ERR_INVALID_ARG, "%s: negative stride", who);
-  if (!rows16(a->q, a->q_stride) || !aligned(a->q_out, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16) ||
-      (kv && (!rows16(a->k, a->k_stride) || !rows16(a->v, a->v_stride) || !aligned(a->k_pages, 16) ||
+  if (!rows16(a->q, qs.s) || !aligned(a->q_out, 16) || !aligned(a->cos, 16) || !aligned(a->sin, 16) ||
+      (kv && (!rows16(a->k, ks.s) || !rows16(a->v, vs.s) || !aligned(a->k_pages, 16) ||
               !aligned(a->v_pages, 16))))
     return fail(MCB_ERR_ALIGNMENT, "%s: head vectors, tables and pages must start on 16-byte boundaries", who);
   mcb::PagedAppendParams p = {};
@@ -160,9 +169,9 @@ int paged_append(const mcb_paged_append_args* a, void* stream) {
   p.k = static_cast<const uint16_t*>(a->k);
   p.v = static_cast<const uint16_t*>(a->v);
   for (int i = 0; i < 2; ++i) {
-    p.qs[i] = a->q_stride[i];
-    p.ks[i] = a->k_stride[i];
-    p.vs[i] = a->v_stride[i];
+    p.qs[i] = qs.s[i];
+    p.ks[i] = ks.s[i];
+    p.vs[i] = vs.s[i];
   }
   p.q_out = static_cast<uint16_t*>(a->q_out);
   p.k_pages = static_cast<uint16_t*>(a->k_pages);
@@ -376,11 +385,10 @@ int paged_attn(const mcb_paged_attn_args* a, void* stream) {
   if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr ||
       a->cu_new == nullptr || (a->R > 0 && (a->block_table == nullptr || a->cache_seqlens == nullptr)))
     return fail(MCB_ERR_INVALID_ARG, "%s: NULL pointer argument", who);
-  if (a->q_stride[0] < 0 || a->q_stride[1] < 0 || a->table_stride < a->max_pages)
+  const PackedStrides qs(a->q_stride, a->N, a->Hq, a->D);
+  const auto& q_stride = qs.s;
+  if (q_stride[0] < 0 || q_stride[1] < 0 || a->table_stride < a->max_pages)
     return fail(MCB_ERR_INVALID_ARG, "%s: negative q stride or table_stride below max_pages", who);
-  // the stride of a dimension of one is arbitrary (and not used)
-  const int64_t q_stride[2] = {a->N > 1 ? a->q_stride[0] : static_cast<int64_t>(a->Hq) * a->D,
-                               a->Hq > 1 ? a->q_stride[1] : a->D};
   if (!rows16(a->q, q_stride) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
     return fail(MCB_ERR_ALIGNMENT, "%s: q rows, out and pages must start on 16-byte boundaries", who);
   const PagedAttnPlan pl = plan_paged_attn(a);

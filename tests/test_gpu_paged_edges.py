@@ -220,3 +220,27 @@ def test_large_values_behind_scores_that_rise(ops, D, G, fresh, rise):
     err = np.abs(got.double().cpu().numpy() - want)
     # (a score below 2^7 is a sum of fp32 products: off by 2^-13 at most, its weight by that relatively)
     assert np.isfinite(err).all() and (err <= (2.25 * U + 8.0 * 2.0 ** -13) * bound).all(), (err / bound).max()
+
+
+def test_a_dimension_of_one_has_any_stride(ops):
+    """One token, or one head: torch may give its dimension any stride, and it is not used."""
+    from test_gpu_paged import append_inputs, tables
+    cos, sin = tables(300, 64)
+    odd = lambda x, d: x.contiguous().as_strided(x.shape, [13 if i == d else s for i, s in
+                                                           enumerate(x.contiguous().stride())])
+    for N, H, d in ((1, 4, 0), (6, 1, 1)):
+        (q, k, v), slots, pos, (kp, vp) = append_inputs(N, H, H, 64, 16, 9)
+        kp2, vp2 = kp.clone(), vp.clone()
+        want = ops.paged_append_rope(q, k, v, kp, vp, pos, slots, cos, sin)
+        got = ops.paged_append_rope(odd(q, d), odd(k, d), odd(v, d), kp2, vp2, pos, slots, cos, sin)
+        assert torch.equal(got, want) and torch.equal(kp2[slots // 16, :, slots % 16], kp[slots // 16, :, slots % 16])
+        assert torch.equal(vp2[slots // 16, :, slots % 16], vp[slots // 16, :, slots % 16])
+
+
+def test_one_query_for_all(ops):
+    """Queries expanded over tokens or heads (a stride of 0) are what their copies are."""
+    for fresh in ([40, 3], [1, 1]):
+        c, _, _ = attn_case([90, 10], fresh, 4, 2, 64, 16)
+        for q in (c["q"][:1].expand(sum(fresh), 4, 64), c["q"][:, :1].expand(sum(fresh), 4, 64)):
+            call = lambda x: ops.paged_attn(x, c["kp"], c["vp"], c["table"], c["cached"], c["cu"])
+            assert torch.equal(call(q), call(q.contiguous()))
