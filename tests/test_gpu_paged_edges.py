@@ -244,3 +244,42 @@ def test_one_query_for_all(ops):
         for q in (c["q"][:1].expand(sum(fresh), 4, 64), c["q"][:, :1].expand(sum(fresh), 4, 64)):
             call = lambda x: ops.paged_attn(x, c["kp"], c["vp"], c["table"], c["cached"], c["cu"])
             assert torch.equal(call(q), call(q.contiguous()))
+
+
+def test_the_paged_step_under_torch_compile(ops):
+    """plan, append (keys and values, and queries alone), attention and release as nodes of a compiled graph:
+    the results and what is written in place are the eager step's."""
+    from test_gpu_paged import tables
+    Hq, Hkv, D, page, R = 8, 2, 128, 16, 3
+    cos, sin = tables(400, D)
+    g = torch.Generator("cuda").manual_seed(5)
+    qkv = torch.randn(R, Hq + 2 * Hkv, D, device="cuda", generator=g).to(torch.bfloat16)
+    q, k, v = qkv.split([Hq, Hkv, Hkv], 1)
+    ones, done = i32([1] * R), i32([0, 1, 0])
+    from modelcore_b200 import torch_ops  # noqa: F401
+    m = torch.ops.mcb200
+
+    def step(lens, table, queue, state, kp, vp):
+        state2 = torch.empty_like(state)
+        cu, pos, slots = m.page_plan(lens, ones, table, queue, state, state2, page, R)
+        qr = m.paged_append_rope(q, k, v, kp, vp, pos, slots, cos, sin)
+        alone = m.paged_append_rope(q, None, None, None, None, pos, None, cos, sin)
+        out = m.paged_attn(qr, kp, vp, table, lens, cu, window=100, max_new=1)
+        lens += ones
+        m.page_release(done, lens, table, queue, state2, state2, lens, page)
+        return out * 1.0, alone, state2, cu, pos, slots
+
+    def fresh():
+        pool = lambda s: torch.randn(40, Hkv, page, D, device="cuda", generator=torch.Generator("cuda").manual_seed(s)
+                                     ).to(torch.bfloat16)
+        return [i32([0, 90, 300]), i32(np.arange(R * 30).reshape(R, 30) % 30), i32(np.arange(40)),
+                torch.tensor([30, 40], device="cuda"), pool(1), pool(2)]
+
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    a, b = fresh(), fresh()
+    for _ in range(3):
+        for x, y in zip(step(*a), compiled(*b)):
+            assert torch.equal(x, y)
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+        a[3], b[3] = (torch.tensor([30, 40], device="cuda") for _ in range(2))
