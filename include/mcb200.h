@@ -494,10 +494,12 @@ int mcb_paged_append_rope(const mcb_paged_append_args* args, void* stream);
 /* mcb_paged_attn: out[t, h] = softmax_c(q[t, h] . K[c, h / G] * softmax_scale) . V[c, h / G] for
  * the packed new tokens t of every request, over the request's keys c at positions c <= pos and
  * (window < 0 or pos - c <= window), pos = cache_seqlens[r] + t - cu_new[r].  The new tokens' keys
- * and values are already in the pages.  Tokens past cu_new[R] get zeros; nothing past a request's
- * last position, or before the first its tokens see, reaches the result, whatever the pages hold
- * there.  max_new: an upper bound on the requests' new tokens when the caller knows one, 0 when
- * not: it chooses which kernels are launched, never the result's meaning. */
+ * and values are already in the pages.  Tokens before cu_new[0] and past cu_new[R] get zeros.
+ * Nothing past a request's last position, or before the first its tokens see, reaches the result,
+ * whatever the pages hold there.  (A value of infinity or NaN that some tokens of a request see
+ * reaches the tokens just before it too, as a product of masked weights with it would have it.)
+ * max_new: an upper bound on the requests' new tokens when the caller knows one, 0 when not: it
+ * chooses which kernels are launched, never the result's meaning. */
 typedef struct {
   const void* q;                  /* (N, Hq, D) bf16, element strides q_stride (token, head)    */
   int64_t q_stride[2];

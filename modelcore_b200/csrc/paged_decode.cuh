@@ -171,14 +171,16 @@ __device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedWalk& 
   }
 }
 
-// Zeroes the output of the padding tokens, [cu_new[R], N): threads 0 .. threads - 1 of every CTA.
+// Zeroes the output of the tokens that no request has, [0, cu_new[0]) and [cu_new[R], N): threads 0 ..
+// threads - 1 of every CTA.
 __device__ __forceinline__ void paged_fill(const PagedAttnParams& p, int D, int threads) {
   const long long per = static_cast<long long>(p.Hq) * D / 8;  // 16-byte words a token
-  const long long from = static_cast<long long>(min(max(p.cu_new[p.R], 0), p.N)) * per;
+  const int first = min(max(p.cu_new[0], 0), p.N), last = max(min(p.cu_new[p.R], p.N), first);
+  const long long lead = first * per, gap = (last - first) * per, end = p.N * per;
   uint4* out = reinterpret_cast<uint4*>(p.out);
-  for (long long i = from + static_cast<long long>(blockIdx.x) * threads + threadIdx.x;
-       i < static_cast<long long>(p.N) * per; i += static_cast<long long>(gridDim.x) * threads)
-    out[i] = make_uint4(0, 0, 0, 0);
+  for (long long i = static_cast<long long>(blockIdx.x) * threads + threadIdx.x; i < end - gap;
+       i += static_cast<long long>(gridDim.x) * threads)
+    out[i < lead ? i : i + gap] = make_uint4(0, 0, 0, 0);
 }
 
 // Merges the partials of a cut unit into its output rows, one warp a row: contributors g_first ..

@@ -754,7 +754,7 @@ def paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, *, windo
     on and see every earlier position and their own, within `window` back (< 0: all).  Chunks of
     prompts and single-token steps mix freely.  max_new: the largest number of new tokens of a
     request when the caller knows it (0: unknown; a decode step with 1 needs one launch less).
-    Returns (N, Hq, D) bf16, zeros past cu_new[R]."""
+    Returns (N, Hq, D) bf16, zeros before cu_new[0] and past cu_new[R]."""
     return _PAGED.paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new,
                                -1 if window is None else window, softmax_scale, max_new)
 

@@ -283,3 +283,15 @@ def test_the_paged_step_under_torch_compile(ops):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
         a[3], b[3] = (torch.tensor([30, 40], device="cuda") for _ in range(2))
+
+
+def test_tokens_before_the_first_request_are_padding_too(ops):
+    """A batch whose first request starts after token 0: nobody's tokens come out as zeros, before and after."""
+    for fresh in ([1, 2], [70, 5]):
+        c, ks, vs = attn_case([30, 200], fresh, 4, 2, 64, 16, tail=9)
+        at = c["cu"] + 4
+        want = ops.paged_attn(c["q"][4:].contiguous(), c["kp"], c["vp"], c["table"], c["cached"], c["cu"])
+        junk = torch.full_like(c["q"].contiguous(), float("nan"))
+        del junk  # (the output's memory, as like as not)
+        got = ops.paged_attn(c["q"], c["kp"], c["vp"], c["table"], c["cached"], at)
+        assert not got[:4].any() and torch.equal(got[4:], want)
