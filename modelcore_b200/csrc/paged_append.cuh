@@ -13,8 +13,10 @@
 // and the heads go by in steps of 32 / (D/16) vectors, D/16 lanes each, the next step's loads in flight.
 // With a vector's position and table row read per vector the two dependent loads ahead of every
 // vector bounded it.  16,381 tokens of 16/4 heads of 128 (206 MB): 43 us so, 40 us now, 5.2 TB/s; two
-// or more steps in flight cost registers and with them warps (44 to 65 us).  Bound by HBM (each
-// byte read and written once) for long batches, by launch and dependent-load latency for a decode step.
+// or more steps in flight cost registers and with them warps (44 to 65 us).  Every step rounded to bf16
+// 41 us (both 33.5 at 12/12 heads of 64, 153 MB).  64 registers, with 28 bytes spilled in the form rounded once.
+// Bound by HBM (each byte read and written once) for long batches, by launch and dependent-load
+// latency for a decode step.
 #pragma once
 
 #include "common.cuh"

@@ -27,10 +27,12 @@
 // products, which it does not (1,600 cycles against 1,024), and both then waited: 3,700 cycles a key
 // tile where the products take 2,048.  N = 64 costs the tensor cores a quarter more (S reads Q from
 // shared memory once for 64 keys: 384 cycles for 256 worth) and the rest overlaps: 2,560 of some 3,300.
-// Measured, 16/4 heads of 128: 8,192 tokens after 8,192 767 us, 1,075 TFLOP/s at the 1.45 GHz that the
-// power limit leaves; five chunks of 2,041 under a window of 1,024 119 us, 600 TFLOP/s -- nine key tiles
-// a unit there, and a unit costs some 12,000 cycles beside its tiles: the first tile's maximum and the
-// masks at both ends (5,500), the last product and O's way out (6,000).
+// Measured, 16/4 heads of 128, as called (and back to back in a graph): 8,192 tokens after 8,192 766 us
+// (741), 1,077 TFLOP/s at the 1.45 GHz that the power limit leaves; five chunks of 2,041 under a window of
+// 1,024 124 us (118), 574 TFLOP/s -- nine key tiles a unit there, and a unit costs some 12,000 cycles beside
+// its tiles: the first tile's maximum and the masks at both ends (5,500), the last product and O's way out
+// (6,000).  96 registers a thread, the most that 640 threads allow, with 48 bytes spilled (44 at head size
+// 64) around the rare branches.
 //
 // Softmax without a maximum on the critical path: the exponent's reference m is the row's maximum over
 // the first tile in which it sees a key, and stays.  P and l may then exceed 1 -- fp32 and bf16
@@ -341,8 +343,8 @@ __device__ __noinline__ float tmem_prep(uint32_t addr, bool mask, int lo, int hi
 
 // 32 of a row's weights, 2^(s * scale - m): packed bf16 into w, the unrounded ones added to acc.  (A
 // polynomial on the FMA pipe for some of them, to spare the special function unit's 16 a clock, lost: it
-// costs the issue slots that the four chains' warps share.  8,192 after 8,192: 748 us without, 750, 760,
-// 789 and 818 with one pair of sixteen, one, two and three of eight.)
+// costs the issue slots that the four chains' warps share.  8,192 after 8,192, in one run back to back in
+// a graph: 748 us without, 750, 760, 789 and 818 with one pair of sixteen, one, two and three of eight.)
 __device__ __forceinline__ void exp32(const uint32_t (&s)[32], uint64_t sc2, uint64_t nm2, uint32_t (&w)[16],
                                       uint64_t& acc0, uint64_t& acc1) {
 #pragma unroll

@@ -24,9 +24,11 @@
 // with an online softmax in fp32 a warp, P rounded to bf16 for the product (its sum l is of the
 // unrounded values), and a merge of the eight through shared memory after each unit.
 //
-// Measured: 128 requests at 1,024 to 8,192 positions, 16/4 heads of 128 (1.27 GB): 192 us, 6.6 TB/s; 13
-// of 4 tokens at 8,192 to 32,700, 32/8 heads (0.97 GB) 159 us; 3 requests of 12 heads of 64 at 500 to
-// 1,023 6.6 us, all of it latency (launch, lengths, page numbers, keys, merge: a chain of loads).
+// Measured as called (and back to back in a graph): 128 requests at 1,024 to 8,192 positions, 16/4 heads of
+// 128 (1.27 GB) 199 us (193), 6.4 TB/s; 13 of 4 tokens at 8,192 to 32,700, 32/8 heads (0.97 GB) 167 us (160);
+// 64 of 12/12 heads of 64 at 1,024 to 8,192 (0.97 GB) 149 in a graph, 16 query rows a kv head (16/1 heads of
+// 128, 128 requests, 0.32 GB) 72; 3 requests of 12 heads of 64 at 500 to 1,023 8.4 us (6.6), all of it
+// latency (launch, lengths, page numbers, keys, merge: a chain of loads).
 //
 // Positions of a tile outside [lo, hi] may hold anything (another request's old values, NaN): their
 // scores are replaced by -inf and their value rows are zeroed in shared memory, since 0 * NaN is NaN.
