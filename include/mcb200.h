@@ -526,13 +526,148 @@ size_t mcb_paged_attn_counter_count(const mcb_paged_attn_args* args);
 int mcb_paged_attn(const mcb_paged_attn_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Speculative decoding over the paged cache.  A request's new tokens of a step may be a tree: token t
+ * follows its parent, parents[t], an earlier one of the request's (counted from its first), or the
+ * cached tokens (-1).  Not in the reference, which generates a token at a time (modelcore/generate.py:88-94).
+ *
+ * mcb_draft_tree: positions[t] = cache_seqlens[r] + the number of t's ancestors among the new tokens,
+ * and mask, bit j % 32 of word j / 32 of token t set where new token j is t or an ancestor.  A
+ * request of more than 32 words new tokens is a chunk of a prompt: positions follow each other, and its masks
+ * are zero.  Tokens that no request has get position -1.  A parent that is no earlier token sets device error 8
+ * and counts as -1.  The slots remain mcb_page_plan's: token t of a request at cache_seqlens[r] + t.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  const int32_t* parents;         /* (N,)                                                       */
+  const int32_t* cu_new;          /* (R + 1,)                                                   */
+  const int32_t* cache_seqlens;   /* (R,)                                                       */
+  int32_t* positions;             /* (N,)                                                       */
+  int32_t* mask;                  /* (N, words)                                                 */
+  int32_t R, N, words;            /* words: 1 to 8                                              */
+} mcb_draft_tree_args;
+
+int mcb_draft_tree(const mcb_draft_tree_args* args, void* stream);
+
+/* mcb_paged_tree_attn: mcb_paged_attn for such trees.  Token t sees the cached positions c < cache_seqlens[r]
+ * with positions[t] - c <= window, and the new tokens j of its request with mask bit j and positions[t] -
+ * positions[j] <= window (window < 0: all).  Any mask is taken, draft_tree's or another; a token that sees
+ * nothing gets zeros.  positions below cache_seqlens[r] count as that.  A request of more than 32 words new
+ * tokens is a chunk, as in mcb_paged_attn (its positions and masks are not read).  What is said there of
+ * padding tokens and of what the pages hold elsewhere holds here; a new token's value of infinity or NaN
+ * reaches the request's other new tokens too. */
+typedef struct {
+  mcb_paged_attn_args attn;
+  const int32_t* positions;       /* (N,)                                                       */
+  const int32_t* mask;            /* (N, words)                                                 */
+  int32_t words;                  /* 1 to 8                                                     */
+} mcb_paged_tree_attn_args;
+
+size_t mcb_paged_tree_attn_workspace_size(const mcb_paged_tree_attn_args* args);
+int mcb_paged_tree_attn(const mcb_paged_tree_attn_args* args, void* stream);
+
+/* mcb_verify_drafts: which drafted tokens the target keeps, and the token after them.  logits[t] are the
+ * target's after token t; token 0 of a request is part of its answer already, the others were drafted to
+ * follow their parents.  A walk from token 0: at token u, with rest = p = softmax(logits[u] /
+ * temperature), u's children c in order, x their token:
+ *   c is kept where accept[c] * q(x) * sum(rest) < rest(x), and the walk goes on at c; else
+ *   rest = max(rest / sum(rest) - q, 0)       with q = draft_probs[u], which the children were drawn from,
+ *   rest(x) = 0                               without draft_probs (q(x) = 1 above),
+ *   rest = p again where nothing is left.
+ * Where no child is kept, next_token is the first x with rest(0) + ... + rest(x) > draws[r] * sum(rest).
+ * accept and draws in [0, 1): the tokens are then distributed as the target's own.  temperature 0: a child is
+ * kept where its token is the first of the largest logit, which is next_token otherwise.  path: the kept
+ * tokens' places in the request, token 0 first, then -1; accepted: how many.  A walk ends after max_path
+ * tokens, and at most 256 children of a token are tried.  A request without tokens: 0 and -1.  A
+ * row of logits with a NaN, +infinity or nothing above -infinity: device error 9, and the walk ends
+ * with next_token -1; a token outside [0, V): device error 4, not kept. */
+typedef struct {
+  const void* logits;             /* (N, V) fp32 or bf16, rows logits_stride elements apart     */
+  int64_t logits_stride;
+  const int64_t* tokens;          /* (N,)                                                       */
+  const int32_t* parents;         /* (N,)                                                       */
+  const int32_t* cu_new;          /* (R + 1,)                                                   */
+  const float* accept;            /* (N,) uniforms, a token's own                               */
+  const float* draws;             /* (R,) uniforms                                              */
+  const float* draft_probs;       /* (N, V) fp32 or NULL                                        */
+  int64_t draft_stride;
+  int32_t* accepted;              /* (R,)                                                       */
+  int32_t* path;                  /* (R, max_path)                                              */
+  int64_t* next_token;            /* (R,)                                                       */
+  int32_t R, N, V, max_path;
+  int32_t logits_bf16;
+  float temperature;
+} mcb_verify_drafts_args;
+
+int mcb_verify_drafts(const mcb_verify_drafts_args* args, void* stream);
+
+/* mcb_paged_keep: a step's kept path becomes part of its rows.  In every slot and head position
+ * cache_seqlens[r] + i gets what cache_seqlens[r] + path[r][i] holds, i < accepted[r] (path as
+ * mcb_verify_drafts writes it: growing); seqlens_out[r] = cache_seqlens[r] + accepted[r]; the pages
+ * from there to the step's last, cache_seqlens[r] + new_lens[r], go to the queue's tail in request order.
+ * free_state_out may be free_state, seqlens_out cache_seqlens.  accepted above new_lens or P, or a path
+ * entry below its place or past new_lens, sets device error 8: the former counts as the limit, the latter is not
+ * moved.  Device errors 1, 5 and 6 as in mcb_page_release. */
+typedef struct {
+  const int32_t* path;            /* (R, P), rows path_stride apart                             */
+  int64_t path_stride;
+  const int32_t* accepted;        /* (R,)                                                       */
+  const int32_t* cache_seqlens;   /* (R,) before the step                                       */
+  const int32_t* new_lens;        /* (R,) the step's                                            */
+  const int32_t* block_table;     /* (R, max_pages)                                             */
+  int64_t table_stride;
+  int32_t* free_pages;            /* (n_pages,)                                                 */
+  const int64_t* free_state;      /* (2,)                                                       */
+  int64_t* free_state_out;        /* (2,)                                                       */
+  int32_t* seqlens_out;           /* (R,)                                                       */
+  void* k_pages;                  /* (slots, n_pages, Hkv, page_size, D) bf16                   */
+  void* v_pages;
+  int32_t* counter;               /* one int32, zero before the call and after it               */
+  int32_t R, P, slots, Hkv, D, n_pages, max_pages, page_size;
+} mcb_paged_keep_args;
+
+int mcb_paged_keep(const mcb_paged_keep_args* args, void* stream);
+
+/* mcb_page_fork: row r becomes what row source[r] was (-1: empty), all rows at once: samples of one
+ * prompt, a beam search's step, finished rows given back.  Full pages are shared: shares[x] is one less
+ * than the rows that hold page x (0 for one row's own and for free ones).  A last page that is not
+ * full stays with the first row that takes it over; every other one gets a fresh page from the queue, in row
+ * order, and a copy of the positions in use in every slot.  Pages that no row holds any more go to the
+ * queue's tail in page order.  block_table_out gets -1 beyond a row's pages.  Each output may be the
+ * input of its kind.  source above R - 1 sets device error 8 and counts as -1; a queue that runs out 5 (the
+ * page is -1), an entry outside the pool 6, a length past the table 1.
+ * A row that shares pages is given back by this call, not by mcb_page_release, and is not shortened below
+ * the length it was forked at. */
+typedef struct {
+  const int32_t* source;          /* (R,)                                                       */
+  const int32_t* cache_seqlens;   /* (R,)                                                       */
+  const int32_t* block_table;     /* (R, max_pages)                                             */
+  int64_t table_stride;
+  const int32_t* shares;          /* (n_pages,)                                                 */
+  int32_t* free_pages;            /* (n_pages,)                                                 */
+  const int64_t* free_state;      /* (2,)                                                       */
+  void* k_pages;                  /* (slots, n_pages, Hkv, page_size, D) bf16                   */
+  void* v_pages;
+  int32_t* block_table_out;       /* (R, max_pages)                                             */
+  int64_t table_out_stride;
+  int32_t* shares_out;            /* (n_pages,)                                                 */
+  int64_t* free_state_out;        /* (2,)                                                       */
+  int32_t* seqlens_out;           /* (R,)                                                       */
+  void* workspace;                /* mcb_page_fork_workspace_size() bytes, 256-byte aligned     */
+  size_t workspace_bytes;
+  int32_t R, slots, Hkv, D, n_pages, max_pages, page_size;
+} mcb_page_fork_args;
+
+size_t mcb_page_fork_workspace_size(const mcb_page_fork_args* args);
+int mcb_page_fork(const mcb_page_fork_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Device-side status.  Kernels never trap: an out-of-range position (a cache or rotary table
  * overflow) or a timed-out pipeline wait sets a device error word and skips the access.
  * mcb_device_error synchronises `stream`, returns the word in *code and clears it.
  * Codes: 0 none, 1 position beyond Tmax, 2 position beyond the rotary table, 3 pipeline wait
  * timed out, 4 token id outside the embedding table, 5 the free pages do not match the request
  * (too few to take, or returned twice), 6 a page or slot outside the pool, 7 more new tokens than
- * the packed batch holds.
+ * the packed batch holds, 8 a drafted token's parent, a kept path or a fork's source out of its range, 9
+ * logits without probabilities.
  * ------------------------------------------------------------------------------------------- */
 int mcb_device_error(int32_t* code, void* stream);
 

@@ -37,6 +37,8 @@ DEVICE_ERRORS = {
     5: "the free pages do not match the request (too few to take, or returned twice)",
     6: "a page or slot outside the pool",
     7: "more new tokens than the packed batch holds",
+    8: "a drafted token's parent, a kept path or a fork's source out of its range",
+    9: "logits without probabilities (NaN, +infinity or nothing above -infinity)",
 }
 
 ABI_VERSION = 9
@@ -67,6 +69,13 @@ EXPORTED_SYMBOLS = (
     "mcb_page_plan",
     "mcb_page_release",
     "mcb_page_release_to",
+    "mcb_draft_tree",
+    "mcb_paged_tree_attn_workspace_size",
+    "mcb_paged_tree_attn",
+    "mcb_verify_drafts",
+    "mcb_paged_keep",
+    "mcb_page_fork_workspace_size",
+    "mcb_page_fork",
     "mcb_paged_append_rope",
     "mcb_paged_attn_workspace_size",
     "mcb_paged_attn_counter_count",
@@ -254,6 +263,58 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+class DraftTreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("parents", ctypes.c_void_p), ("cu_new", ctypes.c_void_p), ("cache_seqlens", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("R", ctypes.c_int32),
+        ("N", ctypes.c_int32), ("words", ctypes.c_int32),
+    ]
+
+
+class PagedTreeAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("attn", PagedAttnArgs), ("positions", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("words", ctypes.c_int32),
+    ]
+
+
+class VerifyDraftsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("logits_stride", ctypes.c_int64), ("tokens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p), ("cu_new", ctypes.c_void_p), ("accept", ctypes.c_void_p),
+        ("draws", ctypes.c_void_p), ("draft_probs", ctypes.c_void_p), ("draft_stride", ctypes.c_int64),
+        ("accepted", ctypes.c_void_p), ("path", ctypes.c_void_p), ("next_token", ctypes.c_void_p),
+        ("R", ctypes.c_int32), ("N", ctypes.c_int32), ("V", ctypes.c_int32), ("max_path", ctypes.c_int32),
+        ("logits_bf16", ctypes.c_int32), ("temperature", ctypes.c_float),
+    ]
+
+
+class PagedKeepArgs(ctypes.Structure):
+    _fields_ = [
+        ("path", ctypes.c_void_p), ("path_stride", ctypes.c_int64), ("accepted", ctypes.c_void_p),
+        ("cache_seqlens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64), ("free_pages", ctypes.c_void_p), ("free_state", ctypes.c_void_p),
+        ("free_state_out", ctypes.c_void_p), ("seqlens_out", ctypes.c_void_p), ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p), ("counter", ctypes.c_void_p), ("R", ctypes.c_int32),
+        ("P", ctypes.c_int32), ("slots", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class PageForkArgs(ctypes.Structure):
+    _fields_ = [
+        ("source", ctypes.c_void_p), ("cache_seqlens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64), ("shares", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("free_state", ctypes.c_void_p), ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+        ("block_table_out", ctypes.c_void_p), ("table_out_stride", ctypes.c_int64),
+        ("shares_out", ctypes.c_void_p), ("free_state_out", ctypes.c_void_p),
+        ("seqlens_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t), ("R", ctypes.c_int32), ("slots", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
 class McbError(RuntimeError):
     """A C-ABI call returned a non-zero mcb_status."""
 
@@ -317,6 +378,15 @@ def _declare(lib):
     for name in ("mcb_paged_attn_workspace_size", "mcb_paged_attn_counter_count"):
         getattr(lib, name).restype = ctypes.c_size_t
         getattr(lib, name).argtypes = [P(PagedAttnArgs)]
+    for name, cls in (("mcb_draft_tree", DraftTreeArgs), ("mcb_paged_tree_attn", PagedTreeAttnArgs),
+                      ("mcb_verify_drafts", VerifyDraftsArgs), ("mcb_paged_keep", PagedKeepArgs),
+                      ("mcb_page_fork", PageForkArgs)):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [P(cls), ctypes.c_void_p]
+    for name, cls in (("mcb_paged_tree_attn_workspace_size", PagedTreeAttnArgs),
+                      ("mcb_page_fork_workspace_size", PageForkArgs)):
+        getattr(lib, name).restype = ctypes.c_size_t
+        getattr(lib, name).argtypes = [P(cls)]
     lib.mcb_last_attn_kernel.restype = ctypes.c_int
     lib.mcb_last_attn_kernel.argtypes = [ctypes.c_char_p, ctypes.c_size_t]
 

@@ -21,6 +21,8 @@ enum DeviceError : int {
   kErrPagesExhausted = 5,
   kErrPageOutOfRange = 6,
   kErrTooManyTokens = 7,
+  kErrDraftOutOfRange = 8,
+  kErrNoProbabilities = 9,
 };
 // Defined once here: the library is a single translation unit (mcb200.cu).
 __device__ int g_device_error = 0;

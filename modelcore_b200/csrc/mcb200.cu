@@ -18,15 +18,19 @@
 #include "common.cuh"
 #include "decode_attn.cuh"
 #include "decode_attn_split.cuh"
+#include "draft_tree.cuh"
 #include "kv_append.cuh"
 #include "kv_copy.cuh"
+#include "page_fork.cuh"
 #include "paged_append.cuh"
 #include "paged_chunk.cuh"
 #include "paged_plan.cuh"
+#include "paged_tree.cuh"
 #include "prefill_attn.cuh"
 #include "decode_proj.cuh"
 #include "sample.cuh"
 #include "step_fused.cuh"
+#include "verify.cuh"
 
 namespace {
 
@@ -1676,3 +1680,4 @@ int mcb_device_error(int32_t* code, void* stream) {
 }  // extern "C"
 
 #include "paged_api.cuh"
+#include "draft_api.cuh"

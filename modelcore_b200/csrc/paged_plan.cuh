@@ -62,7 +62,7 @@ __device__ __forceinline__ bool last_cta(int* counter, bool& flag) {
   const int mine = __syncthreads_or(flag) ? kFlag + 1 : 1;
   if (threadIdx.x == 0) {
     const int all = atom_add_acq_rel_gpu(counter, mine) + mine;
-    s_last = (all & (kFlag - 1)) == static_cast<int>(gridDim.x) ? (all >= kFlag ? 3 : 1) : 0;
+    s_last = (all & (kFlag - 1)) == static_cast<int>(gridDim.x * gridDim.y) ? (all >= kFlag ? 3 : 1) : 0;
     if (s_last) *counter = 0;
   }
   __syncthreads();

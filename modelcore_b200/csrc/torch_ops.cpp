@@ -18,6 +18,10 @@
 //   page_plan, page_release, paged_append_rope, paged_attn
 //                   the paged cache: one step's block tables and slots, a finished request's
 //                   pages back, the append and the attention over pages (include/mcb200.h)
+//   draft_tree, paged_tree_attn, verify_drafts, paged_keep
+//                   trees of drafted tokens over the paged cache: positions and masks, attention,
+//                   verification, the kept path's keys and values moved together
+//   page_fork       rows of the paged cache become copies of rows, full pages shared
 //
 // Every op runs on the current CUDA stream of its tensors' device, checks dtypes, devices and
 // dimensions here (TORCH_CHECK: a RuntimeError in Python) and leaves sizes, strides and
@@ -609,28 +613,23 @@ at::Tensor paged_append_rope(const at::Tensor& q, const std::optional<at::Tensor
   return q_out;
 }
 
-at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                      const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
-                      int64_t window, std::optional<double> softmax_scale, int64_t max_new) {
-  need(q, "q", 3, at::kBFloat16);
-  c10::cuda::CUDAGuard guard(q.device());
+// What paged_attn and paged_tree_attn have alike: everything but the output, workspace and counters.
+void fill_paged_attn(mcb_paged_attn_args& a, const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                     const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
+                     int64_t window, std::optional<double> softmax_scale, int64_t max_new) {
   check_pages(k_pages, v_pages, q);
   need(cache_seqlens, "cache_seqlens", 1, at::kInt);
   const int64_t R = cache_seqlens.size(0);
   int_vec(cache_seqlens, "cache_seqlens", R, q, at::kInt);
   int_vec(cu_new, "cu_new", R + 1, q, at::kInt);
-  const int64_t table_stride = check_block_table(block_table, R, q);
-  at::Tensor out = new_tensor(q.sizes(), q, at::kBFloat16);
-  mcb_paged_attn_args a = {};
+  a.table_stride = check_block_table(block_table, R, q);
   a.q = q.data_ptr();
   packed_strides(q, "q", a.q_stride);
   a.k_pages = k_pages.data_ptr();
   a.v_pages = v_pages.data_ptr();
   a.block_table = block_table.data_ptr<int32_t>();
-  a.table_stride = table_stride;
   a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
   a.cu_new = cu_new.data_ptr<int32_t>();
-  a.out = out.data_ptr();
   a.R = to_i32(R, "R");
   a.N = to_i32(q.size(0), "N");
   a.Hq = to_i32(q.size(1), "Hq");
@@ -643,6 +642,17 @@ at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::
   a.max_new = to_i32(max_new, "max_new");
   a.softmax_scale = softmax_scale.has_value() ? static_cast<float>(*softmax_scale)
                                               : static_cast<float>(1.0 / std::sqrt(static_cast<double>(q.size(2))));
+}
+
+at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                      const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
+                      int64_t window, std::optional<double> softmax_scale, int64_t max_new) {
+  need(q, "q", 3, at::kBFloat16);
+  c10::cuda::CUDAGuard guard(q.device());
+  mcb_paged_attn_args a = {};
+  fill_paged_attn(a, q, k_pages, v_pages, block_table, cache_seqlens, cu_new, window, softmax_scale, max_new);
+  at::Tensor out = new_tensor(q.sizes(), q, at::kBFloat16);
+  a.out = out.data_ptr();
   if (a.N == 0) return out;
   at::Tensor ws;
   const size_t bytes = mcb_paged_attn_workspace_size(&a);
@@ -658,6 +668,222 @@ at::Tensor paged_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::
   }
   check_status(mcb_paged_attn(&a, stream_of(q)), "mcb200::paged_attn");
   return out;
+}
+
+// -- speculative decoding and shared pages ---------------------------------------------------
+std::tuple<at::Tensor, at::Tensor> draft_tree(const at::Tensor& parents, const at::Tensor& cu_new,
+                                              const at::Tensor& cache_seqlens, int64_t max_tree) {
+  need(parents, "parents", 1, at::kInt);
+  c10::cuda::CUDAGuard guard(parents.device());
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  const int64_t N = parents.size(0), R = cache_seqlens.size(0);
+  int_vec(parents, "parents", N, parents, at::kInt);
+  int_vec(cache_seqlens, "cache_seqlens", R, parents, at::kInt);
+  int_vec(cu_new, "cu_new", R + 1, parents, at::kInt);
+  TORCH_CHECK(max_tree >= 1 && max_tree <= 256, "max_tree must be from 1 to 256 new tokens, got ", max_tree);
+  mcb_draft_tree_args a = {};
+  a.words = static_cast<int32_t>((max_tree + 31) / 32);
+  at::Tensor positions = new_tensor({N}, parents, at::kInt);
+  at::Tensor mask = new_tensor({N, a.words}, parents, at::kInt);
+  a.parents = parents.data_ptr<int32_t>();
+  a.cu_new = cu_new.data_ptr<int32_t>();
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.positions = positions.data_ptr<int32_t>();
+  a.mask = mask.data_ptr<int32_t>();
+  a.R = to_i32(R, "R");
+  a.N = to_i32(N, "N");
+  check_status(mcb_draft_tree(&a, stream_of(parents)), "mcb200::draft_tree");
+  return {positions, mask};
+}
+
+at::Tensor paged_tree_attn(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                           const at::Tensor& block_table, const at::Tensor& cache_seqlens, const at::Tensor& cu_new,
+                           const at::Tensor& positions, const at::Tensor& mask, int64_t window,
+                           std::optional<double> softmax_scale, int64_t max_new) {
+  need(q, "q", 3, at::kBFloat16);
+  c10::cuda::CUDAGuard guard(q.device());
+  mcb_paged_tree_attn_args t = {};
+  const int64_t N = q.size(0);
+  fill_paged_attn(t.attn, q, k_pages, v_pages, block_table, cache_seqlens, cu_new, window, softmax_scale, max_new);
+  int_vec(positions, "positions", N, q, at::kInt);
+  need(mask, "mask", 2, at::kInt);
+  same_device(q, mask, "mask");
+  TORCH_CHECK(mask.size(0) == N && mask.is_contiguous(), "mask must be a contiguous (", N, ", words) int32 tensor, got ",
+              mask.sizes());
+  at::Tensor out = new_tensor(q.sizes(), q, at::kBFloat16);
+  t.attn.out = out.data_ptr();
+  t.positions = positions.data_ptr<int32_t>();
+  t.mask = mask.data_ptr<int32_t>();
+  t.words = to_i32(mask.size(1), "mask words");
+  at::Tensor ws;
+  if (N > 0) {
+    const size_t bytes = mcb_paged_tree_attn_workspace_size(&t);
+    if (bytes > 0) {
+      ws = new_tensor({static_cast<int64_t>(bytes)}, q, at::kByte);
+      t.attn.workspace = ws.data_ptr();
+      t.attn.workspace_bytes = bytes;
+    }
+  }
+  check_status(mcb_paged_tree_attn(&t, stream_of(q)), "mcb200::paged_tree_attn");
+  return out;
+}
+
+// Rows of V values with any row stride; a single row's stride is arbitrary in torch.
+int64_t vocab_rows(const at::Tensor& t, const char* name, int64_t N, int64_t V, const at::Tensor& ref) {
+  same_device(ref, t, name);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == N && t.size(1) == V && (V <= 1 || N == 0 || t.stride(1) == 1) &&
+                  (N <= 1 || t.stride(0) >= V),
+              name, " must be (", N, ", ", V, ") with contiguous rows, got ", t.sizes(), " strides ", t.strides());
+  return N <= 1 ? V : t.stride(0);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(
+    const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& parents, const at::Tensor& cu_new,
+    const at::Tensor& accept, const at::Tensor& draws, double temperature, const std::optional<at::Tensor>& draft_probs,
+    int64_t max_path) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(logits.device());
+  TORCH_CHECK(logits.dim() == 2 && (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
+              "logits must be (N, V) float32 or bfloat16, got ", logits.sizes(), " ", logits.scalar_type());
+  const int64_t N = logits.size(0), V = logits.size(1);
+  need(cu_new, "cu_new", 1, at::kInt);
+  const int64_t R = cu_new.size(0) - 1;
+  TORCH_CHECK(R >= 0, "cu_new must hold one offset more than requests");
+  int_vec(cu_new, "cu_new", R + 1, logits, at::kInt);
+  int_vec(tokens, "tokens", N, logits, at::kLong);
+  int_vec(parents, "parents", N, logits, at::kInt);
+  int_vec(accept, "accept", N, logits, at::kFloat);
+  int_vec(draws, "draws", R, logits, at::kFloat);
+  TORCH_CHECK(max_path >= 1, "max_path must be positive, got ", max_path);
+  mcb_verify_drafts_args a = {};
+  a.max_path = to_i32(max_path, "max_path");
+  at::Tensor accepted = new_tensor({R}, logits, at::kInt);
+  at::Tensor path = new_tensor({R, max_path}, logits, at::kInt);
+  at::Tensor next = new_tensor({R}, logits, at::kLong);
+  a.logits = logits.data_ptr();
+  a.logits_stride = vocab_rows(logits, "logits", N, V, logits);
+  a.logits_bf16 = logits.scalar_type() == at::kBFloat16;
+  a.tokens = tokens.data_ptr<int64_t>();
+  a.parents = parents.data_ptr<int32_t>();
+  a.cu_new = cu_new.data_ptr<int32_t>();
+  a.accept = accept.data_ptr<float>();
+  a.draws = draws.data_ptr<float>();
+  if (draft_probs.has_value()) {
+    TORCH_CHECK(draft_probs->scalar_type() == at::kFloat, "draft_probs must be float32, got ",
+                draft_probs->scalar_type());
+    a.draft_stride = vocab_rows(*draft_probs, "draft_probs", N, V, logits);
+    a.draft_probs = draft_probs->data_ptr<float>();
+  }
+  a.accepted = accepted.data_ptr<int32_t>();
+  a.path = path.data_ptr<int32_t>();
+  a.next_token = next.data_ptr<int64_t>();
+  a.R = to_i32(R, "R");
+  a.N = to_i32(N, "N");
+  a.V = to_i32(V, "V");
+  a.temperature = static_cast<float>(temperature);
+  check_status(mcb_verify_drafts(&a, stream_of(logits)), "mcb200::verify_drafts");
+  return {accepted, path, next};
+}
+
+// The pools of all slots: (slots, n_pages, Hkv, page_size, D), or one slot's without the first dimension.
+template <typename Args>
+void fill_slots(Args& a, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ref) {
+  same_device(ref, k, "k_pages");
+  same_device(ref, v, "v_pages");
+  TORCH_CHECK((k.dim() == 5 || k.dim() == 4) && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 &&
+                  k.is_contiguous() && v.is_contiguous() && k.sizes() == v.sizes(),
+              "k_pages and v_pages must be contiguous bf16 ([slots,] n_pages, Hkv, page_size, D), got ", k.sizes(), " and ",
+              v.sizes());
+  const int64_t d = k.dim() - 4;
+  a.k_pages = k.data_ptr();
+  a.v_pages = v.data_ptr();
+  a.slots = d == 1 ? to_i32(k.size(0), "slots") : 1;
+  a.n_pages = to_i32(k.size(d), "n_pages");
+  a.Hkv = to_i32(k.size(d + 1), "Hkv");
+  a.page_size = to_i32(k.size(d + 2), "page_size");
+  a.D = to_i32(k.size(d + 3), "D");
+}
+
+void paged_keep(const at::Tensor& path, const at::Tensor& accepted, const at::Tensor& cache_seqlens,
+                const at::Tensor& new_lens, const at::Tensor& block_table, const at::Tensor& free_pages,
+                const at::Tensor& free_state, const at::Tensor& free_state_out, const at::Tensor& seqlens_out,
+                const at::Tensor& k_pages, const at::Tensor& v_pages) {
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  c10::cuda::CUDAGuard guard(cache_seqlens.device());
+  const int64_t R = cache_seqlens.size(0);
+  int_vec(cache_seqlens, "cache_seqlens", R, cache_seqlens, at::kInt);
+  int_vec(accepted, "accepted", R, cache_seqlens, at::kInt);
+  int_vec(new_lens, "new_lens", R, cache_seqlens, at::kInt);
+  int_vec(seqlens_out, "seqlens_out", R, cache_seqlens, at::kInt);
+  need(path, "path", 2, at::kInt);
+  same_device(cache_seqlens, path, "path");
+  TORCH_CHECK(path.size(0) == R && (path.size(1) <= 1 || R == 0 || path.stride(1) == 1) &&
+                  (R <= 1 || path.stride(0) >= path.size(1)),
+              "path must be (", R, ", P) with contiguous rows, got ", path.sizes(), " strides ", path.strides());
+  mcb_paged_keep_args a = {};
+  fill_slots(a, k_pages, v_pages, cache_seqlens);
+  a.table_stride = check_block_table(block_table, R, cache_seqlens);
+  int_vec(free_pages, "free_pages", a.n_pages, cache_seqlens, at::kInt);
+  int_vec(free_state, "free_state", 2, cache_seqlens, at::kLong);
+  int_vec(free_state_out, "free_state_out", 2, cache_seqlens, at::kLong);
+  a.path = path.data_ptr<int32_t>();
+  a.path_stride = R <= 1 ? path.size(1) : path.stride(0);
+  a.accepted = accepted.data_ptr<int32_t>();
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.free_pages = free_pages.data_ptr<int32_t>();
+  a.free_state = free_state.data_ptr<int64_t>();
+  a.free_state_out = free_state_out.data_ptr<int64_t>();
+  a.seqlens_out = seqlens_out.data_ptr<int32_t>();
+  a.R = to_i32(R, "R");
+  a.P = to_i32(path.size(1), "P");
+  a.max_pages = to_i32(block_table.size(1), "max_pages");
+  a.counter = paged_counters(cache_seqlens, 1);
+  check_status(mcb_paged_keep(&a, stream_of(cache_seqlens)), "mcb200::paged_keep");
+}
+
+void page_fork(const at::Tensor& source, const at::Tensor& cache_seqlens, const at::Tensor& block_table,
+               const at::Tensor& shares, const at::Tensor& free_pages, const at::Tensor& free_state,
+               const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& block_table_out,
+               const at::Tensor& shares_out, const at::Tensor& free_state_out, const at::Tensor& seqlens_out) {
+  need(cache_seqlens, "cache_seqlens", 1, at::kInt);
+  c10::cuda::CUDAGuard guard(cache_seqlens.device());
+  const int64_t R = cache_seqlens.size(0);
+  int_vec(cache_seqlens, "cache_seqlens", R, cache_seqlens, at::kInt);
+  int_vec(source, "source", R, cache_seqlens, at::kInt);
+  int_vec(seqlens_out, "seqlens_out", R, cache_seqlens, at::kInt);
+  mcb_page_fork_args a = {};
+  fill_slots(a, k_pages, v_pages, cache_seqlens);
+  a.table_stride = check_block_table(block_table, R, cache_seqlens);
+  a.table_out_stride = check_block_table(block_table_out, R, cache_seqlens);
+  TORCH_CHECK(block_table_out.size(1) == block_table.size(1), "block_table_out must have ", block_table.size(1),
+              " columns, got ", block_table_out.size(1));
+  int_vec(shares, "shares", a.n_pages, cache_seqlens, at::kInt);
+  int_vec(shares_out, "shares_out", a.n_pages, cache_seqlens, at::kInt);
+  int_vec(free_pages, "free_pages", a.n_pages, cache_seqlens, at::kInt);
+  int_vec(free_state, "free_state", 2, cache_seqlens, at::kLong);
+  int_vec(free_state_out, "free_state_out", 2, cache_seqlens, at::kLong);
+  a.source = source.data_ptr<int32_t>();
+  a.cache_seqlens = cache_seqlens.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.shares = shares.data_ptr<int32_t>();
+  a.free_pages = free_pages.data_ptr<int32_t>();
+  a.free_state = free_state.data_ptr<int64_t>();
+  a.block_table_out = block_table_out.data_ptr<int32_t>();
+  a.shares_out = shares_out.data_ptr<int32_t>();
+  a.free_state_out = free_state_out.data_ptr<int64_t>();
+  a.seqlens_out = seqlens_out.data_ptr<int32_t>();
+  a.R = to_i32(R, "R");
+  a.max_pages = to_i32(block_table.size(1), "max_pages");
+  const size_t bytes = mcb_page_fork_workspace_size(&a);
+  at::Tensor ws;
+  if (bytes > 0) {
+    ws = new_tensor({static_cast<int64_t>(bytes)}, cache_seqlens, at::kByte);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  check_status(mcb_page_fork(&a, stream_of(cache_seqlens)), "mcb200::page_fork");
 }
 
 }  // namespace
@@ -694,6 +920,21 @@ TORCH_LIBRARY(mcb200, m) {
   m.def(
       "paged_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cache_seqlens, "
       "Tensor cu_new, int window=-1, float? softmax_scale=None, int max_new=0) -> Tensor");
+  m.def("draft_tree(Tensor parents, Tensor cu_new, Tensor cache_seqlens, int max_tree) -> (Tensor, Tensor)");
+  m.def(
+      "paged_tree_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor cache_seqlens, "
+      "Tensor cu_new, Tensor positions, Tensor mask, int window=-1, float? softmax_scale=None, int max_new=0) -> Tensor");
+  m.def(
+      "verify_drafts(Tensor logits, Tensor tokens, Tensor parents, Tensor cu_new, Tensor accept, Tensor draws, "
+      "float temperature, Tensor? draft_probs, int max_path) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "paged_keep(Tensor path, Tensor accepted, Tensor cache_seqlens, Tensor new_lens, Tensor block_table, "
+      "Tensor(a!) free_pages, Tensor free_state, Tensor(b!) free_state_out, Tensor(c!) seqlens_out, "
+      "Tensor(d!) k_pages, Tensor(e!) v_pages) -> ()");
+  m.def(
+      "page_fork(Tensor source, Tensor cache_seqlens, Tensor block_table, Tensor shares, Tensor(a!) free_pages, "
+      "Tensor free_state, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) block_table_out, Tensor(e!) shares_out, "
+      "Tensor(f!) free_state_out, Tensor(g!) seqlens_out) -> ()");
   m.def("add_rms_norm(Tensor x, Tensor? delta, Tensor(a!)? x_out, Tensor(b!) h_out, float? eps=None) -> ()");
 }
 
@@ -709,4 +950,9 @@ TORCH_LIBRARY_IMPL(mcb200, CUDA, m) {
   m.impl("page_release", &page_release);
   m.impl("paged_append_rope", &paged_append_rope);
   m.impl("paged_attn", &paged_attn);
+  m.impl("draft_tree", &draft_tree);
+  m.impl("paged_tree_attn", &paged_tree_attn);
+  m.impl("verify_drafts", &verify_drafts);
+  m.impl("paged_keep", &paged_keep);
+  m.impl("page_fork", &page_fork);
 }

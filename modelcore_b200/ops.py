@@ -759,6 +759,110 @@ def paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, *, windo
                                -1 if window is None else window, softmax_scale, max_new)
 
 
+class DraftTree(NamedTuple):
+    """Trees of drafted tokens of a packed batch (draft_tree)."""
+    positions: torch.Tensor   # (N,) int32, -1 for padding
+    mask: torch.Tensor        # (N, words) int32: bit j % 32 of word j / 32 of a token: it sees its request's j-th
+
+
+class Verified(NamedTuple):
+    """What verify_drafts keeps of each request's drafted tokens."""
+    accepted: torch.Tensor    # (R,) int32: tokens kept, the first one (part of the answer already) among them
+    path: torch.Tensor        # (R, max_path) int32: their places in the request, then -1
+    next_token: torch.Tensor  # (R,) int64: the token after them
+
+
+class PageFork(NamedTuple):
+    """A paged cache's tables after page_fork."""
+    block_table: torch.Tensor
+    shares: torch.Tensor
+    free_state: torch.Tensor
+    seqlens: torch.Tensor
+
+
+def draft_tree(parents, cu_new, cache_seqlens, *, max_tree):
+    """Positions and ancestor masks of trees of drafted tokens.  parents (N,) int32: each new token's
+    parent, an earlier token of its request counted from the request's first, or -1 after the cached tokens.
+    A token's position is its request's cached length plus its ancestors (for paged_append_rope, in place of
+    the plan's; its slot stays the plan's), its mask has its ancestors' bits and its own (for
+    paged_tree_attn).  max_tree: the most new tokens of a request that is a tree, 256 at most; requests of
+    more than that, rounded up to 32, are chunks of prompts: their positions follow each other and their
+    parents are not read.  Device error 8: a parent that is no earlier token (counts as -1).
+    Returns a DraftTree."""
+    return DraftTree(*_PAGED.draft_tree(parents, cu_new, cache_seqlens, max_tree))
+
+
+def paged_tree_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, positions, mask, *, window=-1,
+                    softmax_scale=None, max_new=0):
+    """paged_attn for trees of drafted tokens: a new token sees its request's cached tokens and the new ones
+    that its mask names, each within `window` positions back (< 0: all).  positions and mask as draft_tree
+    gives them, or any others: a token that sees nothing gets zeros.  Requests of more new tokens than
+    the mask has bits are chunks of prompts, as in paged_attn.  max_new: the largest number of new tokens
+    of a request when the caller knows it (0: unknown).  Returns (N, Hq, D) bf16, zeros for padding."""
+    return _PAGED.paged_tree_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, positions, mask,
+                                  -1 if window is None else window, softmax_scale, max_new)
+
+
+def verify_drafts(logits, tokens, parents, cu_new, accept, draws, *, temperature=1.0, draft_probs=None, max_path):
+    """Which drafted tokens the target keeps, and the token after them, so that the tokens are
+    distributed as the target's own (sample over the whole vocabulary, at each position).
+
+    logits (N, V) fp32 or bf16: the target's after each token of the packed trees; tokens (N,) int64 and
+    parents (N,) int32 as draft_tree takes them -- a request's first token is part of its answer already,
+    the others were drafted.  accept (N,) and draws (R,) fp32: uniforms in [0, 1).  draft_probs (N, V) fp32: row u
+    is the distribution that u's children were drawn from, each for itself; None: they are the draft's
+    choices (its largest, say), kept with the target's probability.  temperature == 0: the tokens that
+    the greedy pick would give.  include/mcb200.h (mcb_verify_drafts) has the rule.  max_path: the width of
+    the path, and the most tokens kept.  Device errors: 9 a row without probabilities (its request's
+    next_token is -1), 4 a token outside the vocabulary (not kept).  Returns a Verified."""
+    if temperature < 0:
+        raise RuntimeError("temperature must be non-negative")
+    return Verified(*_PAGED.verify_drafts(logits, tokens, parents, cu_new, accept, draws, float(temperature), draft_probs,
+                                          max_path))
+
+
+def paged_keep(path, accepted, cache_seqlens, new_lens, block_table, free_pages, free_state, k_pages, v_pages, *,
+               free_state_out=None, seqlens_out=None):
+    """A step's kept path becomes part of its rows: path (R, P) int32 and accepted (R,) int32 as
+    verify_drafts gives them.  In every slot the path's keys and values move to the positions after the
+    cached tokens (k_pages / v_pages (n_slots, n_pages, Hkv, page_size, D) or one slot's, in place), the pages
+    that only the step's other tokens needed (new_lens (R,) as given to page_plan) go back to the queue's tail
+    in request order.  Returns (free_state, seqlens) after it: new tensors, or free_state_out /
+    seqlens_out, which may be the inputs.  Device errors as page_release's, and 8 for a path that does not
+    fit its request."""
+    if free_state_out is None:
+        free_state_out = torch.empty_like(free_state)
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens)
+    _PAGED.paged_keep(path, accepted, cache_seqlens, new_lens, block_table, free_pages, free_state, free_state_out,
+                      seqlens_out, k_pages, v_pages)
+    return free_state_out, seqlens_out
+
+
+def page_fork(source, cache_seqlens, block_table, shares, free_pages, free_state, k_pages, v_pages, *,
+              block_table_out=None, shares_out=None, free_state_out=None, seqlens_out=None):
+    """Row r becomes what row source[r] was ((R,) int32, -1: empty), all rows at once: samples of one prompt,
+    a beam search's step, finished rows given back.  Full pages are shared (shares (n_pages,) int32: one less
+    than the rows that hold a page); a last page that is not full stays with the first row that takes it
+    over and is copied, in every slot, to a fresh page for each other one; pages that no row holds any more
+    go back to the queue's tail in page order.  free_pages and the pools (n_slots, n_pages, Hkv, page_size,
+    D), or one slot's, are written in place; the rest is returned as a PageFork: new tensors, or the ones
+    given, which may be the inputs.  Rows that share pages are given back by this call and not by
+    page_release.  Device errors: 5 too few free pages (the row's last page is -1), 8 a source past the rows
+    (counts as -1), 1 and 6 as page_plan's."""
+    if block_table_out is None:
+        block_table_out = torch.empty_like(block_table)
+    if shares_out is None:
+        shares_out = torch.empty_like(shares)
+    if free_state_out is None:
+        free_state_out = torch.empty_like(free_state)
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens)
+    _PAGED.page_fork(source, cache_seqlens, block_table, shares, free_pages, free_state, k_pages, v_pages,
+                     block_table_out, shares_out, free_state_out, seqlens_out)
+    return PageFork(block_table_out, shares_out, free_state_out, seqlens_out)
+
+
 def device_error(device=None):
     """Reads and clears the library's device error word (synchronises the current stream).
     Returns (code, description)."""

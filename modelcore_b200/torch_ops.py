@@ -34,6 +34,16 @@ functions, so that torch.compile can trace through them:
     torch.ops.mcb200.paged_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, window=-1,
                                 softmax_scale=None, max_new=0) -> y
         the paged cache (modelcore_b200.ops documents each)
+    torch.ops.mcb200.draft_tree(parents, cu_new, cache_seqlens, max_tree) -> positions, mask
+    torch.ops.mcb200.paged_tree_attn(q, k_pages, v_pages, block_table, cache_seqlens, cu_new, positions, mask,
+                                     window=-1, softmax_scale=None, max_new=0) -> y
+    torch.ops.mcb200.verify_drafts(logits, tokens, parents, cu_new, accept, draws, temperature, draft_probs,
+                                   max_path) -> accepted, path, next_token
+    torch.ops.mcb200.paged_keep(path, accepted, cache_seqlens, new_lens, block_table, free_pages, free_state,
+                                free_state_out, seqlens_out, k_pages, v_pages)
+    torch.ops.mcb200.page_fork(source, cache_seqlens, block_table, shares, free_pages, free_state, k_pages, v_pages,
+                               block_table_out, shares_out, free_state_out, seqlens_out)
+        trees of drafted tokens over the paged cache, and rows that share pages
 
 bf16 slots only (the fp8 cache format is reached through modelcore_b200.ops).  The results are
 those of the ctypes entry points bit for bit: one library does the work.  Without the built
@@ -47,7 +57,8 @@ from . import _native
 from .build import TORCH_OPS_PATH
 
 OPS = ("kv_append_rope", "kv_broadcast", "decode_attn", "append_attn", "kv_advance", "linear",
-       "add_rms_norm", "page_plan", "page_release", "paged_append_rope", "paged_attn")
+       "add_rms_norm", "page_plan", "page_release", "paged_append_rope", "paged_attn", "draft_tree",
+       "paged_tree_attn", "verify_drafts", "paged_keep", "page_fork")
 
 
 def _register_fakes():
@@ -62,10 +73,20 @@ def _register_fakes():
         ints = [cache_seqlens.new_empty(n) for n in (cache_seqlens.shape[0] + 1, num_tokens)]
         return (*ints, cache_seqlens.new_empty(num_tokens, dtype=torch.int64))
 
+    def tree(parents, cu_new, cache_seqlens, max_tree):
+        n = parents.shape[0]
+        return parents.new_empty(n), parents.new_empty((n, (max_tree + 31) // 32))
+
+    def verified(logits, tokens, parents, cu_new, accept, draws, temperature, draft_probs, max_path):
+        rows = draws.shape[0]
+        return cu_new.new_empty(rows), cu_new.new_empty((rows, max_path)), tokens.new_empty(rows)
+
     for name, fn in (("kv_append_rope", like_q), ("decode_attn", like_q), ("append_attn", like_q),
                      ("kv_broadcast", nothing), ("kv_advance", nothing), ("linear", nothing),
                      ("add_rms_norm", nothing), ("page_plan", plan), ("page_release", nothing),
-                     ("paged_append_rope", like_q), ("paged_attn", like_q)):
+                     ("paged_append_rope", like_q), ("paged_attn", like_q), ("draft_tree", tree),
+                     ("paged_tree_attn", like_q), ("verify_drafts", verified), ("paged_keep", nothing),
+                     ("page_fork", nothing)):
         torch.library.register_fake(f"mcb200::{name}")(fn)
 
 
