@@ -51,6 +51,55 @@ int check_paged_tree(const mcb_paged_tree_attn_args* a, const char* who) {
   return rc != MCB_OK ? rc : check_words(a->words, who);
 }
 
+// How a call runs, from its shapes alone: the workspace's parts are the tree kernel's partials and cut units, then
+// the chunk kernel's.
+struct PagedTreePlan {
+  bool chunk;  // some request may be a chunk of a prompt
+  int grid;
+  size_t o, lse, cuts, ws_bytes;
+};
+
+PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
+  PagedTreePlan pl = {};
+  pl.chunk = t->attn.max_new == 0 || t->attn.max_new > 32 * t->words;
+  pl.grid = device_sm_count();
+  const size_t rows = static_cast<size_t>(pl.grid) * 2 * 256;
+  pl.o = round256(rows * t->attn.D * 4);
+  pl.lse = round256(rows * 4);
+  pl.cuts = round256(pl.grid * sizeof(mcb::PagedCut));
+  pl.ws_bytes = (pl.o + pl.lse + pl.cuts) * (pl.chunk ? 2 : 1);
+  return pl;
+}
+
+template <int D>
+int launch_paged_tree(const mcb_paged_attn_args* a, const mcb::PagedTreeParams& p, const int64_t (&q_stride)[2], int grid,
+                      cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int smem = mcb::PagedTreeConfig<D>::kBytes;
+  CUtensorMap qm, km, vm;
+  const int box = std::min(a->page_size, mcb::kPtTile);
+  int rc = encode_packed_q_map(&qm, a, q_stride, p.a.tpb);
+  if (rc == MCB_OK) rc = encode_page_map(&km, a->k_pages, a, box, 1);
+  if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, 1);
+  if (rc != MCB_OK) return rc;
+  cudaError_t e = ensure_smem(mcb::paged_tree_kernel<D>, smem, done);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_tree)");
+  e = launch_pdl(mcb::paged_tree_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(mcb::kPtThreads),
+                 static_cast<size_t>(smem), st, qm, km, vm, p);
+  g_launches++;
+  note_attn_kernel("paged_tree_kernel", D, 0, 0, false);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_tree launch");
+  mcb::PagedChunkParams c = {};
+  c.a = p.a;
+  c.cuts = p.cuts;
+  e = launch_pdl(mcb::paged_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 8), dim3(256), 0, st, c);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_combine launch");
+  return MCB_OK;
+}
+
 int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
   const char* who = "mcb_paged_tree_attn";
   int rc = check_paged_tree(t, who);
@@ -66,6 +115,10 @@ int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
     return fail(MCB_ERR_INVALID_ARG, "%s: negative q stride or table_stride below max_pages", who);
   if (!rows16(a->q, qs.s) || !aligned(a->out, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16))
     return fail(MCB_ERR_ALIGNMENT, "%s: q rows, out and pages must start on 16-byte boundaries", who);
+  const PagedTreePlan pl = plan_paged_tree(t);
+  if (a->workspace == nullptr || a->workspace_bytes < pl.ws_bytes || !aligned(a->workspace, 256))
+    return fail(MCB_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, got %zu", who, pl.ws_bytes,
+                a->workspace_bytes);
   mcb::PagedTreeParams p = {};
   p.a.q = static_cast<const uint16_t*>(a->q);
   p.a.qs[0] = qs.s[0];
@@ -85,20 +138,31 @@ int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
   p.a.page_shift = page_shift_of(a->page_size);
   p.a.window = a->window;
   p.a.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  p.k_pages = static_cast<const uint16_t*>(a->k_pages);
-  p.v_pages = static_cast<const uint16_t*>(a->v_pages);
+  p.a.few_rows = 32 * t->words * p.a.G;  // the chunk kernel's share begins above
+  p.a.tpb = mcb::kPtTile / p.a.G;
+  p.a.all = !pl.chunk;
+  p.a.fill = 1;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  auto parts = [&](mcb::PagedAttnParams& q, mcb::PagedCut*& cuts) {
+    q.part_o = reinterpret_cast<float*>(ws);
+    q.part_lse = reinterpret_cast<float*>(ws + pl.o);
+    cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.o + pl.lse);
+    ws += pl.o + pl.lse + pl.cuts;
+  };
+  parts(p.a, p.cuts);
   p.positions = t->positions;
   p.mask = reinterpret_cast<const uint32_t*>(t->mask);
   p.words = t->words;
-  const long long warps = static_cast<long long>(a->N) * a->Hq;
-  const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = a->D == 64 ? launch_pdl(mcb::paged_tree_simple_kernel<64>, grid, dim3(128), 0, st, p)
-                             : launch_pdl(mcb::paged_tree_simple_kernel<128>, grid, dim3(128), 0, st, p);
-  g_launches++;
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "paged_tree launch");
-  return MCB_OK;
+  rc = a->D == 64 ? launch_paged_tree<64>(a, p, qs.s, pl.grid, st) : launch_paged_tree<128>(a, p, qs.s, pl.grid, st);
+  if (rc != MCB_OK || !pl.chunk) return rc;
+  mcb::PagedChunkParams c = {};
+  c.a = p.a;
+  c.a.all = 0;
+  c.a.fill = 0;
+  parts(c.a, c.cuts);
+  c.wait_last = 1;
+  return a->D == 64 ? launch_paged_chunk<64>(a, c, qs.s, pl.grid, st) : launch_paged_chunk<128>(a, c, qs.s, pl.grid, st);
 }
 
 int verify_drafts(const mcb_verify_drafts_args* a, void* stream) {
@@ -319,9 +383,13 @@ int mcb_draft_tree(const mcb_draft_tree_args* a, void* stream) {
   return guarded("mcb_draft_tree", [&] { return draft_tree(a, stream); });
 }
 size_t mcb_paged_tree_attn_workspace_size(const mcb_paged_tree_attn_args* a) {
-  guarded("mcb_paged_tree_attn_workspace_size",
-          [&] { return check_paged_tree(a, "mcb_paged_tree_attn_workspace_size"); });
-  return 0;
+  size_t n = 0;
+  guarded("mcb_paged_tree_attn_workspace_size", [&] {
+    const int rc = check_paged_tree(a, "mcb_paged_tree_attn_workspace_size");
+    if (rc == MCB_OK) n = plan_paged_tree(a).ws_bytes;
+    return rc;
+  });
+  return n;
 }
 int mcb_paged_tree_attn(const mcb_paged_tree_attn_args* a, void* stream) {
   return guarded("mcb_paged_tree_attn", [&] { return paged_tree_attn(a, stream); });

@@ -3,70 +3,729 @@
 //   out[t, h] = sum_c softmax_c(q[t, h] . K[c, h / G] * softmax_scale) V[c, h / G]
 // over the cached keys c < L with position_t - c <= window, and the request's new tokens j with mask
 // bit j of t and position_t - position_j <= window (window < 0: all).  A request of more new tokens
-// than the mask has bits is a chunk of a prompt: token t sees the new tokens up to itself.
+// than the mask has bits is a chunk of a prompt, the chunk kernel's where that is launched.
+//
+// A tree has few query rows for many keys (16 tokens of 4 heads a kv head over 8,000 keys: 64 rows, 64
+// FLOP a byte): bound by HBM, if products and softmax keep up with 44 GB/s an SM, a 128-key tile of K and V
+// in 2,800 cycles at head size 128 and in 1,400 at 64.  The query rows of a kv head are packed as in the
+// chunk kernel, row = token * G + head, 128 a tile; a *unit* is (request, two tiles Q0, Q1, kv head), its
+// keys from the first that any of its rows may see to the request's last.  All units' 128-key tiles form one
+// sequence that the CTAs (one an SM) share evenly, computed on the device from the lengths; a cut unit leaves
+// (O / l, log2 sum) in workspace and paged_combine_kernel, launched after, merges them.
+//
+// Roles of a CTA's warps:
+//   warp 0      TMA producer and walker: describes each part of a unit in shared memory, loads its queries,
+//               and K and V tiles into one ring that runs on across units
+//   warps 1, 2  (warp 1 allocates TMEM) products of group 0, of group 1:
+//                 S_t = Q K_j^T   M=128 N=128 K=D   (both operands from shared memory)
+//                 O_t += P_t V_j  M=128 N=D K=128   (P from TMEM, over its S)
+//   warps 4-7   softmax of group 0, warps 8-11 of group 1: a thread a query row
+// Two groups, each with its own S, running maximum, sum and accumulator, so that one group's products run
+// beside the other's softmax.  Where a unit has one query tile -- up to 128 rows, most trees -- the groups
+// take its key tiles in turn, each key tile read once, and merge their two results in TMEM at the
+// unit's end; with two tiles each group has one and both read every key tile.
+// TMEM: S_0, S_1 of 128 columns, O_0, O_1 of D: all 512 at D = 128.
+//
+// The running maximum m moves only when a row's scores exceed it by 2^8 (P and l stay far below 2^127):
+// then the row's O, in TMEM, is rescaled, which no product can be at: a group's S is complete after its
+// P V before.  P is rounded to bf16 for the product; l sums the unrounded values.
+//
+// Masks: only the tiles with new tokens, at a window's start or at the unit's end look at them; a row's
+// 32 bits at a time are made from its interval of cached keys and its mask words, shifted to the
+// tile.  A key tile's positions outside the unit's [lo, hi] may hold anything: scores there are replaced by
+// -inf, and their rows of V are zeroed in shared memory before the product reads them (0 * NaN is NaN).
+// Every wait is bounded; a timeout raises the abort flag, the issuers wait for their products, the
+// producer for its copies, and TMEM is freed.
 #pragma once
 
-#include "paged_decode.cuh"
+#include "paged_chunk.cuh"
 
 namespace mcb {
 
 struct PagedTreeParams {
   PagedAttnParams a;
-  const uint16_t* k_pages;
-  const uint16_t* v_pages;
+  PagedCut* cuts;            // [grid]
   const int32_t* positions;  // (N,)
   const uint32_t* mask;      // (N, words)
   int words;
 };
 
-// One warp a token and query head, one key after another.
+constexpr int kPtTile = 128;      // query rows a tile, keys a key tile
+constexpr int kPtThreads = 384;   // producer, two issuers, an idle warp, 2 x 4 softmax warps
+constexpr int kPtWarps = kPtThreads / 32;
+
 template <int D>
-__global__ void __launch_bounds__(128) paged_tree_simple_kernel(const PagedTreeParams p) {
-  constexpr int E = D / 32;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const long long id = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (id >= static_cast<long long>(p.a.N) * p.a.Hq) return;
-  const int t = static_cast<int>(id / p.a.Hq), h = static_cast<int>(id % p.a.Hq), kvh = h / p.a.G;
-  int r = 0;
-  while (r < p.a.R && !(t >= p.a.cu_new[r] && t < p.a.cu_new[r + 1])) ++r;
-  float acc[E] = {}, m = -CUDART_INF_F, l = 0.f;
-  if (r < p.a.R) {
+struct PagedTreeConfig {
+  static constexpr int kPanels = D / 64;
+  static constexpr int kTileBytes = kPanels * kPtTile * 128;
+  static constexpr int kStages = D == 128 ? 5 : 12;      // K and V tiles in turn
+  static constexpr uint32_t kOCol = 2 * kPtTile;         // TMEM: S (and P) below, O_0, O_1 above
+  static constexpr int kRingOff = 2 * kTileBytes;        // Q0, Q1, then the ring
+  static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
+  static constexpr int kNumBars = 2 * kStages + 21;
+  static constexpr int kSegOff = (kBarOff + kNumBars * 8 + 32 + 63) / 64 * 64;
+  static constexpr int kXchOff = kSegOff + 4 * 64;       // a float a row of either group
+  static constexpr int kBytes = kXchOff + 2 * kPtTile * 4 + 1024;
+  // above half of an SM's shared memory: two CTAs never meet on one SM, whose TMEM each needs whole
+  static_assert(kBytes > 118784 && kBytes <= 232448, "one CTA an SM");
+};
+
+// A unit (kv head aside).
+struct TreeUnit {
+  PagedRow row;
+  int r, qb, nqb;
+  int c0, c1;       // tokens in Q0 and Q1 (first tokens: qb * 2 tpb, + tpb)
+  int lo, hi, kb, n;
+};
+
+__device__ __forceinline__ bool tree_causal(const PagedTreeParams& p, const PagedRow& x) {
+  return x.T > 32 * p.words;
+}
+
+__device__ __forceinline__ int tree_blocks(const PagedTreeParams& p, const PagedRow& x) {
+  return p.a.all || !tree_causal(p, x) ? (x.T + 2 * p.a.tpb - 1) / (2 * p.a.tpb) : 0;
+}
+
+__device__ __forceinline__ TreeUnit tree_unit(const PagedTreeParams& p, const PagedRow& x, int r, int qb, int nqb) {
+  TreeUnit u;
+  u.row = x;
+  u.r = r;
+  u.qb = qb;
+  u.nqb = nqb;
+  const int first = qb * 2 * p.a.tpb, left = x.T - first;
+  u.c0 = min(left, p.a.tpb);
+  u.c1 = min(max(left - p.a.tpb, 0), p.a.tpb);
+  const bool causal = tree_causal(p, x);
+  const long long cap = (static_cast<long long>(p.a.max_pages) << p.a.page_shift) - 1;
+  const int last = causal ? first + u.c0 + u.c1 - 1 : x.T - 1;  // a tree's token may see any other
+  u.lo = p.a.window >= 0 ? max(0, x.L + (causal ? first : 0) - p.a.window) : 0;
+  u.hi = static_cast<int>(min(static_cast<long long>(x.L) + last, cap));
+  u.kb = min(u.lo, u.hi) / kPtTile * kPtTile;
+  u.n = (u.hi - u.kb) / kPtTile + 1;
+  return u;
+}
+
+// The part of a unit in one CTA's share, as the producer describes it to the other roles.
+struct TreeSeg {
+  int seg;             // key tiles (0: no more parts)
+  int kt0;             // the first one's first key
+  int lo, hi;          // the unit's keys
+  int L, T, tok0;      // the request's
+  int first;           // the unit's first token, counted from the request's first
+  int c0, c1;          // tokens in Q0, Q1
+  int h;               // kv head
+  int part;            // -1: the whole unit; else the slot of the partial result
+  int q;               // one tile: which of the two places its queries have; parities of q_full << 1, << 2
+  int pad[3];
+};
+static_assert(sizeof(TreeSeg) == 64, "four descriptions of 64 bytes");
+
+struct TreeWalk {
+  TreeUnit u;
+  int h, local;
+  long long t;
+};
+
+__device__ __forceinline__ void tree_next(const PagedTreeParams& p, TreeWalk& w) {
+  w.local = 0;
+  if (++w.h < p.a.Hkv) return;
+  w.h = 0;
+  if (w.u.qb + 1 < w.u.nqb) {
+    w.u = tree_unit(p, w.u.row, w.u.r, w.u.qb + 1, w.u.nqb);
+    return;
+  }
+  for (int r = w.u.r + 1; r < p.a.R; ++r) {
     const PagedRow x = paged_row(p.a, r);
-    if (t == x.tok0 && h == 0 && lane == 0 && !paged_row_fits(p.a, r, x)) record_error(kErrPositionBeyondCache);
-    const int i = t - x.tok0, page = 1 << p.a.page_shift;
-    const bool chunk = x.T > 32 * p.words;
-    const int pos = chunk ? x.L + i : max(p.positions[t], x.L);
-    float q[E];
-    for (int e = 0; e < E; ++e) q[e] = bf16_bits_to_float(p.a.q[t * p.a.qs[0] + h * p.a.qs[1] + lane * E + e]);
-    for (int c = p.a.window >= 0 ? max(0, min(x.L, pos - p.a.window)) : 0; c < x.L + x.T; ++c) {
-      const int j = c - x.L;
-      if (j >= 0) {
-        const bool seen = chunk ? j <= i : (p.mask[static_cast<long long>(t) * p.words + (j >> 5)] >> (j & 31)) & 1;
-        const int kp = chunk ? c : max(p.positions[x.tok0 + j], x.L);
-        if (!seen || (p.a.window >= 0 && pos - kp > p.a.window)) continue;
-      }
-      const int pg = p.a.block_table[r * p.a.table_stride + (c >> p.a.page_shift)];
-      if (pg < 0 || pg >= p.a.n_pages) {
-        record_error(kErrPageOutOfRange);
-        continue;
-      }
-      const long long at = ((static_cast<long long>(pg) * p.a.Hkv + kvh) * page + (c & (page - 1))) * D + lane * E;
-      float s = 0.f;
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], bf16_bits_to_float(p.k_pages[at + e]), s);
-      for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= p.a.scale_log2;
-      const float mn = fmaxf(m, s);
-      if (mn == -CUDART_INF_F) continue;
-      const float alpha = fast_exp2(m - mn), w = fast_exp2(s - mn);
-      m = mn;
-      l = fmaf(l, alpha, w);
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], alpha, w * bf16_bits_to_float(p.v_pages[at + e]));
+    const int nqb = tree_blocks(p, x);
+    if (nqb > 0) {
+      w.u = tree_unit(p, x, r, 0, nqb);
+      return;
     }
   }
-  for (int e = 0; e < E; ++e)
-    p.a.out[id * D + lane * E + e] = float_to_bf16_bits(l == 0.f ? 0.f : acc[e] / l);
+}
+
+// chunk_rows for this kernel's units: rows [row_a, row_b) 32 at a time (a lane each), the blocks of each row
+// in turn (a lane each).  Stops when visit(request, first block, this lane's tiles) returns true (uniform).
+template <typename F>
+__device__ __forceinline__ void tree_rows(const PagedTreeParams& p, int row_a, int row_b, F visit) {
+  const int lane = threadIdx.x & 31;
+  for (int base = row_a; base < row_b; base += 32) {
+    PagedRow x = {0, 0, 0};
+    int nqb = 0;
+    if (base + lane < row_b) {
+      x = paged_row(p.a, base + lane);
+      if (blockIdx.x == 0 && !paged_row_fits(p.a, base + lane, x)) record_error(kErrPositionBeyondCache);
+      nqb = tree_blocks(p, x);
+    }
+    unsigned have = __ballot_sync(0xffffffffu, nqb > 0);
+    while (have) {
+      const int src = __ffs(have) - 1;
+      have &= have - 1;
+      PagedRow y;
+      y.tok0 = __shfl_sync(0xffffffffu, x.tok0, src);
+      y.T = __shfl_sync(0xffffffffu, x.T, src);
+      y.L = __shfl_sync(0xffffffffu, x.L, src);
+      const int nb = __shfl_sync(0xffffffffu, nqb, src);
+      for (int qb = 0; qb < nb; qb += 32) {
+        const int n = qb + lane < nb ? tree_unit(p, y, base + src, qb + lane, nb).n : 0;
+        if (visit(base + src, qb, n)) return;
+      }
+    }
+  }
+}
+
+// Bits a .. b of a word (none when b < a; 0 <= a, b <= 31).
+__device__ __forceinline__ uint32_t bit_range(int a, int b) {
+  return b < a ? 0u : (b - a == 31 ? 0xffffffffu : ((1u << (b - a + 1)) - 1)) << a;
+}
+
+// Which of the 32 keys from k0 on a row sees.  Out of line: a tile in a request's interior asks for none.
+struct TreeRowView {
+  int see_lo, see_hi;  // its interval of cached keys (a chunk's token: of all)
+  int L, T, tok0, tok; // the request's, and its own place in the packed batch (-1: a tree without masks)
+  int pos;
+};
+__device__ __noinline__ uint32_t tree_bits(const PagedTreeParams& p, const TreeRowView& v, int k0) {
+  uint32_t bits = bit_range(max(v.see_lo - k0, 0), min(v.see_hi - k0, 31));
+  const int j0 = k0 - v.L;  // the first key's place among the new tokens
+  if (v.tok < 0 || j0 <= -32 || j0 >= v.T) return bits;
+  const int w = j0 >> 5, sh = j0 & 31;
+  const uint32_t* row = p.mask + static_cast<long long>(v.tok) * p.words;
+  const uint32_t a = w >= 0 && w < p.words ? row[w] : 0u, b = w + 1 < p.words ? row[w + 1] : 0u;
+  uint32_t fresh = __funnelshift_r(a, b, sh) & bit_range(max(-j0, 0), min(v.T - 1 - j0, 31));
+  if (p.a.window >= 0 && v.pos - v.L > p.a.window)  // (a new token's position is L or more)
+    for (uint32_t left = fresh; left != 0; left &= left - 1) {
+      const int e = __ffs(left) - 1;
+      if (v.pos - max(p.positions[v.tok0 + j0 + e], v.L) > p.a.window) fresh &= ~(1u << e);
+    }
+  return bits | fresh;
+}
+
+// COLS columns of this warp's rows, O_0 w0 + O_1 w1 (a weight of 0: not read): as chunk_store.
+template <int COLS>
+__device__ __noinline__ void tree_store(uint32_t o0, uint32_t o1, float w0, float w1, int orow, uint16_t* out,
+                                        long long pitch, float* part) {
+  const int lane = threadIdx.x & 31;
+  const bool any0 = __any_sync(0xffffffffu, w0 != 0.f), any1 = __any_sync(0xffffffffu, w1 != 0.f);
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t o[32];
+    if (any0) {
+      tmem_ld32(o0 + c, o);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = w0 != 0.f ? __float_as_uint(__uint_as_float(o[e]) * w0) : 0u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0u;
+    }
+    if (any1) {
+      uint32_t b[32];
+      tmem_ld32(o1 + c, b);
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (w1 != 0.f) o[e] = __float_as_uint(fmaf(__uint_as_float(b[e]), w1, __uint_as_float(o[e])));
+    }
+    if (part != nullptr) {
+      if (orow >= 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(part + (c / 4 + e) * (256 * 4)) =
+              make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      continue;
+    }
+    uint32_t v[4][4];  // four 16-byte chunks of this lane's row
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      v[e >> 2][e & 3] = pack_bf16x2_rn(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+#pragma unroll
+    for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i & b) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & b) ? v[i][e] : v[i | b][e], b);
+          if (lane & b) v[i][e] = got;
+          else v[i | b][e] = got;
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // now v[i]: this lane's chunk of the group's i-th row
+      const int ri = __shfl_sync(0xffffffffu, orow, (lane & ~3) + i);
+      if (ri >= 0)
+        *reinterpret_cast<uint4*>(out + ri * pitch + c + (lane & 3) * 8) = make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]);
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPtThreads, 1)
+    paged_tree_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedTreeParams p) {
+  using Cfg = PagedTreeConfig<D>;
+  constexpr int ST = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
+  uint64_t* full = bars;             // [ST] the ring: K of key tile g at 2 g, V at 2 g + 1
+  // [ST] two arrivals: both groups' products; one tile's keys: its group's and the producer's own
+  uint64_t* empty = full + ST;
+  uint64_t* q_full = empty + ST;     // [2]
+  uint64_t* q_empty = q_full + 2;    // [2] two arrivals, as empty
+  uint64_t* s_full = q_empty + 2;    // [2]
+  uint64_t* p_full = s_full + 2;     // [2] 128 arrivals
+  uint64_t* o_done = p_full + 2;     // [2] a part's products are complete
+  uint64_t* epi_done = o_done + 2;   // [2] 128 arrivals: ... and its O has been read
+  // [4] a description is there.  Description x is written once the queries' place of part x - 2 or later is
+  // free, so after every thread is past x - 4
+  uint64_t* seg_full = epi_done + 2;
+  uint64_t* pair_bar = seg_full + 4; // [4] two arrivals: the two warps of a row quarter
+  uint64_t* drained = pair_bar + 4;  // two arrivals
+  static_assert(2 * ST + 21 == Cfg::kNumBars, "the barriers above");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* ctl = reinterpret_cast<int*>(tmem_slot + 2);  // start: r, qb, h, local
+  TreeSeg* segs = reinterpret_cast<TreeSeg*>(smem + Cfg::kSegOff);
+  float* xch = reinterpret_cast<float*>(smem + Cfg::kXchOff);  // [2][128]
+  long long* warp_tot = reinterpret_cast<long long*>(xch);     // [12], before the roles begin
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Cfg::kNumBars; ++i) {
+      uint64_t* b = bars + i;
+      const bool two = (b >= empty && b < q_full) || (b >= q_empty && b < s_full) || b >= pair_bar;
+      const bool threads = (b >= p_full && b < o_done) || (b >= epi_done && b < seg_full);
+      mbar_init(b, threads ? 128 : two ? 2 : 1);
+    }
+    *abort_flag = 0;
+    fence_mbarrier_init();
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the sequence's length and this CTA's first tile ----
+  const int per = (p.a.R + kPtWarps - 1) / kPtWarps;
+  const int row_a = min(warp * per, p.a.R), row_b = min(row_a + per, p.a.R);
+  long long mine = 0;
+  tree_rows(p, row_a, row_b, [&](int, int, int n) {
+    mine += n;
+    return false;
+  });
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+  mine *= p.a.Hkv;
+  if (lane == 0) warp_tot[warp] = mine;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  long long total = 0, before = 0;
+#pragma unroll
+  for (int i = 0; i < kPtWarps; ++i) {
+    if (i < warp) before += warp_tot[i];
+    total += warp_tot[i];
+  }
+  if (p.a.fill) paged_fill(p.a, D, blockDim.x);
+  const int ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const bool active = static_cast<int>(blockIdx.x) < ng;
+  const long long t_begin = active ? share_begin(blockIdx.x, total, ng) : 0;
+  const long long t_end = active ? share_begin(blockIdx.x + 1, total, ng) : 0;
+  if (active && before <= t_begin && t_begin < before + mine) {
+    long long left = t_begin - before;
+    tree_rows(p, row_a, row_b, [&](int r, int qb, int n) {
+      int incl = n;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, m);
+        if (lane >= m) incl += o;
+      }
+      const long long all = static_cast<long long>(__shfl_sync(0xffffffffu, incl, 31)) * p.a.Hkv;
+      if (left >= all) {
+        left -= all;
+        return false;
+      }
+      const long long mine0 = static_cast<long long>(incl - n) * p.a.Hkv;
+      if (n > 0 && mine0 <= left && left < mine0 + static_cast<long long>(n) * p.a.Hkv) {
+        ctl[0] = r;
+        ctl[1] = qb + lane;
+        ctl[2] = static_cast<int>((left - mine0) / n);
+        ctl[3] = static_cast<int>((left - mine0) % n);
+      }
+      return true;
+    });
+  }
+  if (threadIdx.x == 0) p.cuts[blockIdx.x].h = -1;
+  __syncthreads();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t base = smem_u32(smem);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
+    return __all_sync(0xffffffffu, mbar_wait_small(bar, parity, abort_flag)) != 0;
+  };
+  // the x-th description, once it is there; false on a timeout
+  auto next_seg = [&](int x, TreeSeg& d) {
+    if (!wait(&seg_full[x & 3], (x >> 2) & 1)) return false;
+    const int4* src = reinterpret_cast<const int4*>(&segs[x & 3]);
+    int4* dst = reinterpret_cast<int4*>(&d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = src[i];
+    return true;
+  };
+
+  if (warp < 4) {
+    if (warp == 0) {
+      // ---------------- producer and walker ----------------
+      const uint64_t q_pol = l2_policy_evict_first(), kv_pol = l2_policy_evict_first();
+      const int box_shift = min(p.a.page_shift, 7);  // positions a box: min(page, 128)
+      const int box = 1 << box_shift, nch = kPtTile >> box_shift;
+      const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+      const uint32_t q_bytes = static_cast<uint32_t>(p.a.tpb * p.a.G) * 128u;
+      const int lch = lane / Cfg::kPanels, lpn = lane % Cfg::kPanels;
+      TreeWalk w;
+      w.t = t_begin;
+      if (active) {
+        const PagedRow x = paged_row(p.a, ctl[0]);
+        w.u = tree_unit(p, x, ctl[0], ctl[1], tree_blocks(p, x));
+        w.h = ctl[2];
+        w.local = ctl[3];
+      }
+      uint32_t idx = 0;       // K and V tiles so far
+      int k = 0, place = 1;   // parts so far; the queries' place of the last one with one tile
+      int uses[2] = {0, 0};   // of the two places
+      bool ok = true;
+      while (ok && w.t < t_end) {
+        const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
+        const bool both = w.u.c1 > 0;
+        if (!both) place ^= 1;
+        for (int s = 0; s < 2 && ok; ++s)
+          if ((both || s == place) && uses[s] > 0) ok = wait(&q_empty[s], (uses[s] - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          const bool whole = w.local == 0 && seg == w.u.n;
+          TreeSeg d;
+          d.seg = seg;
+          d.kt0 = w.u.kb + w.local * kPtTile;
+          d.lo = w.u.lo;
+          d.hi = w.u.hi;
+          d.L = w.u.row.L;
+          d.T = w.u.row.T;
+          d.tok0 = w.u.row.tok0;
+          d.first = w.u.qb * 2 * p.a.tpb;
+          d.c0 = w.u.c0;
+          d.c1 = w.u.c1;
+          d.h = w.h;
+          d.part = whole ? -1 : k > 0 ? 1 : 0;
+          d.q = place | (uses[0] & 1) << 1 | (uses[1] & 1) << 2;
+          d.pad[0] = d.pad[1] = d.pad[2] = 0;
+          segs[k & 3] = d;
+          mbar_arrive(&seg_full[k & 3]);
+          const long long start = w.t - w.local;
+          if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
+            PagedCut c;
+            c.tok0 = d.tok0 + d.first;
+            c.tok1 = c.tok0 + d.c0 + d.c1;
+            c.h = w.h;
+            c.g_last = share_owner(start + w.u.n - 1, total, ng);
+            c.slot1 = d.part;
+            c.pad[0] = c.pad[1] = c.pad[2] = 0;
+            p.cuts[blockIdx.x] = c;
+          }
+          for (int s = 0; s < 2; ++s) {
+            if (!both && s != place) continue;
+            if (both) mbar_arrive(&q_empty[s]);  // one group reads it; the other's arrival
+            mbar_arrive_expect_tx(&q_full[s], Cfg::kPanels * q_bytes);
+#pragma unroll
+            for (int pn = 0; pn < Cfg::kPanels; ++pn)
+              tma_load_3d(smem + s * Cfg::kTileBytes + pn * kPtTile * 128, &qmap, &q_full[s], pn * 64, w.h * p.a.G,
+                          d.tok0 + d.first + (both ? s * p.a.tpb : 0), q_pol);
+          }
+        }
+        __syncwarp();
+        for (int s = 0; s < 2; ++s) uses[s] += both || s == place;
+        ++k;
+        const int32_t* table = p.a.block_table + w.u.r * p.a.table_stride;
+        int pbase = 0, pg = 0;  // lane l holds the page of chunk pbase + l
+        auto pages_from = [&](int c) {
+          pbase = c;
+          const long long key = static_cast<long long>(c + lane) << box_shift;
+          pg = p.a.n_pages;  // outside the pool: a box there reads zeros
+          if (key <= w.u.hi && key + box > w.u.lo) {
+            pg = table[key >> p.a.page_shift];
+            if (pg < 0 || pg >= p.a.n_pages) {
+              record_error(kErrPageOutOfRange);
+              pg = p.a.n_pages;
+            }
+          }
+        };
+        pages_from((w.u.kb + w.local * kPtTile) >> box_shift);
+        for (int i = 0; ok && i < seg; ++i) {
+          const int c0 = (w.u.kb + (w.local + i) * kPtTile) >> box_shift;
+          if (c0 + nch > pbase + 32) pages_from(c0);
+          // a lane a box: chunk lch, panel lpn of the tile's, those with visible keys
+          const int key0 = (c0 + lch) << box_shift;
+          const bool load = lch < nch && key0 <= w.u.hi && key0 + box > w.u.lo;
+          const int row = __shfl_sync(0xffffffffu, pg, (c0 - pbase + lch) & 31) * p.a.Hkv + w.h;
+          const int pos = key0 & ((1 << p.a.page_shift) - 1);
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box_bytes;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++idx) {
+            const uint32_t st = idx % ST;
+            if (idx >= ST && !(ok = wait(&empty[st], ((idx / ST) - 1) & 1))) break;
+            if (lane == 0) {
+              if (!both) mbar_arrive(&empty[st]);  // one group reads it; the other's arrival
+              mbar_arrive_expect_tx(&full[st], bytes);
+            }
+            __syncwarp();
+            if (load)
+              tma_load_4d(smem + Cfg::kRingOff + st * Cfg::kTileBytes + lpn * kPtTile * 128 + lch * box_bytes,
+                          kv ? &vmap : &kmap, &full[st], 0, pos, lpn, row, kv_pol);
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
+        w.t += seg;
+        w.local += seg;
+        if (w.local == w.u.n && w.t < t_end) tree_next(p, w);
+      }
+      if (ok && lane == 0) {
+        segs[k & 3].seg = 0;
+        mbar_arrive(&seg_full[k & 3]);
+      }
+      if (*abort_flag && lane == 0) {  // the copies in flight land before the CTA can exit
+        for (uint32_t f = idx > ST ? idx - ST : 0; f < idx; ++f) mbar_wait(&full[f % ST], (f / ST) & 1);
+        for (int s = 0; s < 2; ++s)
+          if (uses[s] > 0) mbar_wait(&q_full[s], (uses[s] - 1) & 1);
+      }
+      __syncwarp();
+    } else if (warp < 3) {
+      // ---------------- product issuers, one a group ----------------
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPtTile, 0);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
+      const int t = __shfl_sync(0xffffffffu, warp - 1, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t s_col = tm + t * kPtTile, o_col = tm + Cfg::kOCol + t * D;
+      const uint64_t q0_desc = smem_desc_sw128(base, 16, 1024);
+      const uint64_t k0_desc = smem_desc_sw128(base + Cfg::kRingOff, 16, 1024);
+      const uint64_t v0_desc = smem_desc_sw128(base + Cfg::kRingOff, kPtTile * 128, 1024);
+      uint32_t g = 0, cnt = 0;  // key tiles of the parts before; this group's own
+      bool ok = true;
+      TreeSeg d;
+      for (int k = 0; ok; ++k) {
+        if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+        const bool both = d.c1 > 0;
+        const int place = both ? t : d.q & 1, step = both ? 1 : 2, j0 = both ? 0 : t;
+        const uint64_t q_desc = q0_desc + place * (Cfg::kTileBytes >> 4);
+        if (j0 >= d.seg) {
+          if (lane == 0) mbar_arrive(&q_empty[place]);
+        } else {
+          ok = wait(&q_full[place], (d.q >> (1 + place)) & 1);
+        }
+        for (int j = j0; ok && j < d.seg; j += step, ++cnt) {
+          const uint32_t ik = 2 * (g + j), iv = ik + 1, sk = ik % ST, sv = iv % ST;
+          if (!(ok = wait(&full[sk], (ik / ST) & 1))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t ka = k0_desc + sk * (Cfg::kTileBytes >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const int off = (kk >> 2) * ((kPtTile * 128) >> 4) + (kk & 3) * (32 >> 4);
+              umma_ss(s_col, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[t]);
+            umma_commit(&empty[sk]);
+            if (j + step >= d.seg) umma_commit(&q_empty[place]);
+          }
+          __syncwarp();
+          if (!(ok = wait(&full[sv], (iv / ST) & 1))) break;
+          if (!(ok = wait(&p_full[t], cnt & 1))) break;
+          // (a part's first product overwrites O_t: the last part's has been read)
+          if (j == j0 && k > 0 && !(ok = wait(&epi_done[t], (k - 1) & 1))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t va = v0_desc + sv * (Cfg::kTileBytes >> 4);
+#pragma unroll
+            for (int kk = 0; kk < kPtTile / 16; ++kk)
+              umma_ts(o_col, s_col + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o, kk > 0 || j > j0 ? 1u : 0u);
+            umma_commit(&empty[sv]);
+            if (j + step >= d.seg) umma_commit(&o_done[t]);
+          }
+          __syncwarp();
+        }
+        g += d.seg;
+      }
+      if (elect_one()) umma_commit(drained);  // every product has completed before TMEM is freed
+      __syncwarp();
+      mbar_wait(drained, 0);
+      __syncwarp();
+    }
+  } else {
+    // ---------------- softmax: four warps a group, a thread a query row ----------------
+    const int t = (warp - 4) >> 2, quarter = warp & 3;  // group; TMEM lanes 32 * quarter .. +31
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_off + t * kPtTile;  // S, and P over it
+    const uint32_t o_addr = tmem + lane_off + Cfg::kOCol;   // O_0; O_1 D columns on
+    const int rt = row / p.a.G;                             // the row's token in its tile
+    const float sc = p.a.scale_log2;
+    const uint64_t sc2 = pair_f32(sc, sc);
+    uint32_t g = 0, cnt = 0, ends = 0, ex = 0;
+    bool ok = true;
+    // the other group's v of this row (both warps of the quarter take part)
+    auto exchange = [&](float v) -> float {
+      xch[t * kPtTile + row] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair_bar[quarter]);
+      if (!wait(&pair_bar[quarter], ex++ & 1)) ok = false;
+      const float o = xch[(t ^ 1) * kPtTile + row];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair_bar[quarter]);  // read: the slots are free again
+      if (!wait(&pair_bar[quarter], ex++ & 1)) ok = false;
+      return o;
+    };
+    for (int k = 0; ok; ++k) {
+      TreeSeg d;
+      if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+      const bool both = d.c1 > 0, causal = d.T > 32 * p.words;
+      const int tile = both ? t : 0, step = both ? 1 : 2;
+      const int local = d.first + tile * p.a.tpb + rt;  // the row's token, counted from the request's first
+      const bool valid = rt < (tile ? d.c1 : d.c0);     // (rows past tpb * G have rt >= tpb)
+      TreeRowView view;
+      view.L = d.L;
+      view.T = d.T;
+      view.tok0 = d.tok0;
+      view.tok = -1;
+      view.pos = d.L;
+      view.see_lo = 0;
+      view.see_hi = -1;
+      if (valid) {
+        view.pos = causal ? d.L + local : max(p.positions[d.tok0 + local], d.L);
+        view.tok = causal ? -1 : d.tok0 + local;
+        view.see_lo = p.a.window >= 0 ? max(view.pos - p.a.window, 0) : 0;
+        view.see_hi = min(causal ? view.pos : d.L - 1, d.hi);
+      }
+      const bool warp_rows = __any_sync(0xffffffffu, valid);
+      float m_used = -INFINITY, l = 0.f;
+      bool own = false;  // this group has tiles of the part
+      for (int j = both ? 0 : t; j < d.seg; j += step, ++cnt) {
+        const int kt = d.kt0 + j * kPtTile;
+        const bool plain = __all_sync(0xffffffffu, !valid || (kt >= view.see_lo && kt + kPtTile - 1 <= view.see_hi));
+        if (kt < d.lo || kt + kPtTile - 1 > d.hi) {
+          // rows of V outside [lo, hi] to zero, a thread a row
+          const uint32_t iv = 2 * (g + j) + 1;
+          if (!(ok = wait(&full[iv % ST], (iv / ST) & 1))) break;
+          if (kt + row < d.lo || kt + row > d.hi) {
+            const uint32_t at = base + Cfg::kRingOff + (iv % ST) * Cfg::kTileBytes + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8 * Cfg::kPanels; ++c)
+              sts128(at + (c >> 3) * (kPtTile * 128) + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+          }
+          fence_proxy_async_shared();
+        }
+        if (!(ok = wait(&s_full[t], cnt & 1))) break;
+        tc_fence_after();
+        if (warp_rows) {  // (else P may be anything)
+          uint32_t bits[4];
+          if (!plain)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bits[c] = tree_bits(p, view, kt + 32 * c);
+          uint32_t s[128];
+          tmem_ld128(s_addr, s);
+          if (!plain)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(bits[c] >> e & 1)) s[32 * c + e] = __float_as_uint(-INFINITY);
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 128; e += 8) {
+            mx0 = fmax3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            mx1 = fmax3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+            mx2 = fmax3(mx2, __uint_as_float(s[e + 4]), __uint_as_float(s[e + 5]));
+            mx3 = fmax3(mx3, __uint_as_float(s[e + 6]), __uint_as_float(s[e + 7]));
+          }
+          const float mx = fmaxf(fmax3(mx0, mx1, mx2), mx3) * sc;
+          float alpha = 1.f;
+          if (mx > m_used + 8.f) {
+            alpha = fast_exp2(m_used - mx);  // 0 when m was -inf
+            m_used = mx;
+            l *= alpha;
+          }
+          if (own && __any_sync(0xffffffffu, alpha != 1.f)) tmem_scale(o_addr + t * D, D, alpha);
+          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+          const uint64_t nm2 = pair_f32(neg_m, neg_m);
+          uint64_t acc0 = 0, acc1 = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[16];
+            exp32(*reinterpret_cast<const uint32_t(*)[32]>(&s[32 * c]), sc2, nm2, w, acc0, acc1);
+            tmem_st16_nowait(s_addr + 16 * c, w);
+          }
+          acc0 = add2(acc0, acc1);
+          l += lo_f(acc0) + hi_f(acc0);
+          tmem_st_wait();
+        }
+        own = true;
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      if (own && !(ok = wait(&o_done[t], ends++ & 1))) break;
+      tc_fence_after();
+      if (__any_sync(0xffffffffu, valid) || !both) {
+        float w_own = 0.f, w_other = 0.f, lse;
+        if (both) {
+          w_own = l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
+          lse = l == 0.f ? -INFINITY : m_used + __log2f(l);
+        } else {
+          tc_fence_before();
+          const float m_other = exchange(m_used);  // (and the other group's O is complete)
+          const float m = fmaxf(m_used, m_other);
+          const float f_own = m_used == -INFINITY ? 0.f : fast_exp2(m_used - m);
+          const float f_other = m_other == -INFINITY ? 0.f : fast_exp2(m_other - m);
+          // (a sum of NaN under a maximum of -inf: every score was a NaN)
+          const float l_own = m_used == -INFINITY ? l : l * f_own, l_other = exchange(l_own);
+          tc_fence_after();
+          const float all = t ? l_other + l_own : l_own + l_other;
+          const float inv = all == 0.f ? 0.f : 1.f / all;
+          w_own = all != all ? all : f_own * inv;
+          w_other = all != all ? all : f_other * inv;
+          lse = all == 0.f ? -INFINITY : (m == -INFINITY ? all : m + __log2f(all));
+        }
+        if (!ok) break;
+        const long long slot = static_cast<long long>(blockIdx.x) * 2 + d.part;
+        const int prow = tile * kPtTile + row;
+        if (d.part >= 0 && valid && (both || t == 0)) p.a.part_lse[slot * 256 + prow] = lse;
+        const int orow = valid ? (d.tok0 + local) * p.a.Hq + d.h * p.a.G + (row - rt * p.a.G) : -1;
+        if (both) {
+          float* part = d.part < 0 ? nullptr : p.a.part_o + (slot * (D / 4) * 256 + prow) * 4;
+          tree_store<D>(o_addr + t * D, 0, w_own, 0.f, orow, p.a.out, D, part);
+        } else {  // half of the columns each
+          float* part = d.part < 0 ? nullptr : p.a.part_o + ((slot * (D / 4) + t * (D / 8)) * 256 + prow) * 4;
+          tree_store<D / 2>(o_addr + t * (D / 2), o_addr + D + t * (D / 2), t ? w_other : w_own, t ? w_own : w_other, orow,
+                            p.a.out + t * (D / 2), D, part);
+          tc_fence_before();
+          exchange(0.f);  // both have read both
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&epi_done[t]);  // O is read: the issuer may overwrite it
+      g += d.seg;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 }  // namespace mcb
