@@ -62,7 +62,7 @@ struct PagedTreeConfig {
   static constexpr uint32_t kOCol = 2 * kPtTile;         // TMEM: S (and P) below, O_0, O_1 above
   static constexpr int kRingOff = 2 * kTileBytes;        // Q0, Q1, then the ring
   static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
-  static constexpr int kNumBars = 2 * kStages + 21;
+  static constexpr int kNumBars = 4 * kStages + 29;
   static constexpr int kSegOff = (kBarOff + kNumBars * 8 + 32 + 63) / 64 * 64;
   static constexpr int kXchOff = kSegOff + 4 * 64;       // a float a row of either group
   static constexpr int kBytes = kXchOff + 2 * kPtTile * 4 + 1024;
@@ -107,7 +107,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const PagedTreeParams& p, const Pa
 
 // The part of a unit in one CTA's share, as the producer describes it to the other roles.
 struct TreeSeg {
-  int seg;             // key tiles (0: no more parts)
+  int seg;             // key tiles
   int kt0;             // the first one's first key
   int lo, hi;          // the unit's keys
   int L, T, tok0;      // the request's
@@ -116,7 +116,8 @@ struct TreeSeg {
   int h;               // kv head
   int part;            // -1: the whole unit; else the slot of the partial result
   int q;               // one tile: which of the two places its queries have; parities of q_full << 1, << 2
-  int pad[3];
+  int last;            // no more parts
+  int pad[2];
 };
 static_assert(sizeof(TreeSeg) == 64, "four descriptions of 64 bytes");
 
@@ -268,21 +269,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
-  uint64_t* full = bars;             // [ST] the ring: K of key tile g at 2 g, V at 2 g + 1
+  // [3][ST] the ring: K of key tile g at 2 g, V at 2 g + 1.  A set a reader -- group 0, group 1, both -- whose
+  // phases only its reader's uses advance: a wait is for the phase after the last one waited for, never
+  // for one that another reader's copy, still on its way, would have to complete first
+  uint64_t* full = bars;
   // [ST] two arrivals: both groups' products; one tile's keys: its group's and the producer's own
-  uint64_t* empty = full + ST;
+  uint64_t* empty = full + 3 * ST;
   uint64_t* q_full = empty + ST;     // [2]
   uint64_t* q_empty = q_full + 2;    // [2] two arrivals, as empty
-  uint64_t* s_full = q_empty + 2;    // [2]
-  uint64_t* p_full = s_full + 2;     // [2] 128 arrivals
-  uint64_t* o_done = p_full + 2;     // [2] a part's products are complete
+  uint64_t* s_full = q_empty + 2;    // [4] group * 2 + half of the key tile
+  uint64_t* p_full = s_full + 4;     // [4] 128 arrivals
+  uint64_t* pv_done = p_full + 4;    // [2] a half's P V is complete
+  uint64_t* v_ready = pv_done + 2;   // [2] a tile's values have landed, told for tiles with keys outside [lo, hi]
+  uint64_t* o_done = v_ready + 2;    // [2] a part's products are complete
   uint64_t* epi_done = o_done + 2;   // [2] 128 arrivals: ... and its O has been read
   // [4] a description is there.  Description x is written once the queries' place of part x - 2 or later is
   // free, so after every thread is past x - 4
   uint64_t* seg_full = epi_done + 2;
   uint64_t* pair_bar = seg_full + 4; // [4] two arrivals: the two warps of a row quarter
   uint64_t* drained = pair_bar + 4;  // two arrivals
-  static_assert(2 * ST + 21 == Cfg::kNumBars, "the barriers above");
+  static_assert(4 * ST + 29 == Cfg::kNumBars, "the barriers above");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* ctl = reinterpret_cast<int*>(tmem_slot + 2);  // start: r, qb, h, local
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int i = 0; i < Cfg::kNumBars; ++i) {
       uint64_t* b = bars + i;
       const bool two = (b >= empty && b < q_full) || (b >= q_empty && b < s_full) || b >= pair_bar;
-      const bool threads = (b >= p_full && b < o_done) || (b >= epi_done && b < seg_full);
+      const bool threads = (b >= p_full && b < pv_done) || (b >= epi_done && b < seg_full);
       mbar_init(b, threads ? 128 : two ? 2 : 1);
     }
     *abort_flag = 0;
@@ -396,6 +402,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         w.local = ctl[3];
       }
       uint32_t idx = 0;       // K and V tiles so far
+      uint32_t sets = 0, armed[3] = {0, 0, 0};  // two bits a stage: the set of its last copy; a bit: that set's phase
       int k = 0, place = 1;   // parts so far; the queries' place of the last one with one tile
       int uses[2] = {0, 0};   // of the two places
       bool ok = true;
@@ -422,7 +429,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           d.h = w.h;
           d.part = whole ? -1 : k > 0 ? 1 : 0;
           d.q = place | (uses[0] & 1) << 1 | (uses[1] & 1) << 2;
-          d.pad[0] = d.pad[1] = d.pad[2] = 0;
+          d.last = w.t + seg >= t_end;
+          d.pad[0] = d.pad[1] = 0;
           segs[k & 3] = d;
           mbar_arrive(&seg_full[k & 3]);
           const long long start = w.t - w.local;
@@ -477,14 +485,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           for (int kv = 0; kv < 2; ++kv, ++idx) {
             const uint32_t st = idx % ST;
             if (idx >= ST && !(ok = wait(&empty[st], ((idx / ST) - 1) & 1))) break;
+            const int set = both ? 2 : i & 1;
+            uint64_t* bar = full + set * ST + st;
             if (lane == 0) {
               if (!both) mbar_arrive(&empty[st]);  // one group reads it; the other's arrival
-              mbar_arrive_expect_tx(&full[st], bytes);
+              mbar_arrive_expect_tx(bar, bytes);
             }
+            sets = (sets & ~(3u << 2 * st)) | static_cast<uint32_t>(set) << 2 * st;
+#pragma unroll
+            for (int x = 0; x < 3; ++x) armed[x] ^= x == set ? 1u << st : 0u;
             __syncwarp();
             if (load)
               tma_load_4d(smem + Cfg::kRingOff + st * Cfg::kTileBytes + lpn * kPtTile * 128 + lch * box_bytes,
-                          kv ? &vmap : &kmap, &full[st], 0, pos, lpn, row, kv_pol);
+                          kv ? &vmap : &kmap, bar, 0, pos, lpn, row, kv_pol);
             __syncwarp();
           }
         }
@@ -493,19 +506,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         w.local += seg;
         if (w.local == w.u.n && w.t < t_end) tree_next(p, w);
       }
-      if (ok && lane == 0) {
-        segs[k & 3].seg = 0;
-        mbar_arrive(&seg_full[k & 3]);
-      }
       if (*abort_flag && lane == 0) {  // the copies in flight land before the CTA can exit
-        for (uint32_t f = idx > ST ? idx - ST : 0; f < idx; ++f) mbar_wait(&full[f % ST], (f / ST) & 1);
+        for (uint32_t st = 0; st < min(idx, static_cast<uint32_t>(ST)); ++st) {
+          const int set = sets >> 2 * st & 3;
+          const uint32_t a = set == 0 ? armed[0] : set == 1 ? armed[1] : armed[2];
+          mbar_wait(full + set * ST + st, ((a >> st) & 1) ^ 1);
+        }
         for (int s = 0; s < 2; ++s)
           if (uses[s] > 0) mbar_wait(&q_full[s], (uses[s] - 1) & 1);
       }
       __syncwarp();
     } else if (warp < 3) {
       // ---------------- product issuers, one a group ----------------
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPtTile, 0);
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
       const int t = __shfl_sync(0xffffffffu, warp - 1, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -513,11 +526,25 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const uint64_t q0_desc = smem_desc_sw128(base, 16, 1024);
       const uint64_t k0_desc = smem_desc_sw128(base + Cfg::kRingOff, 16, 1024);
       const uint64_t v0_desc = smem_desc_sw128(base + Cfg::kRingOff, kPtTile * 128, 1024);
-      uint32_t g = 0, cnt = 0;  // key tiles of the parts before; this group's own
+      uint32_t g = 0, cnt = 0;  // key tiles of the parts before; this group's own products'
+      uint32_t own_phase = 0, both_phase = 0;  // a bit a stage: the phases of this group's set and of both's
+      auto landed = [&](bool both, uint32_t st, bool poll) {
+        uint64_t* bar = full + (both ? 2 : t) * ST + st;
+        const uint32_t parity = (both ? both_phase : own_phase) >> st & 1;
+        if (poll) {
+          if (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return false;
+        } else if (!wait(bar, parity)) {
+          return false;
+        }
+        if (both) both_phase ^= 1u << st;
+        else own_phase ^= 1u << st;
+        return true;
+      };
       bool ok = true;
       TreeSeg d;
-      for (int k = 0; ok; ++k) {
-        if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+      d.last = t_begin >= t_end;
+      for (int k = 0; ok && !d.last; ++k) {
+        if (!(ok = next_seg(k, d))) break;
         const bool both = d.c1 > 0;
         const int place = both ? t : d.q & 1, step = both ? 1 : 2, j0 = both ? 0 : t;
         const uint64_t q_desc = q0_desc + place * (Cfg::kTileBytes >> 4);
@@ -526,36 +553,69 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         } else {
           ok = wait(&q_full[place], (d.q >> (1 + place)) & 1);
         }
-        for (int j = j0; ok && j < d.seg; j += step, ++cnt) {
-          const uint32_t ik = 2 * (g + j), iv = ik + 1, sk = ik % ST, sv = iv % ST;
-          if (!(ok = wait(&full[sk], (ik / ST) & 1))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t ka = k0_desc + sk * (Cfg::kTileBytes >> 4);
+        // Half by half: P V of key tile j and, over its S, the S of this group's next one (first both
+        // halves' S of the part's first tile).
+#pragma unroll 1
+        for (int j = j0 - step; ok && j0 < d.seg && j < d.seg; j += step) {
+          const bool pv = j >= j0, sn = j + step < d.seg;
+          const uint32_t sv = (2 * (g + j) + 1) % ST, sk = 2 * (g + j + step) % ST;
+          if (pv) {
+            if (!(ok = landed(both, sv, false))) break;
+            const int kt = d.kt0 + j * kPtTile;
+            if ((kt < d.lo || kt + kPtTile - 1 > d.hi) && lane == 0) mbar_arrive(&v_ready[t]);
+          }
+          auto issue_pv = [&](int h) {
+            if (!(ok = wait(&p_full[t * 2 + h], cnt & 1))) return;
+            // (a part's first product overwrites O_t: the last part's has been read)
+            if (j == j0 && h == 0 && k > 0 && !(ok = wait(&epi_done[t], (k - 1) & 1))) return;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t va = v0_desc + sv * (Cfg::kTileBytes >> 4) + h * ((64 * 128) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const int off = (kk >> 2) * ((kPtTile * 128) >> 4) + (kk & 3) * (32 >> 4);
-              umma_ss(s_col, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                umma_ts(o_col, s_col + h * 64 + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o,
+                        kk > 0 || h > 0 || j > j0 ? 1u : 0u);
+              umma_commit(&pv_done[t]);
+              if (h) umma_commit(&empty[sv]);
+              if (h && !sn) umma_commit(&o_done[t]);
             }
-            umma_commit(&s_full[t]);
-            umma_commit(&empty[sk]);
-            if (j + step >= d.seg) umma_commit(&q_empty[place]);
-          }
-          __syncwarp();
-          if (!(ok = wait(&full[sv], (iv / ST) & 1))) break;
-          if (!(ok = wait(&p_full[t], cnt & 1))) break;
-          // (a part's first product overwrites O_t: the last part's has been read)
-          if (j == j0 && k > 0 && !(ok = wait(&epi_done[t], (k - 1) & 1))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t va = v0_desc + sv * (Cfg::kTileBytes >> 4);
+            __syncwarp();
+          };
+          auto issue_s = [&](int h) {
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t ka = k0_desc + sk * (Cfg::kTileBytes >> 4) + h * ((64 * 128) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < kPtTile / 16; ++kk)
-              umma_ts(o_col, s_col + kk * 8, va + kk * ((16 * 128) >> 4), idesc_o, kk > 0 || j > j0 ? 1u : 0u);
-            umma_commit(&empty[sv]);
-            if (j + step >= d.seg) umma_commit(&o_done[t]);
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const int off = (kk >> 2) * ((kPtTile * 128) >> 4) + (kk & 3) * (32 >> 4);
+                umma_ss(s_col + h * 64, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[t * 2 + h]);
+              if (h) umma_commit(&empty[sk]);
+              if (h && j + 2 * step >= d.seg) umma_commit(&q_empty[place]);
+            }
+            __syncwarp();
+          };
+          // S of the next tile's first half goes between the two P V where its keys are there already
+          bool first_s = false;
+          if (pv) {
+            issue_pv(0);
+            if (!ok) break;
+            if (sn && landed(both, sk, true)) {
+              issue_s(0);
+              first_s = true;
+            }
+            issue_pv(1);
+            if (!ok) break;
           }
-          __syncwarp();
+          if (sn) {
+            if (!first_s) {
+              if (!(ok = landed(both, sk, false))) break;
+              issue_s(0);
+            }
+            issue_s(1);
+          }
+          cnt += pv;
         }
         g += d.seg;
       }
@@ -574,7 +634,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int rt = row / p.a.G;                             // the row's token in its tile
     const float sc = p.a.scale_log2;
     const uint64_t sc2 = pair_f32(sc, sc);
-    uint32_t g = 0, cnt = 0, ends = 0, ex = 0;
+    uint32_t g = 0, cnt = 0, all_halves = 0, edges = 0, ends = 0, ex = 0;
     bool ok = true;
     // the other group's v of this row (both warps of the quarter take part)
     auto exchange = [&](float v) -> float {
@@ -588,9 +648,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (!wait(&pair_bar[quarter], ex++ & 1)) ok = false;
       return o;
     };
-    for (int k = 0; ok; ++k) {
-      TreeSeg d;
-      if (!(ok = next_seg(k, d)) || d.seg == 0) break;
+    TreeSeg d;
+    d.last = t_begin >= t_end;
+    for (int k = 0; ok && !d.last; ++k) {
+      if (!(ok = next_seg(k, d))) break;
       const bool both = d.c1 > 0, causal = d.T > 32 * p.words;
       const int tile = both ? t : 0, step = both ? 1 : 2;
       const int local = d.first + tile * p.a.tpb + rt;  // the row's token, counted from the request's first
@@ -611,14 +672,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
-      bool own = false;  // this group has tiles of the part
+      int halves = 0;  // of this group's, of the part
       for (int j = both ? 0 : t; j < d.seg; j += step, ++cnt) {
         const int kt = d.kt0 + j * kPtTile;
-        const bool plain = __all_sync(0xffffffffu, !valid || (kt >= view.see_lo && kt + kPtTile - 1 <= view.see_hi));
         if (kt < d.lo || kt + kPtTile - 1 > d.hi) {
           // rows of V outside [lo, hi] to zero, a thread a row
           const uint32_t iv = 2 * (g + j) + 1;
-          if (!(ok = wait(&full[iv % ST], (iv / ST) & 1))) break;
+          if (!(ok = wait(&v_ready[t], edges++ & 1))) break;
           if (kt + row < d.lo || kt + row > d.hi) {
             const uint32_t at = base + Cfg::kRingOff + (iv % ST) * Cfg::kTileBytes + row * 128;
 #pragma unroll
@@ -627,56 +687,68 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           fence_proxy_async_shared();
         }
-        if (!(ok = wait(&s_full[t], cnt & 1))) break;
-        tc_fence_after();
-        if (warp_rows) {  // (else P may be anything)
-          uint32_t bits[4];
-          if (!plain)
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int k0 = kt + h * 64;
+          const bool plain = __all_sync(0xffffffffu, !valid || (k0 >= view.see_lo && k0 + 63 <= view.see_hi));
+          uint32_t bits[2];
+          if (!plain && warp_rows)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) bits[c] = tree_bits(p, view, kt + 32 * c);
-          uint32_t s[128];
-          tmem_ld128(s_addr, s);
-          if (!plain)
+            for (int c = 0; c < 2; ++c) bits[c] = tree_bits(p, view, k0 + 32 * c);
+          if (!(ok = wait(&s_full[t * 2 + h], cnt & 1))) break;
+          tc_fence_after();
+          if (warp_rows) {  // (else P may be anything)
+            uint32_t s[64];
+            tmem_ld64(s_addr + h * 64, s);
+            if (!plain)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(bits[c] >> e & 1)) s[32 * c + e] = __float_as_uint(-INFINITY);
-          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+                for (int e = 0; e < 32; ++e)
+                  if (!(bits[c] >> e & 1)) s[32 * c + e] = __float_as_uint(-INFINITY);
+            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 128; e += 8) {
-            mx0 = fmax3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-            mx1 = fmax3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-            mx2 = fmax3(mx2, __uint_as_float(s[e + 4]), __uint_as_float(s[e + 5]));
-            mx3 = fmax3(mx3, __uint_as_float(s[e + 6]), __uint_as_float(s[e + 7]));
+            for (int e = 0; e < 64; e += 8) {
+              mx0 = fmax3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+              mx1 = fmax3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+              mx2 = fmax3(mx2, __uint_as_float(s[e + 4]), __uint_as_float(s[e + 5]));
+              mx3 = fmax3(mx3, __uint_as_float(s[e + 6]), __uint_as_float(s[e + 7]));
+            }
+            const float mx = fmaxf(fmax3(mx0, mx1, mx2), mx3) * sc;
+            float alpha = 1.f;
+            if (mx > m_used + 8.f) {
+              alpha = fast_exp2(m_used - mx);  // 0 when m was -inf
+              m_used = mx;
+              l *= alpha;
+            }
+            if (halves > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+              // the half's before: the one product that S does not say is complete
+              if (!(ok = wait(&pv_done[t], (all_halves - 1) & 1))) break;
+              tc_fence_after();
+              tmem_scale(o_addr + t * D, D, alpha);
+            }
+            const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+            const uint64_t nm2 = pair_f32(neg_m, neg_m);
+            uint64_t acc0 = 0, acc1 = 0;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t w[16];
+              exp32(*reinterpret_cast<const uint32_t(*)[32]>(&s[32 * c]), sc2, nm2, w, acc0, acc1);
+              tmem_st16_nowait(s_addr + h * 64 + 16 * c, w);
+            }
+            acc0 = add2(acc0, acc1);
+            l += lo_f(acc0) + hi_f(acc0);
+            tmem_st_wait();
           }
-          const float mx = fmaxf(fmax3(mx0, mx1, mx2), mx3) * sc;
-          float alpha = 1.f;
-          if (mx > m_used + 8.f) {
-            alpha = fast_exp2(m_used - mx);  // 0 when m was -inf
-            m_used = mx;
-            l *= alpha;
-          }
-          if (own && __any_sync(0xffffffffu, alpha != 1.f)) tmem_scale(o_addr + t * D, D, alpha);
-          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-          const uint64_t nm2 = pair_f32(neg_m, neg_m);
-          uint64_t acc0 = 0, acc1 = 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[16];
-            exp32(*reinterpret_cast<const uint32_t(*)[32]>(&s[32 * c]), sc2, nm2, w, acc0, acc1);
-            tmem_st16_nowait(s_addr + 16 * c, w);
-          }
-          acc0 = add2(acc0, acc1);
-          l += lo_f(acc0) + hi_f(acc0);
-          tmem_st_wait();
+          ++halves;
+          ++all_halves;
+          tc_fence_before();
+          mbar_arrive(&p_full[t * 2 + h]);
         }
-        own = true;
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
+        if (!ok) break;
       }
       if (!ok) break;
-      if (own && !(ok = wait(&o_done[t], ends++ & 1))) break;
+      if (halves > 0 && !(ok = wait(&o_done[t], ends++ & 1))) break;
       tc_fence_after();
       if (__any_sync(0xffffffffu, valid) || !both) {
         float w_own = 0.f, w_other = 0.f, lse;
