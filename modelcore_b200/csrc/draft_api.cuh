@@ -55,20 +55,56 @@ int check_paged_tree(const mcb_paged_tree_attn_args* a, const char* who) {
 // the chunk kernel's.
 struct PagedTreePlan {
   bool chunk;  // some request may be a chunk of a prompt
+  int rows;    // query rows a unit: 16 or 32 with the keys on the M side, 256 the other kernel
   int grid;
-  size_t o, lse, cuts, ws_bytes;
+  size_t o, lse, cuts, chunk_o, chunk_lse, ws_bytes;
 };
 
 PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
   PagedTreePlan pl = {};
+  const long long G = t->attn.Hq / t->attn.Hkv;
   pl.chunk = t->attn.max_new == 0 || t->attn.max_new > 32 * t->words;
   pl.grid = device_sm_count();
-  const size_t rows = static_cast<size_t>(pl.grid) * 2 * 256;
+  // trees of at most max_new tokens, where that is known: as few rows as hold them
+  const long long most = std::min(t->attn.max_new > 0 ? t->attn.max_new : 32 * t->words, 32 * t->words) * G;
+  pl.rows = most <= 16 ? 16 : most <= 32 ? 32 : 256;
+  const size_t rows = static_cast<size_t>(pl.grid) * 2 * pl.rows, chunk_rows = static_cast<size_t>(pl.grid) * 2 * 256;
   pl.o = round256(rows * t->attn.D * 4);
   pl.lse = round256(rows * 4);
   pl.cuts = round256(pl.grid * sizeof(mcb::PagedCut));
-  pl.ws_bytes = (pl.o + pl.lse + pl.cuts) * (pl.chunk ? 2 : 1);
+  pl.ws_bytes = pl.o + pl.lse + pl.cuts;
+  if (pl.chunk) {
+    pl.chunk_o = round256(chunk_rows * t->attn.D * 4);
+    pl.chunk_lse = round256(chunk_rows * 4);
+    pl.ws_bytes += pl.chunk_o + pl.chunk_lse + pl.cuts;
+  }
   return pl;
+}
+
+template <int D, int R>
+int launch_tree_few(const mcb_paged_attn_args* a, const mcb::PagedTreeParams& p, const int64_t (&q_stride)[2], int grid,
+                    cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int smem = mcb::TreeFewConfig<D, R>::kBytes;
+  CUtensorMap qm, km, vm;
+  const int box = std::min(a->page_size, mcb::kPtTile);
+  int rc = encode_packed_q_map(&qm, a, q_stride, p.a.tpb);
+  if (rc == MCB_OK) rc = encode_page_map(&km, a->k_pages, a, box, 1);
+  if (rc == MCB_OK) rc = encode_page_map(&vm, a->v_pages, a, box, 1);
+  if (rc != MCB_OK) return rc;
+  cudaError_t e = ensure_smem(mcb::paged_tree_few_kernel<D, R>, smem, done);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged_tree_few)");
+  e = launch_pdl(mcb::paged_tree_few_kernel<D, R>, dim3(static_cast<unsigned>(grid)), dim3(mcb::kPtThreads),
+                 static_cast<size_t>(smem), st, qm, km, vm, p);
+  g_launches++;
+  note_attn_kernel("paged_tree_few_kernel", D, 0, R, false);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged_tree_few launch");
+  e = launch_pdl(mcb::tree_few_combine_kernel<D, R>, dim3(static_cast<unsigned>(grid), R / 8), dim3(256), 0, st, p);
+  g_launches++;
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "tree_few_combine launch");
+  return MCB_OK;
 }
 
 template <int D>
@@ -139,28 +175,37 @@ int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
   p.a.window = a->window;
   p.a.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.a.few_rows = 32 * t->words * p.a.G;  // the chunk kernel's share begins above
-  p.a.tpb = mcb::kPtTile / p.a.G;
+  p.a.tpb = std::min(pl.rows, mcb::kPtTile) / p.a.G;
+  p.unit_tok = pl.rows == 256 ? 2 * p.a.tpb : p.a.tpb;
   p.a.all = !pl.chunk;
   p.a.fill = 1;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  auto parts = [&](mcb::PagedAttnParams& q, mcb::PagedCut*& cuts) {
-    q.part_o = reinterpret_cast<float*>(ws);
-    q.part_lse = reinterpret_cast<float*>(ws + pl.o);
-    cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.o + pl.lse);
-    ws += pl.o + pl.lse + pl.cuts;
-  };
-  parts(p.a, p.cuts);
+  p.a.part_o = reinterpret_cast<float*>(ws);
+  p.a.part_lse = reinterpret_cast<float*>(ws + pl.o);
+  p.cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.o + pl.lse);
   p.positions = t->positions;
   p.mask = reinterpret_cast<const uint32_t*>(t->mask);
   p.words = t->words;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  rc = a->D == 64 ? launch_paged_tree<64>(a, p, qs.s, pl.grid, st) : launch_paged_tree<128>(a, p, qs.s, pl.grid, st);
+  auto launch = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    switch (pl.rows) {
+      case 16: return launch_tree_few<D, 16>(a, p, qs.s, pl.grid, st);
+      case 32: return launch_tree_few<D, 32>(a, p, qs.s, pl.grid, st);
+      default: return launch_paged_tree<D>(a, p, qs.s, pl.grid, st);
+    }
+  };
+  rc = a->D == 64 ? launch(std::integral_constant<int, 64>()) : launch(std::integral_constant<int, 128>());
   if (rc != MCB_OK || !pl.chunk) return rc;
   mcb::PagedChunkParams c = {};
   c.a = p.a;
   c.a.all = 0;
   c.a.fill = 0;
-  parts(c.a, c.cuts);
+  c.a.tpb = mcb::kPcTile / p.a.G;
+  ws += pl.o + pl.lse + pl.cuts;
+  c.a.part_o = reinterpret_cast<float*>(ws);
+  c.a.part_lse = reinterpret_cast<float*>(ws + pl.chunk_o);
+  c.cuts = reinterpret_cast<mcb::PagedCut*>(ws + pl.chunk_o + pl.chunk_lse);
   c.wait_last = 1;
   return a->D == 64 ? launch_paged_chunk<64>(a, c, qs.s, pl.grid, st) : launch_paged_chunk<128>(a, c, qs.s, pl.grid, st);
 }

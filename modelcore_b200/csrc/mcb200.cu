@@ -26,6 +26,7 @@
 #include "paged_chunk.cuh"
 #include "paged_plan.cuh"
 #include "paged_tree.cuh"
+#include "paged_tree_few.cuh"
 #include "prefill_attn.cuh"
 #include "decode_proj.cuh"
 #include "sample.cuh"

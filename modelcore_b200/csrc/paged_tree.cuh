@@ -15,7 +15,8 @@
 //
 // Roles of a CTA's warps:
 //   warp 0      TMA producer and walker: describes each part of a unit in shared memory, loads its queries,
-//               and K and V tiles into one ring that runs on across units
+//               and K tiles into a ring that runs on across units
+//   warp 3      the same walk, V tiles
 //   warps 1, 2  (warp 1 allocates TMEM) products of group 0, of group 1:
 //                 S_t = Q K_j^T   M=128 N=128 K=D   (both operands from shared memory)
 //                 O_t += P_t V_j  M=128 N=D K=128   (P from TMEM, over its S)
@@ -48,17 +49,19 @@ struct PagedTreeParams {
   const int32_t* positions;  // (N,)
   const uint32_t* mask;      // (N, words)
   int words;
+  int unit_tok;              // new tokens a unit: a tile's or two tiles'
 };
 
 constexpr int kPtTile = 128;      // query rows a tile, keys a key tile
-constexpr int kPtThreads = 384;   // producer, two issuers, an idle warp, 2 x 4 softmax warps
+constexpr int kPtThreads = 384;   // two producers, two issuers, 2 x 4 softmax warps
 constexpr int kPtWarps = kPtThreads / 32;
 
 template <int D>
 struct PagedTreeConfig {
   static constexpr int kPanels = D / 64;
   static constexpr int kTileBytes = kPanels * kPtTile * 128;
-  static constexpr int kStages = D == 128 ? 5 : 12;      // K and V tiles in turn
+  static constexpr int kK = D == 128 ? 2 : 5, kV = D == 128 ? 3 : 7;  // (V's wait for the softmax)
+  static constexpr int kStages = kK + kV;                // K's ring, then V's
   static constexpr uint32_t kOCol = 2 * kPtTile;         // TMEM: S (and P) below, O_0, O_1 above
   static constexpr int kRingOff = 2 * kTileBytes;        // Q0, Q1, then the ring
   static constexpr int kBarOff = kRingOff + kStages * kTileBytes;
@@ -74,7 +77,7 @@ struct PagedTreeConfig {
 struct TreeUnit {
   PagedRow row;
   int r, qb, nqb;
-  int c0, c1;       // tokens in Q0 and Q1 (first tokens: qb * 2 tpb, + tpb)
+  int c0, c1;       // tokens in Q0 and Q1 (first tokens: qb * unit_tok, + tpb)
   int lo, hi, kb, n;
 };
 
@@ -83,7 +86,7 @@ __device__ __forceinline__ bool tree_causal(const PagedTreeParams& p, const Page
 }
 
 __device__ __forceinline__ int tree_blocks(const PagedTreeParams& p, const PagedRow& x) {
-  return p.a.all || !tree_causal(p, x) ? (x.T + 2 * p.a.tpb - 1) / (2 * p.a.tpb) : 0;
+  return p.a.all || !tree_causal(p, x) ? (x.T + p.unit_tok - 1) / p.unit_tok : 0;
 }
 
 __device__ __forceinline__ TreeUnit tree_unit(const PagedTreeParams& p, const PagedRow& x, int r, int qb, int nqb) {
@@ -92,9 +95,9 @@ __device__ __forceinline__ TreeUnit tree_unit(const PagedTreeParams& p, const Pa
   u.r = r;
   u.qb = qb;
   u.nqb = nqb;
-  const int first = qb * 2 * p.a.tpb, left = x.T - first;
+  const int first = qb * p.unit_tok, left = min(x.T - first, p.unit_tok);
   u.c0 = min(left, p.a.tpb);
-  u.c1 = min(max(left - p.a.tpb, 0), p.a.tpb);
+  u.c1 = left - u.c0;
   const bool causal = tree_causal(p, x);
   const long long cap = (static_cast<long long>(p.a.max_pages) << p.a.page_shift) - 1;
   const int last = causal ? first + u.c0 + u.c1 - 1 : x.T - 1;  // a tree's token may see any other
@@ -181,23 +184,22 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b) {
 }
 
 // Which of the 32 keys from k0 on a row sees.  Out of line: a tile in a request's interior asks for none.
-struct TreeRowView {
-  int see_lo, see_hi;  // its interval of cached keys (a chunk's token: of all)
-  int L, T, tok0, tok; // the request's, and its own place in the packed batch (-1: a tree without masks)
-  int pos;
-};
-__device__ __noinline__ uint32_t tree_bits(const PagedTreeParams& p, const TreeRowView& v, int k0) {
-  uint32_t bits = bit_range(max(v.see_lo - k0, 0), min(v.see_hi - k0, 31));
-  const int j0 = k0 - v.L;  // the first key's place among the new tokens
-  if (v.tok < 0 || j0 <= -32 || j0 >= v.T) return bits;
+// (Arguments by value: what has an address lives in local memory, and shared memory leaves the L1 cache next to
+// nothing to keep it.)  [see_lo, see_hi]: its interval of cached keys (a chunk's token: of all); L, T, tok0 the
+// request's; tok its own place in the packed batch (-1: by the interval alone), pos its position.
+__device__ __noinline__ uint32_t tree_bits(const PagedTreeParams& p, int see_lo, int see_hi, int L, int T, int tok0,
+                                           int tok, int pos, int k0) {
+  uint32_t bits = bit_range(max(see_lo - k0, 0), min(see_hi - k0, 31));
+  const int j0 = k0 - L;  // the first key's place among the new tokens
+  if (tok < 0 || j0 <= -32 || j0 >= T) return bits;
   const int w = j0 >> 5, sh = j0 & 31;
-  const uint32_t* row = p.mask + static_cast<long long>(v.tok) * p.words;
+  const uint32_t* row = p.mask + static_cast<long long>(tok) * p.words;
   const uint32_t a = w >= 0 && w < p.words ? row[w] : 0u, b = w + 1 < p.words ? row[w + 1] : 0u;
-  uint32_t fresh = __funnelshift_r(a, b, sh) & bit_range(max(-j0, 0), min(v.T - 1 - j0, 31));
-  if (p.a.window >= 0 && v.pos - v.L > p.a.window)  // (a new token's position is L or more)
+  uint32_t fresh = __funnelshift_r(a, b, sh) & bit_range(max(-j0, 0), min(T - 1 - j0, 31));
+  if (p.a.window >= 0 && pos - L > p.a.window)  // (a new token's position is L or more)
     for (uint32_t left = fresh; left != 0; left &= left - 1) {
       const int e = __ffs(left) - 1;
-      if (v.pos - max(p.positions[v.tok0 + j0 + e], v.L) > p.a.window) fresh &= ~(1u << e);
+      if (pos - max(p.positions[tok0 + j0 + e], L) > p.a.window) fresh &= ~(1u << e);
     }
   return bits | fresh;
 }
@@ -264,12 +266,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     paged_tree_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedTreeParams p) {
   using Cfg = PagedTreeConfig<D>;
-  constexpr int ST = Cfg::kStages;
+  constexpr int ST = Cfg::kStages, SK = Cfg::kK, SV = Cfg::kV;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOff);
-  // [3][ST] the ring: K of key tile g at 2 g, V at 2 g + 1.  A set a reader -- group 0, group 1, both -- whose
+  // [3][ST] the rings: K of key tile g at g mod kK, V at kK + g mod kV.  A set a reader -- group 0, group 1, both -- whose
   // phases only its reader's uses advance: a wait is for the phase after the last one waited for, never
   // for one that another reader's copy, still on its way, would have to complete first
   uint64_t* full = bars;
@@ -385,14 +387,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   };
 
   if (warp < 4) {
-    if (warp == 0) {
-      // ---------------- producer and walker ----------------
-      const uint64_t q_pol = l2_policy_evict_first(), kv_pol = l2_policy_evict_first();
+    if (warp == 0 || warp == 3) {
+      // ---------------- producers: of K, the queries and the descriptions; of V ----------------
+      // (one warp for both tiles, a chain of some 100 dependent instructions a tile and 1,000 cycles, was what
+      // bounded head size 64)
+      const int kv = warp == 3;
+      const CUtensorMap* map = kv ? &vmap : &kmap;
+      const uint64_t policy = l2_policy_evict_first();
       const int box_shift = min(p.a.page_shift, 7);  // positions a box: min(page, 128)
       const int box = 1 << box_shift, nch = kPtTile >> box_shift;
       const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
       const uint32_t q_bytes = static_cast<uint32_t>(p.a.tpb * p.a.G) * 128u;
       const int lch = lane / Cfg::kPanels, lpn = lane % Cfg::kPanels;
+      const uint32_t lane_dst = Cfg::kRingOff + lpn * kPtTile * 128 + lch * box_bytes;
       TreeWalk w;
       w.t = t_begin;
       if (active) {
@@ -401,105 +408,109 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         w.h = ctl[2];
         w.local = ctl[3];
       }
-      uint32_t idx = 0;       // K and V tiles so far
+      uint32_t gt = 0;        // key tiles so far
       uint32_t sets = 0, armed[3] = {0, 0, 0};  // two bits a stage: the set of its last copy; a bit: that set's phase
+      uint32_t mine = 0;                        // stages with a copy of this warp's last
       int k = 0, place = 1;   // parts so far; the queries' place of the last one with one tile
       int uses[2] = {0, 0};   // of the two places
       bool ok = true;
       while (ok && w.t < t_end) {
         const int seg = static_cast<int>(min(static_cast<long long>(w.u.n - w.local), t_end - w.t));
         const bool both = w.u.c1 > 0;
-        if (!both) place ^= 1;
-        for (int s = 0; s < 2 && ok; ++s)
-          if ((both || s == place) && uses[s] > 0) ok = wait(&q_empty[s], (uses[s] - 1) & 1);
-        if (!ok) break;
-        if (lane == 0) {
-          const bool whole = w.local == 0 && seg == w.u.n;
-          TreeSeg d;
-          d.seg = seg;
-          d.kt0 = w.u.kb + w.local * kPtTile;
-          d.lo = w.u.lo;
-          d.hi = w.u.hi;
-          d.L = w.u.row.L;
-          d.T = w.u.row.T;
-          d.tok0 = w.u.row.tok0;
-          d.first = w.u.qb * 2 * p.a.tpb;
-          d.c0 = w.u.c0;
-          d.c1 = w.u.c1;
-          d.h = w.h;
-          d.part = whole ? -1 : k > 0 ? 1 : 0;
-          d.q = place | (uses[0] & 1) << 1 | (uses[1] & 1) << 2;
-          d.last = w.t + seg >= t_end;
-          d.pad[0] = d.pad[1] = 0;
-          segs[k & 3] = d;
-          mbar_arrive(&seg_full[k & 3]);
-          const long long start = w.t - w.local;
-          if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
-            PagedCut c;
-            c.tok0 = d.tok0 + d.first;
-            c.tok1 = c.tok0 + d.c0 + d.c1;
-            c.h = w.h;
-            c.g_last = share_owner(start + w.u.n - 1, total, ng);
-            c.slot1 = d.part;
-            c.pad[0] = c.pad[1] = c.pad[2] = 0;
-            p.cuts[blockIdx.x] = c;
-          }
-          for (int s = 0; s < 2; ++s) {
-            if (!both && s != place) continue;
-            if (both) mbar_arrive(&q_empty[s]);  // one group reads it; the other's arrival
-            mbar_arrive_expect_tx(&q_full[s], Cfg::kPanels * q_bytes);
-#pragma unroll
-            for (int pn = 0; pn < Cfg::kPanels; ++pn)
-              tma_load_3d(smem + s * Cfg::kTileBytes + pn * kPtTile * 128, &qmap, &q_full[s], pn * 64, w.h * p.a.G,
-                          d.tok0 + d.first + (both ? s * p.a.tpb : 0), q_pol);
-          }
-        }
-        __syncwarp();
-        for (int s = 0; s < 2; ++s) uses[s] += both || s == place;
-        ++k;
         const int32_t* table = p.a.block_table + w.u.r * p.a.table_stride;
-        int pbase = 0, pg = 0;  // lane l holds the page of chunk pbase + l
-        auto pages_from = [&](int c) {
-          pbase = c;
+        // lane l holds the page of chunk pbase + l; the next 32 are on their way
+        int pbase = 0, pg = 0, pg_next = 0;
+        bool in_next = false;
+        auto page_at = [&](int c) {
           const long long key = static_cast<long long>(c + lane) << box_shift;
-          pg = p.a.n_pages;  // outside the pool: a box there reads zeros
-          if (key <= w.u.hi && key + box > w.u.lo) {
-            pg = table[key >> p.a.page_shift];
-            if (pg < 0 || pg >= p.a.n_pages) {
-              record_error(kErrPageOutOfRange);
-              pg = p.a.n_pages;
+          in_next = key <= w.u.hi && key + box > w.u.lo;
+          return in_next ? table[key >> p.a.page_shift] : 0;
+        };
+        const int c_first = (w.u.kb + w.local * kPtTile) >> box_shift;
+        pg_next = page_at(c_first);
+        pbase = c_first - 32;
+        if (!kv) {
+          if (!both) place ^= 1;
+          for (int s = 0; s < 2 && ok; ++s)
+            if ((both || s == place) && uses[s] > 0) ok = wait(&q_empty[s], (uses[s] - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) {
+            const bool whole = w.local == 0 && seg == w.u.n;
+            TreeSeg d;
+            d.seg = seg;
+            d.kt0 = w.u.kb + w.local * kPtTile;
+            d.lo = w.u.lo;
+            d.hi = w.u.hi;
+            d.L = w.u.row.L;
+            d.T = w.u.row.T;
+            d.tok0 = w.u.row.tok0;
+            d.first = w.u.qb * p.unit_tok;
+            d.c0 = w.u.c0;
+            d.c1 = w.u.c1;
+            d.h = w.h;
+            d.part = whole ? -1 : k > 0 ? 1 : 0;
+            d.q = place | (uses[0] & 1) << 1 | (uses[1] & 1) << 2;
+            d.last = w.t + seg >= t_end;
+            d.pad[0] = d.pad[1] = 0;
+            segs[k & 3] = d;
+            mbar_arrive(&seg_full[k & 3]);
+            const long long start = w.t - w.local;
+            if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
+              PagedCut c;
+              c.tok0 = d.tok0 + d.first;
+              c.tok1 = c.tok0 + d.c0 + d.c1;
+              c.h = w.h;
+              c.g_last = share_owner(start + w.u.n - 1, total, ng);
+              c.slot1 = d.part;
+              c.pad[0] = c.pad[1] = c.pad[2] = 0;
+              p.cuts[blockIdx.x] = c;
+            }
+            for (int s = 0; s < 2; ++s) {
+              if (!both && s != place) continue;
+              if (both) mbar_arrive(&q_empty[s]);  // one group reads it; the other's arrival
+              mbar_arrive_expect_tx(&q_full[s], Cfg::kPanels * q_bytes);
+#pragma unroll
+              for (int pn = 0; pn < Cfg::kPanels; ++pn)
+                tma_load_3d(smem + s * Cfg::kTileBytes + pn * kPtTile * 128, &qmap, &q_full[s], pn * 64, w.h * p.a.G,
+                            d.tok0 + d.first + (both ? s * p.a.tpb : 0), policy);
             }
           }
-        };
-        pages_from((w.u.kb + w.local * kPtTile) >> box_shift);
-        for (int i = 0; ok && i < seg; ++i) {
-          const int c0 = (w.u.kb + (w.local + i) * kPtTile) >> box_shift;
-          if (c0 + nch > pbase + 32) pages_from(c0);
+          __syncwarp();
+          for (int s = 0; s < 2; ++s) uses[s] += both || s == place;
+          ++k;
+        }
+        for (int i = 0; i < seg; ++i, ++gt) {
+          const int c0 = c_first + i * nch;
+          if (c0 + nch > pbase + 32) {
+            pbase = c0;
+            pg = pg_next;
+            if (pg < 0 || pg >= p.a.n_pages) {
+              if (in_next) record_error(kErrPageOutOfRange);
+              pg = p.a.n_pages;  // outside the pool: a box there reads zeros
+            }
+            pg_next = page_at(c0 + 32);
+          }
           // a lane a box: chunk lch, panel lpn of the tile's, those with visible keys
           const int key0 = (c0 + lch) << box_shift;
           const bool load = lch < nch && key0 <= w.u.hi && key0 + box > w.u.lo;
           const int row = __shfl_sync(0xffffffffu, pg, (c0 - pbase + lch) & 31) * p.a.Hkv + w.h;
           const int pos = key0 & ((1 << p.a.page_shift) - 1);
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box_bytes;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++idx) {
-            const uint32_t st = idx % ST;
-            if (idx >= ST && !(ok = wait(&empty[st], ((idx / ST) - 1) & 1))) break;
-            const int set = both ? 2 : i & 1;
-            uint64_t* bar = full + set * ST + st;
-            if (lane == 0) {
-              if (!both) mbar_arrive(&empty[st]);  // one group reads it; the other's arrival
-              mbar_arrive_expect_tx(bar, bytes);
-            }
-            sets = (sets & ~(3u << 2 * st)) | static_cast<uint32_t>(set) << 2 * st;
-#pragma unroll
-            for (int x = 0; x < 3; ++x) armed[x] ^= x == set ? 1u << st : 0u;
-            __syncwarp();
-            if (load)
-              tma_load_4d(smem + Cfg::kRingOff + st * Cfg::kTileBytes + lpn * kPtTile * 128 + lch * box_bytes,
-                          kv ? &vmap : &kmap, bar, 0, pos, lpn, row, kv_pol);
-            __syncwarp();
+          const uint32_t st = kv ? SK + gt % SV : gt % SK, turn = kv ? gt / SV : gt / SK;
+          if (turn > 0 && !(ok = wait(&empty[st], (turn - 1) & 1))) break;
+          const int set = both ? 2 : i & 1;
+          uint64_t* bar = full + set * ST + st;
+          if (lane == 0) {
+            if (!both) mbar_arrive(&empty[st]);  // one group reads it; the other's arrival
+            mbar_arrive_expect_tx(bar, bytes);
           }
+          mine |= 1u << st;
+          sets = (sets & ~(3u << 2 * st)) | static_cast<uint32_t>(set) << 2 * st;
+#pragma unroll
+          for (int x = 0; x < 3; ++x) armed[x] ^= x == set ? 1u << st : 0u;
+          __syncwarp();
+          if (load) tma_load_4d(smem + lane_dst + st * Cfg::kTileBytes, map, bar, 0, pos, lpn, row, policy);
+          __syncwarp();
         }
         if (!ok) break;
         w.t += seg;
@@ -507,7 +518,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (w.local == w.u.n && w.t < t_end) tree_next(p, w);
       }
       if (*abort_flag && lane == 0) {  // the copies in flight land before the CTA can exit
-        for (uint32_t st = 0; st < min(idx, static_cast<uint32_t>(ST)); ++st) {
+        for (int st = 0; st < ST; ++st) {
+          if (!(mine >> st & 1)) continue;
           const int set = sets >> 2 * st & 3;
           const uint32_t a = set == 0 ? armed[0] : set == 1 ? armed[1] : armed[2];
           mbar_wait(full + set * ST + st, ((a >> st) & 1) ^ 1);
@@ -558,7 +570,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll 1
         for (int j = j0 - step; ok && j0 < d.seg && j < d.seg; j += step) {
           const bool pv = j >= j0, sn = j + step < d.seg;
-          const uint32_t sv = (2 * (g + j) + 1) % ST, sk = 2 * (g + j + step) % ST;
+          const uint32_t sv = SK + (g + j) % SV, sk = (g + j + step) % SK;
           if (pv) {
             if (!(ok = landed(both, sv, false))) break;
             const int kt = d.kt0 + j * kPtTile;
@@ -656,19 +668,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int tile = both ? t : 0, step = both ? 1 : 2;
       const int local = d.first + tile * p.a.tpb + rt;  // the row's token, counted from the request's first
       const bool valid = rt < (tile ? d.c1 : d.c0);     // (rows past tpb * G have rt >= tpb)
-      TreeRowView view;
-      view.L = d.L;
-      view.T = d.T;
-      view.tok0 = d.tok0;
-      view.tok = -1;
-      view.pos = d.L;
-      view.see_lo = 0;
-      view.see_hi = -1;
+      int pos = d.L, tok = -1, see_lo = 0, see_hi = -1;
       if (valid) {
-        view.pos = causal ? d.L + local : max(p.positions[d.tok0 + local], d.L);
-        view.tok = causal ? -1 : d.tok0 + local;
-        view.see_lo = p.a.window >= 0 ? max(view.pos - p.a.window, 0) : 0;
-        view.see_hi = min(causal ? view.pos : d.L - 1, d.hi);
+        pos = causal ? d.L + local : max(p.positions[d.tok0 + local], d.L);
+        tok = causal ? -1 : d.tok0 + local;
+        see_lo = p.a.window >= 0 ? max(pos - p.a.window, 0) : 0;
+        see_hi = min(causal ? pos : d.L - 1, d.hi);
       }
       const bool warp_rows = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
@@ -677,10 +682,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int kt = d.kt0 + j * kPtTile;
         if (kt < d.lo || kt + kPtTile - 1 > d.hi) {
           // rows of V outside [lo, hi] to zero, a thread a row
-          const uint32_t iv = 2 * (g + j) + 1;
           if (!(ok = wait(&v_ready[t], edges++ & 1))) break;
           if (kt + row < d.lo || kt + row > d.hi) {
-            const uint32_t at = base + Cfg::kRingOff + (iv % ST) * Cfg::kTileBytes + row * 128;
+            const uint32_t at = base + Cfg::kRingOff + (SK + (g + j) % SV) * Cfg::kTileBytes + row * 128;
 #pragma unroll
             for (int c = 0; c < 8 * Cfg::kPanels; ++c)
               sts128(at + (c >> 3) * (kPtTile * 128) + (c & 7) * 16, make_uint4(0, 0, 0, 0));
@@ -690,11 +694,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           const int k0 = kt + h * 64;
-          const bool plain = __all_sync(0xffffffffu, !valid || (k0 >= view.see_lo && k0 + 63 <= view.see_hi));
+          const bool plain = __all_sync(0xffffffffu, !valid || (k0 >= see_lo && k0 + 63 <= see_hi));
           uint32_t bits[2];
           if (!plain && warp_rows)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) bits[c] = tree_bits(p, view, k0 + 32 * c);
+            for (int c = 0; c < 2; ++c) bits[c] = tree_bits(p, see_lo, see_hi, d.L, d.T, d.tok0, tok, pos, k0 + 32 * c);
           if (!(ok = wait(&s_full[t * 2 + h], cnt & 1))) break;
           tc_fence_after();
           if (warp_rows) {  // (else P may be anything)
