@@ -242,7 +242,8 @@ int verify_drafts(const mcb_verify_drafts_args* a, void* stream) {
   p.V = a->V;
   p.max_path = a->max_path;
   p.temperature = a->temperature;
-  // CTAs a request: as many as fill the GPU, up to the portable cluster, none with less than 2,048 tokens
+  // CTAs a request: as many as the GPU holds at two an SM, up to the portable cluster, none with less than 2,048
+  // tokens
   int c = 1;
   while (c < 8 && 2ll * c * a->R <= 2ll * device_sm_count() && a->V / (2 * c) >= 2048) c *= 2;
   if (static_cast<long long>(a->R) * c > INT32_MAX)

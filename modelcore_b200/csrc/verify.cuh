@@ -12,10 +12,16 @@
 // So the tokens are distributed as if each had been drawn from its p, whatever the draft was.  T = 0: a
 // child is kept when its token is the first one of the largest logit, which is the next token otherwise.
 //
-// Only the rows on the walk are read: a cluster of C CTAs a request, the vocabulary divided among them.
-// Weights, their sums and the draw are in 64 bits: a vocabulary of 10^5 has borders everywhere, and
-// 32-bit sums put a draw on their wrong side now and then.  Every CTA takes the walk's decisions itself,
-// from the same numbers, exchanged through distributed shared memory.
+// Only the rows on the walk are read: a cluster of C CTAs a request, the vocabulary divided among them,
+// and every CTA takes the walk's decisions itself from the same numbers, exchanged through distributed shared
+// memory.  What is decided is what 64-bit sums decide, to their rounding: a vocabulary of 10^5 has borders
+// everywhere, and 32-bit sums put a draw on their wrong side now and then.
+//   A token's row is first summed in 32 bits (one pass, bound by its bytes), with a bound on how far off the
+//   sums can be; children are kept or refused by these while the sides of the comparison are further apart than
+//   that, in nearly all cases.  Where they are not, and where the walk ends and a token is drawn, the row is
+//   summed again in 64 bits (bound by the 64-bit units: about 11 operations a token and pass).
+// 2^t in 64 bits: t = n / 32 + f with |f| <= 1/64, a table of 2^(j/32) and five terms of 2^f's series in f ln 2
+// (the remainder, (ln 2 / 64)^6 / 720, is 2e-15): Tang's table-driven method, ACM TOMS 15, 1989.
 #pragma once
 
 #include "paged_plan.cuh"
@@ -45,116 +51,283 @@ struct VerifyParams {
 
 __device__ __forceinline__ float logit_of(const float* p) { return *p; }
 __device__ __forceinline__ float logit_of(const uint16_t* p) { return bf16_bits_to_float(*p); }
+// Four values from an address that four of them divide.
+__device__ __forceinline__ float4 logits4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 logits4(const uint16_t* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                     __uint_as_float(v.y & 0xffff0000u));
+}
 
-__device__ __forceinline__ void st_dsmem_f64(uint32_t addr, double v) {
-  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+__device__ __forceinline__ void st_dsmem_u64(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
 struct VerifyShared {
-  double xch[2][8];              // what the cluster's CTAs exchange
-  double warp_sum[kVerifyWarps]; // this CTA's warps' sums of the last pass
-  double part[kVerifyWarps];
-  double inv_mass[kVerifyMaxTried];  // with draft: 1 / |rest| after each refused child
-  long long gone[kVerifyMaxTried];   // without: the refused tokens
+  unsigned long long xch[2][8][2];   // what the cluster's CTAs exchange
+  double table[32];                  // 2^(j / 32)
+  double warp_sum[kVerifyWarps];     // this CTA's warps' 64-bit sums of the last pass
+  unsigned long long warp_word[kVerifyWarps];
+  float2 warp_stat[kVerifyWarps];
+  double inv_mass[kVerifyMaxTried];  // with draft: 1 / |rest| before each refused child
+  long long gone[kVerifyMaxTried];   // the refused children's tokens
   int child;
-  int tried;
+};
+
+// This warp's share of a row: the vocabulary in groups of four at the row's own alignment, `mis` elements
+// before the row's first, shared out to the cluster's warps in order.
+struct VerifySpan {
+  int y0, y1, mis;
+  __device__ __forceinline__ VerifySpan(const void* row, int size, int V, int wi, int nw) {
+    mis = static_cast<int>(reinterpret_cast<uintptr_t>(row) / size & 3);
+    const long long total = static_cast<long long>(V) + mis;
+    const long long per = (total + nw * 128ll - 1) / (nw * 128ll) * 128;
+    y0 = static_cast<int>(min(wi * per, total));
+    y1 = static_cast<int>(min(y0 + per, total));
+  }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyParams p) {
+__device__ __forceinline__ void load4(const T* row, int v, int V, float outside, float (&x)[4]) {
+  if (v >= 0 && v + 4 <= V) {
+    const float4 q = logits4(row + v);
+    x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = v + e >= 0 && v + e < V ? logit_of(row + v + e) : outside;
+  }
+}
+
+// Four of the draft's probabilities; its rows may lie otherwise than the logits'.
+__device__ __forceinline__ void draft4(const float* q, bool vec, int v, int V, float (&x)[4]) {
+  if (vec && v >= 0 && v + 4 <= V) {
+    const float4 f = *reinterpret_cast<const float4*>(q + v);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = v + e >= 0 && v + e < V ? q[v + e] : 0.f;
+  }
+}
+
+// f(v, x[4]) for every group of a lane's, four groups' loads on their way at once.
+template <typename T, typename F>
+__device__ __forceinline__ void each4(const T* row, const VerifySpan& s, int V, F f) {
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31;
+  for (int y = s.y0 + lane * 4; y < s.y1; y += U * 128) {
+    float x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = y + u * 128 - s.mis;
+      if (y + u * 128 < s.y1) load4(row, v, V, -CUDART_INF_F, x[u]);
+      else x[u][0] = x[u][1] = x[u][2] = x[u][3] = -CUDART_INF_F;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (y + u * 128 < s.y1) f(y + u * 128 - s.mis, x[u]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
   __shared__ VerifyShared s;
-  pdl_wait();
-  pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank, C;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  if (tid < 32) s.table[tid] = exp2(tid / 32.0);
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
   const int r = blockIdx.x / C;
   const int tok0 = min(max(p.cu[r], 0), p.N), count = min(max(p.cu[r + 1], tok0), p.N) - tok0;
-  // this warp's tokens [v0, v1) of the vocabulary
   const int nw = C * kVerifyWarps, wi = rank * kVerifyWarps + warp;
-  const int per = (p.V + nw - 1) / nw;
-  const int v0 = static_cast<int>(min(static_cast<long long>(wi) * per, static_cast<long long>(p.V)));
-  const int v1 = min(v0 + per, p.V);
   int phase = 0;
-  // A value of every CTA to all of them (thread 0's), reduced in the CTAs' order.
-  auto exchange = [&](double v, auto reduce) -> double {
+  // Two words of every CTA (thread 0's) to all of them, reduced in the CTAs' order.
+  auto exchange = [&](unsigned long long a, unsigned long long b, auto reduce) {
     if (tid == 0)
-      for (uint32_t c = 0; c < C; ++c) st_dsmem_f64(map_to_rank(&s.xch[phase][rank], c), v);
+      for (uint32_t c = 0; c < C; ++c) {
+        st_dsmem_u64(map_to_rank(&s.xch[phase][rank][0], c), a);
+        st_dsmem_u64(map_to_rank(&s.xch[phase][rank][1], c), b);
+      }
     cluster_sync();
-    double a = s.xch[phase][0];
-    for (uint32_t c = 1; c < C; ++c) a = reduce(a, s.xch[phase][c]);
-    phase ^= 1;
-    return a;
+    for (uint32_t c = 0; c < C; ++c) reduce(c, s.xch[phase][c][0], s.xch[phase][c][1]);
+    phase ^= 1;  // (a slot is written again two exchanges on: every thread has read it by the one between)
   };
-  auto add = [](double a, double b) { return a + b; };
-  auto greater = [](double a, double b) { return a != a || a > b ? a : b; };  // (a NaN stays)
-  // A value of every thread, reduced over the CTA in order; the warps' values stay in warp_sum.
-  auto block_reduce = [&](double v, auto reduce) -> double {
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) v = reduce(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = v;
-    __syncthreads();
-    double a = s.warp_sum[0];
-    for (int w = 1; w < kVerifyWarps; ++w) a = reduce(a, s.warp_sum[w]);
-    return a;
-  };
-  const double inv_t = p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0;
+  const float inv_t32 = p.temperature > 0.f ? 1.f / p.temperature : 1.f;
+  const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 1.4426950408889634074;
+  const float scale32 = inv_t32 * 1.4426950408889634f;
   const bool greedy = p.temperature == 0.f;
   int node = 0, kept = 0;
   long long answer = -1;
   while (count > 0) {
-    if (rank == 0 && tid == 0 && kept < p.max_path) p.path[static_cast<long long>(r) * p.max_path + kept] = node;
+    if (rank == 0 && tid == 0) p.path[static_cast<long long>(r) * p.max_path + kept] = node;
     ++kept;
     const T* row = static_cast<const T*>(p.logits) + (tok0 + node) * p.logits_stride;
     const float* q = p.draft != nullptr && !greedy ? p.draft + (tok0 + node) * p.draft_stride : nullptr;
-    // ---- the largest logit ----
-    double mx = -CUDART_INF;
-    bool nan = false;
-    for (int i = v0 + lane; i < v1; i += 32) {
-      const double x = logit_of(row + i);
-      nan |= x != x;
-      mx = fmax(mx, x);
+    const VerifySpan span(row, sizeof(T), p.V, wi, nw);
+    const bool q_vec = q != nullptr && (reinterpret_cast<uintptr_t>(q) / 4 & 3) == span.mis;
+
+    // ---- the largest logit, and the first that is; or the sum of the weights, in 32 bits ----
+    float top;
+    long long best = -1;
+    float total32 = 0.f;
+    if (greedy) {
+      unsigned long long word = 0;  // order-preserving image of the logit, then of the first index
+      each4(row, span, p.V, [&](int v, const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = __float_as_uint(x[e] + 0.f);  // (no -0)
+          const uint32_t key = x[e] != x[e] ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
+          const unsigned long long w = static_cast<unsigned long long>(key) << 32 | static_cast<uint32_t>(~(v + e));
+          if (w > word && v + e >= 0 && v + e < p.V) word = w;
+        }
+      });
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, word, o);
+        word = max(word, other);
+      }
+      __syncthreads();
+      if (lane == 0) s.warp_word[warp] = word;
+      __syncthreads();
+      for (int w = 0; w < kVerifyWarps; ++w) word = max(word, s.warp_word[w]);
+      exchange(word, 0, [&](uint32_t, unsigned long long a, unsigned long long) { word = max(word, a); });
+      const uint32_t key = static_cast<uint32_t>(word >> 32);
+      top = key == 0xffffffffu ? CUDART_NAN_F : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+      best = static_cast<uint32_t>(~static_cast<uint32_t>(word));
+    } else {
+      float m = -CUDART_INF_F, sum = 0.f;
+      bool odd = false;  // NaN or +infinity
+      each4(row, span, p.V, [&](int, const float (&x)[4]) {
+        const float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        odd |= !(x[0] < CUDART_INF_F) | !(x[1] < CUDART_INF_F) | !(x[2] < CUDART_INF_F) | !(x[3] < CUDART_INF_F);
+        if (big > m) {
+          sum *= fast_exp2((m - big) * scale32);
+          m = big;
+        }
+        if (m > -CUDART_INF_F)
+          sum += (fast_exp2((x[0] - m) * scale32) + fast_exp2((x[1] - m) * scale32)) +
+                 (fast_exp2((x[2] - m) * scale32) + fast_exp2((x[3] - m) * scale32));
+      });
+      if (odd) m = CUDART_INF_F;
+      auto join = [&](float m2, float sum2) {
+        const float big = fmaxf(m, m2);
+        if (big > -CUDART_INF_F && big < CUDART_INF_F)
+          sum = sum * fast_exp2((m - big) * scale32) + sum2 * fast_exp2((m2 - big) * scale32);
+        m = big;
+      };
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+        join(m2, sum2);
+      }
+      __syncthreads();
+      if (lane == 0) s.warp_stat[warp] = make_float2(m, sum);
+      __syncthreads();
+      m = -CUDART_INF_F, sum = 0.f;
+      for (int w = 0; w < kVerifyWarps; ++w) join(s.warp_stat[w].x, s.warp_stat[w].y);
+      const unsigned long long mine =
+          static_cast<unsigned long long>(__float_as_uint(m)) << 32 | __float_as_uint(sum);
+      m = -CUDART_INF_F, sum = 0.f;
+      exchange(mine, 0, [&](uint32_t, unsigned long long a, unsigned long long) {
+        join(__uint_as_float(static_cast<uint32_t>(a >> 32)), __uint_as_float(static_cast<uint32_t>(a)));
+      });
+      top = m;
+      total32 = sum;
     }
-    if (nan) mx = CUDART_NAN;
-    const double top = exchange(block_reduce(mx, greater), greater);
-    if (!(top > -CUDART_INF && top < CUDART_INF)) {  // NaN, an infinity, or no token at all
+    if (!(top > -CUDART_INF_F && top < CUDART_INF_F)) {  // NaN, an infinity, or no token at all
       if (rank == 0 && tid == 0) record_error(kErrNoProbabilities);
       break;
     }
-    double total = 0.0;
-    long long best = -1;
-    if (greedy) {
-      int first = p.V;
-      for (int i = v0 + lane; i < v1 && first == p.V; i += 32)
-        if (logit_of(row + i) == top) first = i;
-      auto less = [](double a, double b) { return a < b ? a : b; };
-      best = static_cast<long long>(exchange(block_reduce(static_cast<double>(first), less), less));
-    } else {
-      double sum = 0.0;
-      for (int i = v0 + lane; i < v1; i += 32) sum += exp((logit_of(row + i) - top) * inv_t);
-      total = exchange(block_reduce(sum, add), add);
-    }
-    // ---- its children in turn ----
-    const double inv_total = 1.0 / total;
-    double mass = 1.0;
-    int tried = 0;  // refused so far (0 again where nothing was left)
-    auto rest = [&](int x) {  // of p, after the refused children
-      double v = exp((logit_of(row + x) - top) * inv_t) * inv_total;
+
+    // ---- the same in 64 bits ----
+    const double top64 = top;
+    auto weight = [&](float x) -> double {
+      const double t = (static_cast<double>(x) - top64) * scale;  // <= 0
+      constexpr double magic = 6755399441055744.0;                // 1.5 * 2^52
+      const double kd = fma(t, 32.0, magic);
+      const int n = __double2loint(kd);
+      const double f = fma(kd - magic, -0.03125, t);
+      double e = 1.3333558146428443e-3;                           // ln 2^k / k!, k = 5 .. 1
+      e = fma(e, f, 9.6181291076284772e-3);
+      e = fma(e, f, 5.5504108664821580e-2);
+      e = fma(e, f, 2.4022650695910071e-1);
+      e = fma(e, f, 6.9314718055994531e-1);
+      const double tab = s.table[n & 31];
+      const double w = fma(tab * f, e, tab);
+      // times 2^(n / 32); below 2^-1000 nothing (a logit of -infinity among them)
+      return t > -1000.0 ? __hiloint2double(__double2hiint(w) + ((n >> 5) << 20), __double2loint(w)) : 0.0;
+    };
+    int tried = 0;                  // refused so far, of those that the rest is without
+    bool exact = false;             // total, mass and inv_mass are 64-bit sums
+    double total = 0.0, mass = 1.0; // (mass: of the rest, 1 before any is refused)
+    double inv_total = 1.0 / static_cast<double>(total32);
+    auto rest_of = [&](double w, float qx, int x) {  // of token x with weight w
+      double v = w * inv_total;
       if (q != nullptr) {
-        for (int k = 0; k < tried; ++k) v = fmax(v * s.inv_mass[k] - static_cast<double>(q[x]), 0.0);
+        for (int k = 0; k < tried; ++k) v = fmax(fma(v, s.inv_mass[k], -static_cast<double>(qx)), 0.0);
       } else {
         for (int k = 0; k < tried; ++k)
           if (s.gone[k] == x) v = 0.0;
       }
       return v;
     };
-    auto rest_sum = [&] {
+    // The rest's sum over the vocabulary, in 64 bits: warp_sum and the last exchange's slots keep its parts.
+    int positive = -1;              // this lane's last token with any
+    auto sum64 = [&](bool raw) {    // raw: of the weights themselves
       double sum = 0.0;
-      for (int i = v0 + lane; i < v1; i += 32) sum += rest(i);
-      return exchange(block_reduce(sum, add), add);
+      positive = -1;
+      each4(row, span, p.V, [&](int v, const float (&x)[4]) {
+        float qx[4] = {0.f, 0.f, 0.f, 0.f};
+        if (q != nullptr && !raw && tried > 0) draft4(q, q_vec, v, p.V, qx);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double w = weight(x[e]), y = raw ? w : rest_of(w, qx[e], v + e);
+          sum += y;
+          if (y > 0.0) positive = v + e;
+        }
+      });
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      __syncthreads();
+      if (lane == 0) s.warp_sum[warp] = sum;
+      __syncthreads();
+      double a = s.warp_sum[0];
+      for (int w = 1; w < kVerifyWarps; ++w) a += s.warp_sum[w];
+      double all = 0.0;
+      exchange(__double_as_longlong(a), 0,
+               [&](uint32_t, unsigned long long x, unsigned long long) { all += __longlong_as_double(x); });
+      return all;
     };
+    // Everything so far at this token again in 64 bits.
+    auto make_exact = [&] {
+      const int n = tried;
+      tried = 0;
+      total = sum64(true);
+      inv_total = 1.0 / total;
+      mass = 1.0;
+      exact = true;
+      if (q == nullptr) {
+        tried = n;
+        if (n > 0) mass = sum64(false);
+        return;
+      }
+      while (tried < n) {
+        if (tid == 0) s.inv_mass[tried] = 1.0 / mass;
+        ++tried;
+        __syncthreads();
+        mass = sum64(false);
+        if (!(mass > 0.0)) {  // (only where 32 bits saw something left that is not)
+          tried = 0;
+          mass = 1.0;
+          break;
+        }
+      }
+    };
+
+    // ---- its children in turn ----
+    double off = 1e-5;  // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms
     int next = -1, last = node;
     for (int tries = 0; kept < p.max_path && tries < kVerifyMaxTried; ++tries) {
       if (warp == 0) {  // the next child
@@ -168,33 +341,83 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
       }
       __syncthreads();
       const int c = s.child;
+      __syncthreads();
       if (c < 0) break;
       last = c;
       const long long x = p.tokens[tok0 + c];
       if (x < 0 || x >= p.V) {
         if (rank == 0 && tid == 0) record_error(kErrTokenOutOfRange);
-        __syncthreads();
         continue;
       }
       if (greedy) {
-        if (x == best) next = c;
-      } else {
-        const double of_draft = q != nullptr ? static_cast<double>(q[x]) : 1.0;
-        if (static_cast<double>(p.accept[tok0 + c]) * of_draft * mass < rest(static_cast<int>(x))) next = c;
+        if (x == best) {
+          next = c;
+          break;
+        }
+        continue;
+      }
+      const float qx = q != nullptr ? q[x] : 1.f;
+      const double w = weight(logit_of(row + x)), bar = static_cast<double>(p.accept[tok0 + c]) * qx;
+      double have = rest_of(w, qx, static_cast<int>(x));
+      if (!exact && !(fabs(bar * mass - have) > 2.0 * off)) {  // too close for 32 bits (or a NaN)
+        make_exact();
+        have = rest_of(w, qx, static_cast<int>(x));
+      }
+      if (bar * mass < have) {
+        next = c;
+        break;
+      }
+      // refused: the rest is without it
+      if (tid == 0) {
+        s.inv_mass[tried] = 1.0 / mass;
+        s.gone[tried] = x;
       }
       __syncthreads();
-      if (next >= 0) break;
-      if (greedy) continue;
-      if (tid == 0) {
-        if (q != nullptr) s.inv_mass[tried] = 1.0 / mass;
-        else s.gone[tried] = x;
+      if (q == nullptr) {
+        mass -= have;
+        ++tried;
+        // a difference says little of a small rest, and nothing of an empty one
+        if (mass < 1e-3) {
+          make_exact();
+          if (!(mass > 0.0)) {
+            tried = 0;
+            mass = 1.0;
+          }
+        }
+        continue;
       }
       ++tried;
-      __syncthreads();
-      mass = rest_sum();
-      if (!(mass > 0.0)) {
-        tried = 0;
-        mass = 1.0;
+      if (!exact) {
+        const float inv32 = static_cast<float>(inv_total);
+        float sum = 0.f;
+        each4(row, span, p.V, [&](int v, const float (&x)[4]) {
+          float qv[4];
+          draft4(q, q_vec, v, p.V, qv);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = fast_exp2((x[e] - top) * scale32) * inv32;
+            for (int k = 0; k < tried; ++k) y = fmaxf(fmaf(y, static_cast<float>(s.inv_mass[k]), -qv[e]), 0.f);
+            sum += y;
+          }
+        });
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        __syncthreads();
+        if (lane == 0) s.warp_stat[warp].x = sum;
+        __syncthreads();
+        double a = 0.0, all = 0.0;
+        for (int v = 0; v < kVerifyWarps; ++v) a += s.warp_stat[v].x;
+        exchange(__double_as_longlong(a), 0,
+                 [&](uint32_t, unsigned long long y, unsigned long long) { all += __longlong_as_double(y); });
+        off = 2.0 * off / mass + 1e-5;
+        mass = all;
+        if (!(mass > 4.0 * off)) make_exact();  // nothing left, as far as 32 bits can tell
+      } else {
+        mass = sum64(false);
+        if (!(mass > 0.0)) {
+          tried = 0;
+          mass = 1.0;
+        }
       }
     }
     if (next >= 0) {
@@ -206,45 +429,70 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
       answer = rank == 0 ? best : -1;
       break;
     }
-    double sum = 0.0;
-    int positive = -1;
-    for (int i = v0 + lane; i < v1; i += 32) {
-      const double v = rest(i);
-      sum += v;
-      if (v > 0.0) positive = i;
+    // The rest's parts in 64 bits, in any unit; without draft_probs, or with no child refused, from the weights alone.
+    if (q != nullptr && tried > 0 && !exact) {
+      make_exact();
+      if (tried == 0) mass = sum64(false);  // (nothing left after all)
+    } else {
+      if (q == nullptr || tried == 0) inv_total = 1.0;
+      mass = sum64(false);
+      if (!(mass > 0.0)) {
+        tried = 0;
+        mass = sum64(false);
+      }
     }
-    const double mine = block_reduce(sum, add);
-    if (tid == 0)
-      for (uint32_t c = 0; c < C; ++c) st_dsmem_f64(map_to_rank(&s.xch[phase][rank], c), mine);
-    cluster_sync();
     double before = 0.0, all = 0.0;
     for (uint32_t c = 0; c < C; ++c) {
       if (c == rank) before = all;
-      all += s.xch[phase][c];
+      all += __longlong_as_double(s.xch[phase ^ 1][c][0]);
     }
-    phase ^= 1;
     const double target = static_cast<double>(p.draws[r]) * all;
     // the warp that the target falls into: the last one whose tokens begin at or below it (all compute
     // the same borders, in the same order)
     for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
-    auto last_of = [](double a, double b) { return a > b ? a : b; };
     const bool may = s.warp_sum[warp] > 0.0 && before <= target;
-    const double owner = exchange(block_reduce(may ? static_cast<double>(wi) : -1.0, last_of), last_of);
-    if (owner == wi) {
-      double cum = before;
-      long long pick = -1;
-      for (int i0 = v0; i0 < v1 && pick < 0; i0 += 32) {
-        const int i = i0 + lane;
-        const double v = i < v1 ? rest(i) : 0.0;
-        double incl = v;
+    __syncthreads();
+    if (lane == 0) s.warp_word[warp] = may ? wi + 1 : 0;
+    __syncthreads();
+    unsigned long long owner = 0;
+    for (int w = 0; w < kVerifyWarps; ++w) owner = max(owner, s.warp_word[w]);
+    exchange(owner, 0, [&](uint32_t, unsigned long long a, unsigned long long) { owner = max(owner, a); });
+    if (owner == static_cast<unsigned long long>(wi) + 1) {
+      // within it: the lanes' 32 spans first, then the one's tokens
+      auto rest_at = [&](int v) {
+        if (v < 0 || v >= p.V) return 0.0;
+        return rest_of(weight(logit_of(row + v)), q != nullptr ? q[v] : 0.f, v);
+      };
+      auto scan = [&](double v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
+          const double y = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += y;
         }
-        const unsigned b = __ballot_sync(0xffffffffu, v > 0.0 && cum + incl > target);
-        if (b) pick = i0 + __ffs(b) - 1;
-        cum += __shfl_sync(0xffffffffu, incl, 31);
+        return v;
+      };
+      const int per = (span.y1 - span.y0 + 31) / 32, a = span.y0 + lane * per - span.mis;
+      const int end = span.y1 - span.mis;
+      double sum = 0.0;
+      for (int i = 0; i < per; ++i) sum += a + i < end ? rest_at(a + i) : 0.0;
+      double incl = scan(sum);
+      unsigned b = __ballot_sync(0xffffffffu, sum > 0.0 && before + incl > target);
+      long long pick = -1;
+      if (b) {
+        const int l = __ffs(b) - 1;
+        double cum = before + __shfl_sync(0xffffffffu, incl - sum, l);
+        const int from = __shfl_sync(0xffffffffu, a, l), to = min(from + per, end);
+        int some = -1;
+        for (int i0 = from; i0 < to && pick < 0; i0 += 32) {
+          const double v = i0 + lane < to ? rest_at(i0 + lane) : 0.0;
+          incl = scan(v);
+          const unsigned has = __ballot_sync(0xffffffffu, v > 0.0);
+          b = __ballot_sync(0xffffffffu, v > 0.0 && cum + incl > target);
+          if (b) pick = i0 + __ffs(b) - 1;
+          if (has) some = i0 + 31 - __clz(has);
+          cum += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (pick < 0) pick = some;  // (the span's last: its sum in another order went past the target)
       }
       if (pick < 0) {  // the target is past the last one: rounding, or a draw of 1
 #pragma unroll
@@ -257,7 +505,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
     break;
   }
   if (rank == 0 && tid == 0) {
-    p.accepted[r] = min(kept, p.max_path);
+    p.accepted[r] = kept;
     if (answer != -2) p.next[r] = answer;
   }
   if (rank == 0)
