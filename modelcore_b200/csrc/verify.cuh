@@ -24,6 +24,8 @@
 // (the remainder, (ln 2 / 64)^6 / 720, is 2e-15): Tang's table-driven method, ACM TOMS 15, 1989.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_plan.cuh"
 
 namespace mcb {
@@ -70,7 +72,8 @@ struct VerifyShared {
   unsigned long long warp_word[kVerifyWarps];
   float2 warp_stat[kVerifyWarps];
   double inv_mass[kVerifyMaxTried];  // with draft: 1 / |rest| before each refused child
-  long long gone[kVerifyMaxTried];   // the refused children's tokens
+  float inv_mass32[kVerifyMaxTried];
+  int gone[kVerifyMaxTried];         // the refused children's tokens
   int child;
 };
 
@@ -109,22 +112,57 @@ __device__ __forceinline__ void draft4(const float* q, bool vec, int v, int V, f
   }
 }
 
-// f(v, x[4]) for every group of a lane's, four groups' loads on their way at once.
-template <typename T, typename F>
-__device__ __forceinline__ void each4(const T* row, const VerifySpan& s, int V, F f) {
-  constexpr int U = 4;
+// f(v, x[4], q[4]) for every group of a lane's, the loads of several on their way at once: those of whole turns
+// inside the row without a branch between them (a branch each cost a trip to memory each: 20,000 cycles for
+// 33,000 logits).  Without WITH_Q the q are not read.
+template <bool WITH_Q, typename T, typename F>
+__device__ __forceinline__ void each4(const T* row, const float* q, bool q_vec, const VerifySpan& s, int V, F f) {
+  constexpr int U = WITH_Q ? 2 : 4;
   const int lane = threadIdx.x & 31;
-  for (int y = s.y0 + lane * 4; y < s.y1; y += U * 128) {
-    float x[U][4];
+  int b = s.y0;  // (the same in all lanes)
+  auto turn = [&](auto u_const) {
+    constexpr int N = decltype(u_const)::value;
+    float x[N][4], d[N][4];
+    const int v0 = b + lane * 4 - s.mis;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = y + u * 128 - s.mis;
-      if (y + u * 128 < s.y1) load4(row, v, V, -CUDART_INF_F, x[u]);
-      else x[u][0] = x[u][1] = x[u][2] = x[u][3] = -CUDART_INF_F;
+    for (int u = 0; u < N; ++u) {
+      const float4 t = logits4(row + v0 + u * 128);
+      x[u][0] = t.x, x[u][1] = t.y, x[u][2] = t.z, x[u][3] = t.w;
+    }
+    if constexpr (WITH_Q) {
+      if (q_vec) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          const float4 t = *reinterpret_cast<const float4*>(q + v0 + u * 128);
+          d[u][0] = t.x, d[u][1] = t.y, d[u][2] = t.z, d[u][3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[u][e] = q[v0 + u * 128 + e];
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (y + u * 128 < s.y1) f(y + u * 128 - s.mis, x[u]);
+    for (int u = 0; u < N; ++u) f(v0 + u * 128, x[u], d[u]);
+    b += N * 128;
+  };
+  while (b < s.y1) {
+    const int room = min(s.y1, V + s.mis) - b;
+    if (b >= s.mis && room >= U * 128) {
+      turn(std::integral_constant<int, U>());
+    } else if (b >= s.mis && room >= 128) {
+      turn(std::integral_constant<int, 1>());
+    } else {  // a row's ends
+      const int y = b + lane * 4;
+      float x[4], d[4] = {0.f, 0.f, 0.f, 0.f};
+      if (y < s.y1) {
+        load4(row, y - s.mis, V, -CUDART_INF_F, x);
+        if constexpr (WITH_Q) draft4(q, q_vec, y - s.mis, V, d);
+        f(y - s.mis, x, d);
+      }
+      b += 128;
+    }
   }
 }
 
@@ -174,7 +212,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     float total32 = 0.f;
     if (greedy) {
       unsigned long long word = 0;  // order-preserving image of the logit, then of the first index
-      each4(row, span, p.V, [&](int v, const float (&x)[4]) {
+      each4<false>(row, nullptr, false, span, p.V, [&](int v, const float (&x)[4], const float (&)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t u = __float_as_uint(x[e] + 0.f);  // (no -0)
@@ -199,7 +237,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     } else {
       float m = -CUDART_INF_F, sum = 0.f;
       bool odd = false;  // NaN or +infinity
-      each4(row, span, p.V, [&](int, const float (&x)[4]) {
+      each4<false>(row, nullptr, false, span, p.V, [&](int, const float (&x)[4], const float (&)[4]) {
         const float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         odd |= !(x[0] < CUDART_INF_F) | !(x[1] < CUDART_INF_F) | !(x[2] < CUDART_INF_F) | !(x[3] < CUDART_INF_F);
         if (big > m) {
@@ -278,16 +316,27 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     auto sum64 = [&](bool raw) {    // raw: of the weights themselves
       double sum = 0.0;
       positive = -1;
-      each4(row, span, p.V, [&](int v, const float (&x)[4]) {
-        float qx[4] = {0.f, 0.f, 0.f, 0.f};
-        if (q != nullptr && !raw && tried > 0) draft4(q, q_vec, v, p.V, qx);
+      auto add = [&](double y, int v) {
+        sum += y;
+        if (y > 0.0) positive = v;
+      };
+      if (raw || tried == 0) {
+        const double unit = raw ? 1.0 : inv_total;
+        each4<false>(row, nullptr, false, span, p.V, [&](int v, const float (&x)[4], const float (&)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double w = weight(x[e]), y = raw ? w : rest_of(w, qx[e], v + e);
-          sum += y;
-          if (y > 0.0) positive = v + e;
-        }
-      });
+          for (int e = 0; e < 4; ++e) add(weight(x[e]) * unit, v + e);
+        });
+      } else if (q != nullptr) {
+        each4<true>(row, q, q_vec, span, p.V, [&](int v, const float (&x)[4], const float (&d)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) add(rest_of(weight(x[e]), d[e], v + e), v + e);
+        });
+      } else {
+        each4<false>(row, nullptr, false, span, p.V, [&](int v, const float (&x)[4], const float (&)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) add(rest_of(weight(x[e]), 0.f, v + e), v + e);
+        });
+      }
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       __syncthreads();
@@ -370,7 +419,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       // refused: the rest is without it
       if (tid == 0) {
         s.inv_mass[tried] = 1.0 / mass;
-        s.gone[tried] = x;
+        s.inv_mass32[tried] = static_cast<float>(1.0 / mass);
+        s.gone[tried] = static_cast<int>(x);
       }
       __syncthreads();
       if (q == nullptr) {
@@ -390,15 +440,16 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       if (!exact) {
         const float inv32 = static_cast<float>(inv_total);
         float sum = 0.f;
-        each4(row, span, p.V, [&](int v, const float (&x)[4]) {
-          float qv[4];
-          draft4(q, q_vec, v, p.V, qv);
+        each4<true>(row, q, q_vec, span, p.V, [&](int, const float (&x)[4], const float (&d)[4]) {
+          float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = fast_exp2((x[e] - top) * scale32) * inv32;
-            for (int k = 0; k < tried; ++k) y = fmaxf(fmaf(y, static_cast<float>(s.inv_mass[k]), -qv[e]), 0.f);
-            sum += y;
+          for (int e = 0; e < 4; ++e) y[e] = fast_exp2((x[e] - top) * scale32) * inv32;
+          for (int k = 0; k < tried; ++k) {
+            const float by = s.inv_mass32[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = fmaxf(fmaf(y[e], by, -d[e]), 0.f);
           }
+          sum += (y[0] + y[1]) + (y[2] + y[3]);
         });
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
