@@ -7,6 +7,8 @@
 //   otherwise     rest <- max(rest / |rest| - q, 0)   with q = draft_probs_u, of which the x_i were drawn
 //                 rest <- rest, but rest(x_i) = 0     without draft_probs: q is 1 at x_i
 //   (rest = p again should nothing be left of it).
+// With q >= 0 the steps' maxima can wait: a term that is below 0 once stays there, so after refusals with
+// |rest| = m_0 = 1, m_1, ... the rest is max(A p - B q, 0), A = A / m_i and B = B / m_i + 1 a step.
 // The walk goes on at a kept child; where none is kept the next token is the first x with
 //   rest(0) + ... + rest(x) > draw |rest|.
 // So the tokens are distributed as if each had been drawn from its p, whatever the draft was.  T = 0: a
@@ -66,16 +68,22 @@ __device__ __forceinline__ void st_dsmem_u64(uint32_t addr, unsigned long long v
 }
 
 struct VerifyShared {
-  unsigned long long xch[2][8][2];   // what the cluster's CTAs exchange
+  unsigned long long xch[2][8];      // what the cluster's CTAs exchange
   double table[32];                  // 2^(j / 32)
   double warp_sum[kVerifyWarps];     // this CTA's warps' 64-bit sums of the last pass
   unsigned long long warp_word[kVerifyWarps];
-  float2 warp_stat[kVerifyWarps];
-  double inv_mass[kVerifyMaxTried];  // with draft: 1 / |rest| before each refused child
-  float inv_mass32[kVerifyMaxTried];
-  int gone[kVerifyMaxTried];         // the refused children's tokens
-  int child;
+  int gone[kVerifyMaxTried];         // without draft: the refused children's tokens
+  int parent[kVerifyMaxTried], token[kVerifyMaxTried];  // the request's first tokens' (those behind are read)
+  float accept[kVerifyMaxTried];
 };
+
+// A float as a double by integer operations (the conversion unit takes 16 a clock): exact for normal numbers; a 0
+// becomes 2^-127, an infinity 2^128.
+__device__ __forceinline__ double double_of(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double(static_cast<int>((u & 0x80000000u) | ((u & 0x7fffffffu) >> 3) + 0x38000000u),
+                          static_cast<int>(u << 29));
+}
 
 // This warp's share of a row: the vocabulary in groups of four at the row's own alignment, `mis` elements
 // before the row's first, shared out to the cluster's warps in order.
@@ -181,17 +189,32 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   const int tok0 = min(max(p.cu[r], 0), p.N), count = min(max(p.cu[r + 1], tok0), p.N) - tok0;
   const int nw = C * kVerifyWarps, wi = rank * kVerifyWarps + warp;
   int phase = 0;
-  // Two words of every CTA (thread 0's) to all of them, reduced in the CTAs' order.
-  auto exchange = [&](unsigned long long a, unsigned long long b, auto reduce) {
-    if (tid == 0)
-      for (uint32_t c = 0; c < C; ++c) {
-        st_dsmem_u64(map_to_rank(&s.xch[phase][rank][0], c), a);
-        st_dsmem_u64(map_to_rank(&s.xch[phase][rank][1], c), b);
-      }
+  // A word of every CTA (the same in all its threads) to all of them: lane c gets CTA c's.
+  auto exchange = [&](unsigned long long a) {
+    if (warp == 0 && lane < C) st_dsmem_u64(map_to_rank(&s.xch[phase][rank], lane), a);
     cluster_sync();
-    for (uint32_t c = 0; c < C; ++c) reduce(c, s.xch[phase][c][0], s.xch[phase][c][1]);
+    const unsigned long long got = s.xch[phase][lane & 7];
     phase ^= 1;  // (a slot is written again two exchanges on: every thread has read it by the one between)
+    return got;
   };
+  // A warp's word to all warps: lane w gets warp w's.
+  auto spread = [&](unsigned long long a) {
+    __syncthreads();
+    if (lane == 0) s.warp_word[warp] = a;
+    __syncthreads();
+    return s.warp_word[lane & (kVerifyWarps - 1)];
+  };
+  auto sum_lanes = [&](double v, int n) {  // over lanes 0 .. n - 1, n a power of two; the same in all lanes
+    for (int o = n >> 1; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+  };
+  for (int i = tid; i < min(count, kVerifyMaxTried); i += kVerifyThreads) {
+    s.parent[i] = p.parents[tok0 + i];
+    const long long x = p.tokens[tok0 + i];
+    s.token[i] = x < 0 || x >= p.V ? -1 : static_cast<int>(x);
+    s.accept[i] = p.accept[tok0 + i];
+  }
+  __syncthreads();
   const float inv_t32 = p.temperature > 0.f ? 1.f / p.temperature : 1.f;
   const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 1.4426950408889634074;
   const float scale32 = inv_t32 * 1.4426950408889634f;
@@ -226,11 +249,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         const unsigned long long other = __shfl_xor_sync(0xffffffffu, word, o);
         word = max(word, other);
       }
-      __syncthreads();
-      if (lane == 0) s.warp_word[warp] = word;
-      __syncthreads();
-      for (int w = 0; w < kVerifyWarps; ++w) word = max(word, s.warp_word[w]);
-      exchange(word, 0, [&](uint32_t, unsigned long long a, unsigned long long) { word = max(word, a); });
+      auto largest = [&](unsigned long long v) {
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, o);
+          v = max(v, other);
+        }
+        return v;
+      };
+      word = largest(spread(word));
+      word = exchange(word);
+      word = largest(lane < C ? word : 0);
       const uint32_t key = static_cast<uint32_t>(word >> 32);
       top = key == 0xffffffffu ? CUDART_NAN_F : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
       best = static_cast<uint32_t>(~static_cast<uint32_t>(word));
@@ -249,28 +278,27 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
                  (fast_exp2((x[2] - m) * scale32) + fast_exp2((x[3] - m) * scale32));
       });
       if (odd) m = CUDART_INF_F;
-      auto join = [&](float m2, float sum2) {
-        const float big = fmaxf(m, m2);
-        if (big > -CUDART_INF_F && big < CUDART_INF_F)
-          sum = sum * fast_exp2((m - big) * scale32) + sum2 * fast_exp2((m2 - big) * scale32);
-        m = big;
+      auto join = [&](int n) {  // over groups of n lanes
+        for (int o = n >> 1; o >= 1; o >>= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+          const float big = fmaxf(m, m2);
+          if (big > -CUDART_INF_F && big < CUDART_INF_F)
+            sum = sum * fast_exp2((m - big) * scale32) + sum2 * fast_exp2((m2 - big) * scale32);
+          m = big;
+        }
       };
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
-        join(m2, sum2);
-      }
-      __syncthreads();
-      if (lane == 0) s.warp_stat[warp] = make_float2(m, sum);
-      __syncthreads();
-      m = -CUDART_INF_F, sum = 0.f;
-      for (int w = 0; w < kVerifyWarps; ++w) join(s.warp_stat[w].x, s.warp_stat[w].y);
-      const unsigned long long mine =
-          static_cast<unsigned long long>(__float_as_uint(m)) << 32 | __float_as_uint(sum);
-      m = -CUDART_INF_F, sum = 0.f;
-      exchange(mine, 0, [&](uint32_t, unsigned long long a, unsigned long long) {
-        join(__uint_as_float(static_cast<uint32_t>(a >> 32)), __uint_as_float(static_cast<uint32_t>(a)));
-      });
+      auto word = [&] { return static_cast<unsigned long long>(__float_as_uint(m)) << 32 | __float_as_uint(sum); };
+      auto unpack = [&](unsigned long long a) {
+        m = __uint_as_float(static_cast<uint32_t>(a >> 32));
+        sum = __uint_as_float(static_cast<uint32_t>(a));
+      };
+      join(32);
+      unpack(spread(word()));
+      join(kVerifyWarps);
+      unpack(exchange(word()));
+      join(static_cast<int>(C));
+      m = __shfl_sync(0xffffffffu, m, 0);  // (C lanes have it)
+      sum = __shfl_sync(0xffffffffu, sum, 0);
       top = m;
       total32 = sum;
     }
@@ -282,7 +310,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     // ---- the same in 64 bits ----
     const double top64 = top;
     auto weight = [&](float x) -> double {
-      const double t = (static_cast<double>(x) - top64) * scale;  // <= 0
+      const double t = fma(double_of(x), scale, -top64 * scale);  // <= 0, to rounding
       constexpr double magic = 6755399441055744.0;                // 1.5 * 2^52
       const double kd = fma(t, 32.0, magic);
       const int n = __double2loint(kd);
@@ -297,19 +325,32 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       // times 2^(n / 32); below 2^-1000 nothing (a logit of -infinity among them)
       return t > -1000.0 ? __hiloint2double(__double2hiint(w) + ((n >> 5) << 20), __double2loint(w)) : 0.0;
     };
-    int tried = 0;                  // refused so far, of those that the rest is without
-    bool exact = false;             // total, mass and inv_mass are 64-bit sums
-    double total = 0.0, mass = 1.0; // (mass: of the rest, 1 before any is refused)
-    double inv_total = 1.0 / static_cast<double>(total32);
-    auto rest_of = [&](double w, float qx, int x) {  // of token x with weight w
-      double v = w * inv_total;
+    int tried = 0;                  // without draft: refused so far, of those that the rest is without
+    bool exact = false;             // mass and the factors come of 64-bit sums
+    double mass = 1.0;              // of the rest
+    // the rest is max(of_p w - of_q q, 0), w the weight before its division by all; history: the masses so far
+    double of_p = 1.0 / static_cast<double>(total32), of_q = 0.0;
+    int refused = 0;
+    auto rest_of = [&](double w, float qx, int x) {  // of token x
       if (q != nullptr) {
-        for (int k = 0; k < tried; ++k) v = fmax(fma(v, s.inv_mass[k], -static_cast<double>(qx)), 0.0);
-      } else {
-        for (int k = 0; k < tried; ++k)
-          if (s.gone[k] == x) v = 0.0;
+        const double v = fma(w, of_p, -(static_cast<double>(qx) * of_q));
+        return v > 0.0 ? v : 0.0;
       }
+      double v = w * of_p;
+      for (int k = 0; k < tried; ++k)
+        if (s.gone[k] == x) v = 0.0;
       return v;
+    };
+    auto refuse = [&] {  // a draft's child, the rest's sum being mass
+      of_p /= mass;
+      of_q = of_q / mass + 1.0;
+      ++refused;
+    };
+    auto restart = [&](double all) {
+      of_p = 1.0 / all;
+      of_q = 0.0;
+      mass = 1.0;
+      refused = tried = 0;
     };
     // The rest's sum over the vocabulary, in 64 bits: warp_sum and the last exchange's slots keep its parts.
     int positive = -1;              // this lane's last token with any
@@ -320,16 +361,20 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         sum += y;
         if (y > 0.0) positive = v;
       };
-      if (raw || tried == 0) {
-        const double unit = raw ? 1.0 : inv_total;
+      if (raw || (q != nullptr && refused == 0) || (q == nullptr && tried == 0)) {
+        const double unit = raw ? 1.0 : of_p;
         each4<false>(row, nullptr, false, span, p.V, [&](int v, const float (&x)[4], const float (&)[4]) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) add(weight(x[e]) * unit, v + e);
         });
       } else if (q != nullptr) {
+        const double a = of_p, b = -of_q;
         each4<true>(row, q, q_vec, span, p.V, [&](int v, const float (&x)[4], const float (&d)[4]) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) add(rest_of(weight(x[e]), d[e], v + e), v + e);
+          for (int e = 0; e < 4; ++e) {
+            const double y = fma(weight(x[e]), a, double_of(d[e]) * b);
+            if (y > 0.0) add(y, v + e);
+          }
         });
       } else {
         each4<false>(row, nullptr, false, span, p.V, [&](int v, const float (&x)[4], const float (&)[4]) {
@@ -342,34 +387,24 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       __syncthreads();
       if (lane == 0) s.warp_sum[warp] = sum;
       __syncthreads();
-      double a = s.warp_sum[0];
-      for (int w = 1; w < kVerifyWarps; ++w) a += s.warp_sum[w];
-      double all = 0.0;
-      exchange(__double_as_longlong(a), 0,
-               [&](uint32_t, unsigned long long x, unsigned long long) { all += __longlong_as_double(x); });
-      return all;
+      const double mine = sum_lanes(s.warp_sum[lane & (kVerifyWarps - 1)], kVerifyWarps);
+      return sum_lanes(__longlong_as_double(exchange(__double_as_longlong(mine))), static_cast<int>(C));
     };
     // Everything so far at this token again in 64 bits.
     auto make_exact = [&] {
-      const int n = tried;
-      tried = 0;
-      total = sum64(true);
-      inv_total = 1.0 / total;
-      mass = 1.0;
+      const int n = refused, gone = tried;
+      restart(sum64(true));
       exact = true;
       if (q == nullptr) {
-        tried = n;
-        if (n > 0) mass = sum64(false);
+        tried = gone;
+        if (tried > 0) mass = sum64(false);
         return;
       }
-      while (tried < n) {
-        if (tid == 0) s.inv_mass[tried] = 1.0 / mass;
-        ++tried;
-        __syncthreads();
+      while (refused < n) {
+        refuse();
         mass = sum64(false);
         if (!(mass > 0.0)) {  // (only where 32 bits saw something left that is not)
-          tried = 0;
-          mass = 1.0;
+          restart(sum64(true));
           break;
         }
       }
@@ -379,21 +414,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     double off = 1e-5;  // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms
     int next = -1, last = node;
     for (int tries = 0; kept < p.max_path && tries < kVerifyMaxTried; ++tries) {
-      if (warp == 0) {  // the next child
-        int found = -1;
-        for (int j0 = last + 1; j0 < count && found < 0; j0 += 32) {
-          const int j = j0 + lane;
-          const unsigned b = __ballot_sync(0xffffffffu, j < count && p.parents[tok0 + j] == node);
-          if (b) found = j0 + __ffs(b) - 1;
-        }
-        if (lane == 0) s.child = found;
+      // the next child (every warp looks for itself)
+      int c = -1;
+      for (int j0 = last + 1; j0 < count && c < 0; j0 += 32) {
+        const int j = j0 + lane;
+        int parent = -1;
+        if (j < count) parent = j < kVerifyMaxTried ? s.parent[j] : p.parents[tok0 + j];
+        const unsigned b = __ballot_sync(0xffffffffu, parent == node);
+        if (b) c = j0 + __ffs(b) - 1;
       }
-      __syncthreads();
-      const int c = s.child;
-      __syncthreads();
       if (c < 0) break;
       last = c;
-      const long long x = p.tokens[tok0 + c];
+      long long x = c < kVerifyMaxTried ? s.token[c] : p.tokens[tok0 + c];
       if (x < 0 || x >= p.V) {
         if (rank == 0 && tid == 0) record_error(kErrTokenOutOfRange);
         continue;
@@ -406,7 +438,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         continue;
       }
       const float qx = q != nullptr ? q[x] : 1.f;
-      const double w = weight(logit_of(row + x)), bar = static_cast<double>(p.accept[tok0 + c]) * qx;
+      const double w = weight(logit_of(row + x)), bar = static_cast<double>(c < kVerifyMaxTried ? s.accept[c] : p.accept[tok0 + c]) * qx;
       double have = rest_of(w, qx, static_cast<int>(x));
       if (!exact && !(fabs(bar * mass - have) > 2.0 * off)) {  // too close for 32 bits (or a NaN)
         make_exact();
@@ -417,13 +449,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         break;
       }
       // refused: the rest is without it
-      if (tid == 0) {
-        s.inv_mass[tried] = 1.0 / mass;
-        s.inv_mass32[tried] = static_cast<float>(1.0 / mass);
-        s.gone[tried] = static_cast<int>(x);
-      }
-      __syncthreads();
       if (q == nullptr) {
+        __syncthreads();
+        if (tid == 0) s.gone[tried] = static_cast<int>(x);
+        __syncthreads();
         mass -= have;
         ++tried;
         // a difference says little of a small rest, and nothing of an empty one
@@ -436,39 +465,26 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         }
         continue;
       }
-      ++tried;
+      const double before = mass;
+      refuse();
       if (!exact) {
-        const float inv32 = static_cast<float>(inv_total);
+        const float a = static_cast<float>(of_p), b = -static_cast<float>(of_q);
         float sum = 0.f;
         each4<true>(row, q, q_vec, span, p.V, [&](int, const float (&x)[4], const float (&d)[4]) {
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = fast_exp2((x[e] - top) * scale32) * inv32;
-          for (int k = 0; k < tried; ++k) {
-            const float by = s.inv_mass32[k];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = fmaxf(fmaf(y[e], by, -d[e]), 0.f);
-          }
+          for (int e = 0; e < 4; ++e) y[e] = fmaxf(fmaf(fast_exp2((x[e] - top) * scale32), a, d[e] * b), 0.f);
           sum += (y[0] + y[1]) + (y[2] + y[3]);
         });
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        __syncthreads();
-        if (lane == 0) s.warp_stat[warp].x = sum;
-        __syncthreads();
-        double a = 0.0, all = 0.0;
-        for (int v = 0; v < kVerifyWarps; ++v) a += s.warp_stat[v].x;
-        exchange(__double_as_longlong(a), 0,
-                 [&](uint32_t, unsigned long long y, unsigned long long) { all += __longlong_as_double(y); });
-        off = 2.0 * off / mass + 1e-5;
-        mass = all;
+        const double mine = sum_lanes(__longlong_as_double(spread(__double_as_longlong(static_cast<double>(sum)))), kVerifyWarps);
+        mass = sum_lanes(__longlong_as_double(exchange(__double_as_longlong(mine))), static_cast<int>(C));
+        off = 2.0 * off / before + 1e-5 * of_q;
         if (!(mass > 4.0 * off)) make_exact();  // nothing left, as far as 32 bits can tell
       } else {
         mass = sum64(false);
-        if (!(mass > 0.0)) {
-          tried = 0;
-          mass = 1.0;
-        }
+        if (!(mass > 0.0)) restart(sum64(true));
       }
     }
     if (next >= 0) {
@@ -481,33 +497,38 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       break;
     }
     // The rest's parts in 64 bits, in any unit; without draft_probs, or with no child refused, from the weights alone.
-    if (q != nullptr && tried > 0 && !exact) {
-      make_exact();
-      if (tried == 0) mass = sum64(false);  // (nothing left after all)
+    if (q != nullptr && refused > 0 && !exact) {
+      make_exact();  // (ends with the rest's sum, or the weights')
+      if (refused == 0) of_p = 1.0;
     } else {
-      if (q == nullptr || tried == 0) inv_total = 1.0;
+      if (q == nullptr || refused == 0) of_p = 1.0;
       mass = sum64(false);
       if (!(mass > 0.0)) {
-        tried = 0;
-        mass = sum64(false);
+        restart(1.0);
+        mass = sum64(true);
       }
     }
     double before = 0.0, all = 0.0;
     for (uint32_t c = 0; c < C; ++c) {
       if (c == rank) before = all;
-      all += __longlong_as_double(s.xch[phase ^ 1][c][0]);
+      all += __longlong_as_double(s.xch[phase ^ 1][c]);
     }
     const double target = static_cast<double>(p.draws[r]) * all;
     // the warp that the target falls into: the last one whose tokens begin at or below it (all compute
     // the same borders, in the same order)
     for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
     const bool may = s.warp_sum[warp] > 0.0 && before <= target;
-    __syncthreads();
-    if (lane == 0) s.warp_word[warp] = may ? wi + 1 : 0;
-    __syncthreads();
-    unsigned long long owner = 0;
-    for (int w = 0; w < kVerifyWarps; ++w) owner = max(owner, s.warp_word[w]);
-    exchange(owner, 0, [&](uint32_t, unsigned long long a, unsigned long long) { owner = max(owner, a); });
+    auto largest = [&](unsigned long long v) {
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, o);
+        v = max(v, other);
+      }
+      return v;
+    };
+    unsigned long long owner = largest(spread(may ? wi + 1 : 0));
+    owner = exchange(owner);
+    owner = largest(lane < C ? owner : 0);
     if (owner == static_cast<unsigned long long>(wi) + 1) {
       // within it: the lanes' 32 spans first, then the one's tokens
       auto rest_at = [&](int v) {
