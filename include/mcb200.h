@@ -603,6 +603,7 @@ int mcb_verify_drafts(const mcb_verify_drafts_args* args, void* stream);
  * cache_seqlens[r] + i gets what cache_seqlens[r] + path[r][i] holds, i < accepted[r] (path as
  * mcb_verify_drafts writes it: growing); seqlens_out[r] = cache_seqlens[r] + accepted[r]; the pages
  * from there to the step's last, cache_seqlens[r] + new_lens[r], go to the queue's tail in request order.
+ * accepted[r] < 0: the request's whole step is kept as it is (a prompt's chunk); its path is not read.
  * free_state_out may be free_state, seqlens_out cache_seqlens.  accepted above new_lens or P, or a path
  * entry below its place or past new_lens, sets device error 8: the former counts as the limit, the latter is not
  * moved.  Device errors 1, 5 and 6 as in mcb_page_release. */

@@ -17,7 +17,8 @@
 // paged_keep: the tokens path_0 < path_1 < ... of a row's new ones are kept: position L + i of every slot
 // and head gets what L + path_i holds, the row is L + kept long, and the pages behind it that the step
 // took are free again.  path_i >= i, so moves in the order of i never overwrite one still to be read, and a
-// thread that carries 16 bytes of one head through all of a row's moves needs no other.
+// thread that carries 16 bytes of one head through all of a row's moves needs no other.  kept < 0: the whole step
+// as it is.
 #pragma once
 
 #include "paged_plan.cuh"
@@ -255,12 +256,15 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKee
     const long long cap = static_cast<long long>(p.max_pages) << p.page_shift;
     return static_cast<int>(min(static_cast<long long>(max(p.seqlens[r], 0)), cap));
   };
-  auto kept_of = [&](int r, int fresh) { return min(max(p.kept[r], 0), min(fresh, p.P)); };
+  auto kept_of = [&](int r, int fresh) {  // (below 0: the whole step as it is)
+    const int kept = p.kept[r];
+    return kept < 0 ? fresh : min(kept, min(fresh, p.P));
+  };
   const int r = blockIdx.y;
   const bool row = r < p.R;  // (no rows: one block row for the counters alone)
   const int len = row ? len_of(r) : 0, fresh = row ? max(p.new_lens[r], 0) : 0, kept = row ? kept_of(r, fresh) : 0;
   if (row && blockIdx.x == 0 && tid == 0) {
-    if (p.kept[r] != kept) record_error(kErrDraftOutOfRange);
+    if (p.kept[r] > kept) record_error(kErrDraftOutOfRange);
     if (p.seqlens[r] != len || ((static_cast<long long>(len) + fresh + page_len - 1) >> p.page_shift) > p.max_pages)
       record_error(kErrPositionBeyondCache);
   }
@@ -275,11 +279,12 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKee
     base = (vec & 1 ? p.v_pages : p.k_pages) + ((slot * p.n_pages * p.Hkv + h) << p.page_shift) * p.D +
            column % per_vec * 8;
   }
-  for (int i0 = 0; i0 < kept; i0 += kKeepThreads) {
+  const int moving = row && p.kept[r] >= 0 ? kept : 0;
+  for (int i0 = 0; i0 < moving; i0 += kKeepThreads) {
     const int i = i0 + tid;
     bool move = false;
     long long src = 0, dst = 0;
-    if (i < kept) {
+    if (i < moving) {
       const int from = p.path[r * p.path_stride + i];
       if (from < i || from >= fresh) record_error(kErrDraftOutOfRange);
       else if (from > i) {

@@ -827,8 +827,9 @@ def paged_keep(path, accepted, cache_seqlens, new_lens, block_table, free_pages,
     verify_drafts gives them.  In every slot the path's keys and values move to the positions after the
     cached tokens (k_pages / v_pages (n_slots, n_pages, Hkv, page_size, D) or one slot's, in place), the pages
     that only the step's other tokens needed (new_lens (R,) as given to page_plan) go back to the queue's tail
-    in request order.  Returns (free_state, seqlens) after it: new tensors, or free_state_out /
-    seqlens_out, which may be the inputs.  Device errors as page_release's, and 8 for a path that does not
+    in request order.  accepted[r] < 0: the whole step of that request is kept as it is (a prompt's chunk beside
+    the trees).  Returns (free_state, seqlens) after it: new tensors, or free_state_out / seqlens_out, which
+    may be the inputs.  Device errors as page_release's, and 8 for a path that does not
     fit its request."""
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)

@@ -16,6 +16,9 @@ finished request's pages serve the next:
     cache.release([2])                                # row 2 is done: its pages are free
 
 Of drafted tokens that were verified in one step, advance(step, kept=[2, 0, 1, 4]) keeps the accepted ones.
+Drafted tokens may be trees: plan(new_lens, parents=parents) gives a step whose tokens see their ancestors
+alone, and keep(step, path, accepted) what ops.verify_drafts says of them.  fork(source) makes rows copies of
+rows -- samples of one prompt, beams -- that share the pages that are full.
 
 A plan takes its pages only when the step is advanced: until then it can be dropped (planned again, or
 never followed), and the cache is what it was.
@@ -40,6 +43,7 @@ class PagedStep(NamedTuple):
     host_lens: np.ndarray      # the same, on the host
     num_tokens: int            # of the packed batch, padding included
     max_new: int
+    tree: Optional[ops.DraftTree] = None  # the tokens' positions and masks, where they are trees
 
     def last_tokens(self):
         """Indices into the packed batch of the last new token of every row that has any, and those rows
@@ -77,8 +81,13 @@ class PagedKVCache:
         self.cache_seqlens = torch.zeros(max_rows, **ints)
         self.free_pages = torch.arange(n_pages, **ints)
         self.free_state = torch.tensor([0, n_pages], dtype=torch.int64, device=device)
+        self.page_shares = torch.zeros(n_pages, **ints)  # the rows that hold a page, less one
         self._host_lens = np.zeros(max_rows, dtype=np.int64)
         self._step = None  # the planned step that advance has not followed yet
+        # a row's first pages that were full when it was last forked or forked from, by numbers of the host's own:
+        # equal numbers are one page
+        self._shared = [[] for _ in range(max_rows)]
+        self._page_numbers = 0
 
     def _held(self, lens):
         return -(-lens // self.page_size)
@@ -93,7 +102,12 @@ class PagedKVCache:
 
     def free_page_count(self):
         """Pages that no row holds (no device read)."""
-        return int(self.n_pages - self._held(self._host_lens).sum())
+        return int(self.n_pages - self._held(self._host_lens).sum()) + self._shared_count()
+
+    def _shared_count(self):
+        """Pages that rows would hold besides if none were shared."""
+        numbers = [x for pages in self._shared for x in pages]
+        return len(numbers) - len(set(numbers))
 
     def pages_needed(self, new_lens):
         """Pages a step of these new tokens a row would take from the free ones."""
@@ -108,11 +122,16 @@ class PagedKVCache:
         new[:given.size] = given
         return new
 
-    def plan(self, new_lens, num_tokens: Optional[int] = None):
+    def plan(self, new_lens, num_tokens: Optional[int] = None, *, parents=None, max_tree: Optional[int] = None):
         """Plans a step of new_lens[r] new tokens for each row (missing rows: 0): pages are chosen for
         them and the packed batch's offsets, positions and slots computed, on the GPU.  num_tokens pads
         the batch (for a fixed shape).  The rows' lengths and the free pages stay until advance(step);
-        planning again drops a step that has not been advanced."""
+        planning again drops a step that has not been advanced.
+
+        parents: the new tokens are trees; for each of the packed batch its parent, an earlier new token of its
+        row counted from the row's first, or -1 after the cached ones (a list or an int32 tensor of num_tokens, as
+        ops.draft_tree takes it).  Rows of more new tokens than max_tree (256 at most, and unless given) rounded up
+        to 32 are chunks of prompts, whose parents are not read."""
         new = self._rows(new_lens)
         total = int(new.sum())
         num_tokens = total if num_tokens is None else int(num_tokens)
@@ -124,10 +143,17 @@ class PagedKVCache:
             raise RuntimeError(f"row {row} would grow to {int(end[row])} tokens, beyond {self.max_seq_len}")
         if self.pages_needed(new) > self.free_page_count():
             raise RuntimeError(f"the step needs {self.pages_needed(new)} pages and {self.free_page_count()} are free")
+        if parents is not None:
+            if not isinstance(parents, torch.Tensor):
+                parents = self._to_device(parents)
+            if tuple(parents.shape) != (num_tokens,):
+                raise RuntimeError(f"parents must name one for each of {num_tokens} tokens, got {tuple(parents.shape)}")
+            max_tree = min(256, max(1, int(new.max(initial=0)))) if max_tree is None else int(max_tree)
         lens = self._to_device(new)
         p = ops.page_plan(self.cache_seqlens, lens, self.block_table, self.free_pages, self.free_state,
                           page_size=self.page_size, num_tokens=num_tokens)
-        self._step = PagedStep(p, lens, new, num_tokens, int(new.max(initial=0)))
+        tree = None if parents is None else ops.draft_tree(parents, p.cu_new, self.cache_seqlens, max_tree=max_tree)
+        self._step = PagedStep(p, lens, new, num_tokens, int(new.max(initial=0)), tree)
         return self._step
 
     def _current(self, step):
@@ -142,12 +168,17 @@ class PagedKVCache:
         produces_kv=False).  Returns the processed q."""
         self._current(step)
         pages = (self.k_pages[slot], self.v_pages[slot], step.plan.slot_map) if k is not None else (None,) * 3
-        return ops.paged_append_rope(q, k, v, pages[0], pages[1], step.plan.positions, pages[2], cos, sin, eps=eps,
+        positions = step.plan.positions if step.tree is None else step.tree.positions
+        return ops.paged_append_rope(q, k, v, pages[0], pages[1], positions, pages[2], cos, sin, eps=eps,
                                      scale=scale, rotate_k=rotate_k, round_each=round_each)
 
     def attend(self, slot, q, step, *, window=-1, softmax_scale=None):
         """Attention of the step's packed queries over their rows' pages of one slot."""
         self._current(step)
+        if step.tree is not None:
+            return ops.paged_tree_attn(q, self.k_pages[slot], self.v_pages[slot], self.block_table, self.cache_seqlens,
+                                       step.plan.cu_new, step.tree.positions, step.tree.mask, window=window,
+                                       softmax_scale=softmax_scale, max_new=step.max_new)
         return ops.paged_attn(q, self.k_pages[slot], self.v_pages[slot], self.block_table, self.cache_seqlens,
                               step.plan.cu_new, window=window, softmax_scale=softmax_scale, max_new=step.max_new)
 
@@ -172,11 +203,58 @@ class PagedKVCache:
         if fewer.any():
             self._release(fewer, self._to_device(self._host_lens))
 
+    def keep(self, step, path, accepted):
+        """advance for a step of trees: each row keeps the path that ops.verify_drafts gives for it (path
+        (max_rows, P) and accepted (max_rows,) int32 on the GPU; accepted < 0: the row's new tokens all, as they
+        are), moved together in every slot, and the pages that only its other tokens needed are free again.
+        Reads accepted from the GPU, and returns how many tokens each row has kept."""
+        self._current(step)
+        if accepted.numel() != self.max_rows or path.shape[0] != self.max_rows:
+            raise RuntimeError(f"path and accepted must have a row for each of {self.max_rows}, got "
+                               f"{tuple(path.shape)} and {tuple(accepted.shape)}")
+        state = step.plan.free_state
+        ops.paged_keep(path, accepted, self.cache_seqlens, step.new_lens, self.block_table, self.free_pages, state,
+                       self.k_pages, self.v_pages, free_state_out=state, seqlens_out=self.cache_seqlens)
+        self._step = None
+        self.free_state = state
+        kept = accepted.cpu().numpy().astype(np.int64)
+        kept = np.where(kept < 0, step.host_lens, np.minimum(kept, np.minimum(step.host_lens, path.shape[1])))
+        self._host_lens += kept
+        return kept.tolist()
+
+    def fork(self, source):
+        """Row r becomes what row source[r] was (-1: empty; rows not given stay), all rows at once.  Full pages
+        are shared, a last page that is not full is copied for every row but the first that takes it over.
+        Drops a planned step."""
+        given = np.asarray(source, dtype=np.int64)
+        if given.ndim != 1 or given.size > self.max_rows or (given < -1).any() or (given >= self.max_rows).any():
+            raise RuntimeError(f"source must name at most {self.max_rows} rows, each -1 or below that, got {source}")
+        source = np.arange(self.max_rows)
+        source[:given.size] = given
+        heirs = np.bincount(source[source >= 0], minlength=self.max_rows)
+        copies = int((np.maximum(heirs - 1, 0) * (self._host_lens % self.page_size > 0)).sum())
+        if copies > self.free_page_count():
+            raise RuntimeError(f"the fork copies {copies} pages and {self.free_page_count()} are free")
+        self._step = None
+        ops.page_fork(self._to_device(source), self.cache_seqlens, self.block_table, self.page_shares, self.free_pages,
+                      self.free_state, self.k_pages, self.v_pages, block_table_out=self.block_table,
+                      shares_out=self.page_shares, free_state_out=self.free_state, seqlens_out=self.cache_seqlens)
+        for r in np.nonzero(heirs > 1)[0]:
+            fresh = int(self._host_lens[r] // self.page_size) - len(self._shared[r])
+            self._shared[r] = self._shared[r] + list(range(self._page_numbers, self._page_numbers + fresh))
+            self._page_numbers += fresh
+        self._shared = [list(self._shared[s]) if s >= 0 else [] for s in source]
+        self._host_lens = np.where(source >= 0, self._host_lens[source], 0)
+
     def release(self, rows):
-        """Frees the pages of the given rows and sets their lengths to 0.  A planned step that has new tokens
-        of one of them is dropped; any other stays the current one."""
+        """Frees the pages of the given rows and sets their lengths to 0 (a page that other rows share stays
+        theirs).  A planned step that has new tokens of one of them, or any where rows share pages, is
+        dropped; any other stays the current one."""
         done = np.zeros(self.max_rows, dtype=bool)
         done[np.asarray(rows, dtype=np.int64)] = True
+        if any(self._shared[r] for r in np.nonzero(done)[0]):
+            self.fork(np.where(done, -1, np.arange(self.max_rows)))
+            return
         if self._step is not None and self._step.host_lens[done].any():
             self._step = None
         self._release(done)

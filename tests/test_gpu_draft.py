@@ -665,7 +665,7 @@ def test_keep_moves_the_path_and_gives_pages_back(ops, in_place, cached, fresh, 
 
 def test_keep_with_paths_that_do_not_fit(ops, expects_device_error):
     g = torch.Generator("cuda").manual_seed(1)
-    for path, kept, want in (([[0, 0, 3]], 3, 3), ([[0, 9, 3]], 3, 3), ([[0, 1, 2]], 7, 3), ([[0, 1, 2]], -1, 0),
+    for path, kept, want in (([[0, 0, 3]], 3, 3), ([[0, 9, 3]], 3, 3), ([[0, 1, 2]], 7, 3),
                              ([[0, -1, 2]], 3, 3)):
         kp, vp = pools(g, 1, 4, 1, 16, 64)
         before = kp.clone()
@@ -674,6 +674,20 @@ def test_keep_with_paths_that_do_not_fit(ops, expects_device_error):
         assert ops.device_error()[0] == 8 and lens.tolist() == [3 + want]
         moved = [p for p in range(16) if not torch.equal(kp[0, 2, :, p], before[0, 2, :, p])]
         assert moved == ([5] if path[0][2] == 3 else [])
+
+
+def test_keep_of_whole_steps(ops):
+    """accepted < 0: as it is, its path not read; the pages up to its end stay."""
+    g = torch.Generator("cuda").manual_seed(1)
+    kp, vp = pools(g, 2, 8, 1, 16, 64)
+    before = kp.clone()
+    state, lens = ops.paged_keep(i32([[9, 9], [0, 3]]), i32([-1, 2]), i32([3, 20]), i32([40, 30]),
+                                 i32([[2, 1, 0, -1], [3, 4, 5, 6]]), i32([7, -1, -1, -1, -1, -1, -1, -1]),
+                                 torch.tensor([0, 1], device="cuda"), kp, vp)
+    assert lens.tolist() == [43, 22] and state.tolist() == [0, 3]
+    assert torch.equal(kp[:, 4, :, 5], before[:, 4, :, 7])
+    kp[:, 4, :, 5] = before[:, 4, :, 5]
+    assert torch.equal(kp, before)
 
 
 def test_keep_without_requests(ops):
