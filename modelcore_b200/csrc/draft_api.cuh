@@ -63,10 +63,12 @@ struct PagedTreePlan {
 PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
   PagedTreePlan pl = {};
   const long long G = t->attn.Hq / t->attn.Hkv;
-  pl.chunk = t->attn.max_new == 0 || t->attn.max_new > 32 * t->words;
-  pl.grid = device_sm_count();
+  // Chunks of up to 1,024 tokens share the tree kernel's launch: two of 300 beside 22 trees of 41, window 1,024, 95
+  // -> 54 us.  Above that the chunk kernel's products are worth its launch.
+  pl.chunk = t->attn.max_new == 0 || t->attn.max_new > std::max(32 * t->words, 1024);
+  pl.grid = std::min(device_sm_count(), mcb::kTreeMostCuts);
   // trees of at most max_new tokens, where that is known: as few rows as hold them
-  const long long most = std::min(t->attn.max_new > 0 ? t->attn.max_new : 32 * t->words, 32 * t->words) * G;
+  const long long most = (t->attn.max_new == 0 || pl.chunk ? 32 * t->words : t->attn.max_new) * G;
   pl.rows = most <= 16 ? 16 : most <= 32 ? 32 : 256;
   const size_t rows = static_cast<size_t>(pl.grid) * 2 * pl.rows, chunk_rows = static_cast<size_t>(pl.grid) * 2 * 256;
   pl.o = round256(rows * t->attn.D * 4);
@@ -126,13 +128,10 @@ int launch_paged_tree(const mcb_paged_attn_args* a, const mcb::PagedTreeParams& 
   note_attn_kernel("paged_tree_kernel", D, 0, 0, false);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_tree launch");
-  mcb::PagedChunkParams c = {};
-  c.a = p.a;
-  c.cuts = p.cuts;
-  e = launch_pdl(mcb::paged_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 8), dim3(256), 0, st, c);
+  e = launch_pdl(mcb::tree_combine_kernel<D>, dim3(static_cast<unsigned>(grid), 8), dim3(256), 0, st, p);
   g_launches++;
   if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "paged_combine launch");
+  if (e != cudaSuccess) return cuda_fail(e, "tree_combine launch");
   return MCB_OK;
 }
 
@@ -289,7 +288,7 @@ int paged_keep(const mcb_paged_keep_args* a, void* stream) {
   const int rc = check_slots(a, who);
   if (rc != MCB_OK) return rc;
   if (a->P < 0) return fail(MCB_ERR_INVALID_ARG, "%s: bad size P=%d", who, a->P);
-  if (a->R > 65535) return fail(MCB_ERR_UNSUPPORTED, "%s: R %d requests (at most 65,535)", who, a->R);
+  if (a->R >= 65535) return fail(MCB_ERR_UNSUPPORTED, "%s: R %d requests (at most 65,534)", who, a->R);
   if (a->free_state == nullptr || a->free_state_out == nullptr || a->free_pages == nullptr || a->counter == nullptr ||
       a->k_pages == nullptr || a->v_pages == nullptr ||
       (a->R > 0 && ((a->P > 0 && a->path == nullptr) || a->accepted == nullptr || a->cache_seqlens == nullptr ||
@@ -322,14 +321,15 @@ int paged_keep(const mcb_paged_keep_args* a, void* stream) {
   p.slots = a->slots;
   p.Hkv = a->Hkv;
   p.D = a->D;
+  p.in_place = a->seqlens_out == a->cache_seqlens;
   const long long columns = 2ll * a->slots * a->Hkv * (a->D / 8);
   const long long ctas = (columns + mcb::kKeepThreads - 1) / mcb::kKeepThreads;
   // (the arrival counter of the last CTA counts to 2^16)
-  if (ctas * std::max(a->R, 1) >= 1 << 16)
+  if (ctas * (a->R + 1ll) >= 1 << 16)
     return fail(MCB_ERR_UNSUPPORTED, "%s: %lld blocks of %d requests' heads in one call (at most 65,535)", who,
                 ctas * a->R, a->R);
   cudaError_t e = launch_pdl(mcb::paged_keep_kernel,
-                             dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(std::max(a->R, 1))),
+                             dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.in_place ? std::max(a->R, 1) : a->R + 1)),
                              dim3(mcb::kKeepThreads), 0, static_cast<cudaStream_t>(stream), p);
   g_launches++;
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -413,9 +413,12 @@ int page_fork(const mcb_page_fork_args* a, void* stream) {
   cudaError_t e = launch_pdl(mcb::page_fork_plan_kernel,
                              dim3(1 + std::min(blocks, static_cast<unsigned>(sms))), dim3(1024), 0, st, p);
   if (e == cudaSuccess) e = launch_pdl(mcb::page_fork_apply_kernel, dim3(static_cast<unsigned>(8 * sms)), dim3(256), 0, st, p);
-  if (e == cudaSuccess) e = launch_pdl(mcb::page_fork_count_kernel, dim3(blocks), dim3(mcb::kForkBlock), 0, st, p);
-  if (e == cudaSuccess) e = launch_pdl(mcb::page_fork_place_kernel, dim3(blocks), dim3(mcb::kForkBlock), 0, st, p);
-  g_launches += 4;
+  // one CTA counts a pool of up to 32 blocks as it places the pages, a launch (3 us) for some 0.3 us a block
+  const bool one = blocks <= 32;
+  if (e == cudaSuccess && !one) e = launch_pdl(mcb::page_fork_count_kernel, dim3(blocks), dim3(mcb::kForkBlock), 0, st, p);
+  if (e == cudaSuccess)
+    e = launch_pdl(mcb::page_fork_place_kernel, dim3(one ? 1u : blocks), dim3(mcb::kForkBlock), 0, st, p);
+  g_launches += one ? 3 : 4;
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "page_fork launch");
   return MCB_OK;

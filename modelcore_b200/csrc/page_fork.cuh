@@ -9,8 +9,9 @@
 //   freed:     page x with shares_x + change_x < 0, in page order, to queue[(tail + rank) mod n_pages]
 // (Counts, not an order of arrival, decide: the same call gives the same queue.)
 //
-// Four launches, each needing the whole of the one before: the plan (one CTA; the others zero the changes),
-// then the tables, the changes and the copies, then the freed pages of every 1,024 counted, then placed.
+// Three or four launches, each needing the whole of the one before: the plan (one CTA; the others zero the
+// changes), then the tables, the changes and the copies, then, in large pools, the freed pages of every 1,024
+// counted, then all placed.
 // All reads of what may be written in place come before the last.  The copies are bound by HBM (a page's
 // positions of one head are contiguous), all else by launches.
 //
@@ -63,6 +64,7 @@ __device__ __forceinline__ int fork_len(const PageForkParams& p, int s) {
 __global__ void __launch_bounds__(1024) page_fork_plan_kernel(const PageForkParams p) {
   __shared__ unsigned long long warp_sums[33];
   pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     for (long long i = (blockIdx.x - 1ll) * 1024 + tid; i < p.n_pages; i += (gridDim.x - 1ll) * 1024) p.change[i] = 0;
@@ -131,6 +133,7 @@ __global__ void __launch_bounds__(1024) page_fork_plan_kernel(const PageForkPara
 
 __global__ void __launch_bounds__(256) page_fork_apply_kernel(const PageForkParams p) {
   pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x, page_len = 1 << p.page_shift;
   const long long thr = static_cast<long long>(gridDim.x) * 256, me = static_cast<long long>(blockIdx.x) * 256 + tid;
   int32_t* out = p.table_in_place ? p.table_tmp : p.table_out;
@@ -189,42 +192,48 @@ __device__ __forceinline__ bool fork_freed(const PageForkParams& p, long long pa
 
 __global__ void __launch_bounds__(kForkBlock) page_fork_count_kernel(const PageForkParams p) {
   pdl_wait();
+  pdl_launch_dependents();
   const int n = __syncthreads_count(fork_freed(p, static_cast<long long>(blockIdx.x) * kForkBlock + threadIdx.x));
   if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
 }
 
+// A CTA a block; with one CTA for all blocks, in turn.
 __global__ void __launch_bounds__(kForkBlock) page_fork_place_kernel(const PageForkParams p) {
   __shared__ unsigned long long warp_sums[33];
-  pdl_wait();
+  pdl_wait();  // no early trigger: this kernel may write cache_seqlens
   const int tid = threadIdx.x;
-  unsigned long long sum = 0, all = 0;
-  for (int b = tid; b < static_cast<int>(gridDim.x); b += kForkBlock) {
-    if (b < static_cast<int>(blockIdx.x)) sum += p.counts[b];
-    all += p.counts[b];
+  const int blocks = (p.n_pages + kForkBlock - 1) / kForkBlock;
+  const bool alone = gridDim.x == 1;
+  unsigned long long before = 0;
+  if (!alone) {
+    for (int b = tid; b < static_cast<int>(blockIdx.x); b += kForkBlock) before += p.counts[b];
+    block_scan(before, warp_sums);
+    before = warp_sums[32];
+    __syncthreads();
   }
-  block_scan(sum, warp_sums);
-  const unsigned long long before = warp_sums[32];
-  __syncthreads();
-  block_scan(all, warp_sums);
-  all = warp_sums[32];
-  __syncthreads();
   const unsigned long long room = p.meta[3];
-  const long long page = static_cast<long long>(blockIdx.x) * kForkBlock + tid;
-  const bool freed = fork_freed(p, page);
-  const unsigned long long k = before + block_scan(freed ? 1ull : 0ull, warp_sums) - 1;
-  if (freed && k < room) p.queue[wrap(p.meta[4] + static_cast<long long>(k), p.n_pages)] = static_cast<int>(page);
-  if (page < p.n_pages) p.shares_out[page] = max(p.shares[page] + p.change[page], 0);
+  const long long tail_at = p.meta[4];
+  for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long page = static_cast<long long>(b) * kForkBlock + tid;
+    const bool freed = fork_freed(p, page);
+    const unsigned long long k = before + block_scan(freed ? 1ull : 0ull, warp_sums) - 1;
+    before += warp_sums[32];
+    if (freed && k < room) p.queue[wrap(tail_at + static_cast<long long>(k), p.n_pages)] = static_cast<int>(page);
+    if (page < p.n_pages) p.shares_out[page] = max(p.shares[page] + p.change[page], 0);
+    if (b == blocks - 1 && tid == 0) {
+      if (before > room) record_error(kErrPagesExhausted);
+      p.state_out[0] = p.meta[0];
+      p.state_out[1] = p.meta[1] + static_cast<long long>(min(before, room));
+    }
+    __syncthreads();  // warp_sums is free again
+  }
+  const long long me = static_cast<long long>(blockIdx.x) * kForkBlock + tid;
   const long long thr = static_cast<long long>(gridDim.x) * kForkBlock;
-  for (long long i = page; i < p.R; i += thr) p.seqlens_out[i] = p.new_len[i];
+  for (long long i = me; i < p.R; i += thr) p.seqlens_out[i] = p.new_len[i];
   if (p.table_in_place) {
     const long long entries = static_cast<long long>(p.R) * p.max_pages;
-    for (long long i = page; i < entries; i += thr)
+    for (long long i = me; i < entries; i += thr)
       p.table_out[i / p.max_pages * p.out_stride + i % p.max_pages] = p.table_tmp[i];
-  }
-  if (page == 0) {
-    if (all > room) record_error(kErrPagesExhausted);
-    p.state_out[0] = p.meta[0];
-    p.state_out[1] = p.meta[1] + static_cast<long long>(min(all, room));
   }
 }
 
@@ -243,26 +252,66 @@ struct PagedKeepParams {
   int* counter;
   long long table_stride, path_stride;
   int R, P, n_pages, max_pages, page_shift, slots, Hkv, D;
+  int in_place;  // seqlens_out is seqlens
 };
 
 constexpr int kKeepThreads = 256;
+
+__device__ __forceinline__ int keep_len(const PagedKeepParams& p, int r) {
+  const long long cap = static_cast<long long>(p.max_pages) << p.page_shift;
+  return static_cast<int>(min(static_cast<long long>(max(p.seqlens[r], 0)), cap));
+}
+__device__ __forceinline__ int keep_kept(const PagedKeepParams& p, int r, int fresh) {  // (below 0: the whole step as it is)
+  const int kept = p.kept[r];
+  return kept < 0 ? fresh : min(kept, min(fresh, p.P));
+}
+
+// The rows' lengths, and the pages behind them to the queue; one CTA.
+__device__ __noinline__ void keep_books(const PagedKeepParams& p, unsigned long long* warp_sums) {
+  const int tid = threadIdx.x;
+  const long long head = p.state[0], tail = p.state[1], n = p.n_pages;
+  const long long room = min(max(n - (tail - head), 0ll), n);
+  const int tail_at = static_cast<int>(((tail % n) + n) % n);
+  long long back = 0;
+  for (int b0 = 0; b0 < p.R; b0 += kKeepThreads) {
+    const int row = b0 + tid;
+    int c0 = 0, c1 = 0, pages = 0;
+    if (row < p.R) {
+      const int l = keep_len(p, row), f = max(p.new_lens[row], 0), k = keep_kept(p, row, f);
+      c0 = pages_of(static_cast<long long>(l) + k, p.page_shift, p.max_pages);
+      c1 = pages_of(static_cast<long long>(l) + f, p.page_shift, p.max_pages);
+      for (int c = c0; c < c1; ++c) {
+        const int pg = p.table[row * p.table_stride + c];
+        if (pg >= 0 && pg < p.n_pages) ++pages;
+        else record_error(kErrPageOutOfRange);
+      }
+      p.seqlens_out[row] = static_cast<int>(min(static_cast<long long>(l) + k, 2147483647ll));
+    }
+    long long at = back + static_cast<long long>(block_scan(static_cast<unsigned long long>(pages), warp_sums)) - pages;
+    back += static_cast<long long>(warp_sums[32]);
+    for (int c = c0; c < c1; ++c) {
+      const int pg = p.table[row * p.table_stride + c];
+      if (pg < 0 || pg >= p.n_pages) continue;
+      if (at < room) p.queue[wrap(tail_at + at, p.n_pages)] = pg;
+      ++at;
+    }
+    __syncthreads();  // warp_sums is free again
+  }
+  if (tid == 0) {
+    if (back > room) record_error(kErrPagesExhausted);
+    p.state_out[0] = head;
+    p.state_out[1] = tail + min(back, room);
+  }
+}
 
 __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKeepParams p) {
   __shared__ unsigned long long warp_sums[33];
   __shared__ long long s_src[kKeepThreads], s_dst[kKeepThreads];  // the moves' offsets in a slot, in order
   pdl_wait();  // no early trigger: this kernel may write cache_seqlens
   const int tid = threadIdx.x, page_len = 1 << p.page_shift;
-  auto len_of = [&](int r) {
-    const long long cap = static_cast<long long>(p.max_pages) << p.page_shift;
-    return static_cast<int>(min(static_cast<long long>(max(p.seqlens[r], 0)), cap));
-  };
-  auto kept_of = [&](int r, int fresh) {  // (below 0: the whole step as it is)
-    const int kept = p.kept[r];
-    return kept < 0 ? fresh : min(kept, min(fresh, p.P));
-  };
   const int r = blockIdx.y;
   const bool row = r < p.R;  // (no rows: one block row for the counters alone)
-  const int len = row ? len_of(r) : 0, fresh = row ? max(p.new_lens[r], 0) : 0, kept = row ? kept_of(r, fresh) : 0;
+  const int len = row ? keep_len(p, r) : 0, fresh = row ? max(p.new_lens[r], 0) : 0, kept = row ? keep_kept(p, r, fresh) : 0;
   if (row && blockIdx.x == 0 && tid == 0) {
     if (p.kept[r] > kept) record_error(kErrDraftOutOfRange);
     if (p.seqlens[r] != len || ((static_cast<long long>(len) + fresh + page_len - 1) >> p.page_shift) > p.max_pages)
@@ -280,6 +329,13 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKee
            column % per_vec * 8;
   }
   const int moving = row && p.kept[r] >= 0 ? kept : 0;
+  // Where the lengths' outputs are no inputs, one CTA more writes them beside the others' moves; else the last to
+  // arrive, all having read them.  (All arriving before their moves, 1,500 atomics on one word in the way: 19 ->
+  // 23 us for 128 requests of 24 slots.)
+  if (!p.in_place && r >= p.R) {
+    if (blockIdx.x == 0) keep_books(p, warp_sums);
+    return;
+  }
   for (int i0 = 0; i0 < moving; i0 += kKeepThreads) {
     const int i = i0 + tid;
     bool move = false;
@@ -321,41 +377,7 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKee
     __syncthreads();
   }
   bool unused = false;
-  if (!last_cta(p.counter, unused)) return;
-  // the lengths, and the pages behind them
-  const long long head = p.state[0], tail = p.state[1], n = p.n_pages;
-  const long long room = min(max(n - (tail - head), 0ll), n);
-  const int tail_at = static_cast<int>(((tail % n) + n) % n);
-  long long back = 0;
-  for (int b0 = 0; b0 < p.R; b0 += kKeepThreads) {
-    const int row = b0 + tid;
-    int c0 = 0, c1 = 0, pages = 0;
-    if (row < p.R) {
-      const int l = len_of(row), f = max(p.new_lens[row], 0), k = kept_of(row, f);
-      c0 = pages_of(static_cast<long long>(l) + k, p.page_shift, p.max_pages);
-      c1 = pages_of(static_cast<long long>(l) + f, p.page_shift, p.max_pages);
-      for (int c = c0; c < c1; ++c) {
-        const int pg = p.table[row * p.table_stride + c];
-        if (pg >= 0 && pg < p.n_pages) ++pages;
-        else record_error(kErrPageOutOfRange);
-      }
-      p.seqlens_out[row] = static_cast<int>(min(static_cast<long long>(l) + k, 2147483647ll));
-    }
-    long long at = back + static_cast<long long>(block_scan(static_cast<unsigned long long>(pages), warp_sums)) - pages;
-    back += static_cast<long long>(warp_sums[32]);
-    for (int c = c0; c < c1; ++c) {
-      const int pg = p.table[row * p.table_stride + c];
-      if (pg < 0 || pg >= p.n_pages) continue;
-      if (at < room) p.queue[wrap(tail_at + at, p.n_pages)] = pg;
-      ++at;
-    }
-    __syncthreads();  // warp_sums is free again
-  }
-  if (tid == 0) {
-    if (back > room) record_error(kErrPagesExhausted);
-    p.state_out[0] = head;
-    p.state_out[1] = tail + min(back, room);
-  }
+  if (p.in_place && last_cta(p.counter, unused)) keep_books(p, warp_sums);
 }
 
 }  // namespace mcb

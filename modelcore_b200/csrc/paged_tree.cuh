@@ -11,7 +11,7 @@
 // chunk kernel, row = token * G + head, 128 a tile; a *unit* is (request, two tiles Q0, Q1, kv head), its
 // keys from the first that any of its rows may see to the request's last.  All units' 128-key tiles form one
 // sequence that the CTAs (one an SM) share evenly, computed on the device from the lengths; a cut unit leaves
-// (O / l, log2 sum) in workspace and paged_combine_kernel, launched after, merges them.
+// (O / l, log2 sum) in workspace and tree_combine_kernel, launched after, merges them.
 //
 // Roles of a CTA's warps:
 //   warp 0      TMA producer and walker: describes each part of a unit in shared memory, loads its queries,
@@ -178,6 +178,128 @@ __device__ __forceinline__ void tree_rows(const PagedTreeParams& p, int row_a, i
   }
 }
 
+// Where a CTA's share of the tiles begins and ends, and the walk at its start: every warp's own when all requests
+// fit its lanes (no barrier, nothing through shared memory, which a step of few requests is made of), else the
+// CTA's together through `tot` (kPtWarps words) and `ctl` (4).  Ends with all threads past one __syncthreads.
+struct TreeShare {
+  long long total, t_begin, t_end;
+  int ng;
+};
+__device__ __forceinline__ TreeShare tree_share(long long total) {
+  TreeShare s;
+  s.total = total;
+  s.ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const bool active = static_cast<int>(blockIdx.x) < s.ng;
+  s.t_begin = active ? share_begin(blockIdx.x, total, s.ng) : 0;
+  s.t_end = active ? share_begin(blockIdx.x + 1, total, s.ng) : 0;
+  return s;
+}
+__device__ __forceinline__ TreeShare tree_place(const PagedTreeParams& p, TreeWalk& w, long long* tot, int* ctl) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  TreeShare s;
+  if (p.a.R <= 32) {
+    PagedRow x = {0, 0, 0};
+    long long mine = 0;
+    if (lane < p.a.R) {
+      x = paged_row(p.a, lane);
+      if (blockIdx.x == 0 && warp == 0 && !paged_row_fits(p.a, lane, x)) record_error(kErrPositionBeyondCache);
+      const int nqb = tree_blocks(p, x);
+      for (int qb = 0; qb < nqb; ++qb) mine += tree_unit(p, x, lane, qb, nqb).n;
+      mine *= p.a.Hkv;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, m);
+      if (lane >= m) incl += o;
+    }
+    s = tree_share(__shfl_sync(0xffffffffu, incl, 31));
+    w.t = s.t_begin;
+    if (s.t_begin < s.t_end) {
+      const int r = __ffs(__ballot_sync(0xffffffffu, s.t_begin < incl)) - 1;  // (t_begin < total: some lane's)
+      long long left = s.t_begin - __shfl_sync(0xffffffffu, incl - mine, r);
+      x.tok0 = __shfl_sync(0xffffffffu, x.tok0, r);
+      x.T = __shfl_sync(0xffffffffu, x.T, r);
+      x.L = __shfl_sync(0xffffffffu, x.L, r);
+      const int nqb = tree_blocks(p, x);
+      w.u = tree_unit(p, x, r, 0, nqb);
+      while (left >= static_cast<long long>(w.u.n) * p.a.Hkv) {
+        left -= static_cast<long long>(w.u.n) * p.a.Hkv;
+        w.u = tree_unit(p, x, r, w.u.qb + 1, nqb);
+      }
+      const uint32_t at = static_cast<uint32_t>(left);  // < n Hkv
+      w.h = static_cast<int>(at / static_cast<uint32_t>(w.u.n));
+      w.local = static_cast<int>(at % static_cast<uint32_t>(w.u.n));
+    }
+    __syncthreads();
+    return s;
+  }
+  const int per = (p.a.R + kPtWarps - 1) / kPtWarps;
+  const int row_a = min(warp * per, p.a.R), row_b = min(row_a + per, p.a.R);
+  long long mine = 0;
+  tree_rows(p, row_a, row_b, [&](int, int, int n) {
+    mine += n;
+    return false;
+  });
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+  mine *= p.a.Hkv;
+  if (lane == 0) tot[warp] = mine;
+  __syncthreads();
+  long long total = 0, before = 0;
+#pragma unroll
+  for (int i = 0; i < kPtWarps; ++i) {
+    if (i < warp) before += tot[i];
+    total += tot[i];
+  }
+  s = tree_share(total);
+  const long long t_begin = s.t_begin;
+  if (t_begin < s.t_end && before <= t_begin && t_begin < before + mine) {
+    long long left = t_begin - before;
+    tree_rows(p, row_a, row_b, [&](int r, int qb, int n) {
+      int incl = n;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, m);
+        if (lane >= m) incl += o;
+      }
+      const long long all = static_cast<long long>(__shfl_sync(0xffffffffu, incl, 31)) * p.a.Hkv;
+      if (left >= all) {
+        left -= all;
+        return false;
+      }
+      const long long mine0 = static_cast<long long>(incl - n) * p.a.Hkv;
+      if (n > 0 && mine0 <= left && left < mine0 + static_cast<long long>(n) * p.a.Hkv) {
+        ctl[0] = r;
+        ctl[1] = qb + lane;
+        ctl[2] = static_cast<int>((left - mine0) / n);
+        ctl[3] = static_cast<int>((left - mine0) % n);
+      }
+      return true;
+    });
+  }
+  __syncthreads();
+  w.t = t_begin;
+  if (t_begin < s.t_end) {
+    const PagedRow x = paged_row(p.a, ctl[0]);
+    w.u = tree_unit(p, x, ctl[0], ctl[1], tree_blocks(p, x));
+    w.h = ctl[2];
+    w.local = ctl[3];
+  }
+  return s;
+}
+
+// paged_fill by threads 0 .. threads - 1 of every CTA, this one `index`.
+__device__ __forceinline__ void tree_fill(const PagedAttnParams& p, int D, int index, int threads) {
+  const long long per = static_cast<long long>(p.Hq) * D / 8;  // 16-byte words a token
+  const int first = min(max(p.cu_new[0], 0), p.N), last = max(min(p.cu_new[p.R], p.N), first);
+  const long long lead = first * per, gap = (last - first) * per, end = p.N * per;
+  uint4* out = reinterpret_cast<uint4*>(p.out);
+  for (long long i = static_cast<long long>(blockIdx.x) * threads + index; i < end - gap;
+       i += static_cast<long long>(gridDim.x) * threads)
+    out[i < lead ? i : i + gap] = make_uint4(0, 0, 0, 0);
+}
+
 // Bits a .. b of a word (none when b < a; 0 <= a, b <= 31).
 __device__ __forceinline__ uint32_t bit_range(int a, int b) {
   return b < a ? 0u : (b - a == 31 ? 0xffffffffu : ((1u << (b - a + 1)) - 1)) << a;
@@ -320,57 +442,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   pdl_launch_dependents();
 
   // ---- the sequence's length and this CTA's first tile ----
-  const int per = (p.a.R + kPtWarps - 1) / kPtWarps;
-  const int row_a = min(warp * per, p.a.R), row_b = min(row_a + per, p.a.R);
-  long long mine = 0;
-  tree_rows(p, row_a, row_b, [&](int, int, int n) {
-    mine += n;
-    return false;
-  });
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
-  mine *= p.a.Hkv;
-  if (lane == 0) warp_tot[warp] = mine;
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  long long total = 0, before = 0;
-#pragma unroll
-  for (int i = 0; i < kPtWarps; ++i) {
-    if (i < warp) before += warp_tot[i];
-    total += warp_tot[i];
-  }
-  if (p.a.fill) paged_fill(p.a, D, blockDim.x);
-  const int ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  const bool active = static_cast<int>(blockIdx.x) < ng;
-  const long long t_begin = active ? share_begin(blockIdx.x, total, ng) : 0;
-  const long long t_end = active ? share_begin(blockIdx.x + 1, total, ng) : 0;
-  if (active && before <= t_begin && t_begin < before + mine) {
-    long long left = t_begin - before;
-    tree_rows(p, row_a, row_b, [&](int r, int qb, int n) {
-      int incl = n;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, m);
-        if (lane >= m) incl += o;
-      }
-      const long long all = static_cast<long long>(__shfl_sync(0xffffffffu, incl, 31)) * p.a.Hkv;
-      if (left >= all) {
-        left -= all;
-        return false;
-      }
-      const long long mine0 = static_cast<long long>(incl - n) * p.a.Hkv;
-      if (n > 0 && mine0 <= left && left < mine0 + static_cast<long long>(n) * p.a.Hkv) {
-        ctl[0] = r;
-        ctl[1] = qb + lane;
-        ctl[2] = static_cast<int>((left - mine0) / n);
-        ctl[3] = static_cast<int>((left - mine0) % n);
-      }
-      return true;
-    });
-  }
   if (threadIdx.x == 0) p.cuts[blockIdx.x].h = -1;
-  __syncthreads();
+  tc_fence_before();
+  TreeWalk w;
+  const TreeShare share = tree_place(p, w, warp_tot, ctl);
+  tc_fence_after();
+  const long long total = share.total, t_begin = share.t_begin, t_end = share.t_end;
+  const int ng = share.ng;
   const uint32_t tmem = *tmem_slot;
   const uint32_t base = smem_u32(smem);
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
@@ -400,14 +478,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const uint32_t q_bytes = static_cast<uint32_t>(p.a.tpb * p.a.G) * 128u;
       const int lch = lane / Cfg::kPanels, lpn = lane % Cfg::kPanels;
       const uint32_t lane_dst = Cfg::kRingOff + lpn * kPtTile * 128 + lch * box_bytes;
-      TreeWalk w;
-      w.t = t_begin;
-      if (active) {
-        const PagedRow x = paged_row(p.a, ctl[0]);
-        w.u = tree_unit(p, x, ctl[0], ctl[1], tree_blocks(p, x));
-        w.h = ctl[2];
-        w.local = ctl[3];
-      }
       uint32_t gt = 0;        // key tiles so far
       uint32_t sets = 0, armed[3] = {0, 0, 0};  // two bits a stage: the set of its last copy; a bit: that set's phase
       uint32_t mine = 0;                        // stages with a copy of this warp's last
@@ -532,6 +602,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // ---------------- product issuers, one a group ----------------
       constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 1);
+      tree_fill(p.a, D, threadIdx.x - 32, 64);
       const int t = __shfl_sync(0xffffffffu, warp - 1, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t s_col = tm + t * kPtTile, o_col = tm + Cfg::kOCol + t * D;
@@ -801,6 +872,84 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Merges the units cut between CTAs: blockIdx.x is the CTA whose share the unit starts in, blockIdx.y
+// 32 of its rows.  A lane is a row, a warp takes every eighth group of four columns (the partials' layout: a
+// load is 512 contiguous bytes), two groups and four contributors' loads on their way at once; the rows
+// leave through shared memory, whole.
+constexpr int kTreeMostCuts = 160;  // contributors (no GPU of these has as many SMs)
+template <int D>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const PagedTreeParams p) {
+  __shared__ float weight[kTreeMostCuts][32];
+  __shared__ uint2 rows[32][D / 4 + 1];
+  __shared__ int out_row[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const PagedCut c = p.cuts[blockIdx.x];
+  if (c.h < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = blockIdx.y * 32 + lane, rr = n & 127;
+  const int rt = rr / p.a.G, tok = c.tok0 + (n >> 7) * p.a.tpb + rt;
+  const bool valid = rt < p.a.tpb && tok < c.tok1;
+  if (!__syncthreads_or(valid)) return;
+  const int cnt = min(c.g_last - static_cast<int>(blockIdx.x) + 1, kTreeMostCuts);
+  auto slot = [&](int k) { return (static_cast<long long>(blockIdx.x) + k) * 2 + (k == 0 && c.slot1 ? 1 : 0); };
+  for (int k = warp; k < cnt; k += 8) weight[k][lane] = valid ? __ldcg(p.a.part_lse + slot(k) * 256 + n) : -CUDART_INF_F;
+  __syncthreads();
+  float mx = -CUDART_INF_F, wsum = 0.f;
+  for (int k = 0; k < cnt; ++k) mx = fmaxf(mx, weight[k][lane]);
+  for (int k = 0; k < cnt; ++k) {
+    const float ls = weight[k][lane];
+    wsum += ls == -CUDART_INF_F ? 0.f : fast_exp2(ls - mx);
+  }
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
+  __syncthreads();
+  for (int k = warp; k < cnt; k += 8) {
+    const float ls = weight[k][lane];
+    weight[k][lane] = ls == -CUDART_INF_F ? 0.f : fast_exp2(ls - mx) * inv;  // (0: its partial was not written)
+  }
+  if (warp == 0) out_row[lane] = valid ? tok * p.a.Hq + c.h * p.a.G + (rr - rt * p.a.G) : -1;
+  __syncthreads();
+#pragma unroll 1
+  for (int q = warp; q < D / 4; q += 16) {
+    float a[2][4] = {};
+    const bool two = q + 8 < D / 4;
+    for (int k0 = 0; k0 < cnt; k0 += 4) {
+      float4 v[2][4];
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = min(k0 + i, cnt - 1);
+        w[i] = k0 + i < cnt ? weight[k][lane] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (valid && (j == 0 || two))
+            v[j][i] = __ldcg(reinterpret_cast<const float4*>(p.a.part_o) + (slot(k) * (D / 4) + q + 8 * j) * 256 + n);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!valid || w[i] == 0.f) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (j == 1 && !two) continue;
+          a[j][0] = fmaf(w[i], v[j][i].x, a[j][0]);
+          a[j][1] = fmaf(w[i], v[j][i].y, a[j][1]);
+          a[j][2] = fmaf(w[i], v[j][i].z, a[j][2]);
+          a[j][3] = fmaf(w[i], v[j][i].w, a[j][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (j == 0 || two) rows[lane][q + 8 * j] = make_uint2(pack_bf16x2(a[j][0], a[j][1]), pack_bf16x2(a[j][2], a[j][3]));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+    const int r = i / (D / 4), q = i % (D / 4);
+    if (out_row[r] >= 0)
+      *reinterpret_cast<uint2*>(p.a.out + static_cast<long long>(out_row[r]) * D + 4 * q) = rows[r][q];
   }
 }
 

@@ -183,57 +183,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   pdl_launch_dependents();
 
   // ---- the sequence's length and this CTA's first tile ----
-  const int per = (p.a.R + kPtWarps - 1) / kPtWarps;
-  const int row_a = min(warp * per, p.a.R), row_b = min(row_a + per, p.a.R);
-  long long mine = 0;
-  tree_rows(p, row_a, row_b, [&](int, int, int n) {
-    mine += n;
-    return false;
-  });
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
-  mine *= p.a.Hkv;
-  if (lane == 0) warp_tot[warp] = mine;
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  long long total = 0, before = 0;
-#pragma unroll
-  for (int i = 0; i < kPtWarps; ++i) {
-    if (i < warp) before += warp_tot[i];
-    total += warp_tot[i];
-  }
-  if (p.a.fill) paged_fill(p.a, D, blockDim.x);
-  const int ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  const bool active = static_cast<int>(blockIdx.x) < ng;
-  const long long t_begin = active ? share_begin(blockIdx.x, total, ng) : 0;
-  const long long t_end = active ? share_begin(blockIdx.x + 1, total, ng) : 0;
-  if (active && before <= t_begin && t_begin < before + mine) {
-    long long left = t_begin - before;
-    tree_rows(p, row_a, row_b, [&](int r, int qb, int n) {
-      int incl = n;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, m);
-        if (lane >= m) incl += o;
-      }
-      const long long all = static_cast<long long>(__shfl_sync(0xffffffffu, incl, 31)) * p.a.Hkv;
-      if (left >= all) {
-        left -= all;
-        return false;
-      }
-      const long long mine0 = static_cast<long long>(incl - n) * p.a.Hkv;
-      if (n > 0 && mine0 <= left && left < mine0 + static_cast<long long>(n) * p.a.Hkv) {
-        ctl[0] = r;
-        ctl[1] = qb + lane;
-        ctl[2] = static_cast<int>((left - mine0) / n);
-        ctl[3] = static_cast<int>((left - mine0) % n);
-      }
-      return true;
-    });
-  }
   if (threadIdx.x == 0) p.cuts[blockIdx.x].h = -1;
-  __syncthreads();
+  tc_fence_before();
+  TreeWalk w;
+  const TreeShare share = tree_place(p, w, warp_tot, ctl);
+  tc_fence_after();
+  const long long total = share.total, t_begin = share.t_begin, t_end = share.t_end;
+  const int ng = share.ng;
   const uint32_t tmem = *tmem_slot;
   const uint32_t base = smem_u32(smem);
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
@@ -260,14 +216,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t q_bytes = static_cast<uint32_t>(p.a.tpb * p.a.G) * 128u;
     const int lch = lane / Cfg::kPanels, lpn = lane % Cfg::kPanels;
     const uint32_t lane_dst = Cfg::kRingOff + lpn * kPtTile * 128 + lch * box_bytes;
-    TreeWalk w;
-    w.t = t_begin;
-    if (active) {
-      const PagedRow x = paged_row(p.a, ctl[0]);
-      w.u = tree_unit(p, x, ctl[0], ctl[1], tree_blocks(p, x));
-      w.h = ctl[2];
-      w.local = ctl[3];
-    }
     uint32_t gt = 0;  // key tiles so far
     int k = 0;        // parts so far
     bool ok = true;
@@ -366,6 +314,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // ---------------- product issuers: S^T, O^T ----------------
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, R, 0);
     constexpr uint32_t idesc_o = umma_idesc_bf16(128, R, 1) | 1u << 15;  // A and B both MN-major
+    tree_fill(p.a, D, threadIdx.x - 32, 64);
     const bool pv = __shfl_sync(0xffffffffu, warp, 0) == 2;
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t q0_desc = smem_desc_sw128(base + Cfg::kQOff, 16, 1024);
