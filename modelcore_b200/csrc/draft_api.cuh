@@ -214,6 +214,7 @@ int verify_drafts(const mcb_verify_drafts_args* a, void* stream) {
   if (a == nullptr) return fail(MCB_ERR_INVALID_ARG, "%s: args is NULL", who);
   if (a->R < 0 || a->N < 0 || a->V <= 0 || a->max_path <= 0)
     return fail(MCB_ERR_INVALID_ARG, "%s: bad sizes R=%d N=%d V=%d max_path=%d", who, a->R, a->N, a->V, a->max_path);
+  if (a->V > 1 << 30) return fail(MCB_ERR_UNSUPPORTED, "%s: V %d (at most 2^30)", who, a->V);
   if (!(a->temperature >= 0.f) || a->temperature > 3e38f)
     return fail(MCB_ERR_INVALID_ARG, "%s: temperature %g must be finite and not negative", who, a->temperature);
   if (a->R == 0) return MCB_OK;

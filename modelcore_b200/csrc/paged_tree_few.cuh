@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         // a lane a box: chunk lch, panel lpn of the tile's, those with visible keys
         const int key0 = (c0 + lch) << box_shift;
-        const bool load = lch < nch && key0 <= w.u.hi && key0 + box > w.u.lo;
+        const bool load = lch < nch && key0 <= w.u.hi && key0 > w.u.lo - box;
         const int row = __shfl_sync(0xffffffffu, pg, (c0 - pbase + lch) & 31) * p.a.Hkv + w.h;
         const int pos = key0 & ((1 << p.a.page_shift) - 1);
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * box_bytes;

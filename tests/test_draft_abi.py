@@ -76,7 +76,7 @@ def test_verify_rejects_bad_arguments():
     good = dict(logits=P, logits_stride=100, tokens=P, parents=P, cu_new=P, accept=P, draws=P, accepted=P, path=P,
                 next_token=P, R=2, N=5, V=100, max_path=4, temperature=1.0)
     call = _rejects("mcb_verify_drafts", VerifyDraftsArgs, good, [
-        (dict(R=-1), INVALID, "R=-1"), (dict(V=0), INVALID, "V=0"), (dict(max_path=0), INVALID, "max_path=0"),
+        (dict(R=-1), INVALID, "R=-1"), (dict(V=0), INVALID, "V=0"), (dict(V=(1 << 30) + 1), UNSUPPORTED, "2^30"), (dict(max_path=0), INVALID, "max_path=0"),
         (dict(temperature=-1.0), INVALID, "temperature"), (dict(temperature=float("nan")), INVALID, "temperature"),
         (dict(temperature=float("inf")), INVALID, "temperature"), (dict(logits=None), INVALID, "NULL"),
         (dict(draws=None), INVALID, "NULL"), (dict(path=None), INVALID, "NULL"),

@@ -251,6 +251,33 @@ def test_long_requests_cut_between_many_blocks(ops):
     check_attn(ops, [12345, 9000], [100, 250], 8, 1, 128, 32, max_tree=256)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,fresh", [(16, 4, 128, 5), (16, 4, 128, 30), (16, 4, 128, 63), (4, 4, 64, 14),
+                                            (8, 8, 64, 30), (12, 6, 64, 64), (32, 4, 128, 3), (6, 6, 128, 1)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_long_runs_of_tiles(ops, Hq, Hkv, D, fresh, page):
+    """Some 25 tiles a block in one or two runs: every stage of its rings turns many times."""
+    check_attn(ops, [20000, 17777, 23456, 20001], [fresh] * 4, Hq, Hkv, D, page)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,fresh", [(8, 1, 64, 2), (8, 1, 128, 2), (8, 1, 64, 20), (4, 4, 128, 20)])
+def test_positions_up_to_31_bits(ops, Hq, Hkv, D, fresh):
+    """The last tokens that a table of 1,024-position pages can hold, their window's pages the only real ones."""
+    page, window = 1024, 700
+    width = (2 ** 31 - 1) // page
+    past = width * page - fresh
+    parents = random_parents(np.random.default_rng(1), fresh)
+    first = past - past % page - page  # the first position that has a page of its own
+    c = attn_case([past - first], [fresh], [parents], Hq, Hkv, D, page, 32)
+    table = torch.full((1, width), 2 ** 31 - 1, device="cuda", dtype=torch.int32)
+    table[0, first // page:] = c["table"][0, :width - first // page]
+    want, bound = attn_ref(c, [past - first], [fresh], window, D ** -0.5)
+    t = ops.draft_tree(i32(parents + [-1, -1]), c["cu"], i32([past]), max_tree=32)
+    for hint in (0, fresh):
+        got = ops.paged_tree_attn(c["q"], c["kp"], c["vp"], table, i32([past]), c["cu"], t.positions, t.mask, window=window,
+                                  max_new=hint)
+        assert ((got[:-2].double() - want).abs() <= 2.25 * U * bound).all()
+
+
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (3, 3, 64)])
 def test_masks_of_any_kind(ops, Hq, Hkv, D):
     """Rows that see nothing, later tokens, not themselves; positions below the cached length."""
@@ -674,6 +701,25 @@ def test_keep_with_paths_that_do_not_fit(ops, expects_device_error):
         assert ops.device_error()[0] == 8 and lens.tolist() == [3 + want]
         moved = [p for p in range(16) if not torch.equal(kp[0, 2, :, p], before[0, 2, :, p])]
         assert moved == ([5] if path[0][2] == 3 else [])
+
+
+def test_keep_and_fork_past_32_bits(ops):
+    """A pool of 2^32 bytes and more a slot: the last slot's last pages."""
+    slots, n_pages, Hkv, page, D = 2, 34000, 8, 64, 128
+    kp, vp = (torch.zeros(slots, n_pages, Hkv, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    g = torch.Generator("cuda").manual_seed(1)
+    for pool in (kp, vp):
+        pool[:, -2] = torch.randn(slots, Hkv, page, D, device="cuda", dtype=torch.bfloat16, generator=g)
+    before = [pool[:, -2].clone() for pool in (kp, vp)]
+    queue, state = torch.arange(n_pages, device="cuda", dtype=torch.int32), torch.tensor([n_pages - 1, n_pages], device="cuda")
+    ops.paged_keep(i32([[0, 5, 40]]), i32([3]), i32([10]), i32([50]), i32([[n_pages - 2]]), queue.clone(), state, kp, vp)
+    f = ops.page_fork(i32([0, 0]), i32([13, 0]), i32([[n_pages - 2], [-1]]), torch.zeros_like(queue), queue, state, kp, vp)
+    assert f.block_table.tolist() == [[n_pages - 2], [n_pages - 1]]
+    for pool, old in zip((kp, vp), before):
+        for i, at in enumerate((0, 5, 40)):
+            assert torch.equal(pool[:, -2, :, 10 + i], old[:, :, 10 + at])
+        assert torch.equal(pool[:, -1, :, :13], pool[:, -2, :, :13]) and not pool[:, -1, :, 13:].any()
+        assert not pool[:, :-2].any()
 
 
 def test_keep_of_whole_steps(ops):
