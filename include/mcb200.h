@@ -562,6 +562,7 @@ typedef struct {
 } mcb_paged_tree_attn_args;
 
 size_t mcb_paged_tree_attn_workspace_size(const mcb_paged_tree_attn_args* args);
+size_t mcb_paged_tree_attn_counter_count(const mcb_paged_tree_attn_args* args);
 int mcb_paged_tree_attn(const mcb_paged_tree_attn_args* args, void* stream);
 
 /* mcb_verify_drafts: which drafted tokens the target keeps, and the token after them.  logits[t] are the

@@ -71,6 +71,7 @@ EXPORTED_SYMBOLS = (
     "mcb_page_release_to",
     "mcb_draft_tree",
     "mcb_paged_tree_attn_workspace_size",
+    "mcb_paged_tree_attn_counter_count",
     "mcb_paged_tree_attn",
     "mcb_verify_drafts",
     "mcb_paged_keep",
@@ -384,6 +385,7 @@ def _declare(lib):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [P(cls), ctypes.c_void_p]
     for name, cls in (("mcb_paged_tree_attn_workspace_size", PagedTreeAttnArgs),
+                      ("mcb_paged_tree_attn_counter_count", PagedTreeAttnArgs),
                       ("mcb_page_fork_workspace_size", PageForkArgs)):
         getattr(lib, name).restype = ctypes.c_size_t
         getattr(lib, name).argtypes = [P(cls)]

@@ -57,7 +57,7 @@ struct PagedTreePlan {
   bool chunk;  // some request may be a chunk of a prompt
   int rows;    // query rows a unit: 16 or 32 with the keys on the M side, 256 the other kernel
   int grid;
-  size_t o, lse, cuts, chunk_o, chunk_lse, ws_bytes;
+  size_t o, lse, cuts, chunk_o, chunk_lse, ws_bytes, counters;
 };
 
 PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
@@ -71,6 +71,7 @@ PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
   const long long most = (t->attn.max_new == 0 || pl.chunk ? 32 * t->words : t->attn.max_new) * G;
   pl.rows = most <= 16 ? 16 : most <= 32 ? 32 : 256;
   const size_t rows = static_cast<size_t>(pl.grid) * 2 * pl.rows, chunk_rows = static_cast<size_t>(pl.grid) * 2 * 256;
+  pl.counters = pl.rows < 256 ? static_cast<size_t>(pl.grid) : 0;
   pl.o = round256(rows * t->attn.D * 4);
   pl.lse = round256(rows * 4);
   pl.cuts = round256(pl.grid * sizeof(mcb::PagedCut));
@@ -102,10 +103,6 @@ int launch_tree_few(const mcb_paged_attn_args* a, const mcb::PagedTreeParams& p,
   note_attn_kernel("paged_tree_few_kernel", D, 0, R, false);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged_tree_few launch");
-  e = launch_pdl(mcb::tree_few_combine_kernel<D, R>, dim3(static_cast<unsigned>(grid), R / 8), dim3(256), 0, st, p);
-  g_launches++;
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tree_few_combine launch");
   return MCB_OK;
 }
 
@@ -154,6 +151,8 @@ int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
   if (a->workspace == nullptr || a->workspace_bytes < pl.ws_bytes || !aligned(a->workspace, 256))
     return fail(MCB_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed, got %zu", who, pl.ws_bytes,
                 a->workspace_bytes);
+  if (pl.counters > 0 && (a->counters == nullptr || a->counter_count < pl.counters))
+    return fail(MCB_ERR_WORKSPACE, "%s: %zu counters are needed, got %zu", who, pl.counters, a->counter_count);
   mcb::PagedTreeParams p = {};
   p.a.q = static_cast<const uint16_t*>(a->q);
   p.a.qs[0] = qs.s[0];
@@ -162,6 +161,7 @@ int paged_tree_attn(const mcb_paged_tree_attn_args* t, void* stream) {
   p.a.table_stride = a->table_stride;
   p.a.seqlens = a->cache_seqlens;
   p.a.cu_new = a->cu_new;
+  p.a.counters = a->counters;
   p.a.out = static_cast<uint16_t*>(a->out);
   p.a.R = a->R;
   p.a.N = a->N;
@@ -437,6 +437,15 @@ size_t mcb_paged_tree_attn_workspace_size(const mcb_paged_tree_attn_args* a) {
   guarded("mcb_paged_tree_attn_workspace_size", [&] {
     const int rc = check_paged_tree(a, "mcb_paged_tree_attn_workspace_size");
     if (rc == MCB_OK) n = plan_paged_tree(a).ws_bytes;
+    return rc;
+  });
+  return n;
+}
+size_t mcb_paged_tree_attn_counter_count(const mcb_paged_tree_attn_args* a) {
+  size_t n = 0;
+  guarded("mcb_paged_tree_attn_counter_count", [&] {
+    const int rc = check_paged_tree(a, "mcb_paged_tree_attn_counter_count");
+    if (rc == MCB_OK) n = plan_paged_tree(a).counters;
     return rc;
   });
   return n;

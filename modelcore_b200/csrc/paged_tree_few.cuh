@@ -6,7 +6,7 @@
 //   O^T (D x R rows) += V_j^T P^T              M=128 N=R K=128   (both from shared memory)
 // with R = 16, 32 or 64 rows, token * G + head, of one *unit* (request, R / G tokens, kv head).  The tiles of
 // all units are one sequence that the CTAs share evenly, as in the kernel beside this one, whose walk, masks and
-// descriptions these are.  A tile of K and V, 64 KB at head size 128, has some 2,100 cycles at HBM's rate;
+// descriptions these are; a cut unit's last contributor merges it.  A tile of K and V, 64 KB at head size 128, has some 2,100 cycles at HBM's rate;
 // with the rows on the M side it took 1,280 of the tensor cores whatever the rows, and the exponentials of 16
 // rows fell to one warp.
 //
@@ -40,7 +40,7 @@ struct TreeFewConfig {
   static constexpr int kNumBars = 2 * kStages + 23;
   static constexpr int kSegOff = (kBarOff + kNumBars * 8 + 32 + 63) / 64 * 64;
   static constexpr int kRowOff = kSegOff + 4 * 64;       // R tokens' {see_lo, see_hi, pos}
-  static constexpr int kRefOff = kRowOff + R * 12;       // [2][R] -m of either group; at the end the rows' weights
+  static constexpr int kRefOff = kRowOff + R * 12;       // [2][R] -m of either group
   static constexpr int kVoteOff = kRefOff + 2 * R * 4;   // [2][2][4] what a group's warps vote
   static constexpr int kBytes = kVoteOff + 64 + 1024;
   // above half of an SM's shared memory: one CTA an SM
@@ -183,7 +183,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   pdl_launch_dependents();
 
   // ---- the sequence's length and this CTA's first tile ----
-  if (threadIdx.x == 0) p.cuts[blockIdx.x].h = -1;
   tc_fence_before();
   TreeWalk w;
   const TreeShare share = tree_place(p, w, warp_tot, ctl);
@@ -250,22 +249,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           d.c1 = 0;
           d.h = w.h;
           d.part = whole ? -1 : k > 0 ? 1 : 0;
-          d.q = 0;
           d.last = w.t + seg >= t_end;
-          d.pad[0] = d.pad[1] = 0;
+          d.q = d.pad[0] = d.pad[1] = 0;
+          if (!whole) {  // who has its tiles, and whether the first one's partial is in its slot 1
+            const long long start = w.t - w.local;
+            d.pad[0] = share_owner(start, total, ng);
+            d.pad[1] = share_owner(start + w.u.n - 1, total, ng);
+            d.q = start != share_begin(d.pad[0], total, ng);
+          }
           segs[k & 3] = d;
           mbar_arrive(&seg_full[k & 3]);
-          const long long start = w.t - w.local;
-          if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
-            PagedCut c;
-            c.tok0 = d.tok0 + d.first;
-            c.tok1 = c.tok0 + d.c0;
-            c.h = w.h;
-            c.g_last = share_owner(start + w.u.n - 1, total, ng);
-            c.slot1 = d.part;
-            c.pad[0] = c.pad[1] = c.pad[2] = 0;
-            p.cuts[blockIdx.x] = c;
-          }
           mbar_arrive_expect_tx(&q_full[k & 1], Cfg::kPanels * q_bytes);
 #pragma unroll
           for (int pn = 0; pn < Cfg::kPanels; ++pn)
@@ -384,6 +377,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t s_addr = tmem + lane_off + t * R, o_addr = tmem + lane_off + 2 * R;
     const float sc = p.a.scale_log2;
     int* votes = reinterpret_cast<int*>(smem + Cfg::kVoteOff) + t * 8;
+    volatile int* merge = ctl;                          // whether this CTA merges a cut unit
     uint8_t* p_tile = smem + Cfg::kPOff + t * Cfg::kPBytes;
     float* wred = reinterpret_cast<float*>(p_tile);     // [4][R] while no product reads P^T
     float* delta = wred + 4 * R;                        // [R]
@@ -494,7 +488,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         // P^T of this group's last tile has been read: the meeting tells the group
         if (n > 0 && !(ok = wait(&pv_done[t], (n - 1) & 1))) break;
         tc_fence_after();
-        far = group_any(far);
+        if (!unsettled) far = group_any(far);  // (unsettled is the group's)
         if (!ok) break;
         if (__builtin_expect(far || unsettled, 0)) {
           // the rows' maxima over the tile, less their m
@@ -594,11 +588,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const long long slot = static_cast<long long>(blockIdx.x) * 2 + d.part;
-      if (threadIdx.x - 128 < R) {
-        const int r = threadIdx.x - 128;
+      const bool two = d.seg > 1;
+      const int rows = d.c0 * p.a.G;
+      // a lane a row: both groups' sums and weights, by every warp for itself
+      float w0 = 0.f, w1 = 0.f;
+      {
+        const int r = lane < R ? lane : 0;
         const float* red0 = reinterpret_cast<const float*>(smem + Cfg::kPOff);
         const float* red1 = reinterpret_cast<const float*>(smem + Cfg::kPOff + Cfg::kPBytes);
-        const bool two = d.seg > 1;
         const float l0 = (red0[r] + red0[R + r]) + (red0[2 * R + r] + red0[3 * R + r]);
         const float l1 = two ? (red1[r] + red1[R + r]) + (red1[2 * R + r] + red1[3 * R + r]) : 0.f;
         const float m0 = no_ref(ref[r]) ? -INFINITY : -ref[r];
@@ -608,16 +605,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float f1 = m1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : fast_exp2(m1 - m);
         const float all = (f0 == 0.f ? 0.f : l0 * f0) + (f1 == 0.f ? 0.f : l1 * f1);
         const float inv = all == 0.f ? 0.f : 1.f / all;
-        ref[r] = all != all ? all : f0 * inv;
-        ref[R + r] = all != all ? all : f1 * inv;
-        if (d.part >= 0 && r < d.c0 * p.a.G)
-          p.a.part_lse[slot * R + r] = all == 0.f ? -INFINITY : all != all ? all : m + __log2f(all);
+        w0 = all != all ? all : f0 * inv;
+        w1 = all != all ? all : f1 * inv;
+        if (d.part >= 0 && warp == 4 && lane < rows)
+          p.a.part_lse[slot * R + lane] = all == 0.f ? -INFINITY : all != all ? all : m + __log2f(all);
       }
-      all_meet();
-      if (!ok) break;
-      if (key < D) {  // a group half of the rows, a thread a column of the output
-        const bool two = d.seg > 1;
-        const int rows = d.c0 * p.a.G, half = t * (R / 2);
+      if (quarter * 32 < D) {  // a group half of the rows, a thread a column of the output
+        const int half = t * (R / 2);
         int head = half % p.a.G;  // of the group
         uint16_t* out = p.a.out + (static_cast<long long>(d.tok0 + d.first + half / p.a.G) * p.a.Hq + d.h * p.a.G + head) * D + key;
         float* part = p.a.part_o + (slot * R + half) * D + key;
@@ -630,10 +624,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = r0 + i;
-            const float w0 = ref[r], w1 = ref[R + r];
+            const float u0 = __shfl_sync(0xffffffffu, w0, r), u1 = __shfl_sync(0xffffffffu, w1, r);
             const uint32_t av = r0 & 8 ? a[i + 8] : a[i], bv = r0 & 8 ? b[i + 8] : b[i];
-            float o = w0 == 0.f ? 0.f : __uint_as_float(av) * w0;
-            if (two && w1 != 0.f) o = fmaf(__uint_as_float(bv), w1, o);
+            float o = u0 == 0.f ? 0.f : __uint_as_float(av) * u0;
+            if (two && u1 != 0.f) o = fmaf(__uint_as_float(bv), u1, o);
             if (r < rows) {
               if (d.part >= 0) *part = o;
               else *out = float_to_bf16_bits(o);
@@ -650,6 +644,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       tc_fence_before();
       mbar_arrive(epi_done);  // O^T are read: they may be overwritten
       g += d.seg;
+      if (d.part >= 0) {
+        // The contributor that arrives last merges all partials, a warp a row (a kernel after this one for it cost
+        // a small call 4 us of 19).  The meeting orders every thread's stores before the counter's release.
+        all_meet();
+        if (!ok) break;
+        if (warp == 4 && lane == 0) {
+          int* counter = p.a.counters + d.pad[0];
+          const bool last = atom_add_acq_rel_gpu(counter, 1) == d.pad[1] - d.pad[0];
+          if (last) *counter = 0;  // every contributor has arrived: ready for the next call
+          *merge = last;
+        }
+        all_meet();
+        if (!ok) break;
+        if (*merge)
+          for (int n = warp - 4; n < rows; n += 8)
+            paged_merge<D, R>(p.a.part_o, p.a.part_lse, d.pad[0], d.pad[1], d.q, n, [&](int r) {
+              return p.a.out +
+                     (static_cast<long long>(d.tok0 + d.first + r / p.a.G) * p.a.Hq + d.h * p.a.G + r % p.a.G) * D;
+            });
+      }
     }
   }
   tc_fence_before();
@@ -659,21 +673,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kTmemCols);
   }
-}
-
-// Merges the units cut between CTAs, a warp a row: blockIdx.x is the CTA whose share the unit starts in.
-template <int D, int R>
-__global__ void __launch_bounds__(256) tree_few_combine_kernel(const PagedTreeParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const PagedCut c = p.cuts[blockIdx.x];
-  if (c.h < 0) return;
-  const int n = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int tok = c.tok0 + n / p.a.G;
-  if (tok >= c.tok1 || n >= p.a.tpb * p.a.G) return;
-  paged_merge<D, R>(p.a.part_o, p.a.part_lse, blockIdx.x, c.g_last, c.slot1, n, [&](int r) {
-    return p.a.out + (static_cast<long long>(c.tok0 + r / p.a.G) * p.a.Hq + c.h * p.a.G + r % p.a.G) * D;
-  });
 }
 
 }  // namespace mcb

@@ -723,6 +723,11 @@ at::Tensor paged_tree_attn(const at::Tensor& q, const at::Tensor& k_pages, const
       t.attn.workspace = ws.data_ptr();
       t.attn.workspace_bytes = bytes;
     }
+    const size_t counters = mcb_paged_tree_attn_counter_count(&t);
+    if (counters > 0) {
+      t.attn.counters = paged_counters(q, counters);
+      t.attn.counter_count = counters;
+    }
   }
   check_status(mcb_paged_tree_attn(&t, stream_of(q)), "mcb200::paged_tree_attn");
   return out;
