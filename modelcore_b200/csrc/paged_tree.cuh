@@ -184,10 +184,25 @@ __device__ __forceinline__ void tree_rows(const PagedTreeParams& p, int row_a, i
 struct TreeShare {
   long long total, t_begin, t_end;
   int ng;
+  int g_first, g_last;  // the one unit's contributors, where a CTA's share is one unit's (else g_last < 0)
 };
+// Who has the tiles of the unit that the walk is in, and whether the first one's partial is in its slot 1.
+__device__ __forceinline__ void tree_owners(const TreeShare& s, const TreeWalk& w, int& first, int& last, int& slot1) {
+  first = s.g_first, last = s.g_last, slot1 = 0;
+  if (s.g_last >= 0) return;
+  const long long start = w.t - w.local;
+  first = share_owner(start, s.total, s.ng);
+  last = share_owner(start + w.u.n - 1, s.total, s.ng);
+  slot1 = start != share_begin(first, s.total, s.ng);
+}
+// A unit's two ends -- its first maximum, masks, sums, way out -- cost a CTA what some three tiles do.  Where equal
+// numbers of CTAs a unit give no CTA more than that above an even share, no CTA has two units' ends: three requests of
+// 12 heads of 64 at 1,000 some 17 us for the slowest CTA, whose 2 tiles were two units', and 9 for the others.
+constexpr int kUnitEnds = 3;
 __device__ __forceinline__ TreeShare tree_share(long long total) {
   TreeShare s;
   s.total = total;
+  s.g_first = s.g_last = -1;
   s.ng = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
   const bool active = static_cast<int>(blockIdx.x) < s.ng;
   s.t_begin = active ? share_begin(blockIdx.x, total, s.ng) : 0;
@@ -200,20 +215,62 @@ __device__ __forceinline__ TreeShare tree_place(const PagedTreeParams& p, TreeWa
   if (p.a.R <= 32) {
     PagedRow x = {0, 0, 0};
     long long mine = 0;
+    int units = 0, longest = 0;  // (counts stop at 2^20: no more are shared out unit by unit)
     if (lane < p.a.R) {
       x = paged_row(p.a, lane);
       if (blockIdx.x == 0 && warp == 0 && !paged_row_fits(p.a, lane, x)) record_error(kErrPositionBeyondCache);
       const int nqb = tree_blocks(p, x);
-      for (int qb = 0; qb < nqb; ++qb) mine += tree_unit(p, x, lane, qb, nqb).n;
+      for (int qb = 0; qb < nqb; ++qb) {
+        const int n = tree_unit(p, x, lane, qb, nqb).n;
+        mine += n;
+        longest = max(longest, n);
+      }
       mine *= p.a.Hkv;
+      units = static_cast<int>(min(static_cast<long long>(nqb) * p.a.Hkv, 1ll << 20));
     }
     long long incl = mine;
+    int units_incl = units;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
       const long long o = __shfl_up_sync(0xffffffffu, incl, m);
-      if (lane >= m) incl += o;
+      const int u = __shfl_up_sync(0xffffffffu, units_incl, m);
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, m));
+      if (lane >= m) {
+        incl += o;
+        units_incl += u;
+      }
     }
-    s = tree_share(__shfl_sync(0xffffffffu, incl, 31));
+    const int all_units = __shfl_sync(0xffffffffu, units_incl, 31);
+    const int each = all_units > 0 ? static_cast<int>(gridDim.x) / all_units : 0;  // CTAs a unit
+    const long long total = __shfl_sync(0xffffffffu, incl, 31);
+    if (each > 0 && (longest + each - 1) / each <= total / static_cast<int>(gridDim.x) + kUnitEnds) {
+      s.total = total;
+      s.ng = all_units * each;
+      s.t_begin = s.t_end = 0;
+      s.g_first = blockIdx.x / each * each;
+      s.g_last = 0;
+      const int unit = blockIdx.x / each;
+      if (unit < all_units) {
+        const int r = __ffs(__ballot_sync(0xffffffffu, unit < units_incl)) - 1;
+        const int at = unit - __shfl_sync(0xffffffffu, units_incl - units, r);
+        x.tok0 = __shfl_sync(0xffffffffu, x.tok0, r);
+        x.T = __shfl_sync(0xffffffffu, x.T, r);
+        x.L = __shfl_sync(0xffffffffu, x.L, r);
+        w.u = tree_unit(p, x, r, at / p.a.Hkv, tree_blocks(p, x));
+        w.h = at % p.a.Hkv;
+        const int parts = min(each, w.u.n), part = static_cast<int>(blockIdx.x) - s.g_first;
+        s.g_last = s.g_first + parts - 1;
+        if (part < parts) {  // tiles counted from the unit's first
+          s.t_begin = static_cast<long long>(w.u.n) * part / parts;
+          s.t_end = static_cast<long long>(w.u.n) * (part + 1) / parts;
+        }
+      }
+      w.t = s.t_begin;
+      w.local = static_cast<int>(s.t_begin);
+      __syncthreads();
+      return s;
+    }
+    s = tree_share(total);
     w.t = s.t_begin;
     if (s.t_begin < s.t_end) {
       const int r = __ffs(__ballot_sync(0xffffffffu, s.t_begin < incl)) - 1;  // (t_begin < total: some lane's)
@@ -447,8 +504,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   TreeWalk w;
   const TreeShare share = tree_place(p, w, warp_tot, ctl);
   tc_fence_after();
-  const long long total = share.total, t_begin = share.t_begin, t_end = share.t_end;
-  const int ng = share.ng;
+  const long long t_begin = share.t_begin, t_end = share.t_end;
   const uint32_t tmem = *tmem_slot;
   const uint32_t base = smem_u32(smem);
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
@@ -524,13 +580,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             d.pad[0] = d.pad[1] = 0;
             segs[k & 3] = d;
             mbar_arrive(&seg_full[k & 3]);
-            const long long start = w.t - w.local;
             if (!whole && w.local == 0) {  // it starts here and ends in another CTA's share
               PagedCut c;
+              int first, slot1;
+              tree_owners(share, w, first, c.g_last, slot1);
               c.tok0 = d.tok0 + d.first;
               c.tok1 = c.tok0 + d.c0 + d.c1;
               c.h = w.h;
-              c.g_last = share_owner(start + w.u.n - 1, total, ng);
               c.slot1 = d.part;
               c.pad[0] = c.pad[1] = c.pad[2] = 0;
               p.cuts[blockIdx.x] = c;

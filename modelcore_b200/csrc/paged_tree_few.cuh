@@ -187,8 +187,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   TreeWalk w;
   const TreeShare share = tree_place(p, w, warp_tot, ctl);
   tc_fence_after();
-  const long long total = share.total, t_begin = share.t_begin, t_end = share.t_end;
-  const int ng = share.ng;
+  const long long t_begin = share.t_begin, t_end = share.t_end;
   const uint32_t tmem = *tmem_slot;
   const uint32_t base = smem_u32(smem);
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // warp-uniform
@@ -251,12 +250,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           d.part = whole ? -1 : k > 0 ? 1 : 0;
           d.last = w.t + seg >= t_end;
           d.q = d.pad[0] = d.pad[1] = 0;
-          if (!whole) {  // who has its tiles, and whether the first one's partial is in its slot 1
-            const long long start = w.t - w.local;
-            d.pad[0] = share_owner(start, total, ng);
-            d.pad[1] = share_owner(start + w.u.n - 1, total, ng);
-            d.q = start != share_begin(d.pad[0], total, ng);
-          }
+          if (!whole) tree_owners(share, w, d.pad[0], d.pad[1], d.q);
           segs[k & 3] = d;
           mbar_arrive(&seg_full[k & 3]);
           mbar_arrive_expect_tx(&q_full[k & 1], Cfg::kPanels * q_bytes);
