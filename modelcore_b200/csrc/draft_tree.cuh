@@ -8,7 +8,8 @@
 //
 // A request of more than 32 W tokens has no masks: it is a chunk of a prompt, its tokens follow each
 // other (position L + t).  A CTA of 32 W threads a request; a few KB to a few MB of integers: bound by the
-// launch and a chain of dependent loads (lengths, parents, a shared-memory round a doubling).
+// launch and a chain of dependent loads (lengths, parents, a shared-memory round a doubling): 64 trees of 16 7.3 us as
+// called, 1,000 of 200 beside chunks 11 us (7 MB, 1.1 us at HBM's rate).
 #pragma once
 
 #include "paged_plan.cuh"

@@ -13,13 +13,15 @@
 // changes), then the tables, the changes and the copies, then, in large pools, the freed pages of every 1,024
 // counted, then all placed.
 // All reads of what may be written in place come before the last.  The copies are bound by HBM (a page's
-// positions of one head are contiguous), all else by launches.
+// positions of one head are contiguous), all else by launches: 16 rows of 12 slots 17 us as called, a beam search's
+// step of 256 rows of 12 slots (105 MB) 30 us, 16 at HBM's rate.
 //
 // paged_keep: the tokens path_0 < path_1 < ... of a row's new ones are kept: position L + i of every slot
 // and head gets what L + path_i holds, the row is L + kept long, and the pages behind it that the step
 // took are free again.  path_i >= i, so moves in the order of i never overwrite one still to be read, and a
 // thread that carries 16 bytes of one head through all of a row's moves needs no other.  kept < 0: the whole step
-// as it is.
+// as it is.  8 requests of 12 slots 9.2 us as called, 128 of 24 slots (56 MB in rows of 256 bytes) 19 us, 8.6 at HBM's rate:
+// four dependent loads a CTA (lengths, path, table, rows).
 #pragma once
 
 #include "paged_plan.cuh"

@@ -1,10 +1,10 @@
-// paged_tree_attn for requests of few query rows a kv head (at most 64): the products with the keys on
+// paged_tree_attn for requests of few query rows a kv head (at most 32): the products with the keys on
 // the M side of the tensor cores, so that what they and the softmax cost goes with the rows there are.
 //
 //   S^T (128 keys x R rows) = K_j Q^T          M=128 N=R K=D     (both from shared memory)
 //   P^T                      = 2^(S^T scale - m)  a thread a key: R exponentials, stored for the next product
 //   O^T (D x R rows) += V_j^T P^T              M=128 N=R K=128   (both from shared memory)
-// with R = 16, 32 or 64 rows, token * G + head, of one *unit* (request, R / G tokens, kv head).  The tiles of
+// with R = 16 or 32 rows, token * G + head, of one *unit* (request, R / G tokens, kv head).  The tiles of
 // all units are one sequence that the CTAs share evenly, as in the kernel beside this one, whose walk, masks and
 // descriptions these are; a cut unit's last contributor merges it.  A tile of K and V, 64 KB at head size 128, has some 2,100 cycles at HBM's rate;
 // with the rows on the M side it took 1,280 of the tensor cores whatever the rows, and the exponentials of 16
@@ -18,6 +18,12 @@
 // threads hold a key each, so a maximum over keys is a reduction over the group (a butterfly that
 // leaves each lane one row), taken only then and in a part's first tile.  The group agrees on that in one
 // meeting a tile.  l is summed a thread a row and reduced over the keys at the end.
+//
+// Measured, back to back in a graph: 32 requests of 8,192 with 4 tokens of 16/4 heads of 128 (16 rows) 91 us, 5.9
+// TB/s; 32 of 4,096 with one token of 12/12 heads of 64 80 us, 5.0 TB/s, with 16 tokens 84 (the rows on the other
+// side of the products: 104 and 117).  3 requests of 8 tokens of 12/12 heads of 64 at 1,000: 15.2 us, latency: launch
+// and lengths 4, a tile's maximum and masks 4, sums and way out 3.  With 64 rows the registers for them spill or
+// the scores are read twice, and it is no faster than the other kernel (148 against 112 us at head size 64).
 #pragma once
 
 #include "paged_tree.cuh"
@@ -30,8 +36,8 @@ struct TreeFewConfig {
   static constexpr int kTileBytes = kPanels * kPtTile * 128;
   static constexpr int kQBytes = kPanels * R * 128;
   static constexpr int kPBytes = kPtTile * R * 2;
-  // what 226 KB hold beside two query tiles and two P^T: 5 tiles at head size 128 (6 below 64 rows), 11 or 12 at 64
-  static constexpr int kK = D == 128 ? (R == 64 ? 2 : 3) : 5, kV = D == 128 ? 3 : (R == 64 ? 6 : 7);
+  // what 226 KB hold beside two query tiles and two P^T: 6 tiles at head size 128, 12 at 64
+  static constexpr int kK = D == 128 ? 3 : 5, kV = D == 128 ? 3 : 7;
   static constexpr int kStages = kK + kV;
   static constexpr int kRingOff = 0;
   static constexpr int kQOff = kRingOff + kStages * kTileBytes;
@@ -48,10 +54,10 @@ struct TreeFewConfig {
   static constexpr uint32_t kTmemCols = 4 * R;
 };
 
-// Shared-memory descriptor of an MN-major tile of R values a row: the swizzle is as wide as the row.
+// Shared-memory descriptor of an MN-major tile of R values a row: the swizzle is as wide as the row (64 or 32 bytes).
 template <int R>
 __device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr) {
-  constexpr uint64_t mode = R == 64 ? 2 : R == 32 ? 4 : 6;
+  constexpr uint64_t mode = R == 32 ? 4 : 6;
   return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>((R * 16) >> 4) << 16) |
          (static_cast<uint64_t>((R * 16) >> 4) << 32) | (1ull << 46) | (mode << 61);
 }
@@ -93,8 +99,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 }
 template <int R>
 __device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[R]) {
-  if constexpr (R == 64) tmem_ld64(taddr, r);
-  else if constexpr (R == 32) tmem_ld32(taddr, r);
+  if constexpr (R == 32) tmem_ld32(taddr, r);
   else tmem_ld16(taddr, r);
 }
 
@@ -134,7 +139,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     paged_tree_few_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedTreeParams p) {
   using Cfg = TreeFewConfig<D, R>;
-  constexpr int SK = Cfg::kK, SV = Cfg::kV, ST = SK + SV, C = R < 32 ? R : 32;
+  constexpr int SK = Cfg::kK, SV = Cfg::kV, ST = SK + SV, C = R;  // C rows at a time
+  static_assert(R == 16 || R == 32, "a lane a row");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
