@@ -1,10 +1,10 @@
 """Speculative decoding over a paged KV cache: several samples of each prompt share the prompt's pages, and every
 step verifies a tree of drafted tokens a sample.
 
-    python examples/paged_speculative.py [--prompts 6] [--samples 4] [--tokens 60] [--temperature 0.7]
+    python examples/paged_speculative.py [--prompts 6] [--samples 4] [--tokens 60] [--temperature 0.1]
 
 The draft is the text itself: what followed the last tokens where they stood before, as a tree of the continuations
-found.  The model is paged_serving.py's small random-weight decoder.
+found.  The model is paged_serving.py's small random-weight decoder, whose text repeats itself at low temperatures.
 """
 import argparse
 import importlib.util
@@ -120,7 +120,7 @@ def main():
     ap.add_argument("--prompts", type=int, default=6)
     ap.add_argument("--samples", type=int, default=4)
     ap.add_argument("--tokens", type=int, default=60)
-    ap.add_argument("--temperature", type=float, default=0.7)
+    ap.add_argument("--temperature", type=float, default=0.1)
     args = ap.parse_args()
     rng = np.random.default_rng(1)
     model = SpeculativeDecoder()

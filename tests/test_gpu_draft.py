@@ -843,6 +843,51 @@ def test_fork_against_the_plain_one(ops, in_place, kind, name, slots, Hkv, D):
         assert np.array_equal(args["block_table"].cpu().numpy(), table) and args["shares"].tolist() == shares.tolist()
 
 
+def test_calls_without_requests_or_tokens(ops):
+    g = torch.Generator("cuda").manual_seed(1)
+    kp, vp = pools(g, 1, 40, 1, 16, 64)
+    none, state = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.tensor([7, 9], device="cuda")
+    queue = i32(range(40))
+    f = ops.page_fork(none, none, none.view(0, 2), torch.zeros_like(queue), queue, state, kp, vp)
+    assert f.free_state.tolist() == [7, 9] and f.shares.tolist() == [0] * 40 and queue.tolist() == list(range(40))
+    empty = torch.zeros(0, 50, device="cuda")
+    got = ops.verify_drafts(empty, none.long(), none, i32([0, 0, 0]), empty[:, 0], torch.zeros(2, device="cuda"), max_path=3)
+    assert got.accepted.tolist() == [0, 0] and got.next_token.tolist() == [-1, -1] and (got.path == -1).all()
+    got = ops.verify_drafts(empty, none.long(), none, i32([0]), empty[:, 0], empty[:, 0], max_path=3)
+    assert got.path.shape == (0, 3)
+    q = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    out = ops.paged_tree_attn(q + 1, kp[0], vp[0], none.view(0, 2), none, i32([0]), i32([0] * 3), i32([[1]] * 3))
+    assert not out.any()
+    out = ops.paged_tree_attn(q[:0], kp[0], vp[0], i32([[0]]), i32([5]), i32([0, 0]), none, none.view(0, 1))
+    assert out.shape == (0, 2, 64)
+
+
+def test_a_large_pool_is_counted_and_placed_by_blocks(ops):
+    """Above 32 blocks of 1,024 pages: freed pages in page order across them, the queue's ring included."""
+    rng = np.random.default_rng(3)
+    n, rows, page = 40000, 50, 16
+    order = rng.permutation(n)
+    table = np.full((rows, 500), -1)
+    lens = rng.integers(1, 500 * page, rows)
+    at = 0
+    for r in range(rows):
+        held = ceil_div(int(lens[r]), page)
+        table[r, :held] = order[at:at + held]
+        at += held
+    queue = np.full(n, -1)
+    head = n - 5
+    queue[(head + np.arange(n - at)) % n] = order[at:]
+    g = torch.Generator("cuda").manual_seed(1)
+    kp, vp = pools(g, 0, n, 1, page, 64)
+    source = [r if r % 3 else -1 for r in range(rows)]
+    want = fork_ref(source, lens.tolist(), table, np.zeros(n, int), queue, [head, head + n - at], (kp, vp), page)
+    q = i32(queue)
+    f = ops.page_fork(i32(source), i32(lens), i32(table), i32(np.zeros(n)), q, torch.tensor([head, head + n - at], device="cuda"),
+                      kp, vp)
+    assert q.tolist() == want[2].tolist() and f.free_state.tolist() == want[3]
+    assert np.array_equal(f.block_table.cpu().numpy(), want[0]) and not f.shares.any()
+
+
 def test_fork_step_after_step(ops):
     """Random steps on the same tables: every page is free or held, and shared by as many as its shares say."""
     rng = np.random.default_rng(0)
