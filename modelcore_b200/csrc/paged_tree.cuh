@@ -18,8 +18,8 @@
 //               and K tiles into a ring that runs on across units
 //   warp 3      the same walk, V tiles
 //   warps 1, 2  (warp 1 allocates TMEM) products of group 0, of group 1:
-//                 S_t = Q K_j^T   M=128 N=128 K=D   (both operands from shared memory)
-//                 O_t += P_t V_j  M=128 N=D K=128   (P from TMEM, over its S)
+//                 S_th = Q K_jh^T    M=128 N=64 K=D   (both operands from shared memory; h: half of a key tile)
+//                 O_t += P_th V_jh   M=128 N=D K=64   (P from TMEM, over its S)
 //   warps 4-7   softmax of group 0, warps 8-11 of group 1: a thread a query row
 // Two groups, each with its own S, running maximum, sum and accumulator, so that one group's products run
 // beside the other's softmax.  Where a unit has one query tile -- up to 128 rows, most trees -- the groups
@@ -27,9 +27,10 @@
 // unit's end; with two tiles each group has one and both read every key tile.
 // TMEM: S_0, S_1 of 128 columns, O_0, O_1 of D: all 512 at D = 128.
 //
-// The running maximum m moves only when a row's scores exceed it by 2^8 (P and l stay far below 2^127):
-// then the row's O, in TMEM, is rescaled, which no product can be at: a group's S is complete after its
-// P V before.  P is rounded to bf16 for the product; l sums the unrounded values.
+// A group's key tile goes half by half (64 keys), S -> softmax -> P V -> the next tile's S, so that the products of one half
+// run beside the softmax of the other.  The running maximum m moves only when a row's scores exceed it by 2^8 (P and l
+// stay far below 2^127): then the row's O, in TMEM, is rescaled, after the half's before P V, the one product that may
+// still be at it.  P is rounded to bf16 for the product; l sums the unrounded values.
 //
 // Masks: only the tiles with new tokens, at a window's start or at the unit's end look at them; a row's
 // 32 bits at a time are made from its interval of cached keys and its mask words, shifted to the
