@@ -192,8 +192,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   const int tok0 = min(max(p.cu[r], 0), p.N), count = min(max(p.cu[r + 1], tok0), p.N) - tok0;
   const int nw = C * kVerifyWarps, wi = rank * kVerifyWarps + warp;
   int phase = 0;
-  // A word of every CTA (the same in all its threads) to all of them: lane c gets CTA c's.
+  // A word of every CTA, its first thread's, to all of them: lane c gets CTA c's.  (A butterfly of fused products and
+  // sums leaves the lanes results that differ in their last bit; a cluster whose CTAs got a lane each would decide
+  // on different sums, and meet at different barriers.)
   auto exchange = [&](unsigned long long a) {
+    a = __shfl_sync(0xffffffffu, a, 0);
     if (warp == 0 && lane < C) st_dsmem_u64(map_to_rank(&s.xch[phase][rank], lane), a);
     cluster_sync();
     const unsigned long long got = s.xch[phase][lane & 7];

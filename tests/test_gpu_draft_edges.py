@@ -1,0 +1,42 @@
+"""Speculative decoding and shared pages where their parts meet: a cluster's blocks that decide alike, sums
+and comparisons at their bounds, extreme temperatures, many requests of many heads, steps that follow one
+another.  Plain forms and tolerances are test_gpu_draft's."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_draft import i32
+from test_gpu_draft import expects_device_error, no_device_error, ops  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------
+# verify_drafts
+@pytest.mark.parametrize("V,R", [(16384, 30), (9000, 60), (5000, 120), (40000, 18)])
+def test_comparisons_near_the_bound_of_the_32_bit_sums(ops, V, R):
+    """Chains whose tokens are all kept, by 1e-5 to 5e-5: what a comparison is short of lies around the distance at
+    which the row is summed again, now and then within an ulp of it.  Requests of 8, 4 and 2 blocks: all of a
+    request's take the second sum, or none does (a block alone in it would wait at another barrier)."""
+    T = 40
+    g = torch.Generator("cuda").manual_seed(V)
+    logits = torch.randn(R * T, V, device="cuda", generator=g) * 2
+    tokens = torch.randint(0, V, (R, T), device="cuda", generator=g)
+    x = tokens.roll(-1, 1).reshape(-1, 1)  # the token of the only child
+    logits.scatter_(1, x, -math.inf)
+    logits.scatter_(1, x, torch.logsumexp(logits, 1, keepdim=True) - 0.5)
+    p = torch.softmax(logits.double(), 1)
+    short = 1e-5 + 4e-5 * torch.rand(R * T, device="cuda", generator=g, dtype=torch.float64)
+    accept = torch.zeros(R * T, device="cuda")
+    accept.view(R, T)[:, 1:] = (p.gather(1, x)[:, 0] - short).float().view(R, T)[:, :-1]
+    draws = torch.rand(R, device="cuda", generator=g)
+    sums = p.view(R, T, V)[:, -1].cumsum(1)
+    want = (sums <= draws[:, None].double() * sums[:, -1:]).sum(1)
+    for _ in range(10):
+        got = ops.verify_drafts(logits, tokens.reshape(-1), i32([t - 1 for t in range(T)] * R), i32(np.arange(R + 1) * T),
+                                accept, draws, max_path=T)
+        assert got.accepted.tolist() == [T] * R and got.path.tolist() == [list(range(T))] * R
+        assert torch.equal(got.next_token, want)
+        accept.view(R, T)[:, 1:] += 2.0 ** -25  # (3e-8, ten times: far less than 1e-5)
