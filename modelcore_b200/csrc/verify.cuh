@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   uint32_t rank, C;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
+  cluster_arrive_relaxed();  // started: its shared memory may be written
   if (tid < 32) s.table[tid] = exp2(tid / 32.0);
   __syncthreads();
   pdl_wait();
@@ -221,6 +222,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     s.accept[i] = p.accept[tok0 + i];
   }
   __syncthreads();
+  cluster_wait();  // every block has started
   const float inv_t32 = p.temperature > 0.f ? 1.f / p.temperature : 1.f;
   const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 1.4426950408889634074;
   const float scale32 = inv_t32 * 1.4426950408889634f;

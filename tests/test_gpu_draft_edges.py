@@ -40,3 +40,22 @@ def test_comparisons_near_the_bound_of_the_32_bit_sums(ops, V, R):
         assert got.accepted.tolist() == [T] * R and got.path.tolist() == [list(range(T))] * R
         assert torch.equal(got.next_token, want)
         accept.view(R, T)[:, 1:] += 2.0 ** -25  # (3e-8, ten times: far less than 1e-5)
+
+
+def test_rows_of_unlike_length_back_to_back(ops):
+    """Requests with and without tokens, clusters that end at once beside ones that walk, launch after launch: a block's
+    shared memory is written by the others of its cluster once it has started, and as long as it is there."""
+    V = 16384  # 8 blocks of 2,048 tokens
+    g = torch.Generator("cuda").manual_seed(0)
+    fresh = [r % 4 for r in range(37)]
+    cu = np.concatenate([[0], np.cumsum(fresh)])
+    best = torch.randint(0, V, (int(cu[-1]),), device="cuda", generator=g)
+    logits = torch.zeros(len(best), V, device="cuda").scatter_(1, best[:, None], 60.0)  # (others: e^-60 each)
+    parents = i32(sum(([-1, 0, 0][:n] for n in fresh), []))
+    tokens = best.roll(1)  # the first child is kept
+    accept, draws = (torch.full((n,), 0.5, device="cuda") for n in (len(best), len(fresh)))
+    got = [ops.verify_drafts(logits, tokens, parents, i32(cu), accept, draws, max_path=2) for _ in range(200)]
+    last = [cu[r] + min(n, 2) - 1 for r, n in enumerate(fresh)]
+    for v in got:
+        assert v.accepted.tolist() == [min(n, 2) for n in fresh]
+        assert v.next_token.tolist() == [int(best[t]) if n else -1 for t, n in zip(last, fresh)]
