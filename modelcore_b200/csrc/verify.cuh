@@ -19,7 +19,7 @@
 // memory.  What is decided is what 64-bit sums decide, to their rounding: a vocabulary of 10^5 has borders
 // everywhere, and 32-bit sums put a draw on their wrong side now and then.
 //   A token's row is first summed in 32 bits (one pass, bound by its bytes), with a bound on how far off the
-//   sums can be; children are kept or refused by these while the sides of the comparison are further apart than
+//   sums can be (it grows with the tokens a lane adds up); children are kept or refused by these while the sides of the comparison are further apart than
 //   that, in nearly all cases.  Where they are not, and where the walk ends and a token is drawn, the row is
 //   summed again in 64 bits (bound by the 64-bit units: about 11 operations a token and pass).
 // Measured: 64 requests of 16 tokens, wide 3, 131,071 logits of fp32 and draft_probs 141 us (207 MB; the slowest
@@ -227,6 +227,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 1.4426950408889634074;
   const float scale32 = inv_t32 * 1.4426950408889634f;
   const bool greedy = p.temperature == 0.f;
+  // How far a 32-bit sum of weights may be off, relative to it, in e = 2^-24, with n groups of four a lane.  A weight
+  // 2^t: 5 e |t| ln 2 for the difference, the scale and their product, 4 e for the exponential; |t| in the mean over p
+  // is at most log2 V <= 30: 109 e.  A lane's sum: 3 e for a group's additions, 5 e where the maximum moves, at
+  // most with every group.  12 steps that join lanes, warps and blocks: 7 e each.  195 e + 8 n e; more of both for
+  // the products of these factors.  A rest's sum, of a p - b q, stays within that times b (>= a).
+  auto eps32 = [&] { return (224.f + 10.f * ((p.V + nw * 128 + 2) / (nw * 128))) * 0x1p-24f; };
   int node = 0, kept = 0;
   long long answer = -1;
   while (count > 0) {
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     };
 
     // ---- its children in turn ----
-    double off = 1e-5;  // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms
+    double off = eps32();  // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms
     int next = -1, last = node;
     for (int tries = 0; kept < p.max_path && tries < kVerifyMaxTried; ++tries) {
       // the next child (every warp looks for itself)
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const double mine = sum_lanes(__longlong_as_double(spread(__double_as_longlong(static_cast<double>(sum)))), kVerifyWarps);
         mass = sum_lanes(__longlong_as_double(exchange(__double_as_longlong(mine))), static_cast<int>(C));
-        off = 2.0 * off / before + 1e-5 * of_q;
+        off = 2.0 * off / before + eps32() * of_q;
         if (!(mass > 4.0 * off)) make_exact();  // nothing left, as far as 32 bits can tell
       } else {
         mass = sum64(false);

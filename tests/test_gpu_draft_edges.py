@@ -59,3 +59,46 @@ def test_rows_of_unlike_length_back_to_back(ops):
     for v in got:
         assert v.accepted.tolist() == [min(n, 2) for n in fresh]
         assert v.next_token.tolist() == [int(best[t]) if n else -1 for t, n in zip(last, fresh)]
+
+
+def adding(inc, n):
+    """n times inc added up in 32 bits."""
+    s, inc = np.float32(0), np.float32(inc)
+    for _ in range(n):
+        s += inc
+    return float(s)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_vocabulary_whose_32_bit_sums_are_far_off(ops, dtype):
+    """2^25 tokens and one block (more requests than half of a GPU's blocks, all but one without tokens): a lane adds
+    16,384 equal groups, one rounding after another the same way.  Token 7 has half of the probability; a uniform a
+    little above it refuses it, one a little below keeps it, at distances that 1e-5 would take for settled."""
+    V, x = 1 << 25, 7
+    if dtype == torch.float32:
+        tail = math.log(2.0 ** -25 * (1 + 0.75 * 2.0 ** -9))
+    else:
+        tail = -17.25  # (exact)
+    logits = torch.full((2, V), tail, device="cuda", dtype=dtype)
+    tail = float(logits[0, 0])
+    peak = 0.0 if dtype == torch.float32 else 0.125
+    logits[:, x] = peak
+    w = math.exp(tail - peak)
+    exact = 1 / (1 + (V - 1) * w)
+    in32 = 1 / (1 + 512 * adding(4 * np.float32(w), V // 2048))
+    if dtype == torch.float32:
+        assert abs(in32 - exact) > 5e-5  # (what the test is about: more than a bound of 1e-5 allows)
+    R = 300
+    cu = i32([0] + [2] * R)
+    tokens, parents, draws = torch.tensor([0, x], device="cuda"), i32([-1, 0]), torch.full((R,), 0.25, device="cuda")
+    for near in (1e-6, 1e-5, 2.5e-5, 4e-5, 1e-4, 1e-3):
+        for side in (-1, 1):
+            u = np.float32(exact + side * near)
+            got = ops.verify_drafts(logits, tokens, parents, cu, torch.full((2,), float(u), device="cuda"), draws, max_path=2)
+            assert got.accepted.tolist() == [2 if u < exact else 1] + [0] * (R - 1), (near, side)
+            # the draw at a quarter: of the whole row at token 1, of the row without x at token 0
+            if u < exact:
+                want = x if 7 * w <= 0.25 / exact < 7 * w + 1 else 0.25 / exact / w
+            else:
+                want = 0.25 * (V - 1) + 1
+            assert abs(int(got.next_token[0]) - want) <= 1
