@@ -579,7 +579,8 @@ int mcb_paged_tree_attn(const mcb_paged_tree_attn_args* args, void* stream);
  * tokens' places in the request, token 0 first, then -1; accepted: how many.  A walk ends after max_path
  * tokens, and at most 256 children of a token are tried.  A request without tokens: 0 and -1.  A
  * row of logits with a NaN, +infinity or nothing above -infinity: device error 9, and the walk ends
- * with next_token -1; a token outside [0, V): device error 4, not kept. */
+ * with next_token -1; a token outside [0, V): device error 4, not kept.  A uniform that is read and is NaN or below
+ * 0: device error 10, its token not kept, or next_token -1. */
 typedef struct {
   const void* logits;             /* (N, V) fp32 or bf16, rows logits_stride elements apart     */
   int64_t logits_stride;
@@ -669,7 +670,7 @@ int mcb_page_fork(const mcb_page_fork_args* args, void* stream);
  * timed out, 4 token id outside the embedding table, 5 the free pages do not match the request
  * (too few to take, or returned twice), 6 a page or slot outside the pool, 7 more new tokens than
  * the packed batch holds, 8 a drafted token's parent, a kept path or a fork's source out of its range, 9
- * logits without probabilities.
+ * logits without probabilities, 10 a uniform that is NaN or below 0.
  * ------------------------------------------------------------------------------------------- */
 int mcb_device_error(int32_t* code, void* stream);
 

@@ -39,6 +39,7 @@ DEVICE_ERRORS = {
     7: "more new tokens than the packed batch holds",
     8: "a drafted token's parent, a kept path or a fork's source out of its range",
     9: "logits without probabilities (NaN, +infinity or nothing above -infinity)",
+    10: "a uniform that is NaN or below 0",
 }
 
 ABI_VERSION = 9

@@ -23,6 +23,7 @@ enum DeviceError : int {
   kErrTooManyTokens = 7,
   kErrDraftOutOfRange = 8,
   kErrNoProbabilities = 9,
+  kErrUniformOutOfRange = 10,
 };
 // Defined once here: the library is a single translation unit (mcb200.cu).
 __device__ int g_device_error = 0;

@@ -451,8 +451,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         }
         continue;
       }
+      const float u = c < kVerifyMaxTried ? s.accept[c] : p.accept[tok0 + c];
+      if (!(u >= 0.f)) {
+        if (rank == 0 && tid == 0) record_error(kErrUniformOutOfRange);
+        continue;
+      }
       const float qx = q != nullptr ? q[x] : 1.f;
-      const double w = weight(logit_of(row + x)), bar = static_cast<double>(c < kVerifyMaxTried ? s.accept[c] : p.accept[tok0 + c]) * qx;
+      const double w = weight(logit_of(row + x)), bar = static_cast<double>(u) * qx;
       double have = rest_of(w, qx, static_cast<int>(x));
       if (!exact && !(fabs(bar * mass - have) > 2.0 * off)) {  // too close for 32 bits (or a NaN)
         make_exact();
@@ -508,6 +513,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     // ---- the walk ends here: draw ----
     if (greedy) {
       answer = rank == 0 ? best : -1;
+      break;
+    }
+    if (!(p.draws[r] >= 0.f)) {  // (no token's share begins below it)
+      if (rank == 0 && tid == 0) record_error(kErrUniformOutOfRange);
       break;
     }
     // The rest's parts in 64 bits, in any unit; without draft_probs, or with no child refused, from the weights alone.

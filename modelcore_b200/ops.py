@@ -814,7 +814,8 @@ def verify_drafts(logits, tokens, parents, cu_new, accept, draws, *, temperature
     choices (its largest, say), kept with the target's probability.  temperature == 0: the tokens that
     the greedy pick would give.  include/mcb200.h (mcb_verify_drafts) has the rule.  max_path: the width of
     the path, and the most tokens kept.  Device errors: 9 a row without probabilities (its request's
-    next_token is -1), 4 a token outside the vocabulary (not kept).  Returns a Verified."""
+    next_token is -1), 4 a token outside the vocabulary (not kept), 10 a uniform that is NaN or below 0 (its token
+    is not kept, or next_token is -1).  Returns a Verified."""
     if temperature < 0:
         raise RuntimeError("temperature must be non-negative")
     return Verified(*_PAGED.verify_drafts(logits, tokens, parents, cu_new, accept, draws, float(temperature), draft_probs,

@@ -102,3 +102,24 @@ def test_a_vocabulary_whose_32_bit_sums_are_far_off(ops, dtype):
             else:
                 want = 0.25 * (V - 1) + 1
             assert abs(int(got.next_token[0]) - want) <= 1
+
+
+@pytest.mark.parametrize("bad", [math.nan, -1e-3, -math.inf])
+@pytest.mark.parametrize("V", [50, 20000])
+def test_uniforms_that_are_none(ops, expects_device_error, bad, V):
+    """A draw that is NaN or below 0 gives no token, such an accept keeps none, and both are reported; the other requests
+    are as ever, and temperature 0 reads no uniforms."""
+    logits = torch.zeros(6, V, device="cuda")
+    logits[:, 3] = 60.0  # (the others: e^-60 each)
+    tokens, parents, cu = torch.tensor([0, 3] * 3, device="cuda"), i32([-1, 0] * 3), i32([0, 2, 4, 6])
+    fine, half = torch.full((6,), 0.5, device="cuda"), torch.full((3,), 0.5, device="cuda")
+    bent = torch.tensor([0.5, bad, 0.5], device="cuda")
+    for probs in (None, torch.softmax(logits, 1)):
+        got = ops.verify_drafts(logits, tokens, parents, cu, fine, bent, draft_probs=probs, max_path=2)
+        assert ops.device_error()[0] == 10
+        assert got.accepted.tolist() == [2, 2, 2] and got.next_token.tolist() == [3, -1, 3]
+        got = ops.verify_drafts(logits, tokens, parents, cu, bent.repeat_interleave(2), half, draft_probs=probs, max_path=2)
+        assert ops.device_error()[0] == 10
+        assert got.accepted.tolist() == [2, 1, 2] and got.next_token.tolist() == [3, 3, 3]
+    got = ops.verify_drafts(logits, tokens, parents, cu, fine * bad, half * bad, temperature=0, max_path=2)
+    assert ops.device_error()[0] == 0 and got.accepted.tolist() == [2, 2, 2] and got.next_token.tolist() == [3, 3, 3]
