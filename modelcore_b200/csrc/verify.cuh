@@ -229,10 +229,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   const bool greedy = p.temperature == 0.f;
   // How far a 32-bit sum of weights may be off, relative to it, in e = 2^-24, with n groups of four a lane.  A weight
   // 2^t: 5 e |t| ln 2 for the difference, the scale and their product, 4 e for the exponential; |t| in the mean over p
-  // is at most log2 V <= 30: 109 e.  A lane's sum: 3 e for a group's additions, 5 e where the maximum moves, at
-  // most with every group.  12 steps that join lanes, warps and blocks: 7 e each.  195 e + 8 n e; more of both for
-  // the products of these factors.  A rest's sum, of a p - b q, stays within that times b (>= a).
-  auto eps32 = [&] { return (224.f + 10.f * ((p.V + nw * 128 + 2) / (nw * 128))) * 0x1p-24f; };
+  // is at most log2 V.  A lane's sum: 3 e for a group's additions, 5 e where the maximum moves, at most with every
+  // group.  Lanes, warps and blocks joined: 5 e each for their maximum, 12 e of additions.  (33 + 3.5 log2 V + 8 n) e;
+  // 15 e and (8 n e)^2 for the products of these factors.  A rest's sum, of a p - b q, stays within that times b (>= a).
+  auto eps32 = [&] {
+    const float n = static_cast<float>((p.V + nw * 128 + 2) / (nw * 128));
+    return (48.f + 3.5f * (32 - __clz(p.V)) + (8.f + 0x1p-18f * n) * n) * 0x1p-24f;
+  };
   int node = 0, kept = 0;
   long long answer = -1;
   while (count > 0) {
@@ -293,13 +296,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       });
       if (odd) m = CUDART_INF_F;
       auto join = [&](int n) {  // over groups of n lanes
-        for (int o = n >> 1; o >= 1; o >>= 1) {
-          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
-          const float big = fmaxf(m, m2);
-          if (big > -CUDART_INF_F && big < CUDART_INF_F)
-            sum = sum * fast_exp2((m - big) * scale32) + sum2 * fast_exp2((m2 - big) * scale32);
-          m = big;
-        }
+        float big = m;
+        for (int o = n >> 1; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        if (big > -CUDART_INF_F && big < CUDART_INF_F) sum *= fast_exp2((m - big) * scale32);  // (once: each costs precision)
+        m = big;
+        for (int o = n >> 1; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       };
       auto word = [&] { return static_cast<unsigned long long>(__float_as_uint(m)) << 32 | __float_as_uint(sum); };
       auto unpack = [&](unsigned long long a) {
@@ -425,7 +426,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     };
 
     // ---- its children in turn ----
-    double off = eps32();  // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms
+    // how far the 32-bit sums of p, or of the rest, may be off, and any of their terms; and at most how far, relative to
+    // themselves, of_p and of_q, the factors of a child's 64-bit weight and q
+    double off = eps32();
     int next = -1, last = node;
     for (int tries = 0; kept < p.max_path && tries < kVerifyMaxTried; ++tries) {
       // the next child (every warp looks for itself)
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       const float qx = q != nullptr ? q[x] : 1.f;
       const double w = weight(logit_of(row + x)), bar = static_cast<double>(u) * qx;
       double have = rest_of(w, qx, static_cast<int>(x));
-      if (!exact && !(fabs(bar * mass - have) > 2.0 * off)) {  // too close for 32 bits (or a NaN)
+      if (!exact && !(fabs(bar * mass - have) > 2.0 * off * fmin(bar + w * of_p + qx * of_q, 1.0))) {  // too close (or a NaN)
         make_exact();
         have = rest_of(w, qx, static_cast<int>(x));
       }
