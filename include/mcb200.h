@@ -596,7 +596,7 @@ typedef struct {
   int64_t* next_token;            /* (R,)                                                       */
   int32_t R, N, V, max_path;
   int32_t logits_bf16;
-  float temperature;
+  float temperature;              /* 0, or from 1e-20 to 1e20                                   */
 } mcb_verify_drafts_args;
 
 int mcb_verify_drafts(const mcb_verify_drafts_args* args, void* stream);

@@ -217,6 +217,9 @@ int verify_drafts(const mcb_verify_drafts_args* a, void* stream) {
   if (a->V > 1 << 30) return fail(MCB_ERR_UNSUPPORTED, "%s: V %d (at most 2^30)", who, a->V);
   if (!(a->temperature >= 0.f) || a->temperature > 3e38f)
     return fail(MCB_ERR_INVALID_ARG, "%s: temperature %g must be finite and not negative", who, a->temperature);
+  // (outside, a logit of -infinity or 0 as the kernel widens it, 2^128 and 2^-127, would count beside the others)
+  if (a->temperature != 0.f && (a->temperature < 1e-20f || a->temperature > 1e20f))
+    return fail(MCB_ERR_UNSUPPORTED, "%s: temperature %g (0, or from 1e-20 to 1e20)", who, a->temperature);
   if (a->R == 0) return MCB_OK;
   if (a->cu_new == nullptr || a->draws == nullptr || a->accepted == nullptr || a->path == nullptr ||
       a->next_token == nullptr ||

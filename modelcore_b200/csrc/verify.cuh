@@ -25,7 +25,7 @@
 // Measured: 64 requests of 16 tokens, wide 3, 131,071 logits of fp32 and draft_probs 141 us (207 MB; the slowest
 // request's chain of passes, 4 CTAs: 8 us a row in 32 bits, 15 to 30 a pass in 64), 3 requests of 8 tokens and 32,768
 // logits 23 us, latency.
-// 2^t in 64 bits: t = n / 32 + f with |f| <= 1/64, a table of 2^(j/32) and five terms of 2^f's series in f ln 2
+// 2^t in 64 bits: 32 t = n + f with |f| <= 1/2, a table of 2^(j/32) and five terms of 2^(f/32)'s series in f ln 2 / 32
 // (the remainder, (ln 2 / 64)^6 / 720, is 2e-15): Tang's table-driven method, ACM TOMS 15, 1989.
 #pragma once
 
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   __syncthreads();
   cluster_wait();  // every block has started
   const float inv_t32 = p.temperature > 0.f ? 1.f / p.temperature : 1.f;
-  const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 1.4426950408889634074;
+  const double scale = (p.temperature > 0.f ? 1.0 / static_cast<double>(p.temperature) : 1.0) * 32.0 * 1.4426950408889634074;
   const float scale32 = inv_t32 * 1.4426950408889634f;
   const bool greedy = p.temperature == 0.f;
   // How far a 32-bit sum of weights may be off, relative to it, in e = 2^-24, with n groups of four a lane.  A weight
@@ -325,20 +325,20 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     // ---- the same in 64 bits ----
     const double top64 = top;
     auto weight = [&](float x) -> double {
-      const double t = fma(double_of(x), scale, -top64 * scale);  // <= 0, to rounding
-      constexpr double magic = 6755399441055744.0;                // 1.5 * 2^52
-      const double kd = fma(t, 32.0, magic);
+      const double d = double_of(x) - top64;        // (first: with a small temperature's scale neither is exact)
+      constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52
+      const double kd = fma(d, scale, magic);       // 32 t = n + f
       const int n = __double2loint(kd);
-      const double f = fma(kd - magic, -0.03125, t);
-      double e = 1.3333558146428443e-3;                           // ln 2^k / k!, k = 5 .. 1
-      e = fma(e, f, 9.6181291076284772e-3);
-      e = fma(e, f, 5.5504108664821580e-2);
-      e = fma(e, f, 2.4022650695910071e-1);
-      e = fma(e, f, 6.9314718055994531e-1);
+      const double f = fma(d, scale, magic - kd);
+      double e = 0x1p-25 * 1.3333558146428443e-3;   // (ln 2 / 32)^k / k!, k = 5 .. 1
+      e = fma(e, f, 0x1p-20 * 9.6181291076284772e-3);
+      e = fma(e, f, 0x1p-15 * 5.5504108664821580e-2);
+      e = fma(e, f, 0x1p-10 * 2.4022650695910071e-1);
+      e = fma(e, f, 0x1p-5 * 6.9314718055994531e-1);
       const double tab = s.table[n & 31];
       const double w = fma(tab * f, e, tab);
       // times 2^(n / 32); below 2^-1000 nothing (a logit of -infinity among them)
-      return t > -1000.0 ? __hiloint2double(__double2hiint(w) + ((n >> 5) << 20), __double2loint(w)) : 0.0;
+      return kd > magic - 32000.0 ? __hiloint2double(__double2hiint(w) + ((n >> 5) << 20), __double2loint(w)) : 0.0;
     };
     int tried = 0;                  // without draft: refused so far, of those that the rest is without
     bool exact = false;             // mass and the factors come of 64-bit sums

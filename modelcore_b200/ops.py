@@ -811,8 +811,8 @@ def verify_drafts(logits, tokens, parents, cu_new, accept, draws, *, temperature
     parents (N,) int32 as draft_tree takes them -- a request's first token is part of its answer already,
     the others were drafted.  accept (N,) and draws (R,) fp32: uniforms in [0, 1).  draft_probs (N, V) fp32: row u
     is the distribution that u's children were drawn from, each for itself; None: they are the draft's
-    choices (its largest, say), kept with the target's probability.  temperature == 0: the tokens that
-    the greedy pick would give.  include/mcb200.h (mcb_verify_drafts) has the rule.  max_path: the width of
+    choices (its largest, say), kept with the target's probability.  temperature: from 1e-20 to 1e20, or 0, the tokens
+    that the greedy pick would give.  include/mcb200.h (mcb_verify_drafts) has the rule.  max_path: the width of
     the path, and the most tokens kept.  Device errors: 9 a row without probabilities (its request's
     next_token is -1), 4 a token outside the vocabulary (not kept), 10 a uniform that is NaN or below 0 (its token
     is not kept, or next_token is -1).  Returns a Verified."""

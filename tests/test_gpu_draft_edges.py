@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_draft import i32
+from test_gpu_draft import check_verify, i32, verify_case
 from test_gpu_draft import expects_device_error, no_device_error, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +123,20 @@ def test_uniforms_that_are_none(ops, expects_device_error, bad, V):
         assert got.accepted.tolist() == [2, 1, 2] and got.next_token.tolist() == [3, 3, 3]
     got = ops.verify_drafts(logits, tokens, parents, cu, fine * bad, half * bad, temperature=0, max_path=2)
     assert ops.device_error()[0] == 0 and got.accepted.tolist() == [2, 2, 2] and got.next_token.tolist() == [3, 3, 3]
+
+
+@pytest.mark.parametrize("temperature", [1e-20, 1e-15, 1e-10, 1e-6, 1e20])
+@pytest.mark.parametrize("draft", [0.0, 0.3])
+def test_extreme_temperatures(ops, temperature, draft):
+    """Almost greedy and almost flat, among ties of the largest logit, logits of hundreds and of -infinity."""
+    rng = np.random.default_rng(3)
+    c = verify_case(rng, [1, 9, 0, 30, 12], 3001, draft, kind="chain")
+    logits = (c["logits"] * 40).round()  # (whole numbers: equal ones are equal)
+    logits[:, ::7] = -math.inf
+    logits[:, [0, 70]] = 0.0
+    rows, top = torch.arange(len(logits)), torch.tensor(c["tokens"]).roll(-1)
+    logits[rows, top] = logits.amax(1)  # a drafted token shares the first place
+    c["logits"] = logits
+    for scale in (0.3, 1.0):
+        c["accept"] = (rng.random(len(logits)) * scale).astype(np.float32)
+        check_verify(ops, c, temperature)
