@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // again when all have passed the next meeting, so have read it.)
     auto group_any = [&](bool v) {
       const bool any = __any_sync(0xffffffffu, v);
+      __syncwarp();  // (a vote orders no memory: lane 0's arrival is to release all lanes' stores)
       if (lane == 0) {
         votes[(met & 1) * 4 + quarter] = any;
         mbar_arrive(&meet[t]);

@@ -7,10 +7,39 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_draft import check_verify, i32, verify_case
+from test_gpu_draft import U, attn_case, attn_ref, check_verify, i32, random_parents, verify_case
 from test_gpu_draft import expects_device_error, no_device_error, ops  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------
+# paged_tree_attn
+@pytest.mark.parametrize("Hq,Hkv,D,fresh", [(8, 2, 128, 4), (8, 1, 64, 2), (16, 4, 128, 8), (4, 1, 64, 7)])
+def test_maxima_at_every_place_of_a_tile(ops, Hq, Hkv, D, fresh):
+    """Few rows a kv head, tile after tile of 128 keys whose maximum is 40 above the tile's before, at another key for each
+    of 128 requests: every thread's maximum, reference and sum in turn is the one that counts, for rows that
+    see it rise, fall or not at all.  Tolerance as for scores that leap by hundreds (test_gpu_draft)."""
+    R, cached, scale = 128, 640, 8.0
+    c = attn_case([cached] * R, [fresh] * R, [random_parents(None, fresh, "chain")] * R, Hq, Hkv, D, 64, 32, seed=5)
+    key = torch.arange(cached + fresh, device="cuda")
+    at = key.new_tensor([[t * 128 + (r * 37 + t * 11) % 128 for t in range(5)] for r in range(R)])
+    q = c["q"].contiguous().mul(0.25)
+    q[:-2, :, 0] = (torch.arange(R * fresh, device="cuda") % 3 - 1).to(torch.bfloat16)[:, None]
+    c["q"] = q
+    for r in range(R):
+        c["ks"][r][..., 0] = 0
+        c["ks"][r][at[r], :, 0] = (40.0 * torch.arange(1, 6, device="cuda")).to(torch.bfloat16)[:, None]
+        c["kp"][c["table"][r].long()[key // 64], :, key % 64] = c["ks"][r]
+    want, bound = attn_ref(c, [cached] * R, [fresh] * R, -1, scale)
+    call = lambda: ops.paged_tree_attn(q, c["kp"], c["vp"], c["table"], c["cached"], c["cu"], c["pos"], c["mask"],
+                                       softmax_scale=scale, max_new=fresh)
+    got = call()
+    err = (got[:-2].double() - want).abs()
+    # scores up to 8 * 200 and some tens: 1,700 2^-20 of a weight
+    slack = (2.25 * U + 8.0 * 1700 * 2.0 ** -20) * bound
+    assert err.isfinite().all() and (err <= slack).all(), (err - slack).max()
+    assert all(torch.equal(call(), got) for _ in range(20))
 
 
 # ---------------------------------------------------------------------------------------------
