@@ -608,7 +608,7 @@ int mcb_verify_drafts(const mcb_verify_drafts_args* args, void* stream);
  * accepted[r] < 0: the request's whole step is kept as it is (a prompt's chunk); its path is not read.
  * free_state_out may be free_state, seqlens_out cache_seqlens.  accepted above new_lens or P, or a path
  * entry below its place or past new_lens, sets device error 8: the former counts as the limit, the latter is not
- * moved.  Device errors 1, 5 and 6 as in mcb_page_release. */
+ * moved.  Device errors 1, 5 and 6 as in mcb_page_release.  R is at most 65,534. */
 typedef struct {
   const int32_t* path;            /* (R, P), rows path_stride apart                             */
   int64_t path_stride;

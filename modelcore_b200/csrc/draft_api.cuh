@@ -328,10 +328,9 @@ int paged_keep(const mcb_paged_keep_args* a, void* stream) {
   p.in_place = a->seqlens_out == a->cache_seqlens;
   const long long columns = 2ll * a->slots * a->Hkv * (a->D / 8);
   const long long ctas = (columns + mcb::kKeepThreads - 1) / mcb::kKeepThreads;
-  // (the arrival counter of the last CTA counts to 2^16)
-  if (ctas * (a->R + 1ll) >= 1 << 16)
-    return fail(MCB_ERR_UNSUPPORTED, "%s: %lld blocks of %d requests' heads in one call (at most 65,535)", who,
-                ctas * a->R, a->R);
+  if (ctas * (a->R + 1ll) > INT32_MAX)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: slots %d * Hkv %d * D %d of %d requests above 2^41", who, a->slots, a->Hkv, a->D,
+                a->R);
   cudaError_t e = launch_pdl(mcb::paged_keep_kernel,
                              dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.in_place ? std::max(a->R, 1) : a->R + 1)),
                              dim3(mcb::kKeepThreads), 0, static_cast<cudaStream_t>(stream), p);

@@ -378,8 +378,7 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedKee
     }
     __syncthreads();
   }
-  bool unused = false;
-  if (p.in_place && last_cta(p.counter, unused)) keep_books(p, warp_sums);
+  if (p.in_place && last_cta(p.counter)) keep_books(p, warp_sums);
 }
 
 }  // namespace mcb

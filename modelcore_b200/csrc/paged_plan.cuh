@@ -62,12 +62,24 @@ __device__ __forceinline__ bool last_cta(int* counter, bool& flag) {
   const int mine = __syncthreads_or(flag) ? kFlag + 1 : 1;
   if (threadIdx.x == 0) {
     const int all = atom_add_acq_rel_gpu(counter, mine) + mine;
-    s_last = (all & (kFlag - 1)) == static_cast<int>(gridDim.x * gridDim.y) ? (all >= kFlag ? 3 : 1) : 0;
+    s_last = (all & (kFlag - 1)) == static_cast<int>(gridDim.x) ? (all >= kFlag ? 3 : 1) : 0;
     if (s_last) *counter = 0;
   }
   __syncthreads();
   flag = (s_last & 2) != 0;
   return s_last != 0;
+}
+
+// The same without a flag, of two dimensions and up to 2^31 - 1 CTAs.
+__device__ __forceinline__ bool last_cta(int* counter) {
+  __shared__ bool s_last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_last = atom_add_acq_rel_gpu(counter, 1) + 1 == static_cast<int>(gridDim.x * gridDim.y);
+    if (s_last) *counter = 0;
+  }
+  __syncthreads();
+  return s_last;
 }
 
 // Counts of tokens and pages stop at 2^31, above every N and n_pages: lengths may be anything, and the

@@ -830,7 +830,7 @@ def paged_keep(path, accepted, cache_seqlens, new_lens, block_table, free_pages,
     that only the step's other tokens needed (new_lens (R,) as given to page_plan) go back to the queue's tail
     in request order.  accepted[r] < 0: the whole step of that request is kept as it is (a prompt's chunk beside
     the trees).  Returns (free_state, seqlens) after it: new tensors, or free_state_out / seqlens_out, which
-    may be the inputs.  Device errors as page_release's, and 8 for a path that does not
+    may be the inputs.  At most 65,534 requests.  Device errors as page_release's, and 8 for a path that does not
     fit its request."""
     if free_state_out is None:
         free_state_out = torch.empty_like(free_state)

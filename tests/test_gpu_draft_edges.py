@@ -169,3 +169,38 @@ def test_extreme_temperatures(ops, temperature, draft):
     for scale in (0.3, 1.0):
         c["accept"] = (rng.random(len(logits)) * scale).astype(np.float32)
         check_verify(ops, c, temperature)
+
+
+# ---------------------------------------------------------------------------------------------
+# paged_keep
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("R,slots,Hkv,D", [(520, 32, 32, 128), (1100, 80, 8, 128), (3000, 12, 12, 64)])
+def test_keep_of_many_requests_of_many_heads(ops, in_place, R, slots, Hkv, D):
+    """More blocks than 2^16 (but for the last): every slot's and head's move, the lengths and
+    the counter, twice."""
+    page, g = 16, torch.Generator("cuda").manual_seed(R)
+    kp, vp = (torch.zeros(slots, R + 1, Hkv, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table = torch.randperm(R, device="cuda", generator=g).to(torch.int32).view(R, 1)
+    new, cached = torch.full((R,), 6, device="cuda", dtype=torch.int32), torch.full((R,), 3, device="cuda", dtype=torch.int32)
+    path, kept = i32([[0, 2, 5]] * R), i32([3, 2, 1, 0] * (R // 4))
+    queue, state = torch.full((R + 1,), R, device="cuda", dtype=torch.int32), torch.tensor([0, 1], device="cuda")
+    lens = cached.clone()
+    for turn in range(2):
+        want = []
+        for pool in (kp, vp):
+            pool[:, :, :, 3 + 2 * turn:9 + 2 * turn] = torch.randn(Hkv, 6, D, device="cuda", dtype=torch.bfloat16, generator=g)
+            pool[:, :, :, 3 + 2 * turn:9 + 2 * turn] += torch.arange(R + 1, device="cuda").view(1, -1, 1, 1, 1) % 7
+        cached = lens.clone() if turn == 0 else torch.full_like(lens, 5)
+        start = cached.clone()
+        before = [pool.clone() for pool in (kp, vp)]
+        out = dict(free_state_out=state, seqlens_out=cached) if in_place else {}
+        state, lens = ops.paged_keep(path, kept, cached, new, table, queue, state, kp, vp, **out)
+        assert torch.equal(lens, start + kept) and state.tolist() == [0, 1]
+        at = int(start[0])
+        rows = table[:, 0].long()
+        for pool, old in zip((kp, vp), before):
+            for i, src in ((1, 2), (2, 5)):
+                moves = rows[kept > i]
+                old[:, moves, :, at + i] = old[:, moves, :, at + src]
+            assert torch.equal(pool, old)
+        del before
