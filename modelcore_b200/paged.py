@@ -15,7 +15,7 @@ finished request's pages serve the next:
     cache.advance(step)
     cache.release([2])                                # row 2 is done: its pages are free
 
-Of drafted tokens that were verified in one step, advance(step, kept=[2, 0, 1, 4]) keeps the accepted ones.
+Of chains of drafted tokens that were verified in one step, advance(step, kept=[2, 0, 1, 4]) keeps the accepted ones.
 Drafted tokens may be trees: plan(new_lens, parents=parents) gives a step whose tokens see their ancestors
 alone, and keep(step, path, accepted) what ops.verify_drafts says of them.  fork(source) makes rows copies of
 rows -- samples of one prompt, beams -- that share the pages that are full.
@@ -185,13 +185,17 @@ class PagedKVCache:
     def advance(self, step, kept=None):
         """The step's new tokens become part of their rows, and its pages theirs.  kept: how many of its new
         tokens each row keeps, the first ones (a list as plan's; drafted tokens that verification
-        rejects are not kept); the pages that only the others needed are free again."""
+        rejects are not kept); the pages that only the others needed are free again.
+        Tokens of a tree that do not follow one another where they lie are refused: keep moves a path
+        together.  (Of a step of trees this reads the positions from the GPU.)"""
         self._current(step)
         if kept is not None:
             kept = self._rows(kept)
             if (kept > step.host_lens).any():
                 row = int((kept - step.host_lens).argmax())
                 raise RuntimeError(f"row {row} has {step.host_lens[row]} new tokens in the step, not {kept[row]} to keep")
+        if step.tree is not None:
+            self._check_chain(step, step.host_lens if kept is None else kept)
         self._step = None
         self.cache_seqlens.add_(step.new_lens)
         self.free_state = step.plan.free_state
@@ -203,11 +207,20 @@ class PagedKVCache:
         if fewer.any():
             self._release(fewer, self._to_device(self._host_lens))
 
+    def _check_chain(self, step, kept):
+        # a token as deep as its place is, and all before it, is the end of a chain
+        bent = (step.tree.positions != step.plan.positions).cpu().numpy()
+        first = np.cumsum(step.host_lens) - step.host_lens
+        for row in np.nonzero(kept)[0]:
+            if bent[first[row]:first[row] + kept[row]].any():
+                raise RuntimeError(f"the {kept[row]} new tokens of row {row} are a tree and no chain: keep(step, path, "
+                                   "accepted) moves a path of it together")
+
     def keep(self, step, path, accepted):
         """advance for a step of trees: each row keeps the path that ops.verify_drafts gives for it (path
         (max_rows, P) and accepted (max_rows,) int32 on the GPU; accepted < 0: the row's new tokens all, as they
-        are), moved together in every slot, and the pages that only its other tokens needed are free again.
-        Reads accepted from the GPU, and returns how many tokens each row has kept."""
+        lie, for chunks of prompts and chains), moved together in every slot, and the pages that only its other
+        tokens needed are free again.  Reads accepted from the GPU, and returns how many tokens each row has kept."""
         self._current(step)
         if accepted.numel() != self.max_rows or path.shape[0] != self.max_rows:
             raise RuntimeError(f"path and accepted must have a row for each of {self.max_rows}, got "

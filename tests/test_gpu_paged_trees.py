@@ -1,0 +1,35 @@
+"""PagedKVCache's steps of trees against calls that do not fit them."""
+import pytest
+import torch
+
+from test_gpu_speculative import check, make, put, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+def test_advance_takes_chains_and_refuses_trees():
+    """advance leaves keys where they lie: row 0 has a chunk, row 1 a chain, row 2 a chain that branches at its third
+    token, row 3 two roots."""
+    g = torch.Generator("cuda").manual_seed(0)
+    parents = [t - 1 for t in range(70)] + [-1, 0, 1, 2] + [-1, 0, 0, 1] + [-1, -1]
+    new = [70, 4, 4, 2]
+    for as_list in (True, False):
+        cache = make()
+        cache.advance(cache.plan([3, 20, 0, 17]))
+        given = parents if as_list else torch.tensor(parents, dtype=torch.int32, device="cuda")
+        step = cache.plan(new, parents=given, max_tree=32)
+        put(cache, step, g)
+        for kept, row in ((None, 2), ([70, 4, 3, 1], 2), ([0, 0, 0, 2], 3), ([70, 4, 4, 0], 2)):
+            with pytest.raises(RuntimeError, match=f"of row {row} are a tree"):
+                cache.advance(step, kept=kept)
+        before = [x.clone() for x in rows_of(cache)]
+        cache.advance(step, kept=[70, 3, 2, 1])  # (the refusals have left the step)
+        check(cache)
+        assert cache.host_lens().tolist() == [73, 23, 2, 18, 0, 0]
+        for old, now in zip(before, rows_of(cache)):
+            assert torch.equal(now[:len(old)], old)
+    cache = make()
+    step = cache.plan([5, 40], parents=[t - 1 for t in range(5)] + [t - 1 for t in range(40)], max_tree=32)
+    cache.advance(step)
+    check(cache)
+    assert cache.host_lens().tolist() == [5, 40, 0, 0, 0, 0]
