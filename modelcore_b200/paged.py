@@ -150,6 +150,7 @@ class PagedKVCache:
                 raise RuntimeError(f"parents must name one for each of {num_tokens} tokens, got {tuple(parents.shape)}")
             max_tree = min(256, max(1, int(new.max(initial=0)))) if max_tree is None else int(max_tree)
         lens = self._to_device(new)
+        self._step = None  # from here on the table has this step's pages, also where draft_tree refuses its parents
         p = ops.page_plan(self.cache_seqlens, lens, self.block_table, self.free_pages, self.free_state,
                           page_size=self.page_size, num_tokens=num_tokens)
         tree = None if parents is None else ops.draft_tree(parents, p.cu_new, self.cache_seqlens, max_tree=max_tree)

@@ -33,3 +33,20 @@ def test_advance_takes_chains_and_refuses_trees():
     cache.advance(step)
     check(cache)
     assert cache.host_lens().tolist() == [5, 40, 0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("bad", [dict(max_tree=0), dict(max_tree=257), dict(dtype=torch.int64), dict(device="cpu")])
+def test_a_refused_plan_of_trees_drops_the_step_before(bad):
+    """Row 1's pages of the step before are in the table as another row's by the time the parents are refused."""
+    cache = make()
+    cache.advance(cache.plan([5, 5]))
+    step = cache.plan([0, 40])
+    max_tree = bad.get("max_tree", 32)
+    parents = torch.full((40,), -1, dtype=bad.get("dtype", torch.int32), device=bad.get("device", "cuda"))
+    with pytest.raises(RuntimeError):
+        cache.plan([20, 20], parents=parents, max_tree=max_tree)
+    with pytest.raises(RuntimeError, match="not the planned one"):
+        cache.advance(step)
+    check(cache)
+    cache.advance(cache.plan([20, 20]))
+    check(cache)
