@@ -52,6 +52,16 @@ class PagedStep(NamedTuple):
         return np.cumsum(self.host_lens)[rows] - 1, rows
 
 
+class _SharedRun(NamedTuple):
+    """Pages that a fork found full, after those that earlier forks had."""
+    before: Optional["_SharedRun"]
+    pages: int
+    total: int                 # with all before
+
+
+_NO_RUN = _SharedRun(None, 0, 0)
+
+
 class PagedKVCache:
     """k_pages / v_pages: (n_slots, n_pages, n_kv_head, page_size, head_dim) bf16, a head's page one
     contiguous block.  Rows are requests: block_table (max_rows, max_pages) and cache_seqlens
@@ -84,10 +94,9 @@ class PagedKVCache:
         self.page_shares = torch.zeros(n_pages, **ints)  # the rows that hold a page, less one
         self._host_lens = np.zeros(max_rows, dtype=np.int64)
         self._step = None  # the planned step that advance has not followed yet
-        # a row's first pages that were full when it was last forked or forked from, by numbers of the host's own:
-        # equal numbers are one page
-        self._shared = [[] for _ in range(max_rows)]
-        self._page_numbers = 0
+        # a row's first pages that were full when it was last forked or forked from: equal runs are the same pages
+        self._shared = [_NO_RUN] * max_rows
+        self._shared_pages = 0  # _shared_count() after the last fork
 
     def _held(self, lens):
         return -(-lens // self.page_size)
@@ -102,12 +111,18 @@ class PagedKVCache:
 
     def free_page_count(self):
         """Pages that no row holds (no device read)."""
-        return int(self.n_pages - self._held(self._host_lens).sum()) + self._shared_count()
+        return int(self.n_pages - self._held(self._host_lens).sum()) + self._shared_pages
 
     def _shared_count(self):
         """Pages that rows would hold besides if none were shared."""
-        numbers = [x for pages in self._shared for x in pages]
-        return len(numbers) - len(set(numbers))
+        count, seen = 0, set()
+        for run in self._shared:
+            count += run.total
+            while run.before is not None and id(run) not in seen:
+                seen.add(id(run))
+                count -= run.pages
+                run = run.before
+        return count
 
     def pages_needed(self, new_lens):
         """Pages a step of these new tokens a row would take from the free ones."""
@@ -254,10 +269,11 @@ class PagedKVCache:
                       self.free_state, self.k_pages, self.v_pages, block_table_out=self.block_table,
                       shares_out=self.page_shares, free_state_out=self.free_state, seqlens_out=self.cache_seqlens)
         for r in np.nonzero(heirs > 1)[0]:
-            fresh = int(self._host_lens[r] // self.page_size) - len(self._shared[r])
-            self._shared[r] = self._shared[r] + list(range(self._page_numbers, self._page_numbers + fresh))
-            self._page_numbers += fresh
-        self._shared = [list(self._shared[s]) if s >= 0 else [] for s in source]
+            full = int(self._host_lens[r] // self.page_size)
+            if full > self._shared[r].total:
+                self._shared[r] = _SharedRun(self._shared[r], full - self._shared[r].total, full)
+        self._shared = [self._shared[s] if s >= 0 else _NO_RUN for s in source]
+        self._shared_pages = self._shared_count()
         self._host_lens = np.where(source >= 0, self._host_lens[source], 0)
 
     def release(self, rows):
@@ -266,7 +282,7 @@ class PagedKVCache:
         dropped; any other stays the current one."""
         done = np.zeros(self.max_rows, dtype=bool)
         done[np.asarray(rows, dtype=np.int64)] = True
-        if any(self._shared[r] for r in np.nonzero(done)[0]):
+        if any(self._shared[r].total for r in np.nonzero(done)[0]):
             self.fork(np.where(done, -1, np.arange(self.max_rows)))
             return
         if self._step is not None and self._step.host_lens[done].any():

@@ -50,3 +50,25 @@ def test_a_refused_plan_of_trees_drops_the_step_before(bad):
     check(cache)
     cache.advance(cache.plan([20, 20]))
     check(cache)
+
+
+def test_pages_shared_by_many_are_counted_when_they_change(monkeypatch):
+    """16 samples each of two prompts of 40 pages that go on to share more, part by part; a plan and a count of free pages
+    walk nothing that grows with the pages."""
+    cache = make(n_pages=600, rows=32, max_len=1200, slots=1)
+    cache.advance(cache.plan([645] + [0] * 15 + [640]))
+    cache.fork([0] * 16 + [16] * 16)
+    check(cache)
+    cache.advance(cache.plan([30] * 32))
+    cache.fork([0] * 8 + [1] * 8 + [17] * 16)
+    check(cache)
+    cache.advance(cache.plan([1, 40] * 16))
+    cache.fork([-1, 1] * 8 + list(range(16, 32)))
+    check(cache)
+    cache.release([3, 17])
+    check(cache)
+    monkeypatch.setattr(cache, "_shared_count", lambda: pytest.fail("counted again"))
+    free = cache.free_page_count()
+    cache.advance(cache.plan([16] * 32))
+    assert cache.free_page_count() == free - 32
+    check(cache)
