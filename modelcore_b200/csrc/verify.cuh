@@ -75,6 +75,7 @@ struct VerifyShared {
   double table[32];                  // 2^(j / 32)
   double warp_sum[kVerifyWarps];     // this CTA's warps' 64-bit sums of the last pass
   unsigned long long warp_word[kVerifyWarps];
+  double inv[kVerifyMaxTried];       // with draft: 1 / the rest's sum before each refused child, the first's 1 / all
   int gone[kVerifyMaxTried];         // without draft: the refused children's tokens
   int parent[kVerifyMaxTried], token[kVerifyMaxTried];  // the request's first tokens' (those behind are read)
   float accept[kVerifyMaxTried];
@@ -343,12 +344,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     int tried = 0;                  // without draft: refused so far, of those that the rest is without
     bool exact = false;             // mass and the factors come of 64-bit sums
     double mass = 1.0;              // of the rest
-    // the rest is max(of_p w - of_q q, 0), w the weight before its division by all; history: the masses so far
+    // the rest is max(of_p w - of_q q, 0), w the weight before its division by all.  The two products grow with every
+    // division by a small sum, and cancel; past 2^16 (2^-36 of a rest) it is taken step by step, each rest
+    // divided by its own sum
     double of_p = 1.0 / static_cast<double>(total32), of_q = 0.0;
     int refused = 0;
     auto rest_of = [&](double w, float qx, int x) {  // of token x
       if (q != nullptr) {
-        const double v = fma(w, of_p, -(static_cast<double>(qx) * of_q));
+        double v = w;
+        if (exact && of_q > 65536.0)
+          for (int k = 0; k < refused; ++k) v = fma(v, s.inv[k], -static_cast<double>(qx));
+        else v = fma(w, of_p, -(static_cast<double>(qx) * of_q));
         return v > 0.0 ? v : 0.0;
       }
       double v = w * of_p;
@@ -357,6 +363,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       return v;
     };
     auto refuse = [&] {  // a draft's child, the rest's sum being mass
+      if (exact) {
+        __syncthreads();
+        if (tid == 0) s.inv[refused] = refused == 0 ? of_p : 1.0 / mass;
+        __syncthreads();
+      }
       of_p /= mass;
       of_q = of_q / mass + 1.0;
       ++refused;
@@ -382,6 +393,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
 #pragma unroll
           for (int e = 0; e < 4; ++e) add(weight(x[e]) * unit, v + e);
         });
+      } else if (q != nullptr && of_q > 65536.0) {  // (rare: a token at a time)
+        for (int y = span.y0 + lane; y < span.y1; y += 32) {
+          const int v = y - span.mis;
+          if (v >= 0 && v < p.V) add(rest_of(weight(logit_of(row + v)), q[v], v), v);
+        }
       } else if (q != nullptr) {
         const double a = of_p, b = -of_q;
         each4<true>(row, q, q_vec, span, p.V, [&](int v, const float (&x)[4], const float (&d)[4]) {

@@ -171,6 +171,47 @@ def test_extreme_temperatures(ops, temperature, draft):
         check_verify(ops, c, temperature)
 
 
+@pytest.mark.parametrize("V", [5, 58, 20000])
+def test_a_rest_of_one_token_refusal_after_refusal(ops, V):
+    """p has 1e-8 on a token and all else on another, q more of the first, up to 1e-3.  A child of the first token
+    is refused; what is left is the other token alone, and of p's 1e-8 nothing: no child of the first is kept any more,
+    however small its uniform, and the other one is drawn."""
+    x, y = 1, V - 2
+    parents, uniforms = [-1] + [0] * 12, [0.0] + [0.9] * 6 + [1e-3] * 6
+    logits = torch.full((13, V), -math.inf, device="cuda")
+    logits[:, x], logits[:, y] = math.log(1e-8), 0.0
+    for b in (2e-7, 1.5e-6, 3e-6, 1e-5, 7e-5, 1e-4, 1e-3):
+        probs = torch.zeros(13, V, device="cuda")
+        probs[:, x], probs[:, y] = b, 1 - b
+        for draw in (0.0, 0.4, 0.99):
+            got = ops.verify_drafts(logits, torch.full((13,), x, device="cuda"), i32(parents), i32([0, 13]),
+                                    torch.tensor(uniforms, device="cuda"), torch.tensor([draw], device="cuda"),
+                                    draft_probs=probs, max_path=3)
+            assert (got.accepted.tolist(), got.next_token.tolist()) == ([1], [y]), (b, draw)
+
+
+@pytest.mark.parametrize("V", [5, 58, 1525, 20000])
+@pytest.mark.parametrize("near", [1e-4, 1e-3, 0.3])
+def test_refusal_after_refusal_of_a_draft_that_is_nearly_the_target(ops, V, near):
+    """Rows with most of the probability on one token, drafts near them, and children that the draft would hardly have
+    drawn, refused one after another: what is left of p is 1e-3 to 1e-7 each time, and is divided by itself each time."""
+    rng = np.random.default_rng(V)
+    for spread in (8.0, 14.0):
+        fresh = [20, 7, 3, 12, 25, 2, 9, 16]
+        c = verify_case(rng, fresh, V, near, kind="forest", spread=1.0, few=2)
+        rows = np.arange(len(c["tokens"]))
+        top = rng.integers(0, V, len(rows))
+        logits = c["logits"].double().numpy()
+        logits[rows, top] += spread
+        bent = logits + rng.normal(size=logits.shape) * near
+        probs = np.exp(bent - bent.max(1, keepdims=True))
+        c["logits"] = torch.tensor(logits, dtype=torch.float32)
+        c["probs"] = torch.tensor(probs / probs.sum(1, keepdims=True), dtype=torch.float32)
+        c["tokens"] = rng.integers(0, V, len(rows))
+        c["accept"] = (0.5 + 0.49 * c["accept"]).astype(np.float32)
+        check_verify(ops, c, 1.0)
+
+
 # ---------------------------------------------------------------------------------------------
 # paged_keep
 @pytest.mark.parametrize("in_place", [False, True])
