@@ -63,8 +63,14 @@ struct PagedTreePlan {
 PagedTreePlan plan_paged_tree(const mcb_paged_tree_attn_args* t) {
   PagedTreePlan pl = {};
   const long long G = t->attn.Hq / t->attn.Hkv;
-  // Chunks of up to 1,024 tokens share the tree kernel's launch: two of 300 beside 22 trees of 41, window 1,024, 95
-  // -> 54 us.  Above that the chunk kernel's products are worth its launch.
+  // Chunks of up to 1,024 tokens share the tree kernel's launch, which saves two kernels; longer ones get the chunk
+  // kernel, whose products are faster.  Two chunks beside 22 trees of 41 tokens, one launch against two, us by events:
+  //   16/4 heads of 128 at 4,000 cached: chunks of 300 95, 125; of 1,000 148, 166; of 2,000 232, 237
+  //                     at 16,000:       300 278, 300; 1,000 474, 451; 2,000 761, 682;  window 1,024: 42, 83; 71, 92; 93, 115
+  //   12/12 of 64       at 500:          300 46, 63; 1,000 60, 72; 2,000 87, 98
+  //                     at 4,000:        300 157, 129; 1,000 191, 150; 2,000 249, 197;  window 1,024: 67, 76; 83, 86; 97, 98
+  // So with long cached lengths and no window two would be faster from some 300 to 1,000 tokens on; the lengths are not
+  // known here.
   pl.chunk = t->attn.max_new == 0 || t->attn.max_new > std::max(32 * t->words, 1024);
   pl.grid = std::min(device_sm_count(), mcb::kTreeMostCuts);
   // trees of at most max_new tokens, where that is known: as few rows as hold them
