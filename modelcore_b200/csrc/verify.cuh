@@ -22,7 +22,7 @@
 //   sums can be (it grows with the tokens a lane adds up); children are kept or refused by these while the sides of the comparison are further apart than
 //   that, in nearly all cases.  Where they are not, and where the walk ends and a token is drawn, the row is
 //   summed again in 64 bits (bound by the 64-bit units: about 11 operations a token and pass).
-// Measured: 64 requests of 16 tokens, wide 3, 131,071 logits of fp32 and draft_probs 146 us (207 MB; the slowest
+// Measured: 64 requests of 16 tokens, wide 3, 131,071 logits of fp32 and draft_probs 146 to 156 us by the draws (207 MB; the slowest
 // request's chain of passes, 4 CTAs: 8 us a row in 32 bits, 15 to 30 a pass in 64), 3 requests of 8 tokens and 32,768
 // logits 25 us, latency; greedy 78 and 16 us, bf16 logits 141 and 25.
 // 2^t in 64 bits: 32 t = n + f with |f| <= 1/2, a table of 2^(j/32) and five terms of 2^(f/32)'s series in f ln 2 / 32
